@@ -196,6 +196,69 @@ rtg_result rtg_forward_cached_batched(const rtg_model* model, rtg_cache* cache, 
 rtg_result rtg_generate_cached_batched(const rtg_model* model, const uint32_t* prompts, size_t batch, size_t n,
                                        size_t max_new, uint32_t* out, rtg_timing* timing);
 
+/* ---- 8-bit key/value cache over device tensors (no counterpart in the
+ * reference, whose cache is f32 vectors on the host, gpt2.rs:111-175). For
+ * programs that run their own layers: writing keys and values, reading them
+ * back, and attention over them, for any number of sequences and of query
+ * heads per key/value head. rtg_cache_new_quantised (above) is the same cache
+ * under a GPT-2 model.
+ *
+ * For each (sequence, head), keys and values apart, every `block` consecutive
+ * tokens (16, 32 or 64) share one scale:
+ *   s = f32(max |x| over the block's tokens so far / 127)   (0 where a token's
+ *       maximum is below 127 * 2^-126; NaN where a value is not finite)
+ *   code = the integer nearest to x / s, ties to even; it reads back as code * s.
+ * The last, partly filled block is quantised from its tokens' unrounded values,
+ * which are kept in f32 until it is full: what the cache holds does not depend
+ * on how the tokens were split over appends. 2 bytes per token, head and
+ * column (columns padded to 64 or 128), 8 per block and head, and
+ * 2 * block * columns f32 per sequence and head for the open block.
+ *
+ * Rows are [n_seq][tokens][heads][head_dim] in device memory of the device that
+ * was current when the cache was made, in any strides (elements; a row's
+ * head_dim columns contiguous); counts, start and first are device arrays of
+ * n_seq int32, or NULL. Calls enqueue on `stream` (a hipStream_t of that device,
+ * NULL for the default stream) and return without waiting; they allocate
+ * nothing and may be captured into a graph, each replay acting on the cache as
+ * it then is. Lengths live on the device. A cache must not be used by two
+ * calls (or replays) at once, the reading ones included: they share a
+ * workspace. Calls on different streams need the streams' own ordering. ---- */
+typedef struct rtg_qcache rtg_qcache;
+typedef struct {
+  void* data;
+  ptrdiff_t stride_seq, stride_token, stride_head;
+} rtg_rows;
+/* Errors: "head_dim <hd> is not supported (1 to 128)", "block <b> is not
+ * supported (16, 32 or 64)", capacities over 4000000 tokens. */
+rtg_result rtg_qcache_new(size_t n_seq, size_t n_head, size_t head_dim, size_t capacity, size_t block,
+                          rtg_qcache** out);
+void rtg_qcache_destroy(rtg_qcache* cache);
+/* n_new tokens to every sequence, or the first counts[s] (clamped to 0 ..
+ * n_new) of its rows; behind its length, or with start from token start[s] on:
+ * what lay there and behind is dropped (start of 0: the sequence begins anew;
+ * n_new = 0: only dropped). Where a cut falls into a block that was already
+ * full, that block's remaining tokens count as the values they read back as. A
+ * sequence whose start is negative or behind its length, or whose tokens would
+ * pass the capacity, is left as it was, and rtg_qcache_lengths reports it. */
+rtg_result rtg_qcache_append(rtg_qcache* cache, rtg_dtype dtype, const rtg_rows* k, const rtg_rows* v, size_t n_new,
+                             const int32_t* counts, const int32_t* start, void* stream);
+/* The values of tokens first[s] (0 for NULL) .. first[s] + n - 1 of every
+ * sequence, rounded to dtype; rows that hold no token are set to 0. k or v may be NULL. */
+rtg_result rtg_qcache_read(const rtg_qcache* cache, rtg_dtype dtype, const rtg_rows* k, const rtg_rows* v, size_t n,
+                           const int32_t* first, void* stream);
+/* Causal attention of the last counts[s] (n_q for NULL, clamped to 0 .. n_q)
+ * tokens of every sequence: query i of c sits at position len - c + i and sees
+ * the keys up to its own; softmax of scale * q . k, in f32 or better, results
+ * rounded to dtype once. Query head h reads key/value head h / (n_q_head /
+ * n_head). Rows i >= counts[s], and rows of queries before the sequence's first
+ * token, are set to 0. out must not overlap the queries. */
+rtg_result rtg_qcache_attend(rtg_qcache* cache, rtg_dtype dtype, const rtg_rows* queries, size_t n_q,
+                             size_t n_q_head, const int32_t* counts, float scale, const rtg_rows* out, void* stream);
+/* Waits for the stream and writes the n_seq lengths. Returns an error once
+ * (the lengths are written all the same) where an append since the last call
+ * left a sequence as it was. Not for a stream that is being captured. */
+rtg_result rtg_qcache_lengths(rtg_qcache* cache, uint32_t* out, void* stream);
+
 /* ---- BpeTokenizer, rusttorch-core/src/data/tokenizer.rs (host-side text in
  * and out; used by the reference's example at examples/gpt2.rs:77-95).
  * Text is UTF-8 with an explicit length (a Rust &str). Buffers that a call

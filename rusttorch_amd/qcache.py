@@ -1,0 +1,150 @@
+"""An 8-bit key/value cache over device tensors: torch's side of rtg_qcache_*
+(include/rtgpu.h has what the cache holds and what each call does).
+
+Programs that run their own layers write keys and values with `append`, run
+attention over them with `attend` and get them back with `read`; the calls go
+to the tensors' current stream and do not wait for it. Tensors are
+[n_seq, tokens, heads, head_dim] on the cache's device, f32, bf16 or f16, in any
+strides whose last is 1. There is no counterpart in the reference.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from ._lib import Gpt2Error, Rows, check
+
+__all__ = ["QuantisedCache"]
+
+_TYPES = {torch.float32: _lib.RTG_F32, torch.bfloat16: _lib.RTG_BF16, torch.float16: _lib.RTG_F16}
+
+
+def _one_runtime() -> None:
+    """torch and the library must have loaded the same HIP runtime: streams and
+    memory of one mean nothing to another. They do when torch comes first."""
+    with open("/proc/self/maps") as f:
+        paths = {line.split(None, 5)[5].strip() for line in f if "libamdhip64" in line}
+    if len(paths) > 1:
+        raise Gpt2Error("two HIP runtimes are loaded (" + ", ".join(sorted(paths)) +
+                        "): import torch before the library is first used")
+
+
+class QuantisedCache:
+    """Keys and values of `n_seq` sequences and `n_head` heads, up to `capacity`
+    tokens each, in 8 bits with a scale per `block` (16, 32 or 64) tokens and head."""
+
+    def __init__(self, n_seq: int, n_head: int, head_dim: int, capacity: int, block: int = 32, device=None):
+        self._h = None
+        for name, x in (("n_seq", n_seq), ("n_head", n_head), ("head_dim", head_dim), ("capacity", capacity),
+                        ("block", block)):
+            if x < 0:
+                raise Gpt2Error(f"{name} must not be negative")
+        self._lib = _lib.load()
+        h = C.c_void_p()
+        if torch.cuda.is_available():
+            _one_runtime()
+            self.device = torch.device("cuda" if device is None else device)
+            if self.device.type != "cuda":
+                raise Gpt2Error("the cache's device must be a GPU")
+            if self.device.index is None:
+                self.device = torch.device("cuda", torch.cuda.current_device())
+            with torch.cuda.device(self.device):
+                check(self._lib.rtg_qcache_new(n_seq, n_head, head_dim, capacity, block, C.byref(h)))
+        else:
+            check(self._lib.rtg_qcache_new(n_seq, n_head, head_dim, capacity, block, C.byref(h)))
+        self._h = h
+        self.n_seq, self.n_head, self.head_dim, self.capacity, self.block = n_seq, n_head, head_dim, capacity, block
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            self._lib.rtg_qcache_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    # -- arguments --
+
+    def _stream(self):
+        if self._h is None:
+            raise Gpt2Error("the cache is closed")
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _rows(self, what: str, x: torch.Tensor, heads: int, tokens=None) -> Rows:
+        if x.dim() != 4 or x.shape[0] != self.n_seq or x.shape[3] != self.head_dim or (heads and x.shape[2] != heads):
+            raise Gpt2Error(f"{what} must be [{self.n_seq}, tokens, {heads or 'heads'}, {self.head_dim}], not {list(x.shape)}")
+        if tokens is not None and x.shape[1] != tokens:
+            raise Gpt2Error(f"{what} must have {tokens} tokens, not {x.shape[1]}")
+        if x.dtype not in _TYPES:
+            raise Gpt2Error(f"{what} must be f32, bf16 or f16, not {x.dtype}")
+        if x.device != self.device:
+            raise Gpt2Error(f"{what} is on {x.device}, the cache on {self.device}")
+        seq, tok, head, col = x.stride()
+        if col != 1 and self.head_dim > 1 and x.numel():
+            raise Gpt2Error(f"{what}'s last dimension must be contiguous")
+        return Rows(x.data_ptr(), seq, tok, head)
+
+    def _ints(self, what: str, x):
+        if x is None:
+            return None
+        if x.dtype != torch.int32 or x.dim() != 1 or x.shape[0] != self.n_seq or not x.is_contiguous():
+            raise Gpt2Error(f"{what} must be {self.n_seq} contiguous int32")
+        if x.device != self.device:
+            raise Gpt2Error(f"{what} is on {x.device}, the cache on {self.device}")
+        return x.data_ptr()
+
+    # -- calls --
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, counts=None, start=None) -> None:
+        """Writes k, v [n_seq, tokens, n_head, head_dim] behind the sequences, or from token start[s] on (what lay
+        there and behind is dropped); of sequence s the first counts[s] tokens (clamped to 0 .. tokens)."""
+        stream = self._stream()
+        kr = self._rows("k", k, self.n_head)
+        vr = self._rows("v", v, self.n_head, k.shape[1])
+        if k.dtype != v.dtype:
+            raise Gpt2Error(f"k is {k.dtype}, v {v.dtype}")
+        check(self._lib.rtg_qcache_append(self._h, _TYPES[k.dtype], kr, vr, k.shape[1], self._ints("counts", counts),
+                                          self._ints("start", start), stream))
+
+    def attend(self, q: torch.Tensor, counts=None, scale=None, out=None) -> torch.Tensor:
+        """Attention of the last counts[s] tokens of each sequence, q [n_seq, tokens, query heads, head_dim], over
+        the keys up to their own position; scale: 1 / sqrt(head_dim). Padding rows are 0."""
+        stream = self._stream()
+        qr = self._rows("q", q, 0)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif out.dtype != q.dtype:
+            raise Gpt2Error(f"out is {out.dtype}, q {q.dtype}")
+        outr = self._rows("out", out, q.shape[2], q.shape[1])
+        check(self._lib.rtg_qcache_attend(self._h, _TYPES[q.dtype], qr, q.shape[1], q.shape[2],
+                                          self._ints("counts", counts),
+                                          self.head_dim ** -0.5 if scale is None else scale, outr, stream))
+        return out
+
+    def read(self, n: int, first=None, dtype: torch.dtype = torch.float32, k=None, v=None):
+        """(k, v) [n_seq, n, n_head, head_dim]: the values of tokens first[s] (0) .. + n, 0 where there is none."""
+        stream = self._stream()
+        if n < 0:
+            raise Gpt2Error("n must not be negative")
+        if dtype not in _TYPES:
+            raise Gpt2Error(f"dtype must be f32, bf16 or f16, not {dtype}")
+        shape = (self.n_seq, n, self.n_head, self.head_dim)
+        k = torch.empty(shape, dtype=dtype, device=self.device) if k is None else k
+        v = torch.empty(shape, dtype=dtype, device=self.device) if v is None else v
+        if k.dtype != dtype or v.dtype != dtype:
+            raise Gpt2Error(f"k and v must be {dtype}")
+        check(self._lib.rtg_qcache_read(self._h, _TYPES[dtype], self._rows("k", k, self.n_head, n),
+                                        self._rows("v", v, self.n_head, n), n, self._ints("first", first), stream))
+        return k, v
+
+    def lengths(self) -> list:
+        """Tokens of each sequence (waits for the current stream). Raises once where an append since the last call
+        left a sequence as it was because its tokens did not fit."""
+        out = (C.c_uint32 * self.n_seq)()
+        check(self._lib.rtg_qcache_lengths(self._h, out, self._stream()))
+        return list(out)
