@@ -208,11 +208,11 @@ rtg_result rtg_generate_cached_batched(const rtg_model* model, const uint32_t* p
  *   s = f32(max |x| over the block's tokens so far / 127)   (0 where a token's
  *       maximum is below 127 * 2^-126; NaN where a value is not finite)
  *   code = the integer nearest to x / s, ties to even; it reads back as code * s.
- * The last, partly filled block is quantised from its tokens' unrounded values,
- * which are kept in f32 until it is full: what the cache holds does not depend
- * on how the tokens were split over appends. 2 bytes per token, head and
+ * The last token's block is quantised from its tokens' unrounded values, which
+ * are kept in f32 until the next block begins: what the cache holds does not
+ * depend on how the tokens were split over appends. 2 bytes per token, head and
  * column (columns padded to 64 or 128), 8 per block and head, and
- * 2 * block * columns f32 per sequence and head for the open block.
+ * 2 * block * columns f32 per sequence and head for the last block.
  *
  * Rows are [n_seq][tokens][heads][head_dim] in device memory of the device that
  * was current when the cache was made, in any strides (elements; a row's
@@ -236,8 +236,8 @@ void rtg_qcache_destroy(rtg_qcache* cache);
 /* n_new tokens to every sequence, or the first counts[s] (clamped to 0 ..
  * n_new) of its rows; behind its length, or with start from token start[s] on:
  * what lay there and behind is dropped (start of 0: the sequence begins anew;
- * n_new = 0: only dropped). Where a cut falls into a block that was already
- * full, that block's remaining tokens count as the values they read back as. A
+ * n_new = 0: only dropped). Where a cut falls into a block before
+ * the last token's, that block's remaining tokens count as the values they read back as. A
  * sequence whose start is negative or behind its length, or whose tokens would
  * pass the capacity, is left as it was, and rtg_qcache_lengths reports it. */
 rtg_result rtg_qcache_append(rtg_qcache* cache, rtg_dtype dtype, const rtg_rows* k, const rtg_rows* v, size_t n_new,

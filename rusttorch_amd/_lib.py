@@ -48,15 +48,6 @@ class NamedTensor(C.Structure):
     ]
 
 
-class Rows(C.Structure):
-    _fields_ = [
-        ("data", C.c_void_p),
-        ("stride_seq", C.c_ssize_t),
-        ("stride_token", C.c_ssize_t),
-        ("stride_head", C.c_ssize_t),
-    ]
-
-
 class Timing(C.Structure):
     _fields_ = [
         ("profile_kernels", C.c_int),
@@ -99,14 +90,15 @@ SIGNATURES = {
     "rtg_forward_cached_batched": (Result, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "rtg_generate_cached_batched": (Result, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t,
                                              C.c_void_p, C.POINTER(Timing)]),
+    # (an rtg_rows is passed as its bytes: qcache.py)
     "rtg_qcache_new": (Result, [C.c_size_t] * 5 + [C.POINTER(C.c_void_p)]),
     "rtg_qcache_destroy": (None, [C.c_void_p]),
-    "rtg_qcache_append": (Result, [C.c_void_p, C.c_int, C.POINTER(Rows), C.POINTER(Rows), C.c_size_t, C.c_void_p,
+    "rtg_qcache_append": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_char_p, C.c_size_t, C.c_void_p,
                                    C.c_void_p, C.c_void_p]),
-    "rtg_qcache_read": (Result, [C.c_void_p, C.c_int, C.POINTER(Rows), C.POINTER(Rows), C.c_size_t, C.c_void_p,
+    "rtg_qcache_read": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_char_p, C.c_size_t, C.c_void_p,
                                  C.c_void_p]),
-    "rtg_qcache_attend": (Result, [C.c_void_p, C.c_int, C.POINTER(Rows), C.c_size_t, C.c_size_t, C.c_void_p,
-                                   C.c_float, C.POINTER(Rows), C.c_void_p]),
+    "rtg_qcache_attend": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_size_t, C.c_size_t, C.c_void_p,
+                                   C.c_float, C.c_char_p, C.c_void_p]),
     "rtg_qcache_lengths": (Result, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "rtg_tokenizer_from_files": (Result, [C.c_char_p, C.c_char_p, C.POINTER(C.c_void_p)]),
     "rtg_tokenizer_from_strings": (Result, [C.c_char_p, C.c_size_t, C.c_char_p, C.c_size_t, C.POINTER(C.c_void_p)]),

@@ -138,6 +138,11 @@ template <int HDP>
 struct Tile {
   static constexpr int KS = HDP / 64, DT = HDP / 16;
   i32x4 k[4][KS], v[DT];
+  float2 s;  // lane i: the scales (keys', values') of the tile's block i, over and over
+  // sp: the (sequence, head)'s scales
+  __device__ __forceinline__ void load_s(const float* sp, int tile, int shift, int lane) {
+    s = reinterpret_cast<const float2*>(sp)[(tile << (6 - shift)) + (lane & ((1 << (6 - shift)) - 1))];
+  }
   // kp, vp: the (sequence, head)'s codes
   __device__ __forceinline__ void load_k(const int8_t* kp, int tile, int lane) {
     const int8_t* p = kp + (size_t)tile * kQTile * HDP + (lane & 15) * HDP + (lane >> 4) * 16;
@@ -153,14 +158,17 @@ struct Tile {
   }
 };
 
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
 __device__ __forceinline__ float xmax(float v) { return xor32_max_k(xor16_max_k(v)); }
 __device__ __forceinline__ float xsum(float v) { return xor32_sum_k(xor16_sum_k(v)); }
 
 // One tile (tokens j0 .. j0 + 63) for a wave's columns. edge: some column does
 // not see all of its keys; live: keys below this are in the cache (uniform).
 template <int HDP, int ND>
-__device__ __forceinline__ void tile_step(Cols<HDP, ND>& c, const Tile<HDP>& t, const float* ks, const float* vs,
-                                          int shift, int j0, bool edge, int live, int group) {
+__device__ __forceinline__ void tile_step(Cols<HDP, ND>& c, const Tile<HDP>& t, int shift, int j0, bool edge, int live,
+                                          int group) {
   constexpr int DT = HDP / 16;
   // the tile's scales: of each 16 tokens; those of blocks behind the last key are not read as numbers
   float fk[4], rv[4];
@@ -168,10 +176,10 @@ __device__ __forceinline__ void tile_step(Cols<HDP, ND>& c, const Tile<HDP>& t, 
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int b = (j0 + i * 16) >> shift;
+    const int b = (i * 16) >> shift;
     const bool in = j0 + i * 16 < live;
-    fk[i] = in ? ks[b] : 0.f;
-    rv[i] = in ? vs[b] : 0.f;
+    fk[i] = in ? lane_of(t.s.x, b) : 0.f;
+    rv[i] = in ? lane_of(t.s.y, b) : 0.f;
     vmax = fmaxf(vmax, rv[i]);  // (skips NaN)
     bad |= rv[i] != rv[i];
   }
@@ -325,18 +333,24 @@ __global__ __launch_bounds__(256) void q_attend_cols_kernel(AttnArgs a) {
   const int least = firstq < r.count ? visible(r, firstq) : 0;
   const int tiles = (live + kQTile - 1) / kQTile;
   const int8_t *kp = a.c.k + a.c.codes(sh), *vp = a.c.v + a.c.codes(sh);
-  const float *ks = a.c.ks + a.c.scales(sh), *vs = a.c.vs + a.c.scales(sh);
+  const float* sp = a.c.s + a.c.scales(sh);
+  const int shift = a.c.block_shift;
   Tile<HDP> t;
-  if (tiles) t.load_k(kp, 0, lane);
+  if (tiles) {
+    t.load_s(sp, 0, shift, lane);
+    t.load_k(kp, 0, lane);
+  }
   for (int j = 0; j < tiles; ++j) {
     t.load_v(vp, j, lane);
     Tile<HDP> n;
+    n.load_s(sp, min(j + 1, tiles - 1), shift, lane);
     n.load_k(kp, min(j + 1, tiles - 1), lane);
-    tile_step(c, t, ks, vs, a.c.block_shift, j * kQTile, j * kQTile + kQTile > least, live, group);
+    tile_step(c, t, shift, j * kQTile, j * kQTile + kQTile > least, live, group);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
       for (int y = 0; y < Cols<HDP, ND>::KS; ++y) t.k[x][y] = n.k[x][y];
+    t.s = n.s;
   }
   const float l = xsum(c.l);
   if (!mine) return;
@@ -386,19 +400,22 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
   const T* qrow = static_cast<const T*>(a.q.p) + (long)seq * a.q.seq + (long)i * a.q.tok + (long)qh * a.q.head;
   c.init(used ? qrow : nullptr, a.c.hd, a.qvec, group, a.scale, used ? visible(r, i) : 0);
   const int8_t *kp = a.c.k + a.c.codes(sh), *vp = a.c.v + a.c.codes(sh);
-  const float *ks = a.c.ks + a.c.scales(sh), *vs = a.c.vs + a.c.scales(sh);
+  const float* sp = a.c.s + a.c.scales(sh);
+  const int shift = a.c.block_shift;
   Tile<HDP> t;
   int j = t0 + wave;
   if (j < t1) {
+    t.load_s(sp, j, shift, lane);
     t.load_k(kp, j, lane);
     t.load_v(vp, j, lane);
   }
   for (; j < t1; j += NW) {
     Tile<HDP> n;
     const int nj = min(j + NW, tiles - 1);
+    n.load_s(sp, nj, shift, lane);
     n.load_k(kp, nj, lane);
     n.load_v(vp, nj, lane);
-    tile_step(c, t, ks, vs, a.c.block_shift, j * kQTile, j * kQTile + kQTile > least, live, group);
+    tile_step(c, t, shift, j * kQTile, j * kQTile + kQTile > least, live, group);
     t = n;
   }
   const float l = xsum(c.l);
@@ -451,10 +468,16 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
   }
 }
 
-// Joins the splits of the columns that have more than one: a wave per column.
+// Joins the splits of the columns that have more than one: a workgroup per
+// column, its threads 4 results of a split each.
 template <int HDP, class T>
-__global__ __launch_bounds__(64) void q_attend_join_kernel(AttnArgs a) {
-  const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head, lane = threadIdx.x;
+__global__ __launch_bounds__(256) void q_attend_join_kernel(AttnArgs a) {
+  constexpr int C4 = HDP / 4, ZS = 256 / C4;
+  __shared__ float sm[4];
+  __shared__ __attribute__((aligned(16))) float4 so[4][C4];
+  __shared__ float sl[4];
+  const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int ci = blockIdx.y, cb = ci >> 4, qi = ci / a.group, h = head * a.group + ci - qi * a.group;
   const Seq r = seq_of(a, seq);
   const int last = min((cb * 16 + 15) / a.group, r.count - 1);
@@ -463,15 +486,17 @@ __global__ __launch_bounds__(64) void q_attend_join_kernel(AttnArgs a) {
   if (per >= tiles) return;
   const int n = (tiles + per - 1) / per;
   float m = -INFINITY;
-  for (int z = lane; z < n; z += 64) m = fmaxf(m, part_of<HDP>(a, sh, cb, z, ci & 15)[0]);
+  for (int z = tid; z < n; z += 256) m = fmaxf(m, part_of<HDP>(a, sh, cb, z, ci & 15)[0]);
   for (int w = 1; w < 64; w <<= 1) m = fmaxf(m, __shfl_xor(m, w));
+  if (lane == 0) sm[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
   const float base = m == -INFINITY ? 0.f : m;
-  // lanes: 4 results each, the splits over the lanes left
-  constexpr int C4 = HDP / 4, ZS = 64 / C4;
-  const int c4 = (lane % C4) * 4;
+  const int c4 = (tid % C4) * 4;
   float ls = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int z = lane / C4; z < n; z += ZS) {
+#pragma unroll 4
+  for (int z = tid / C4; z < n; z += ZS) {
     const float* p = part_of<HDP>(a, sh, cb, z, ci & 15);
     const float f = __builtin_amdgcn_exp2f(p[0] - base);
     ls = fmaf(f, p[1], ls);
@@ -487,14 +512,21 @@ __global__ __launch_bounds__(64) void q_attend_join_kernel(AttnArgs a) {
     x.z += __shfl_xor(x.z, w);
     x.w += __shfl_xor(x.w, w);
   }
-  if (lane >= C4) return;
+  if (lane < C4) so[wave][lane] = x;
+  if (lane == 0) sl[wave] = ls;
+  __syncthreads();
+  if (tid >= C4) return;
+  ls = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const float4 y0 = so[0][tid], y1 = so[1][tid], y2 = so[2][tid], y3 = so[3][tid];
   const bool any = qi < r.count && visible(r, qi) > 0;
   const float inv = 1.f / ls;
   put4<T>(a, seq, qi, h, c4,
-          any ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
+          any ? make_float4(((y0.x + y1.x) + (y2.x + y3.x)) * inv, ((y0.y + y1.y) + (y2.y + y3.y)) * inv,
+                            ((y0.z + y1.z) + (y2.z + y3.z)) * inv, ((y0.w + y1.w) + (y2.w + y3.w)) * inv)
+              : make_float4(0.f, 0.f, 0.f, 0.f));
 }
 
-constexpr int kParts = 2048;  // (sequence, head, column block, split)s with partials
+constexpr int kParts = 768;  // (sequence, head, column block, split)s with partials
 
 template <int HDP, int ND, class T>
 void attend(hipStream_t s, AttnArgs& a) {
@@ -509,7 +541,7 @@ void attend(hipStream_t s, AttnArgs& a) {
   const dim3 grid((unsigned)heads, (unsigned)a.cblocks, (unsigned)a.splits);
   q_attend_split_kernel<HDP, ND, T><<<grid, 256, 0, s>>>(a);
   if (a.splits > 1)
-    q_attend_join_kernel<HDP, T><<<dim3((unsigned)heads, (unsigned)(a.n_q * a.group)), 64, 0, s>>>(a);
+    q_attend_join_kernel<HDP, T><<<dim3((unsigned)heads, (unsigned)(a.n_q * a.group)), 256, 0, s>>>(a);
 }
 
 template <int ND, class T>

@@ -6,9 +6,9 @@
 //       (a token whose amax is below 127 * 2^-126 counts as 0, one with a value
 //       that is not finite as NaN, and NaN is the largest)
 //   code = the integer nearest to x / s, ties to even; 0 where s is 0 or NaN.
-// The block that is not full (the open block) is quantised anew from its
-// tokens' f32 values, kept in `tail`, whenever a token raises its scale, so the
-// cache depends on the tokens only and not on how they were split over calls.
+// The block of the last token is quantised anew from its tokens' f32 values,
+// kept in `tail`, whenever a token raises its scale, so the cache depends on the
+// tokens only and not on how they were split over calls.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -29,12 +29,12 @@ struct QStore {
   int block = 0, block_shift = 0;
   int capacity = 0, tiles = 0;  // tokens; tiles per (sequence, head)
   int8_t *k = nullptr, *v = nullptr;
-  float *ks = nullptr, *vs = nullptr;  // scales [seq][head][tiles * 64 / block]
-  float* tail = nullptr;    // open block's values [seq][head][2][block][hdp]
+  float* s = nullptr;       // scales [seq][head][tiles * 64 / block][2]: keys', values'
+  float* tail = nullptr;    // the last block's values [seq][head][2][block][hdp]
   float* tail_s = nullptr;  // and its tokens' own scales [seq][head][2][block]
 
   __host__ __device__ size_t codes(size_t sh) const { return sh * tiles * (size_t)kQTile * hdp; }
-  __host__ __device__ size_t scales(size_t sh) const { return sh * ((size_t)tiles * kQTile >> block_shift); }
+  __host__ __device__ size_t scales(size_t sh) const { return sh * 2 * ((size_t)tiles * kQTile >> block_shift); }
   __host__ __device__ size_t tails(size_t sh, int which) const { return (sh * 2 + which) * (size_t)block * hdp; }
   __host__ __device__ size_t tail_scales(size_t sh, int which) const { return (sh * 2 + which) * (size_t)block; }
   // The sequences from `first` on as a store of their own (a layer of a model's cache).
@@ -44,8 +44,7 @@ struct QStore {
     r.n_seq = n;
     r.k += codes(sh);
     r.v += codes(sh);
-    r.ks += scales(sh);
-    r.vs += scales(sh);
+    r.s += scales(sh);
     r.tail += tails(sh, 0);
     r.tail_s += tail_scales(sh, 0);
     return r;
@@ -74,16 +73,24 @@ struct QLen {
   int stride = 1;
 };
 
+// For appends that move the lengths: how many workgroups of the append in flight
+// have read their sequence's length, counted per (sequence, head) and, as the
+// heads are through, per sequence (0 between appends; a counter per cache line:
+// atomics on one line take turns, 8.6 ns each); and *err = min(*err,
+// seq * 4 + 1 or 2) where a sequence's start (1) or its number of tokens (2) is refused.
+struct QTickets {
+  unsigned* count = nullptr;  // [n_seq * (n_head + 1)][kQTicketStride]
+  unsigned* err = nullptr;
+};
+constexpr int kQTicketStride = 32;
+
 // New tokens k, v (at most n_new for a sequence; counts[seq] of them where
 // counts is given, clamped to 0 .. n_new) behind the length, or from start[seq]
 // on where start is given. A sequence whose start is negative or behind its
-// length, or whose tokens would pass the capacity, is left as it is.
-void launch_q_append(hipStream_t s, const QStore& c, QLen len, QType type, const QRows& k, const QRows& v, int n_new,
-                     const int* counts, const int* start);
-// The lengths after the same append; *err = min(*err, seq * 4 + 1 or 2) where a
-// sequence's start (1) or its number of tokens (2) was refused.
-void launch_q_advance(hipStream_t s, const QStore& c, int* len, int n_new, const int* counts, const int* start,
-                      unsigned* err);
+// length, or whose tokens would pass the capacity, is left as it is. With
+// tickets the lengths are the new ones afterwards, else as they were.
+void launch_q_append(hipStream_t s, const QStore& c, QLen len, QTickets tickets, QType type, const QRows& k,
+                     const QRows& v, int n_new, const int* counts, const int* start);
 // Tokens first[seq] (0 without first) .. + n of every sequence as values; rows
 // that hold no token are set to 0. k or v may have no p.
 void launch_q_read(hipStream_t s, const QStore& c, QLen len, QType type, const QRows& k, const QRows& v, int n,

@@ -36,7 +36,7 @@ struct Parts {
 
 size_t qstore_bytes(const QStore& c) {
   const Parts p(c);
-  return 2 * p.codes + 2 * p.scales + p.tail + p.tail_s;
+  return 2 * p.codes + p.scales + p.tail + p.tail_s;
 }
 
 void qstore_place(QStore* c, void* mem) {
@@ -49,8 +49,7 @@ void qstore_place(QStore* c, void* mem) {
   };
   c->k = reinterpret_cast<int8_t*>(take(p.codes));
   c->v = reinterpret_cast<int8_t*>(take(p.codes));
-  c->ks = reinterpret_cast<float*>(take(p.scales));
-  c->vs = reinterpret_cast<float*>(take(p.scales));
+  c->s = reinterpret_cast<float*>(take(p.scales));
   c->tail = reinterpret_cast<float*>(take(p.tail));
   c->tail_s = reinterpret_cast<float*>(take(p.tail_s));
 }
@@ -60,7 +59,7 @@ namespace {
 // Where an append of a sequence goes: tokens [at, end) over a length of len.
 struct Place {
   int len, at, end;
-  int bad;  // 0, or why it is refused (launch_q_advance)
+  int bad;  // 0, or why it is refused (QTickets)
 };
 __device__ __forceinline__ Place place(int seq, const int* len, int len_stride, int n_new, const int* counts,
                                        const int* start, int capacity) {
@@ -73,6 +72,44 @@ __device__ __forceinline__ Place place(int seq, const int* len, int len_stride, 
   return p;
 }
 
+// The workgroup's Place, read by its first thread, which then counts the
+// workgroup as one that has read its sequence's length; finish() by the last of
+// a sequence's workgroups (per_head of each head) writes the new one. The loads
+// have returned before the barrier (their values went through LDS), so no
+// workgroup can see the new length in place of the old. This saves the launch of
+// a kernel for the lengths alone (3 us of the host's time, 2 of the GPU's).
+class Turn {
+ public:
+  __device__ __forceinline__ Place begin(Place* shared, const QStore& c, int sh, const QLen& len, QTickets tickets,
+                                         int n_new, const int* counts, const int* start) {
+    tickets_ = tickets;
+    seq_ = sh / c.n_head;
+    if (threadIdx.x == 0) *shared = place(seq_, len.p, len.stride, n_new, counts, start, c.capacity);
+    __syncthreads();
+    mine_ = tickets.count + ((size_t)c.n_seq + sh) * kQTicketStride;
+    if (threadIdx.x == 0 && tickets.count) before_ = add(mine_);
+    return *shared;
+  }
+  __device__ __forceinline__ void finish(const Place& p, const QStore& c, const QLen& len, unsigned per_head) {
+    if (threadIdx.x != 0 || !tickets_.count || before_ != per_head - 1) return;
+    *mine_ = 0;
+    unsigned* all = tickets_.count + (size_t)seq_ * kQTicketStride;
+    if (add(all) != (unsigned)c.n_head - 1) return;
+    *all = 0;
+    if (p.bad) atomicMin(tickets_.err, (unsigned)seq_ * 4 + p.bad);
+    else len.p[(size_t)seq_ * len.stride] = p.end;
+  }
+
+ private:
+  static __device__ __forceinline__ unsigned add(unsigned* p) {
+    return __hip_atomic_fetch_add(p, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  QTickets tickets_;
+  unsigned* mine_ = nullptr;
+  int seq_ = 0;
+  unsigned before_ = 0;
+};
+
 constexpr unsigned kNanBits = 0x7FC00000u;
 
 // fl(amax / 127) of a token, as bits (which order like the values): 0 below
@@ -83,17 +120,36 @@ __device__ __forceinline__ unsigned token_scale(float amax) {
   return __float_as_uint(__fdiv_rn(amax, 127.f));
 }
 
-// The integer nearest to x / s, ties to even, |x / s| <= 127: r = rint(x * (1 /
-// s)) may be one off next to a border between two codes; x - r s says on which
+// The integers nearest to x / s, ties to even, |x / s| <= 127, as the bytes of a
+// word: r = x * (1 / s) rounded by adding 1.5 * 2^23, whose sum's low byte is r.
+// That may be one off next to a border between two codes; x - r s says on which
 // side x lies (it is exact there: a multiple of half s's last place below 2^24
-// of those).
-__device__ __forceinline__ int code_of(float x, float s, float inv) {
-  float r = rintf(x * inv);
+// of those), and is looked at again where it reaches half of s, which few words do.
+__device__ __forceinline__ float code_of(float x, float s, float r) {
   const float res = fmaf(-r, s, x), half = 0.5f * s;
   const bool odd = ((int)r & 1) != 0;
-  if (res > half || (res == half && odd)) r += 1.f;
-  else if (res < -half || (res == -half && odd)) r -= 1.f;
-  return (int)r;
+  if (res > half || (res == half && odd)) return r + 1.f;
+  if (res < -half || (res == -half && odd)) return r - 1.f;
+  return r;
+}
+__device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400), __builtin_amdgcn_perm(b, a, 0x0c0c0400),
+                               0x05040100);
+}
+__device__ __forceinline__ unsigned codes_of(const float4& x, float s, float inv) {
+  if (!(s > 0.f)) return 0;
+  constexpr float magic = 12582912.f;
+  const float t[4] = {fmaf(x.x, inv, magic), fmaf(x.y, inv, magic), fmaf(x.z, inv, magic), fmaf(x.w, inv, magic)};
+  float r[4] = {t[0] - magic, t[1] - magic, t[2] - magic, t[3] - magic};
+  const float far = fmaxf(fmaxf(fabsf(fmaf(-r[0], s, x.x)), fabsf(fmaf(-r[1], s, x.y))),
+                          fmaxf(fabsf(fmaf(-r[2], s, x.z)), fabsf(fmaf(-r[3], s, x.w))));
+  if (far < 0.5f * s)
+    return low_bytes(__float_as_uint(t[0]), __float_as_uint(t[1]), __float_as_uint(t[2]), __float_as_uint(t[3]));
+  r[0] = code_of(x.x, s, r[0]);
+  r[1] = code_of(x.y, s, r[1]);
+  r[2] = code_of(x.z, s, r[2]);
+  r[3] = code_of(x.w, s, r[3]);
+  return low_bytes((unsigned)(int)r[0], (unsigned)(int)r[1], (unsigned)(int)r[2], (unsigned)(int)r[3]);
 }
 __device__ __forceinline__ float scale_inv(float s) { return s > 0.f ? __fdiv_rn(1.f, s) : 0.f; }
 
@@ -124,158 +180,310 @@ __device__ __forceinline__ size_t value_byte(int tok, int col, int hdp) {
          (tok & 3);
 }
 
-// One tile (64 tokens) of one (sequence, head) of an append, keys (which = 0)
-// or values. Workgroup y takes the y-th tile that the new tokens touch; tokens
-// and groups of 4 columns go over the threads, a token's row over 16 or 32
-// neighbouring lanes. The first tile's workgroup also quantises the open block's
-// earlier tokens anew and writes the tail.
-template <int HDP, class T>
-__device__ void append_tile(const QStore& c, const Place& p, size_t sh, int y, int which, const T* src, long tok_stride,
-                            bool vec, unsigned* blkmax, unsigned char* image) {
-  constexpr int LPR = HDP / 4, TPP = 256 / LPR, PASSES = kQTile / TPP;  // lanes per row, tokens per pass
-  const int tid = threadIdx.x, c4 = (tid % LPR) * 4, trow = tid / LPR;
-  const int block = c.block;
-  const int tile0 = (p.at / kQTile + y) * kQTile;  // first token of the tile
-  const int blk0 = p.at / block * block;
-  const int first = y == 0 ? blk0 : tile0, hi = min(p.end, tile0 + kQTile);
-  // earlier tokens of the block that `at` lies in: from the tail while it is
-  // the open block, else as they read back
-  const bool open = p.at / block == p.len / block;
-  float* tail = c.tail + c.tails(sh, which);
-  float* tail_s = c.tail_s + c.tail_scales(sh, which);
-  int8_t* codes = (which ? c.v : c.k) + c.codes(sh);
-  float* scales = (which ? c.vs : c.ks) + c.scales(sh);
-
-  if (tid < 4) blkmax[tid] = 0;
-  __syncthreads();
-  float4 x[PASSES];
-  unsigned ts[PASSES];
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int tok = tile0 + i * TPP + trow;
-    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    ts[i] = 0;
-    if (tok >= first && tok < hi) {
-      if (tok >= p.at) {
-        x[i] = load4(src + (long)(tok - p.at) * tok_stride, c4, c.hd, vec);
-      } else if (open) {
-        x[i] = *reinterpret_cast<const float4*>(tail + (size_t)(tok - blk0) * HDP + c4);
-      } else {
-        const float s = scales[tok >> c.block_shift];
-        float* xe = &x[i].x;
-        for (int e = 0; e < 4; ++e)
-          xe[e] = (float)codes[which ? value_byte(tok, c4 + e, HDP) : (size_t)tok * HDP + c4 + e] * s;
-      }
-    }
-    const float amax = __uint_as_float(row_max_bits<HDP>(max_abs4(x[i])));
-    if (tok >= first && tok < hi) {
-      if (tok >= p.at) {
-        ts[i] = token_scale(amax);
-      } else if (open) {
-        ts[i] = __float_as_uint(tail_s[tok - blk0]);
-      } else {
-        // (a token that holds code 127 had the block's scale: amax / 127 may round otherwise)
-        const float s = scales[tok >> c.block_shift];
-        ts[i] = amax == 127.f * s ? __float_as_uint(s) : token_scale(amax);
-      }
-      if (c4 == 0) atomicMax(&blkmax[(tok - tile0) >> c.block_shift], ts[i]);
-    }
-  }
-  __syncthreads();  // (also: every read of the tail and of the codes is done)
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int tok = tile0 + i * TPP + trow;
-    if (tok < first || tok >= hi) continue;
-    const float s = __uint_as_float(blkmax[(tok - tile0) >> c.block_shift]);
-    const float inv = scale_inv(s);
-    const float* xe = &x[i].x;
-    unsigned q = 0;
-    int qe[4];
-    for (int e = 0; e < 4; ++e) {
-      qe[e] = s > 0.f ? code_of(xe[e], s, inv) : 0;
-      q |= (unsigned)(qe[e] & 255) << (8 * e);
-    }
-    if (which == 0) {
-      *reinterpret_cast<unsigned*>(codes + (size_t)tok * HDP + c4) = q;
-    } else {
-      for (int e = 0; e < 4; ++e) image[value_byte(tok - tile0, c4 + e, HDP)] = (unsigned char)qe[e];
-    }
-    if (c4 == 0 && (tok & (block - 1)) == 0) scales[tok >> c.block_shift] = s;
-    // the tail, where the first tile's block stays open (later tiles': append_tail)
-    if (y == 0 && tok / block == p.end / block && !(open && tok < p.at)) {
-      *reinterpret_cast<float4*>(tail + (size_t)(tok & (block - 1)) * HDP + c4) = x[i];
-      if (c4 == 0) tail_s[tok & (block - 1)] = __uint_as_float(ts[i]);
-    }
-  }
-  if (which == 1) {
-    // the tile's values leave in whole groups of 4 tokens (bytes of tokens
-    // behind the end are not part of the cache)
-    __syncthreads();
-    for (int j = tid; j < 4 * HDP; j += 256) {
-      const int g = j / HDP;
-      unsigned* dst = reinterpret_cast<unsigned*>(codes + (size_t)tile0 * HDP + (size_t)j * 16);
-      const unsigned* im = reinterpret_cast<const unsigned*>(image + (size_t)j * 16);
-      for (int t = 0; t < 4; ++t) {
-        const int tok = tile0 + t * 16 + g * 4;
-        if (tok >= first && tok < hi) dst[t] = im[t];
-      }
-    }
-  }
-  __syncthreads();
+// Whether the block that token `at` lies in is the one that the tail holds: the
+// block of the last token.
+__device__ __forceinline__ bool in_tail(const QStore& c, const Place& p) {
+  return p.len > 0 && p.at >> c.block_shift == (p.len - 1) >> c.block_shift;
 }
 
-// The tail of an append whose open block starts behind its first tile: written
+// A value of a full block as it reads back, and its token's own scale: a token
+// that holds code 127 had the block's scale (amax / 127 may round otherwise).
+__device__ __forceinline__ float code_value(int8_t code, float s) { return (float)code * s; }
+__device__ __forceinline__ unsigned read_back_scale(float amax, float s) {
+  return amax == 127.f * s ? __float_as_uint(s) : token_scale(amax);
+}
+
+// The tail of an append whose last block starts behind its first tile: written
 // by the first tile's workgroup, which has read the old tail by then.
 template <int HDP, class T>
 __device__ void append_tail(const QStore& c, const Place& p, size_t sh, int which, const T* src, long tok_stride,
                             bool vec) {
   constexpr int LPR = HDP / 4, TPP = 256 / LPR;
   const int c4 = (threadIdx.x % LPR) * 4, trow = threadIdx.x / LPR;
-  const int ob = p.end / c.block * c.block;
+  const int last = (p.end - 1) & ~(c.block - 1);
   float* tail = c.tail + c.tails(sh, which);
   float* tail_s = c.tail_s + c.tail_scales(sh, which);
   for (int t0 = 0; t0 < c.block; t0 += TPP) {  // (whole rows of lanes for row_max_bits)
     const int t = t0 + trow;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (ob + t < p.end) x = load4(src + (long)(ob + t - p.at) * tok_stride, c4, c.hd, vec);
+    if (last + t < p.end) x = load4(src + (long)(last + t - p.at) * tok_stride, c4, c.hd, vec);
     const float amax = __uint_as_float(row_max_bits<HDP>(max_abs4(x)));
-    if (ob + t < p.end) {
+    if (last + t < p.end) {
       *reinterpret_cast<float4*>(tail + (size_t)t * HDP + c4) = x;
       if (c4 == 0) tail_s[t] = __uint_as_float(token_scale(amax));
     }
   }
 }
 
-// A workgroup per (sequence, head, tile).
+// One tile (64 tokens) of one (sequence, head) of an append, keys (which = 0)
+// or values: the y-th tile that the new tokens touch. A thread has 4 columns of
+// 4 neighbouring tokens (a quad), a quad's columns lie on 16 or 32 neighbouring
+// lanes. The first tile's workgroup also quantises the block's earlier tokens
+// anew and writes the tail.
 template <int HDP, class T>
-__global__ __launch_bounds__(256) void q_append_kernel(QStore c, const int* __restrict__ len, int len_stride, QRows k,
-                                                       QRows v, int n_new, const int* __restrict__ counts,
-                                                       const int* __restrict__ start, bool vec) {
-  __shared__ unsigned blkmax[4];
-  __shared__ __attribute__((aligned(16))) unsigned char image[kQTile * HDP];
-  const int sh = blockIdx.x, seq = sh / c.n_head, head = sh - seq * c.n_head, y = blockIdx.y;
-  const Place p = place(seq, len, len_stride, n_new, counts, start, c.capacity);
-  if (p.bad || (p.at == p.end && p.at == p.len)) return;
-  const int tile0 = (p.at / kQTile + y) * kQTile;
-  if (y > 0 && tile0 >= p.end) return;
-  const T* ks = static_cast<const T*>(k.p) + seq * k.seq + head * k.head;
-  const T* vs = static_cast<const T*>(v.p) + seq * v.seq + head * v.head;
-  append_tile<HDP, T>(c, p, sh, y, 0, ks, k.tok, vec, blkmax, image);
-  append_tile<HDP, T>(c, p, sh, y, 1, vs, v.tok, vec, blkmax, image);
-  if (y == 0 && p.end / kQTile * kQTile > tile0 && p.end % c.block != 0) {
-    append_tail<HDP, T>(c, p, sh, 0, ks, k.tok, vec);
-    append_tail<HDP, T>(c, p, sh, 1, vs, v.tok, vec);
+__device__ __forceinline__ void append_tile(const QStore& c, const Place& p, size_t sh, int y, int which, const T* src,
+                                            long tok_stride, bool vec, unsigned* blkmax, unsigned* image) {
+  constexpr int LPR = HDP / 4, QPP = 256 / LPR, PASSES = 16 / QPP;  // lanes per quad, quads per pass
+  const int tid = threadIdx.x, c4 = (tid % LPR) * 4, qrow = tid / LPR;
+  const int tile0 = (p.at / kQTile + y) * kQTile;  // first token of the tile
+  const int blk0 = p.at & ~(c.block - 1);
+  const int first = y == 0 ? blk0 : tile0, hi = min(p.end, tile0 + kQTile);
+  const bool tailed = in_tail(c, p);
+  float* tail = c.tail + c.tails(sh, which);
+  float* tail_s = c.tail_s + c.tail_scales(sh, which);
+  int8_t* codes = (which ? c.v : c.k) + c.codes(sh);
+  float* scales = c.s + c.scales(sh) + which;
+
+  float4 x[PASSES][4];
+  unsigned ts[PASSES][4];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[i][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.end > p.at) {
+    // (rows outside are read as the nearest inside, so that no load waits for a branch)
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int tok = tile0 + (i * QPP + qrow) * 4 + e;
+        x[i][e] = load4(src + (long)(min(max(tok, p.at), hi - 1) - p.at) * tok_stride, c4, c.hd, vec);
+      }
+  }
+  if (tid < 4) blkmax[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int tok = tile0 + (i * QPP + qrow) * 4 + e;
+      ts[i][e] = token_scale(__uint_as_float(row_max_bits<HDP>(max_abs4(x[i][e]))));
+      if (tok < p.at || tok >= hi) {
+        x[i][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        ts[i][e] = 0;
+      }
+    }
+  if (first < p.at) {  // (uniform; y == 0) the block's earlier tokens
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int tok = tile0 + (i * QPP + qrow) * 4 + e;
+        const bool old = tok >= first && tok < p.at;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        unsigned os = 0;
+        if (old) {
+          if (tailed) {
+            o = *reinterpret_cast<const float4*>(tail + (size_t)(tok - blk0) * HDP + c4);
+            os = __float_as_uint(tail_s[tok - blk0]);
+          } else {
+            const float s = scales[2 * (tok >> c.block_shift)];
+            int8_t q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              q[j] = codes[which ? value_byte(tok, c4 + j, HDP) : (size_t)tok * HDP + c4 + j];
+            o = make_float4(code_value(q[0], s), code_value(q[1], s), code_value(q[2], s), code_value(q[3], s));
+          }
+        }
+        if (!tailed) {
+          const float amax = __uint_as_float(row_max_bits<HDP>(max_abs4(o)));
+          if (old) os = read_back_scale(amax, scales[2 * (tok >> c.block_shift)]);
+        }
+        if (old) {
+          x[i][e] = o;
+          ts[i][e] = os;
+        }
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const unsigned m = max(max(ts[i][0], ts[i][1]), max(ts[i][2], ts[i][3]));
+    if (c4 == 0) atomicMax(&blkmax[((i * QPP + qrow) * 4) >> c.block_shift], m);
+  }
+  __syncthreads();  // (also: every read of the tail, the scales and the codes is done)
+  const int last = (p.end - 1) >> c.block_shift;  // the block that the tail is to hold
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int quad = i * QPP + qrow, tok0 = tile0 + quad * 4;
+    const float s = __uint_as_float(blkmax[(quad * 4) >> c.block_shift]), inv = scale_inv(s);
+    unsigned q[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = codes_of(x[i][e], s, inv);
+    if (which == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (tok0 + e >= first && tok0 + e < hi) *reinterpret_cast<unsigned*>(codes + (size_t)(tok0 + e) * HDP + c4) = q[e];
+    } else {
+      // the quad's bytes by column; they leave in order of the image
+      const unsigned a = __builtin_amdgcn_perm(q[1], q[0], 0x05010400), b = __builtin_amdgcn_perm(q[3], q[2], 0x05010400);
+      const unsigned d = __builtin_amdgcn_perm(q[1], q[0], 0x07030602), f = __builtin_amdgcn_perm(q[3], q[2], 0x07030602);
+      unsigned* im = image + ((quad & 3) * HDP + c4) * 4 + (quad >> 2);
+      im[0] = __builtin_amdgcn_perm(b, a, 0x05040100);
+      im[4] = __builtin_amdgcn_perm(b, a, 0x07060302);
+      im[8] = __builtin_amdgcn_perm(f, d, 0x05040100);
+      im[12] = __builtin_amdgcn_perm(f, d, 0x07060302);
+    }
+    if (c4 == 0 && (tok0 & (c.block - 1)) == 0 && tok0 >= first && tok0 < hi) scales[2 * (tok0 >> c.block_shift)] = s;
+    // the tail, where the first tile holds the last block (else: append_tail)
+    if (y == 0 && tok0 >> c.block_shift == last) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int tok = tok0 + e;
+        if (tok >= first && tok < hi && !(tailed && tok < p.at)) {
+          *reinterpret_cast<float4*>(tail + (size_t)(tok & (c.block - 1)) * HDP + c4) = x[i][e];
+          if (c4 == 0) tail_s[tok & (c.block - 1)] = __uint_as_float(ts[i][e]);
+        }
+      }
+    }
+  }
+  if (which == 1) {
+    // the values leave in whole quads (bytes of tokens behind the end are not part of the cache)
+    __syncthreads();
+    for (int j = tid; j < 4 * HDP; j += 256) {
+      const int g = j / HDP;
+      const uint4 im = *reinterpret_cast<const uint4*>(image + j * 4);
+      unsigned* dst = reinterpret_cast<unsigned*>(codes + (size_t)tile0 * HDP + (size_t)j * 16);
+      if (first <= tile0 && hi == tile0 + kQTile) {
+        *reinterpret_cast<uint4*>(dst) = im;
+      } else {
+        const unsigned w[4] = {im.x, im.y, im.z, im.w};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int tok = tile0 + t * 16 + g * 4;
+          if (tok >= first && tok < hi) dst[t] = w[t];
+        }
+      }
+    }
   }
 }
 
-__global__ __launch_bounds__(256) void q_advance_kernel(int n_seq, int capacity, int* len, int n_new,
-                                                        const int* __restrict__ counts,
-                                                        const int* __restrict__ start, unsigned* err) {
-  const int seq = blockIdx.x * 256 + threadIdx.x;
-  if (seq >= n_seq) return;
-  const Place p = place(seq, len, 1, n_new, counts, start, capacity);
-  if (p.bad) atomicMin(err, (unsigned)seq * 4 + p.bad);
-  else len[seq] = p.end;
+// A workgroup per (sequence, head, tile) and side (keys, values).
+template <int HDP, class T>
+__global__ __launch_bounds__(256) void q_append_kernel(QStore c, QLen len, QTickets tickets, QRows k, QRows v, int n_new,
+                                                       const int* __restrict__ counts, const int* __restrict__ start,
+                                                       bool vec) {
+  __shared__ unsigned blkmax[4];
+  __shared__ Place shared;
+  __shared__ __attribute__((aligned(16))) unsigned image[kQTile * HDP / 4];
+  const int sh = blockIdx.x, seq = sh / c.n_head, head = sh - seq * c.n_head, y = blockIdx.y, which = blockIdx.z;
+  Turn turn;
+  const Place p = turn.begin(&shared, c, sh, len, tickets, n_new, counts, start);
+  const int tile0 = (p.at / kQTile + y) * kQTile;
+  if (!p.bad && (p.end > p.at || p.at < p.len) && (y == 0 || tile0 < p.end)) {
+    const QRows& r = which ? v : k;
+    const T* src = static_cast<const T*>(r.p) + seq * r.seq + head * r.head;
+    append_tile<HDP, T>(c, p, sh, y, which, src, r.tok, vec, blkmax, image);
+    if (y == 0 && p.end > tile0 + kQTile) append_tail<HDP, T>(c, p, sh, which, src, r.tok, vec);
+  }
+  turn.finish(p, c, len, gridDim.y * 2);
+}
+
+// Largest bits over the wave.
+__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {
+  v = row_max_bits<128>(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(r[0], r[1]);
+}
+
+// One new token (or only a cut) for each sequence: a workgroup per (sequence,
+// head), two waves for the keys and two for the values, a lane per column (two
+// for hdp 128). The new scale follows from the tokens' own scales; only where it
+// differs from the block's are the block's codes written anew, the two waves
+// taking every other token.
+template <int HDP, class T>
+__global__ __launch_bounds__(256) void q_append_one_kernel(QStore c, QLen len, QTickets tickets, QRows k, QRows v,
+                                                           int n_new, const int* __restrict__ counts,
+                                                           const int* __restrict__ start) {
+  constexpr int CL = HDP / 64;
+  __shared__ Place shared;
+  const int sh = blockIdx.x, seq = sh / c.n_head, head = sh - seq * c.n_head;
+  const int lane = threadIdx.x & 63, which = threadIdx.x >> 7, part = (threadIdx.x >> 6) & 1;
+  // (the row does not depend on the place: its load is in flight while that is found)
+  const QRows& src = which ? v : k;
+  float x[CL];
+  unsigned top = 0;
+#pragma unroll
+  for (int e = 0; e < CL; ++e) {
+    const int col = lane + e * 64;
+    x[e] = n_new > 0 && col < c.hd ? (float)(static_cast<const T*>(src.p) + seq * src.seq + head * src.head)[col] : 0.f;
+  }
+  Turn turn;
+  const Place p = turn.begin(&shared, c, sh, len, tickets, n_new, counts, start);
+  const bool has = p.end > p.at;  // (false where the append was refused)
+  if (!p.bad && (has || p.at < p.len)) {
+    const int blk = p.at >> c.block_shift, in = p.at & (c.block - 1);  // `in` earlier tokens in the block
+    const bool tailed = in_tail(c, p);
+    float* tail = c.tail + c.tails(sh, which);
+    float* tail_s = c.tail_s + c.tail_scales(sh, which);
+    int8_t* codes = (which ? c.v : c.k) + c.codes(sh);
+    float* scale = c.s + c.scales(sh) + 2 * blk + which;
+    auto code_at = [&](int tok, int col) { return which ? value_byte(tok, col, HDP) : (size_t)tok * HDP + col; };
+    const int blk0 = blk << c.block_shift;
+#pragma unroll
+    for (int e = 0; e < CL; ++e) top = max(top, abs_bits(x[e]));
+    const unsigned mine = has ? token_scale(__uint_as_float(wave_max_bits(top))) : 0;
+    const float old = in > 0 ? *scale : 0.f;
+    // an earlier token's own scale, where the block was full: from its codes
+    auto own_scale = [&](int t) {
+      unsigned m = 0;
+#pragma unroll
+      for (int e = 0; e < CL; ++e) m = max(m, abs_bits(code_value(codes[code_at(blk0 + t, lane + e * 64)], old)));
+      return read_back_scale(__uint_as_float(wave_max_bits(m)), old);
+    };
+    unsigned all = mine;
+    if (tailed) {
+      all = max(all, wave_max_bits(lane < in ? __float_as_uint(tail_s[lane]) : 0));
+    } else {
+      for (int t = 0; t < in; ++t) all = max(all, own_scale(t));
+    }
+    __syncthreads();  // (uniform) both waves have read the scale, the tail's scales and the codes
+    const float s = __uint_as_float(all), inv = scale_inv(s);
+    const bool anew = in > 0 && __float_as_uint(old) != all;
+    auto put = [&](int tok, int col, float value) {
+      codes[code_at(tok, col)] = (int8_t)(s > 0.f ? (int)code_of(value, s, rintf(value * inv)) : 0);
+    };
+    if (anew || !tailed) {
+      constexpr int U = 8;  // tokens in flight
+      for (int t0 = part; t0 < in; t0 += 2 * U) {
+        float y[U][CL];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < CL; ++e) {
+            const int t = min(t0 + 2 * u, in - 1), col = lane + e * 64;
+            y[u][e] = tailed ? tail[t * HDP + col] : code_value(codes[code_at(blk0 + t, col)], old);
+          }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int t = t0 + 2 * u;
+          if (t >= in) break;
+          if (!tailed) {
+            const unsigned ts = own_scale(t);
+            if (lane == 0) tail_s[t] = __uint_as_float(ts);
+          }
+#pragma unroll
+          for (int e = 0; e < CL; ++e) {
+            const int col = lane + e * 64;
+            if (!tailed) tail[t * HDP + col] = y[u][e];
+            if (anew) put(blk0 + t, col, y[u][e]);
+          }
+        }
+      }
+    }
+    if (part == 0) {
+      if (has) {
+#pragma unroll
+        for (int e = 0; e < CL; ++e) {
+          const int col = lane + e * 64;
+          put(p.at, col, x[e]);
+          tail[in * HDP + col] = x[e];
+        }
+        if (lane == 0) tail_s[in] = __uint_as_float(mine);
+      }
+      if (lane == 0 && (has || in > 0)) *scale = s;
+    }
+  }
+  turn.finish(p, c, len, 1);
 }
 
 // code * s rounded to f32 before anything else is done with it: without the
@@ -287,97 +495,142 @@ __device__ __forceinline__ float value_of(int code, float s) {
   return x;
 }
 
-// A workgroup per (sequence, head) and 64 tokens of the cache: keys 4 columns
-// of a token per lane; values 16 tokens of a column per lane.
-template <int HDP, class T>
+// A row's CPL columns from c on.
+template <class T, int CPL>
+__device__ __forceinline__ void put_cols(T* row, int c, int n, const float (&x)[CPL], bool vec) {
+  if (vec) {
+    if (c >= n) return;
+    typedef T TV __attribute__((ext_vector_type(CPL)));
+    TV v;
+#pragma unroll
+    for (int e = 0; e < CPL; ++e) v[e] = (T)x[e];  // to nearest even
+    *reinterpret_cast<TV*>(row + c) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < CPL; ++e)
+      if (c + e < n) row[c + e] = (T)x[e];
+  }
+}
+
+// A wave per (sequence, head), side and so many 64-token tiles of the cache that
+// its lanes have 16 tokens each: CPL columns (16 bytes of T, one store) of the
+// tokens t * 16 + group * 4 + e. Values come as 16 bytes of a column and are
+// transposed in registers, 4 x 4 bytes at a time. Codes and scales are loaded
+// before the sequence's length is known (they lie within the capacity).
+template <int HDP, class T, int CPL>
 __global__ __launch_bounds__(256) void q_read_kernel(QStore c, const int* __restrict__ len, int len_stride, QRows k,
                                                      QRows v, int n, const int* __restrict__ first, bool vec) {
-  constexpr int LPR = HDP / 4, TPP = 256 / LPR;
-  const int sh = blockIdx.x, seq = sh / c.n_head, head = sh - seq * c.n_head, tid = threadIdx.x;
-  const int f = first ? first[seq] : 0, l = min(len[(size_t)seq * len_stride], c.capacity);
-  // rows [r0, r1) of the result are tokens [tile0, tile0 + 64)
-  const long tile0 = (long)(f >= 0 ? f / kQTile : -((-(long)f + kQTile - 1) / kQTile)) * kQTile + (long)blockIdx.y * kQTile;
-  if (tile0 >= (long)f + n) return;
-  if (k.p) {
-    T* out = static_cast<T*>(k.p) + seq * k.seq + head * k.head;
-    const int c4 = (tid % LPR) * 4;
-    for (int t = tid / LPR; t < kQTile; t += TPP) {
-      const long tok = tile0 + t, r = tok - f;
-      if (r < 0 || r >= n || c4 >= c.hd) continue;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (tok >= 0 && tok < l) {
-        const int q = *reinterpret_cast<const int*>(c.k + c.codes(sh) + (size_t)tok * HDP + c4);
-        const float s = c.ks[c.scales(sh) + (tok >> c.block_shift)];
-        x = make_float4(value_of((int8_t)q, s), value_of((int8_t)(q >> 8), s), value_of((int8_t)(q >> 16), s),
-                        value_of((int8_t)(q >> 24), s));
+  constexpr int LPG = HDP / CPL;             // lanes per group of 16 tokens
+  constexpr int GPW = 64 / LPG;              // groups per wave and step
+  const int sh = blockIdx.x, seq = sh / c.n_head, head = sh - seq * c.n_head, which = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = (lane % LPG) * CPL;
+  const QRows& o = which ? v : k;
+  if (!o.p) return;
+  const int f = first ? first[seq] : 0;
+  // tiles before 0 (a first below 0) are counted too
+  const long tile_f = f >= 0 ? f / kQTile : -((-(long)f + kQTile - 1) / kQTile);
+  const long unit = ((long)blockIdx.y * 4 + wave) * GPW + lane / LPG;  // groups of 16 tokens from tile_f's first on
+  const long tile = tile_f + unit / 4;
+  const int group = (int)(unit & 3);
+  if (tile * kQTile >= (long)f + n) return;
+  const bool there = tile >= 0 && tile < c.tiles;
+  const int8_t* codes = (which ? c.v : c.k) + c.codes(sh) + (there ? tile : 0) * (long)kQTile * HDP;
+  const float* scales = c.s + c.scales(sh) + which + 2 * ((there ? tile : 0) * kQTile >> c.block_shift);
+  unsigned q[4][4][CPL / 4];  // [t][token][columns / 4]
+  float s[4];
+  if (which) {
+    uint4 raw[CPL];
+#pragma unroll
+    for (int e = 0; e < CPL; ++e) raw[e] = *reinterpret_cast<const uint4*>(codes + (group * HDP + col + e) * 16);
+#pragma unroll
+    for (int w = 0; w < CPL / 4; ++w)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        unsigned x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = t == 0 ? raw[4 * w + e].x : t == 1 ? raw[4 * w + e].y : t == 2 ? raw[4 * w + e].z : raw[4 * w + e].w;
+        const unsigned a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400), b = __builtin_amdgcn_perm(x[3], x[2], 0x05010400);
+        const unsigned d = __builtin_amdgcn_perm(x[1], x[0], 0x07030602), g = __builtin_amdgcn_perm(x[3], x[2], 0x07030602);
+        q[t][0][w] = __builtin_amdgcn_perm(b, a, 0x05040100);
+        q[t][1][w] = __builtin_amdgcn_perm(b, a, 0x07060302);
+        q[t][2][w] = __builtin_amdgcn_perm(g, d, 0x05040100);
+        q[t][3][w] = __builtin_amdgcn_perm(g, d, 0x07060302);
       }
-      store4(out + r * k.tok, c4, c.hd, x, vec);
-    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int8_t* p = codes + (t * 16 + group * 4 + e) * HDP + col;
+#pragma unroll
+        for (int w = 0; w < CPL / 4; ++w) q[t][e][w] = reinterpret_cast<const unsigned*>(p)[w];
+      }
   }
-  if (v.p) {
-    T* out = static_cast<T*>(v.p) + seq * v.seq + head * v.head;
-    for (int j = tid; j < 4 * HDP; j += 256) {
-      const int g = j / HDP, col = j - g * HDP;
-      if (col >= c.hd) continue;
-      int4 q = make_int4(0, 0, 0, 0);
-      if (tile0 >= 0 && tile0 < l)
-        q = *reinterpret_cast<const int4*>(c.v + c.codes(sh) + (size_t)tile0 * HDP + (size_t)j * 16);
-      const int qe[4] = {q.x, q.y, q.z, q.w};
-      for (int t = 0; t < 4; ++t)
-        for (int e = 0; e < 4; ++e) {
-          const long tok = tile0 + t * 16 + g * 4 + e, r = tok - f;
-          if (r < 0 || r >= n) continue;
-          float x = 0.f;
-          if (tok >= 0 && tok < l)
-            x = value_of((int8_t)(qe[t] >> (8 * e)), c.vs[c.scales(sh) + (tok >> c.block_shift)]);
-          store1(out + r * v.tok + col, x);
-        }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) s[t] = scales[2 * (t * 16 >> c.block_shift)];
+  const int l = min(len[(size_t)seq * len_stride], c.capacity);
+  T* out = static_cast<T*>(o.p) + seq * o.seq + head * o.head;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const long tok = tile * kQTile + t * 16 + group * 4 + e, r = tok - f;
+      if (r < 0 || r >= n) continue;
+      const bool in = there && tok < l;
+      float x[CPL];
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) x[j] = in ? value_of((int8_t)(q[t][e][j / 4] >> (8 * (j & 3))), s[t]) : 0.f;
+      put_cols<T, CPL>(out + r * o.tok, col, c.hd, x, vec);
     }
-  }
 }
 
-template <class T>
+// Whether rows of hd elements are made of aligned vectors of N.
+template <class T, int N>
 bool vec_ok(const QRows& r, int hd) {
-  const long a = sizeof(T) == 4 ? 4 : 4;  // 4 elements at a time
-  return !r.p || (hd % 4 == 0 && r.seq % a == 0 && r.tok % a == 0 && r.head % a == 0 &&
-                  reinterpret_cast<uintptr_t>(r.p) % (4 * sizeof(T)) == 0);
+  return !r.p || (hd % N == 0 && r.seq % N == 0 && r.tok % N == 0 && r.head % N == 0 &&
+                  reinterpret_cast<uintptr_t>(r.p) % (N * sizeof(T)) == 0);
 }
 
 template <class T>
-void append_t(hipStream_t s, const QStore& c, QLen len, const QRows& k, const QRows& v, int n_new, const int* counts,
+void append_t(hipStream_t s, const QStore& c, QLen len, QTickets tickets, const QRows& k, const QRows& v, int n_new, const int* counts,
               const int* start) {
+  if (n_new <= 1) {
+    const unsigned n = (unsigned)(c.n_seq * c.n_head);
+    if (c.hdp == 64)
+      q_append_one_kernel<64, T><<<n, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start);
+    else
+      q_append_one_kernel<128, T><<<n, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start);
+    return;
+  }
   // (n_new tokens touch at most this many tiles, whatever the first one's offset)
-  const dim3 grid((unsigned)(c.n_seq * c.n_head), (unsigned)((n_new + kQTile - 2) / kQTile + 1));
-  const bool vec = vec_ok<T>(k, c.hd) && vec_ok<T>(v, c.hd);
+  const dim3 grid((unsigned)(c.n_seq * c.n_head), (unsigned)((n_new + kQTile - 2) / kQTile + 1), 2);
+  const bool vec = vec_ok<T, 4>(k, c.hd) && vec_ok<T, 4>(v, c.hd);
   if (c.hdp == 64)
-    q_append_kernel<64, T><<<grid, 256, 0, s>>>(c, len.p, len.stride, k, v, n_new, counts, start, vec);
+    q_append_kernel<64, T><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start, vec);
   else
-    q_append_kernel<128, T><<<grid, 256, 0, s>>>(c, len.p, len.stride, k, v, n_new, counts, start, vec);
+    q_append_kernel<128, T><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start, vec);
 }
 
 template <class T>
 void read_t(hipStream_t s, const QStore& c, QLen len, const QRows& k, const QRows& v, int n, const int* first) {
-  const dim3 grid((unsigned)(c.n_seq * c.n_head), (unsigned)((n + kQTile - 2) / kQTile + 1));
-  const bool vec = vec_ok<T>(k, c.hd) && vec_ok<T>(v, c.hd);
+  constexpr int CPL = 16 / sizeof(T);
+  const bool vec = vec_ok<T, CPL>(k, c.hd) && vec_ok<T, CPL>(v, c.hd);
+  const int tiles = (n + kQTile - 2) / kQTile + 1;  // (whatever the first token's offset in its tile)
+  const int per = 4 * (64 / (c.hdp / CPL));         // groups of 16 tokens that a workgroup takes
+  const dim3 grid((unsigned)(c.n_seq * c.n_head), (unsigned)((tiles * 4 + per - 1) / per), 2);
   if (c.hdp == 64)
-    q_read_kernel<64, T><<<grid, 256, 0, s>>>(c, len.p, len.stride, k, v, n, first, vec);
+    q_read_kernel<64, T, CPL><<<grid, 256, 0, s>>>(c, len.p, len.stride, k, v, n, first, vec);
   else
-    q_read_kernel<128, T><<<grid, 256, 0, s>>>(c, len.p, len.stride, k, v, n, first, vec);
+    q_read_kernel<128, T, CPL><<<grid, 256, 0, s>>>(c, len.p, len.stride, k, v, n, first, vec);
 }
 
 }  // namespace
 
-void launch_q_append(hipStream_t s, const QStore& c, QLen len, QType type, const QRows& k, const QRows& v, int n_new,
-                     const int* counts, const int* start) {
-  if (type == Q_F32) append_t<float>(s, c, len, k, v, n_new, counts, start);
-  else if (type == Q_BF16) append_t<__bf16>(s, c, len, k, v, n_new, counts, start);
-  else append_t<_Float16>(s, c, len, k, v, n_new, counts, start);
-}
-
-void launch_q_advance(hipStream_t s, const QStore& c, int* len, int n_new, const int* counts, const int* start,
-                      unsigned* err) {
-  q_advance_kernel<<<(unsigned)((c.n_seq + 255) / 256), 256, 0, s>>>(c.n_seq, c.capacity, len, n_new, counts, start,
-                                                                     err);
+void launch_q_append(hipStream_t s, const QStore& c, QLen len, QTickets tickets, QType type, const QRows& k,
+                     const QRows& v, int n_new, const int* counts, const int* start) {
+  if (type == Q_F32) append_t<float>(s, c, len, tickets, k, v, n_new, counts, start);
+  else if (type == Q_BF16) append_t<__bf16>(s, c, len, tickets, k, v, n_new, counts, start);
+  else append_t<_Float16>(s, c, len, tickets, k, v, n_new, counts, start);
 }
 
 void launch_q_read(hipStream_t s, const QStore& c, QLen len, QType type, const QRows& k, const QRows& v, int n,

@@ -22,6 +22,7 @@ struct rtg_qcache {
   int device = 0;
   void* mem = nullptr;   // the store, lengths, error word and the attention's partial results
   int* len = nullptr;    // [n_seq]
+  unsigned* tickets = nullptr;  // QTickets::count
   unsigned* err = nullptr;
   void* work = nullptr;
   ~rtg_qcache() {
@@ -118,14 +119,16 @@ rtg_result rtg_qcache_new(size_t n_seq, size_t n_head, size_t head_dim, size_t c
     if (strncmp(prop.gcnArchName, "gfx950", 6) != 0)
       return err("rtgpu is built for gfx950 (MI355X); found %s", prop.gcnArchName);
     qstore_shape(&q->c, (int)n_seq, (int)n_head, (int)head_dim, (int)capacity, (int)block);
-    const size_t store = qstore_bytes(q->c), head = (n_seq * 4 + 4 + 255) / 256 * 256;
+    const size_t store = qstore_bytes(q->c), lens = (n_seq * 4 + 4 + 255) / 256 * 256;
+    const size_t head = lens + (n_seq * (n_head + 1) * kQTicketStride * 4 + 255) / 256 * 256;
     hipError_t e = device_malloc(&q->mem, head + store + qattn_work_bytes(q->c.hdp));
     if (e != hipSuccess) return hip_err(e, "rtg_qcache_new");
     q->len = static_cast<int*>(q->mem);
     q->err = reinterpret_cast<unsigned*>(q->len + n_seq);
+    q->tickets = reinterpret_cast<unsigned*>(static_cast<char*>(q->mem) + lens);
     qstore_place(&q->c, static_cast<char*>(q->mem) + head);
     q->work = static_cast<char*>(q->mem) + head + store;
-    e = hipMemset(q->len, 0, n_seq * 4);
+    e = hipMemset(q->mem, 0, head);
     if (e == hipSuccess) e = hipMemset(q->err, 0xFF, 4);
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) return hip_err(e, "rtg_qcache_new");
@@ -154,8 +157,8 @@ rtg_result rtg_qcache_append(rtg_qcache* q, rtg_dtype dtype, const rtg_rows* k, 
   if (dev.status() != hipSuccess) return hip_err(dev.status(), "hipSetDevice");
   (void)hipGetLastError();
   hipStream_t s = static_cast<hipStream_t>(stream);
-  launch_q_append(s, q->c, QLen{q->len, 1}, t, rows(k), rows(v), (int)n_new, counts, start);
-  launch_q_advance(s, q->c, q->len, (int)n_new, counts, start, q->err);
+  launch_q_append(s, q->c, QLen{q->len, 1}, QTickets{q->tickets, q->err}, t, rows(k), rows(v), (int)n_new, counts,
+                  start);
   return launched("rtg_qcache_append");
 }
 
@@ -202,7 +205,6 @@ rtg_result rtg_qcache_lengths(rtg_qcache* q, uint32_t* out, void* stream) {
   if (dev.status() != hipSuccess) return hip_err(dev.status(), "hipSetDevice");
   hipStream_t s = static_cast<hipStream_t>(stream);
   unsigned bad = kNoErr;
-  // (the error word lies behind the lengths, but the caller's array ends there)
   hipError_t e = hipMemcpyAsync(out, q->len, (size_t)q->c.n_seq * 4, hipMemcpyDeviceToHost, s);
   if (e == hipSuccess) e = hipMemcpyAsync(&bad, q->err, 4, hipMemcpyDeviceToHost, s);
   if (e == hipSuccess) e = hipStreamSynchronize(s);

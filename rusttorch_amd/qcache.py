@@ -10,13 +10,19 @@ strides whose last is 1. There is no counterpart in the reference.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
 from . import _lib
-from ._lib import Gpt2Error, Rows, check
+from ._lib import Gpt2Error, check
 
 __all__ = ["QuantisedCache"]
+
+_pack_rows = struct.Struct("Pnnn").pack  # an rtg_rows
+# the current stream of a device as an integer: 0.1 us, where the object that current_stream() makes costs 1 to 2
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 _TYPES = {torch.float32: _lib.RTG_F32, torch.bfloat16: _lib.RTG_BF16, torch.float16: _lib.RTG_F16}
 
@@ -42,6 +48,7 @@ class QuantisedCache:
             if x < 0:
                 raise Gpt2Error(f"{name} must not be negative")
         self._lib = _lib.load()
+        self._index = -1  # of the device
         h = C.c_void_p()
         if torch.cuda.is_available():
             _one_runtime()
@@ -50,6 +57,7 @@ class QuantisedCache:
                 raise Gpt2Error("the cache's device must be a GPU")
             if self.device.index is None:
                 self.device = torch.device("cuda", torch.cuda.current_device())
+            self._index = self.device.index
             with torch.cuda.device(self.device):
                 check(self._lib.rtg_qcache_new(n_seq, n_head, head_dim, capacity, block, C.byref(h)))
         else:
@@ -73,28 +81,35 @@ class QuantisedCache:
     def _stream(self):
         if self._h is None:
             raise Gpt2Error("the cache is closed")
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return _raw_stream(self._index)
 
-    def _rows(self, what: str, x: torch.Tensor, heads: int, tokens=None) -> Rows:
-        if x.dim() != 4 or x.shape[0] != self.n_seq or x.shape[3] != self.head_dim or (heads and x.shape[2] != heads):
-            raise Gpt2Error(f"{what} must be [{self.n_seq}, tokens, {heads or 'heads'}, {self.head_dim}], not {list(x.shape)}")
-        if tokens is not None and x.shape[1] != tokens:
-            raise Gpt2Error(f"{what} must have {tokens} tokens, not {x.shape[1]}")
-        if x.dtype not in _TYPES:
-            raise Gpt2Error(f"{what} must be f32, bf16 or f16, not {x.dtype}")
-        if x.device != self.device:
+    def _rows(self, what: str, x: torch.Tensor, dtype, tokens: int, heads: int) -> bytes:
+        """x as an rtg_rows, once it is known to be [n_seq, tokens, heads, head_dim] of dtype on the cache's device."""
+        shape = (self.n_seq, tokens, heads, self.head_dim)
+        if x.shape != shape:
+            raise Gpt2Error(f"{what} must be {list(shape)}, not {list(x.shape)}")
+        if x.dtype is not dtype:
+            raise Gpt2Error(f"{what} must be {dtype}, not {x.dtype}")
+        if x.get_device() != self._index:
             raise Gpt2Error(f"{what} is on {x.device}, the cache on {self.device}")
         seq, tok, head, col = x.stride()
         if col != 1 and self.head_dim > 1 and x.numel():
             raise Gpt2Error(f"{what}'s last dimension must be contiguous")
-        return Rows(x.data_ptr(), seq, tok, head)
+        return _pack_rows(x.data_ptr(), seq, tok, head)
+
+    def _type(self, what: str, x: torch.Tensor) -> int:
+        if x.dim() != 4:
+            raise Gpt2Error(f"{what} must be [n_seq, tokens, heads, head_dim], not {list(x.shape)}")
+        if x.dtype not in _TYPES:
+            raise Gpt2Error(f"{what} must be f32, bf16 or f16, not {x.dtype}")
+        return _TYPES[x.dtype]
 
     def _ints(self, what: str, x):
         if x is None:
             return None
-        if x.dtype != torch.int32 or x.dim() != 1 or x.shape[0] != self.n_seq or not x.is_contiguous():
+        if x.dtype is not torch.int32 or x.shape != (self.n_seq,) or not x.is_contiguous():
             raise Gpt2Error(f"{what} must be {self.n_seq} contiguous int32")
-        if x.device != self.device:
+        if x.get_device() != self._index:
             raise Gpt2Error(f"{what} is on {x.device}, the cache on {self.device}")
         return x.data_ptr()
 
@@ -103,27 +118,22 @@ class QuantisedCache:
     def append(self, k: torch.Tensor, v: torch.Tensor, counts=None, start=None) -> None:
         """Writes k, v [n_seq, tokens, n_head, head_dim] behind the sequences, or from token start[s] on (what lay
         there and behind is dropped); of sequence s the first counts[s] tokens (clamped to 0 .. tokens)."""
-        stream = self._stream()
-        kr = self._rows("k", k, self.n_head)
-        vr = self._rows("v", v, self.n_head, k.shape[1])
-        if k.dtype != v.dtype:
-            raise Gpt2Error(f"k is {k.dtype}, v {v.dtype}")
-        check(self._lib.rtg_qcache_append(self._h, _TYPES[k.dtype], kr, vr, k.shape[1], self._ints("counts", counts),
-                                          self._ints("start", start), stream))
+        stream, dtype, n = self._stream(), self._type("k", k), k.shape[1]
+        check(self._lib.rtg_qcache_append(self._h, dtype, self._rows("k", k, k.dtype, n, self.n_head),
+                                          self._rows("v", v, k.dtype, n, self.n_head), n,
+                                          self._ints("counts", counts), self._ints("start", start), stream))
 
     def attend(self, q: torch.Tensor, counts=None, scale=None, out=None) -> torch.Tensor:
         """Attention of the last counts[s] tokens of each sequence, q [n_seq, tokens, query heads, head_dim], over
         the keys up to their own position; scale: 1 / sqrt(head_dim). Padding rows are 0."""
-        stream = self._stream()
-        qr = self._rows("q", q, 0)
+        stream, dtype = self._stream(), self._type("q", q)
+        n, heads = q.shape[1], q.shape[2]
+        rows = self._rows("q", q, q.dtype, n, heads)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out.dtype != q.dtype:
-            raise Gpt2Error(f"out is {out.dtype}, q {q.dtype}")
-        outr = self._rows("out", out, q.shape[2], q.shape[1])
-        check(self._lib.rtg_qcache_attend(self._h, _TYPES[q.dtype], qr, q.shape[1], q.shape[2],
-                                          self._ints("counts", counts),
-                                          self.head_dim ** -0.5 if scale is None else scale, outr, stream))
+            out = q.new_empty(q.shape)
+        check(self._lib.rtg_qcache_attend(self._h, dtype, rows, n, heads, self._ints("counts", counts),
+                                          self.head_dim ** -0.5 if scale is None else scale,
+                                          self._rows("out", out, q.dtype, n, heads), stream))
         return out
 
     def read(self, n: int, first=None, dtype: torch.dtype = torch.float32, k=None, v=None):
@@ -135,11 +145,10 @@ class QuantisedCache:
             raise Gpt2Error(f"dtype must be f32, bf16 or f16, not {dtype}")
         shape = (self.n_seq, n, self.n_head, self.head_dim)
         k = torch.empty(shape, dtype=dtype, device=self.device) if k is None else k
-        v = torch.empty(shape, dtype=dtype, device=self.device) if v is None else v
-        if k.dtype != dtype or v.dtype != dtype:
-            raise Gpt2Error(f"k and v must be {dtype}")
-        check(self._lib.rtg_qcache_read(self._h, _TYPES[dtype], self._rows("k", k, self.n_head, n),
-                                        self._rows("v", v, self.n_head, n), n, self._ints("first", first), stream))
+        v = k.new_empty(shape) if v is None else v
+        check(self._lib.rtg_qcache_read(self._h, _TYPES[dtype], self._rows("k", k, dtype, n, self.n_head),
+                                        self._rows("v", v, dtype, n, self.n_head), n, self._ints("first", first),
+                                        stream))
         return k, v
 
     def lengths(self) -> list:

@@ -33,7 +33,7 @@ class Head:
 
     def cut(self, at):
         b = at // self.block
-        if at < self.n and b < self.n // self.block and at % self.block:
+        if at < self.n and b < (self.n - 1) // self.block and at % self.block:
             lo = b * self.block
             s = self.s[b]
             self.x[lo:at] = (self.codes[lo:at].astype(np.float32) * np.float32(s)).astype(np.float64)

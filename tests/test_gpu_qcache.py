@@ -387,8 +387,8 @@ def test_refusals():
     c = QuantisedCache(2, 2, 64, 100)
     x = torch.zeros(2, 3, 2, 64, device="cuda")
     for what, call in (("k must be", lambda: c.append(x[:1], x)), ("v must be", lambda: c.append(x, x[..., :32])),
-                       ("must have 3 tokens", lambda: c.append(x, x[:, :2])),
-                       ("k is torch.float32", lambda: c.append(x, x.half())),
+                       ("v must be", lambda: c.append(x, x[:, :2])),
+                       ("v must be torch.float32", lambda: c.append(x, x.half())),
                        ("f32, bf16 or f16", lambda: c.append(x.double(), x.double())),
                        ("is on cpu", lambda: c.append(x.cpu(), x.cpu())),
                        ("contiguous", lambda: c.append(torch.zeros(2, 3, 2, 128, device="cuda")[..., ::2], x)),
@@ -397,7 +397,7 @@ def test_refusals():
                        ("counts is on cpu", lambda: c.append(x, x, counts=torch.zeros(2, dtype=torch.int32))),
                        ("start must be", lambda: c.append(x, x, start=torch.zeros(3, dtype=torch.int32, device="cuda"))),
                        ("not a multiple", lambda: c.attend(torch.zeros(2, 3, 3, 64, device="cuda"))),
-                       ("out is", lambda: c.attend(x, out=x.half())),
+                       ("out must be torch.float32", lambda: c.attend(x, out=x.half())),
                        ("out must be", lambda: c.attend(x, out=torch.zeros(2, 3, 4, 64, device="cuda"))),
                        ("scale must be finite", lambda: c.attend(x, scale=float("nan"))),
                        ("must not be negative", lambda: c.read(-1)),

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from rusttorch_amd import _lib
-from rusttorch_amd._lib import Gpt2Error, Rows, check
+from rusttorch_amd._lib import Gpt2Error, check
 from tests.qcache_ref import Cache
 
 
@@ -25,7 +25,7 @@ def test_new_refuses(args, what):
 
 
 def test_null_arguments():
-    lib, r, out = _lib.load(), Rows(), C.c_uint32()
+    lib, r, out = _lib.load(), bytes(32), C.c_uint32()
     for res in (lib.rtg_qcache_new(1, 1, 64, 10, 32, None), lib.rtg_qcache_append(None, 0, r, r, 1, None, None, None),
                 lib.rtg_qcache_read(None, 0, r, r, 1, None, None),
                 lib.rtg_qcache_attend(None, 0, r, 1, 1, None, 1.0, r, None), lib.rtg_qcache_lengths(None, C.byref(out), None)):
