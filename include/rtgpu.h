@@ -130,6 +130,14 @@ size_t rtg_num_parameters(const rtg_model* model);
  * holds `batch` sequences and preallocates n_layer*batch*2*n_head*n_positions*
  * head_dim f32 in HBM. batch = 1 is the reference's cache. */
 rtg_result rtg_cache_new(const rtg_model* model, size_t batch, rtg_cache** out);
+/* The same cache in 8 bits, a scale for every `block` (16, 32 or 64) tokens of a
+ * head, keys and values apart (the rules stand with rtg_qcache below; no
+ * counterpart in the reference). A quarter of the memory (and of what a decode
+ * step reads of it), for logits that differ by what the rounding of keys and
+ * values to 8 bits moves. Goes wherever a cache of this batch goes except
+ * rtg_forward_cached_noalloc; one new token runs the batched step's kernel graph
+ * at any batch, more run the prefill kernels. */
+rtg_result rtg_cache_new_quantised(const rtg_model* model, size_t batch, size_t block, rtg_cache** out);
 /* KVCache::len / is_empty / clear, gpt2.rs:137-161. */
 size_t rtg_cache_len(const rtg_cache* cache);
 bool rtg_cache_is_empty(const rtg_cache* cache);
@@ -195,6 +203,10 @@ rtg_result rtg_forward_cached_batched(const rtg_model* model, rtg_cache* cache, 
  * [batch][n + max(1, max_new)]. timing may be NULL. */
 rtg_result rtg_generate_cached_batched(const rtg_model* model, const uint32_t* prompts, size_t batch, size_t n,
                                        size_t max_new, uint32_t* out, rtg_timing* timing);
+
+/* The same over a cache of 8 bits (rtg_cache_new_quantised). */
+rtg_result rtg_generate_cached_quantised(const rtg_model* model, const uint32_t* prompts, size_t batch, size_t n,
+                                         size_t max_new, size_t block, uint32_t* out, rtg_timing* timing);
 
 /* ---- 8-bit key/value cache over device tensors (no counterpart in the
  * reference, whose cache is f32 vectors on the host, gpt2.rs:111-175). For

@@ -74,6 +74,7 @@ SIGNATURES = {
     "rtg_model_destroy": (None, [C.c_void_p]),
     "rtg_num_parameters": (C.c_size_t, [C.c_void_p]),
     "rtg_cache_new": (Result, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p)]),
+    "rtg_cache_new_quantised": (Result, [C.c_void_p, C.c_size_t, C.c_size_t, C.POINTER(C.c_void_p)]),
     "rtg_cache_len": (C.c_size_t, [C.c_void_p]),
     "rtg_cache_is_empty": (C.c_bool, [C.c_void_p]),
     "rtg_cache_clear": (None, [C.c_void_p]),
@@ -90,6 +91,8 @@ SIGNATURES = {
     "rtg_forward_cached_batched": (Result, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "rtg_generate_cached_batched": (Result, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t,
                                              C.c_void_p, C.POINTER(Timing)]),
+    "rtg_generate_cached_quantised": (Result, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t,
+                                               C.c_void_p, C.POINTER(Timing)]),
     # (an rtg_rows is passed as its bytes: qcache.py)
     "rtg_qcache_new": (Result, [C.c_size_t] * 5 + [C.POINTER(C.c_void_p)]),
     "rtg_qcache_destroy": (None, [C.c_void_p]),

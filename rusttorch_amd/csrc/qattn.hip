@@ -299,8 +299,12 @@ __device__ __forceinline__ void put4(const AttnArgs& a, int seq, int i, int head
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (c4 + e >= hd) continue;
+        // (the scale brings the bound of the unrounded values to 2^15 at most;
+        // rounded to 8 bits they are below twice that, which f16 just misses)
+        float y = xe[e] * a.out.scale[col + e];
+        if (fabsf(y) > 65504.f && fabsf(y) <= 65536.f) y = copysignf(65504.f, y);
         unsigned h, l;
-        f16_split(xe[e] * a.out.scale[col + e], &h, &l);
+        f16_split(y, &h, &l);
         uint16_t* p = a.out.pair + pair_index((size_t)seq * a.n_q + i, col + e, d);
         p[0] = (uint16_t)h;
         p[32] = (uint16_t)l;

@@ -27,6 +27,7 @@
 #include "device_memory.h"
 #include "gemm_pair.h"
 #include "kernels.h"
+#include "qcache.h"
 #include "rows.h"
 #include "safetensors_reader.h"
 #include "scratch.h"
@@ -300,9 +301,10 @@ struct rtg_model {
   PrefillHolder pw;           // empty where the f32-MFMA GEMMs run the prefill
   std::mutex bw_mu;
   std::unique_ptr<BatchedWeights> bw;
-  // Pool of caches reused by the generate entry points (keyed by batch).
+  // Pool of caches reused by the generate entry points (keyed by batch and, for
+  // quantised ones, block; else 0).
   std::mutex pool_mu;
-  std::multimap<size_t, rtg_cache*> pool;
+  std::multimap<std::pair<size_t, size_t>, rtg_cache*> pool;
   ~rtg_model();
 };
 
@@ -346,10 +348,20 @@ struct rtg_cache {
   float* bg_spart = nullptr;
   void* sample_work = nullptr;  // of launch_sample, made for the first sampled token
   float* bg_cen = nullptr;  // [2][kBgemvRows]: per-row centres of the folded LayerNorms' inputs
+  // a quantised cache (rtg_cache_new_quantised): sequence l * batch + b of q holds
+  // layer l of sequence b, k and v are null, and a layer's new keys and values pass
+  // through q_new, [2][B][H][new tokens][hd], as c_attn leaves them
+  QStore q;
+  void* q_mem = nullptr;
+  void* q_work = nullptr;  // partial results of its attention
+  int* q_int = nullptr;    // [0]: tokens before a prefill; [kQZero]: 0
+  float* q_new = nullptr;
+  bool quantised() const { return q_mem != nullptr; }
 };
+constexpr int kQZero = 32;
 
 static void free_work(rtg_cache* c) {
-  for (float** p : {&c->x, &c->ln, &c->qkv, &c->att, &c->h, &c->ws}) {
+  for (float** p : {&c->x, &c->ln, &c->qkv, &c->att, &c->h, &c->ws, &c->q_new}) {
     if (*p) hipFree(*p);
     *p = nullptr;
   }
@@ -401,6 +413,7 @@ static void ensure_rows(rtg_cache* c, size_t rows) {
   HIPX(device_malloc(&c->qkv, cap * 3 * d * 4));
   HIPX(device_malloc(&c->att, cap * d * 4));
   HIPX(device_malloc(&c->h, cap * 4 * d * 4));
+  if (c->quantised()) HIPX(device_malloc(&c->q_new, 2 * cap * d * 4));
   ensure_ws(c, cap, c->m->pw.get() != nullptr);
   c->rows_cap = cap;
 }
@@ -421,7 +434,8 @@ static void ensure_sample_work(rtg_cache* c) {
   if (!c->sample_work) HIPX(device_malloc(&c->sample_work, sample_work_bytes((int)c->m->cfg.vocab_size)));
 }
 
-static rtg_cache* cache_create(const rtg_model* m, size_t batch) {
+// block: of a quantised cache, 0 for an f32 one.
+static rtg_cache* cache_create(const rtg_model* m, size_t batch, size_t block = 0) {
   std::unique_ptr<rtg_cache> c(new rtg_cache());
   c->m = m;
   c->batch = batch;
@@ -429,8 +443,17 @@ static rtg_cache* cache_create(const rtg_model* m, size_t batch) {
   c->layer_stride = batch * H * P * hd;
   try {
     HIPX(hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking));
-    HIPX(device_malloc(&c->k, std::max<size_t>(L * c->layer_stride, 1) * 4));
-    HIPX(device_malloc(&c->v, std::max<size_t>(L * c->layer_stride, 1) * 4));
+    if (block) {
+      qstore_shape(&c->q, (int)(L * batch), (int)H, (int)hd, (int)P, (int)block);
+      HIPX(device_malloc(&c->q_mem, std::max<size_t>(qstore_bytes(c->q), 1)));
+      qstore_place(&c->q, c->q_mem);
+      HIPX(device_malloc(&c->q_work, qattn_work_bytes(c->q.hdp)));
+      HIPX(device_malloc(&c->q_int, 256));
+      HIPX(hipMemsetAsync(c->q_int, 0, 256, c->stream));
+    } else {
+      HIPX(device_malloc(&c->k, std::max<size_t>(L * c->layer_stride, 1) * 4));
+      HIPX(device_malloc(&c->v, std::max<size_t>(L * c->layer_stride, 1) * 4));
+    }
     HIPX(device_malloc(&c->pos_dev, 256));
     HIPX(device_malloc(&c->step_dev, 256));
     HIPX(device_malloc(&c->keys, std::max<size_t>(batch, 1) * 8));
@@ -469,6 +492,60 @@ static KvDst kv_layer(const rtg_cache* c, size_t l) {
   kv.n_pos = (int)c->m->cfg.n_positions;
   kv.d = (int)c->m->cfg.n_embd;
   return kv;
+}
+
+// Where c_attn's epilogue puts the k and v columns of T new tokens per sequence
+// of layer l behind `past`, and the position that it is told (as a number or,
+// for a decode step, in device memory): the cache, or what a quantised cache is
+// written from.
+struct NewKv {
+  KvDst kv;
+  int past;
+  const int* pos_dev;
+};
+static NewKv new_kv(const rtg_cache* c, size_t l, size_t T, int past) {
+  if (!c->quantised()) return NewKv{kv_layer(c, l), past, c->pos_dev};
+  KvDst kv;
+  kv.k = c->q_new;
+  kv.v = c->q_new + c->batch * T * c->m->cfg.n_embd;
+  kv.n_head = (int)c->m->cfg.n_head;
+  kv.n_pos = (int)T;
+  kv.d = (int)c->m->cfg.n_embd;
+  return NewKv{kv, 0, c->q_int + kQZero};
+}
+
+// A quantised cache's attention of T new tokens per sequence in layer l: they
+// are quantised into it, then the queries q (row b * T + t, rows of ldq) attend
+// over all of it up to their own positions. len: the tokens before them.
+static void q_attention(rtg_cache* c, size_t l, size_t T, const float* q, int ldq, int* len, QOut out) {
+  const rtg_model* m = c->m;
+  const long hd = m->hd, d = (long)m->cfg.n_embd;
+  const KvDst kv = new_kv(c, l, T, 0).kv;
+  const QStore st = c->q.from(l * c->batch, (int)c->batch);
+  QRows k, v, qr;
+  k.p = kv.k;
+  v.p = kv.v;
+  k.seq = v.seq = (long)T * d;
+  k.tok = v.tok = hd;
+  k.head = v.head = (long)T * hd;
+  qr.p = const_cast<float*>(q);
+  qr.seq = (long)T * ldq;
+  qr.tok = ldq;
+  qr.head = hd;
+  if (out.kind == QO_ROWS) {
+    out.rows.seq = (long)T * d;
+    out.rows.tok = d;
+    out.rows.head = hd;
+  }
+  const QLen at{len, 0};
+  launch_q_append(c->stream, st, at, QTickets{}, Q_F32, k, v, (int)T, nullptr, nullptr);
+  launch_q_attend(c->stream, st, at, (int)T, Q_F32, qr, (int)T, (int)m->cfg.n_head, nullptr,
+                  1.0f / sqrtf((float)hd), out, c->q_work);
+}
+static QOut q_rows(float* p) {
+  QOut o;
+  o.rows.p = p;
+  return o;
 }
 
 // Activation buffers of one forward pass: x, ln [M][d], qkv [M][3d],
@@ -514,17 +591,25 @@ static void enqueue_prefill_pair(rtg_cache* c, const PrefillWeights& pw, const W
     return a;
   };
   launch_embed(s, m->wte, m->wtype, m->wpe, ids_dev, M, (int)T, (int)past, nullptr, d, w.x);
+  if (c->quantised()) launch_set_step(s, nullptr, c->q_int, (int)past, c->q_int + 1, 0);
   for (size_t l = 0; l < m->layers.size(); ++l) {
     const LayerW& L = m->layers[l];
     const PrefillWeights::Layer& P = pw.layers[l];
-    KvDst kv = kv_layer(c, l);
+    const NewKv nkv = new_kv(c, l, T, (int)past);
+    const KvDst& kv = nkv.kv;
     launch_layernorm_pair(s, w.x, d, L.ln1w, L.ln1b, eps, M, d, P.s1, ln);
     PairGemmArgs a = args(ln, d, L.bqkv, w.qkv, 3 * d, EPI_BIAS);
     a.kv = kv;
     a.kv_T = (int)T;
-    a.kv_past = (int)past;
+    a.kv_past = nkv.past;
     launch_pair_gemm(s, P.qkv, a);
-    if (m->hd == 64)
+    if (c->quantised()) {
+      QOut o;
+      o.kind = QO_PAIR;
+      o.pair = att;
+      o.scale = P.att.v;
+      q_attention(c, l, T, w.qkv, 3 * d, c->q_int, o);
+    } else if (m->hd == 64)
       launch_attn_pair(s, w.qkv, (int)S, (int)T, (int)past, kv.k, kv.v, kv.n_head, kv.n_pos, d, P.att, att);
     else
       launch_attn_prefill(s, w.qkv, (int)S, (int)T, (int)past, kv.k, kv.v, kv.n_head, kv.n_pos, d, nullptr, att,
@@ -566,13 +651,16 @@ static void enqueue_prefill(rtg_cache* c, const Work& w, const uint32_t* ids_dev
   const float eps = m->cfg.layer_norm_epsilon;
   hipStream_t s = c->stream;
   launch_embed(s, m->wte, m->wtype, m->wpe, ids_dev, M, (int)T, (int)past, nullptr, d, w.x);
+  if (c->quantised()) launch_set_step(s, nullptr, c->q_int, (int)past, c->q_int + 1, 0);
   for (size_t l = 0; l < m->layers.size(); ++l) {
     const LayerW& L = m->layers[l];
-    KvDst kv = kv_layer(c, l);
+    const NewKv nkv = new_kv(c, l, T, (int)past);
+    const KvDst& kv = nkv.kv;
     launch_layernorm(s, w.x, L.ln1w, L.ln1b, eps, M, d, w.ln);
-    launch_gemm_qkv(s, w.ln, d, L.wqkv, m->wtype, L.bqkv, w.qkv, 3 * d, M, d, (int)S, (int)T, (int)past, kv, w.ws,
+    launch_gemm_qkv(s, w.ln, d, L.wqkv, m->wtype, L.bqkv, w.qkv, 3 * d, M, d, (int)S, (int)T, nkv.past, kv, w.ws,
                     w.ws_floats);
-    launch_attn_prefill(s, w.qkv, (int)S, (int)T, (int)past, kv.k, kv.v, kv.n_head, kv.n_pos, d, w.att);
+    if (c->quantised()) q_attention(c, l, T, w.qkv, 3 * d, c->q_int, q_rows(w.att));
+    else launch_attn_prefill(s, w.qkv, (int)S, (int)T, (int)past, kv.k, kv.v, kv.n_head, kv.n_pos, d, w.att);
     launch_gemm(s, w.att, d, L.waproj, m->wtype, L.baproj, w.x, d, M, d, d, EPI_BIAS_RESID, w.ws, w.ws_floats);
     launch_layernorm(s, w.x, L.ln2w, L.ln2b, eps, M, d, w.ln);
     launch_gemm(s, w.ln, d, L.wfc, m->wtype, L.bfc, w.h, 4 * d, M, 4 * d, d, EPI_BIAS_GELU, w.ws, w.ws_floats);
@@ -743,16 +831,23 @@ static void enqueue_decode_step_batched(rtg_cache* c) {
   for (size_t l = 0; l < m->layers.size(); ++l) {
     const LayerW& L = m->layers[l];
     const BatchedWeights::Layer& T = bw->layers[l];
-    KvDst kv = kv_layer(c, l);
+    const NewKv nkv = new_kv(c, l, 1, 0);
+    const KvDst& kv = nkv.kv;
     {  // LN1 + c_attn; k/v of the new token into the cache
       BgemvArgs a = base();
       a.X = c->ln; a.Wt = T.qkv; a.N = 3 * d; a.K = d; a.bias = T.cq;
       ln_in(a, L.ln1w, T.sq, true);
       a.epi = EPI_BIAS;
-      a.qkv = BgemvQkv{c->qkv, d, d, kv, c->pos_dev};
+      a.qkv = BgemvQkv{c->qkv, d, d, kv, nkv.pos_dev};
       run(bw->pq, a);
     }
-    launch_attn_decode(s, B, c->qkv, d, kv.k, kv.v, kv.n_head, kv.n_pos, c->pos_dev, c->att, d, tk);
+    if (c->quantised()) {
+      QOut o;
+      o.kind = QO_XT;
+      o.xt = c->att;
+      o.tk = tk;
+      q_attention(c, l, 1, c->qkv, d, c->pos_dev, o);
+    } else launch_attn_decode(s, B, c->qkv, d, kv.k, kv.v, kv.n_head, kv.n_pos, c->pos_dev, c->att, d, tk);
     {  // attention c_proj + residual; statistics partials for LN2
       BgemvArgs a = base();
       a.X = c->att; a.Wt = T.proj; a.N = d; a.K = d; a.bias = L.baproj;
@@ -804,10 +899,12 @@ static void enqueue_decode_step(rtg_cache* c, int pos = -1) {
     launch_embed(s, m->wte, m->wtype, m->wpe, c->token_dev, B, 1, 0, c->pos_dev, d, c->x);
     for (size_t l = 0; l < m->layers.size(); ++l) {
       const LayerW& L = m->layers[l];
-      KvDst kv = kv_layer(c, l);
+      const NewKv nkv = new_kv(c, l, 1, 0);
+      const KvDst& kv = nkv.kv;
       launch_layernorm(s, c->x, L.ln1w, L.ln1b, eps, B, d, c->ln);
-      launch_gemv_qkv(s, B, L.wqkv, m->wtype, L.bqkv, c->ln, d, c->qkv, d, d, kv, c->pos_dev);
-      launch_attn_decode(s, B, c->qkv, d, kv.k, kv.v, kv.n_head, kv.n_pos, c->pos_dev, c->att, d);
+      launch_gemv_qkv(s, B, L.wqkv, m->wtype, L.bqkv, c->ln, d, c->qkv, d, d, kv, nkv.pos_dev);
+      if (c->quantised()) q_attention(c, l, 1, c->qkv, d, c->pos_dev, q_rows(c->att));
+      else launch_attn_decode(s, B, c->qkv, d, kv.k, kv.v, kv.n_head, kv.n_pos, c->pos_dev, c->att, d);
       launch_gemv(s, B, L.waproj, m->wtype, L.baproj, c->att, d, c->x, d, d, d, EPI_BIAS_RESID);
       launch_layernorm(s, c->x, L.ln2w, L.ln2b, eps, B, d, c->ln);
       launch_gemv(s, B, L.wfc, m->wtype, L.bfc, c->ln, d, c->h, 4 * d, 4 * d, d, EPI_BIAS_GELU);
@@ -842,7 +939,7 @@ static void set_step(rtg_cache* c, const uint32_t* ids, size_t B) {
 static bool rows_path(const rtg_cache* c, size_t S, size_t T) {
   const char* off = getenv("RTG_NO_ROWS");
   if (off && off[0] == '1') return false;
-  return c->m->rplan && S == c->batch && rows_supported(c->m->rplan, (int)S, (int)T);
+  return c->m->rplan && !c->quantised() && S == c->batch && rows_supported(c->m->rplan, (int)S, (int)T);
 }
 
 // Enqueues the multi-row forward on the cache's stream (the caller holds
@@ -914,7 +1011,7 @@ static void forward_cached_impl(rtg_cache* c, const uint32_t* ids, size_t n, flo
   const size_t B = c->batch, V = m->cfg.vocab_size;
   ensure_rows(c, B * n);
   ensure_logits(c, logits_out ? B * n : B);
-  if (n == 1 && B == 1 && persistent_supported(m->pplan, 1)) {
+  if (n == 1 && B == 1 && !c->quantised() && persistent_supported(m->pplan, 1)) {
     // one new token at batch 1: the persistent decode step, the kernel
     // generate_cached runs per token; its token is read from token_dev at
     // position *pos_dev = past, its logits land in c->logits
@@ -937,7 +1034,7 @@ static void forward_cached_impl(rtg_cache* c, const uint32_t* ids, size_t n, flo
     c->len += 1;
     return;
   }
-  if (n == 1 && B >= 2 && !c->pstate && batched_ok(m, B)) {
+  if (n == 1 && (B >= 2 || c->quantised()) && !c->pstate && batched_ok(m, B)) {
     // one new token per sequence: the batched decode step (the same kernels
     // generate_cached_batched replays), its token read from token_dev at
     // position *pos_dev = past
@@ -968,11 +1065,11 @@ static void forward_cached_impl(rtg_cache* c, const uint32_t* ids, size_t n, flo
   c->len += n;
 }
 
-static rtg_cache* pool_take(const rtg_model* mc, size_t batch) {
+static rtg_cache* pool_take(const rtg_model* mc, size_t batch, size_t block) {
   rtg_model* m = const_cast<rtg_model*>(mc);
   {
     std::lock_guard<std::mutex> g(m->pool_mu);
-    auto it = m->pool.find(batch);
+    auto it = m->pool.find({batch, block});
     if (it != m->pool.end()) {
       rtg_cache* c = it->second;
       m->pool.erase(it);
@@ -980,19 +1077,19 @@ static rtg_cache* pool_take(const rtg_model* mc, size_t batch) {
       return c;
     }
   }
-  return cache_create(mc, batch);
+  return cache_create(mc, batch, block);
 }
 
 static void pool_give(const rtg_model* mc, rtg_cache* c) {
   rtg_model* m = const_cast<rtg_model*>(mc);
   std::lock_guard<std::mutex> g(m->pool_mu);
-  m->pool.emplace(c->batch, c);
+  m->pool.emplace(std::make_pair(c->batch, (size_t)c->q.block), c);
 }
 
 struct PoolLease {
   const rtg_model* m;
   rtg_cache* c;
-  PoolLease(const rtg_model* mm, size_t b) : m(mm), c(pool_take(mm, b)) {}
+  PoolLease(const rtg_model* mm, size_t b, size_t block = 0) : m(mm), c(pool_take(mm, b, block)) {}
   ~PoolLease() {
     if (c) pool_give(m, c);
   }
@@ -1000,10 +1097,11 @@ struct PoolLease {
 
 // generate_cached over B equal-length prompts (gpt2.rs:405-441), greedy or,
 // with sp (B = 1), choosing every token with the device sampler
-// (sample_logits, gpt2.rs:871-906): the whole loop stays on the device.
+// (sample_logits, gpt2.rs:871-906): the whole loop stays on the device. block: of
+// the quantised cache it runs over, 0 for an f32 one.
 static void generate_greedy(const rtg_model* m, const uint32_t* prompts, size_t B, size_t n, size_t max_new,
-                            uint32_t* out, rtg_timing* timing, const SampleParams* sp = nullptr) {
-  PoolLease lease(m, B);
+                            uint32_t* out, rtg_timing* timing, const SampleParams* sp = nullptr, size_t block = 0) {
+  PoolLease lease(m, B, block);
   rtg_cache* c = lease.c;
   const size_t V = m->cfg.vocab_size, P = m->cfg.n_positions;
   const size_t steps = max_new > 0 ? max_new : 1;  // first token comes from prefill
@@ -1022,7 +1120,7 @@ static void generate_greedy(const rtg_model* m, const uint32_t* prompts, size_t 
                              c->sample_work))
       throw HipError{"vocabulary too large for the device sampler"};
   };
-  if (!c->pstate && persistent_supported(m->pplan, (int)B)) {
+  if (!c->pstate && !c->quantised() && persistent_supported(m->pplan, (int)B)) {
     c->pstate = persistent_state_create(m->pplan, c->k, c->v, (int)B, c->token_dev, c->pos_dev, c->logits, c->keys,
                                         c->ids_dev, c->step_dev);
     destroy_graph(c);  // the step graph changes shape
@@ -1527,6 +1625,21 @@ rtg_result rtg_cache_new(const rtg_model* model, size_t batch, rtg_cache** out) 
   return ok();
 }
 
+rtg_result rtg_cache_new_quantised(const rtg_model* model, size_t batch, size_t block, rtg_cache** out) {
+  if (!model || !out) return err("null argument");
+  if (batch == 0) return err("batch must be >= 1");
+  if (block != 16 && block != 32 && block != 64)
+    return err(fmt("block %zu is not supported (16, 32 or 64)", block));
+  try {
+    *out = cache_create(model, batch, block);
+  } catch (const HipError& e) {
+    return err(e.msg);
+  } catch (const std::exception& ex) {
+    return err_internal(ex);
+  }
+  return ok();
+}
+
 size_t rtg_cache_len(const rtg_cache* cache) { return cache ? cache->len : 0; }
 bool rtg_cache_is_empty(const rtg_cache* cache) { return rtg_cache_len(cache) == 0; }
 void rtg_cache_clear(rtg_cache* cache) {
@@ -1543,7 +1656,7 @@ void rtg_cache_destroy(rtg_cache* c) {
   for (void* p : {(void*)c->k, (void*)c->v, (void*)c->pos_dev, (void*)c->step_dev, (void*)c->keys,
                   (void*)c->token_dev, (void*)c->ids_dev, (void*)c->ids_in, (void*)c->logits,
                   (void*)c->bg_part, (void*)c->bg_cnt, (void*)c->bg_spart, (void*)c->bg_cen,
-                  c->sample_work})
+                  c->sample_work, c->q_mem, c->q_work, (void*)c->q_int})
     if (p) hipFree(p);
   for (auto e : c->ev)
     if (e) hipEventDestroy(e);
@@ -1556,6 +1669,31 @@ rtg_result rtg_cache_read(const rtg_cache* c, size_t layer, size_t head, size_t 
   const rtg_model* m = c->m;
   if (layer >= m->cfg.n_layer || head >= m->cfg.n_head || seq >= c->batch) return err("index out of range");
   const size_t P = m->cfg.n_positions, hd = m->hd;
+  if (c->quantised()) {
+    float* tmp = nullptr;
+    try {
+      if (c->len) {
+        // all heads of the sequence, [len][H][hd], then this head's columns
+        const size_t d = m->cfg.n_embd;
+        HIPX(device_malloc(&tmp, c->len * d * 4));
+        QRows r, none;
+        r.p = tmp;
+        r.tok = (long)d;
+        r.head = (long)hd;
+        launch_set_step(c->stream, nullptr, c->q_int, (int)c->len, c->q_int + 1, 0);
+        launch_q_read(c->stream, c->q.from(layer * c->batch + seq, 1), QLen{c->q_int, 0}, Q_F32, values ? none : r,
+                      values ? r : none, (int)c->len, nullptr);
+        HIPX(hipGetLastError());
+        HIPX(hipMemcpy2DAsync(out, hd * 4, tmp + head * hd, d * 4, hd * 4, c->len, hipMemcpyDeviceToHost, c->stream));
+        HIPX(hipStreamSynchronize(c->stream));
+      }
+    } catch (const HipError& e) {
+      if (tmp) hipFree(tmp);
+      return err(e.msg);
+    }
+    if (tmp) hipFree(tmp);
+    return ok();
+  }
   const float* base = (values ? c->v : c->k) + layer * c->layer_stride + ((seq * m->cfg.n_head + head) * P) * hd;
   try {
     if (c->len) HIPX(hipMemcpy(out, base, c->len * hd * 4, hipMemcpyDeviceToHost));
@@ -1629,6 +1767,7 @@ rtg_result rtg_forward_cached_noalloc(const rtg_model* model, rtg_cache* cache, 
   // the pass runs cache->m's kernels on buffers sized from model's shape
   if (cache->m != model) return err("rtg_forward_cached_noalloc: the cache belongs to another model");
   if (cache->batch != 1) return err("rtg_forward_cached_noalloc needs a batch-1 cache");
+  if (cache->quantised()) return err("rtg_forward_cached_noalloc does not take a quantised cache");
   std::string e = check_cached(model, cache->len, ids, n);
   if (!e.empty()) return err(e);
   // x, ln, att [n][d], qkv [n][3d], h [n][4d], logits [n][V] in the device's
@@ -1703,8 +1842,8 @@ rtg_result rtg_forward(const rtg_model* model, const uint32_t* ids, size_t n, fl
   return ok();
 }
 
-rtg_result rtg_generate_cached_batched(const rtg_model* model, const uint32_t* prompts, size_t batch, size_t n,
-                                       size_t max_new, uint32_t* out, rtg_timing* timing) {
+static rtg_result generate_batched(const rtg_model* model, const uint32_t* prompts, size_t batch, size_t n,
+                                   size_t max_new, size_t block, uint32_t* out, rtg_timing* timing) {
   if (!model || !out) return err("null argument");
   if (batch == 0) return err("batch must be >= 1");
   const size_t P = model->cfg.n_positions;
@@ -1716,12 +1855,24 @@ rtg_result rtg_generate_cached_batched(const rtg_model* model, const uint32_t* p
   const size_t steps = max_new > 0 ? max_new : 1;
   if (n + steps - 1 > P) return err(fmt("Total sequence length %zu exceeds max position %zu", P + 1, P));
   try {
-    generate_greedy(model, prompts, batch, n, max_new, out, timing);
+    generate_greedy(model, prompts, batch, n, max_new, out, timing, nullptr, block);
   } catch (const HipError& he) {
     return err(he.msg);  } catch (const std::exception& ex) {
     return err_internal(ex);
   }
   return ok();
+}
+
+rtg_result rtg_generate_cached_batched(const rtg_model* model, const uint32_t* prompts, size_t batch, size_t n,
+                                       size_t max_new, uint32_t* out, rtg_timing* timing) {
+  return generate_batched(model, prompts, batch, n, max_new, 0, out, timing);
+}
+
+rtg_result rtg_generate_cached_quantised(const rtg_model* model, const uint32_t* prompts, size_t batch, size_t n,
+                                         size_t max_new, size_t block, uint32_t* out, rtg_timing* timing) {
+  if (block != 16 && block != 32 && block != 64)
+    return err(fmt("block %zu is not supported (16, 32 or 64)", block));
+  return generate_batched(model, prompts, batch, n, max_new, block, out, timing);
 }
 
 rtg_result rtg_generate_cached(const rtg_model* model, const uint32_t* prompt, size_t n, size_t max_new,

@@ -87,14 +87,21 @@ def _ptr(a: np.ndarray):
 class KVCache:
     """KVCache (gpt2.rs:111-162), preallocated in HBM for n_positions tokens.
 
-    `batch` > 1 is the batched extension: B sequences advancing together."""
+    `batch` > 1 is the batched extension: B sequences advancing together.
+    `bits` 8: keys and values in 8 bits with a scale per `block` tokens and head."""
 
-    def __init__(self, model: "Gpt2Model", batch: int = 1):
+    def __init__(self, model: "Gpt2Model", batch: int = 1, bits: int = 32, block: int = 32):
+        self._h = None
+        if bits not in (32, 8):
+            raise ValueError("bits must be 32 or 8")
         self._lib = _lib.load()
         self.model = model
         self.batch = batch
         h = C.c_void_p()
-        check(self._lib.rtg_cache_new(model._h, batch, C.byref(h)))
+        if bits == 8:
+            check(self._lib.rtg_cache_new_quantised(model._h, batch, block, C.byref(h)))
+        else:
+            check(self._lib.rtg_cache_new(model._h, batch, C.byref(h)))
         self._h = h
 
     def len(self) -> int:
@@ -191,8 +198,8 @@ class Gpt2Model:
     def num_parameters(self) -> int:
         return int(self._lib.rtg_num_parameters(self._h))
 
-    def new_cache(self, batch: int = 1) -> KVCache:
-        return KVCache(self, batch)
+    def new_cache(self, batch: int = 1, bits: int = 32, block: int = 32) -> KVCache:
+        return KVCache(self, batch, bits, block)
 
     # -- forward passes --
     def forward(self, token_ids) -> np.ndarray:
@@ -244,8 +251,9 @@ class Gpt2Model:
         return out.tolist()
 
     def generate_cached_batched(self, prompts, max_new_tokens: int, timing: bool = False,
-                                profile_kernels: bool = False):
-        """Batched greedy generate_cached: prompts [B, n] -> ids [B, n + max(1, max_new)].
+                                profile_kernels: bool = False, bits: int = 32, block: int = 32):
+        """Batched greedy generate_cached: prompts [B, n] -> ids [B, n + max(1, max_new)],
+        over a cache of 32 bits or, with a scale per `block` tokens and head, of 8.
 
         timing=True also returns the device-event timings; profile_kernels=True
         additionally replays the decode steps launch by launch to time the
@@ -256,8 +264,14 @@ class Gpt2Model:
         out = np.empty((B, n + max(1, max_new_tokens)), dtype=np.uint32)
         t = _lib.Timing()
         t.profile_kernels = int(profile_kernels)
-        check(self._lib.rtg_generate_cached_batched(self._h, _ptr(ids), B, n, max_new_tokens, _ptr(out),
-                                                    C.byref(t)))
+        if bits not in (32, 8):
+            raise ValueError("bits must be 32 or 8")
+        if bits == 8:
+            check(self._lib.rtg_generate_cached_quantised(self._h, _ptr(ids), B, n, max_new_tokens, block, _ptr(out),
+                                                          C.byref(t)))
+        else:
+            check(self._lib.rtg_generate_cached_batched(self._h, _ptr(ids), B, n, max_new_tokens, _ptr(out),
+                                                        C.byref(t)))
         if timing:
             return out, {"prefill_ms": t.prefill_ms, "decode_ms": t.decode_ms, "decode_steps": t.decode_steps,
                          "decode_kernel_ms": t.decode_kernel_ms,
