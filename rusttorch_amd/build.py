@@ -28,6 +28,13 @@ DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-m
                 "-amdgpu-kernarg-preload-count=14"]
 COMMON = ["-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", f"-I{os.path.join(PKG, '..', 'include')}"]
 
+# Flags of single files.
+FILE_FLAGS = {
+    # i8 products are read by vector instructions right away: accumulators in VGPRs
+    # save two copies each
+    "qattn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+}
+
 SOURCES = ["kernels.hip", "gemm_pair.hip", "attn_pair.hip", "decode_persistent.hip", "decode_persistent_inst_mini.hip",
            "decode_persistent_inst_small.hip", "decode_persistent_inst_medium.hip",
            "decode_persistent_inst_large.hip", "rtg_runtime.cpp", "device_memory.cpp", "safetensors_reader.cpp",
@@ -39,7 +46,7 @@ def _compile(src: str) -> str:
     path = os.path.join(CSRC, src)
     obj = os.path.join(OBJ, src + ".o")
     if src.endswith(".hip"):
-        cmd = [HIPCC, f"--offload-arch={ARCH}", *DEVICE_FLAGS, *COMMON, "-c", path, "-o", obj]
+        cmd = [HIPCC, f"--offload-arch={ARCH}", *DEVICE_FLAGS, *FILE_FLAGS.get(src, []), *COMMON, "-c", path, "-o", obj]
     else:
         cmd = [HIPCC, *COMMON, "-c", path, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)

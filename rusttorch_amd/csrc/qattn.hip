@@ -70,6 +70,53 @@ __device__ __forceinline__ i32x4 fixed_mfma(const i32x4 (&a)[KS], const i32x4 (&
   return (hi << 8) + mid;
 }
 
+// A query as ND digit planes: this lane's 16 elements (of each 64) group * 16 + e,
+// q[k][digit] bytes e. qrow null: zeros. Returns the score in units of log2 e of a
+// unit of the fixed-point sums (of 256 of them for ND = 3), but for the key's
+// scale; NaN for a row with a value that is not finite. The four lanes 16 apart
+// hold a row.
+template <int KS, int ND, class T>
+__device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, int group, float scale,
+                                             i32x4 (&q)[KS][ND]) {
+  float4 x[KS][4];
+  unsigned top = 0;  // (bits order like the values, NaN above infinity)
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[k][e] = qrow ? load4(qrow, k * 64 + group * 16 + e * 4, hd, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+      top = max(max(top, __float_as_uint(x[k][e].x) & 0x7FFFFFFFu), __float_as_uint(x[k][e].y) & 0x7FFFFFFFu);
+      top = max(max(top, __float_as_uint(x[k][e].z) & 0x7FFFFFFFu), __float_as_uint(x[k][e].w) & 0x7FFFFFFFu);
+    }
+  const auto r = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+  top = max(r[0], r[1]);
+  const auto r2 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+  top = max(r2[0], r2[1]);
+  const float amax = __uint_as_float(top);
+  const bool fine = top < 0x7F800000u;
+  // below 2^-100 a row is as good as 0: no score that exp could tell from 0
+  const bool zero = amax < 7.9e-31f;
+  // (a negative scale goes into the digits: the factor of the sums is not negative)
+  const float inv = fine && !zero ? copysignf(fixed_max<ND>(), scale) / amax : 0.f;
+  constexpr int bias = ND == 3 ? 0x808080 : 0x8080;
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float xe[4] = {x[k][e].x, x[k][e].y, x[k][e].z, x[k][e].w};
+      unsigned u[4], d[ND];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u[i] = (unsigned)((int)rintf(fine ? xe[i] * inv : 0.f) + bias);
+        if constexpr (ND == 3) u[i] ^= 0x800000u;  // (the top digit of planes() carries no 128)
+      }
+      planes<ND>(u[0], u[1], u[2], u[3], d);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) q[k][i][e] = (int)d[i];
+    }
+  return !fine ? NAN : zero ? 0.f : amax * (fabsf(scale) * 1.4426950408889634f * (ND == 3 ? 256.f : 1.f) / fixed_max<ND>());
+}
+
 // A wave's 16 columns: lane = group * 16 + column; the group's 16 (of 64) query
 // elements, and 16 of a tile's keys: t * 16 + group * 4 + i.
 template <int HDP, int ND>
@@ -91,45 +138,7 @@ struct Cols {
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[d][i] = 0.f;
-    float4 x[KS][4];
-    unsigned top = 0;
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[k][e] = qrow ? load4(qrow, k * 64 + group * 16 + e * 4, hd, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
-        top = max(max(top, __float_as_uint(x[k][e].x) & 0x7FFFFFFFu), __float_as_uint(x[k][e].y) & 0x7FFFFFFFu);
-        top = max(max(top, __float_as_uint(x[k][e].z) & 0x7FFFFFFFu), __float_as_uint(x[k][e].w) & 0x7FFFFFFFu);
-      }
-    {
-      const auto r = __builtin_amdgcn_permlane16_swap(top, top, false, false);
-      top = max(r[0], r[1]);
-      const auto r2 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-      top = max(r2[0], r2[1]);
-    }
-    // (bits order like the values, NaN above infinity)
-    const float amax = __uint_as_float(top);
-    const bool fine = top < 0x7F800000u;
-    // below 2^-100 a row is as good as 0: no score that exp could tell from 0
-    const bool zero = amax < 7.9e-31f;
-    const float inv = fine && !zero ? fixed_max<ND>() / amax : 0.f;
-    sq = !fine ? NAN : zero ? 0.f : amax * (scale * 1.4426950408889634f * (ND == 3 ? 256.f : 1.f) / fixed_max<ND>());
-    constexpr int bias = ND == 3 ? 0x808080 : 0x8080;
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float xe[4] = {x[k][e].x, x[k][e].y, x[k][e].z, x[k][e].w};
-        unsigned u[4], d[ND];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          u[i] = (unsigned)((int)rintf(fine ? xe[i] * inv : 0.f) + bias);
-          if constexpr (ND == 3) u[i] ^= 0x800000u;  // (the top digit of planes() carries no 128)
-        }
-        planes<ND>(u[0], u[1], u[2], u[3], d);
-#pragma unroll
-        for (int i = 0; i < ND; ++i) q[k][i][e] = (int)d[i];
-      }
+    sq = fixed_query<KS, ND>(qrow, hd, vec, group, scale, q);
   }
 };
 
@@ -142,6 +151,10 @@ struct Tile {
   // sp: the (sequence, head)'s scales
   __device__ __forceinline__ void load_s(const float* sp, int tile, int shift, int lane) {
     s = reinterpret_cast<const float2*>(sp)[(tile << (6 - shift)) + (lane & ((1 << (6 - shift)) - 1))];
+  }
+  // the same for lane i: the scales of the tile's key i
+  __device__ __forceinline__ void load_s64(const float* sp, int tile, int shift, int lane) {
+    s = reinterpret_cast<const float2*>(sp)[(tile * kQTile + lane) >> shift];
   }
   // kp, vp: the (sequence, head)'s codes
   __device__ __forceinline__ void load_k(const int8_t* kp, int tile, int lane) {
@@ -161,70 +174,114 @@ struct Tile {
 __device__ __forceinline__ float lane_of(float v, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, dpp_row<0xB1>(v));
+  v = fmaxf(v, dpp_row<0x4E>(v));
+  v = fmaxf(v, dpp_row<0x124>(v));
+  v = fmaxf(v, dpp_row<0x128>(v));
+  return v;
+}
 __device__ __forceinline__ float xmax(float v) { return xor32_max_k(xor16_max_k(v)); }
 __device__ __forceinline__ float xsum(float v) { return xor32_sum_k(xor16_sum_k(v)); }
 
-// One tile (tokens j0 .. j0 + 63) for a wave's columns. edge: some column does
-// not see all of its keys; live: keys below this are in the cache (uniform).
-template <int HDP, int ND>
-__device__ __forceinline__ void tile_step(Cols<HDP, ND>& c, const Tile<HDP>& t, int shift, int j0, bool edge, int live,
-                                          int group) {
-  constexpr int DT = HDP / 16;
-  // the tile's scales: of each 16 tokens; those of blocks behind the last key are not read as numbers
-  float fk[4], rv[4];
-  float vmax = 0.f;
-  bool bad = false;
+// Fixed-point probabilities: at most 2^22 (2^14 for two digits) for the tile's
+// largest, of twice that which the digits hold: its exponent is 0 up to rounding,
+// which stays below 1 for scores up to kLargeScore.
+template <int ND>
+__device__ __forceinline__ constexpr float p_one() {
+  return ND == 3 ? 4150000.f : 16200.f;
+}
+constexpr float kLargeScore = 2097152.f;  // 2^21
+
+// A tile's scales for a wave: of each 16 keys f (scores) and r = max(v scale /
+// vmax, 2^-60) as lr = log2 r and 1 / r. (A block of zeros may take any r.)
+struct TileScales {
+  float f[4], lr[4], rinv[4], vmax;
+  unsigned bad;  // bit i: the values of the i-th 16 keys read back as NaN
+  __device__ __forceinline__ bool nan(int i) const { return bad >> i & 1; }
+};
+// sl: a lane's (keys', values') scales, those of the tile's blocks on lanes 0 ..
+// and over and over; live: keys of the tile that are in the cache (or more).
+__device__ __forceinline__ TileScales tile_scales(float2 sl, int shift, int live, int lane) {
+  TileScales t;
+  const int nb = 64 >> shift;
+  const bool in = ((lane & (nb - 1)) << shift) < live;  // blocks behind the last key are not read as numbers
+  const float k = in ? sl.x : 0.f, v = in ? sl.y : 0.f;
+  const unsigned nans = (unsigned)__builtin_amdgcn_ballot_w64(v != v);
+  t.bad = 0;
+  float m = fmaxf(v, dpp_row<0xB1>(v));  // (fmaxf skips NaN)
+  m = fmaxf(m, dpp_row<0x4E>(m));
+  t.vmax = m;
+  // (r to the last place: it is the same for a block's every key)
+  const float r = m > 0.f ? fmaxf(v * __builtin_amdgcn_rcpf(m), 8.6736174e-19f) : 1.f;
+  const float lr = __builtin_amdgcn_logf(r), ri = __builtin_amdgcn_rcpf(r);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int b = (i * 16) >> shift;
-    const bool in = j0 + i * 16 < live;
-    fk[i] = in ? lane_of(t.s.x, b) : 0.f;
-    rv[i] = in ? lane_of(t.s.y, b) : 0.f;
-    vmax = fmaxf(vmax, rv[i]);  // (skips NaN)
-    bad |= rv[i] != rv[i];
+    t.f[i] = lane_of(k, b);
+    t.lr[i] = lane_of(lr, b);
+    t.rinv[i] = lane_of(ri, b);
+    t.bad |= (nans >> b & 1) << i;
   }
-  const float rinv = vmax > 0.f ? 1.f / vmax : 0.f;
-  float s[4][4];
+  return t;
+}
+
+// One tile (keys j0 .. j0 + 63) for a wave's columns. EDGE: some column does not
+// see all of its keys. The running maximum is of score + lr, that is of the
+// probability times the value's scale, so that a tile's largest such product is
+// 1 and needs no second reduction; each probability itself is 1 / r of it.
+template <bool EDGE, int HDP, int ND>
+__device__ __forceinline__ void tile_step(Cols<HDP, ND>& c, const Tile<HDP>& t, const TileScales& ts, int j0, int group) {
+  constexpr int DT = HDP / 16;
+  float s[4][4], f[4];
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const i32x4 d = fixed_mfma<ND, Cols<HDP, ND>::KS>(t.k[i], c.q);
-    const float f = c.sq * fk[i];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[i][e] = (float)d[e] * f;
-  }
-  if (edge) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (j0 + i * 16 + group * 4 + e >= c.lim) s[i][e] = -INFINITY;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
-  const float mn = fmaxf(c.m, xmax(top));
-  const float base = mn == -INFINITY ? 0.f : mn;  // (no key yet: every p is 2^-inf = 0)
-  const float corr = __builtin_amdgcn_exp2f(c.m - base);
-  float sum = 0.f, ptop = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float r = rv[i] * rinv;
+    f[i] = c.sq * ts.f[i];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float p = __builtin_amdgcn_exp2f(s[i][e] - base);
-      sum += p;
-      s[i][e] = edge && j0 + i * 16 + group * 4 + e >= c.lim ? 0.f : p * r;
-      ptop = fmaxf(ptop, s[i][e]);
+      s[i][e] = (float)d[e];
+      if (EDGE) s[i][e] = j0 + i * 16 + group * 4 + e < c.lim ? fmaf(s[i][e], f[i], ts.lr[i]) : -INFINITY;
     }
   }
-  if (bad) {  // a block that reads back as NaN: every column that sees a key of it is NaN
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float m = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+    top = fmaxf(top, EDGE ? m : fmaf(m, f[i], ts.lr[i]));  // (f >= 0)
+  }
+  top = xmax(top);
+  const float base = top == -INFINITY ? 0.f : top;  // (no key here: every p is 2^-inf = 0)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float cc = ts.lr[i] - base;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[i][e] = EDGE ? s[i][e] - base : fmaf(s[i][e], f[i], cc);
+  }
+  if (!EDGE && __builtin_amdgcn_ballot_w64(fabsf(top) > kLargeScore)) {
+    asm volatile("");  // (a branch: hardly ever taken)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (rv[i] != rv[i] && j0 + i * 16 + group * 4 < c.lim) sum = NAN;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] = s[i][e] > 0.f ? 0.f : s[i][e];
   }
-  c.l = c.l * corr + sum;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[i][e] = __builtin_amdgcn_exp2f(s[i][e]);
+    sum = fmaf((s[i][0] + s[i][1]) + (s[i][2] + s[i][3]), ts.rinv[i], sum);
+  }
+  if (ts.bad) {
+    asm volatile("");
+    // every column that sees a key of such a block is NaN
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (ts.nan(i) && j0 + i * 16 + group * 4 < c.lim) sum = NAN;
+  }
+  const float mn = fmaxf(c.m, top), mb = mn == -INFINITY ? 0.f : mn;
+  const float corr = __builtin_amdgcn_exp2f(c.m - mb), g = __builtin_amdgcn_exp2f(top - mb);
+  c.l = fmaf(c.l, corr, sum * g);
   if (__builtin_amdgcn_ballot_w64(mn != c.m)) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -232,18 +289,15 @@ __device__ __forceinline__ void tile_step(Cols<HDP, ND>& c, const Tile<HDP>& t, 
       for (int i = 0; i < 4; ++i) c.o[d][i] *= corr;
   }
   c.m = mn;
-  ptop = xmax(ptop);
-  // (a tile whose largest product is below 2^-100 of its largest scale adds nothing)
-  const float pinv = ptop > 7.9e-31f ? fixed_max<ND>() * __builtin_amdgcn_rcpf(ptop) : 0.f;
-  const float w = ptop * vmax * ((ND == 3 ? 256.f : 1.f) / fixed_max<ND>());
-  // p * pinv rounded to an integer and biased, in the low bits of the sum with 2^23
+  const float w = g * ts.vmax * ((ND == 3 ? 256.f : 1.f) / p_one<ND>());
+  // rounded to an integer and biased, in the low bits of the sum with 2^23
   constexpr float magic = ND == 3 ? 8421504.f : 8388608.f + 32896.f;  // 2^23 + 0x8080
   i32x4 pd[1][ND];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     unsigned u[4], d[ND];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(fmaf(s[i][e], pinv, magic));
+    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(fmaf(s[i][e], p_one<ND>(), magic));
     planes<ND>(u[0], u[1], u[2], u[3], d);
 #pragma unroll
     for (int n = 0; n < ND; ++n) pd[0][n][i] = (int)d[n];
@@ -269,6 +323,7 @@ struct AttnArgs {
   bool qvec, ovec;
   int cblocks;               // blocks of columns per (sequence, head)
   float* part;               // partial results of split keys
+  unsigned* joined;          // per block of columns: how many of its splits are done (0 between calls)
   int splits;
 };
 
@@ -349,7 +404,9 @@ __global__ __launch_bounds__(256) void q_attend_cols_kernel(AttnArgs a) {
     Tile<HDP> n;
     n.load_s(sp, min(j + 1, tiles - 1), shift, lane);
     n.load_k(kp, min(j + 1, tiles - 1), lane);
-    tile_step(c, t, shift, j * kQTile, j * kQTile + kQTile > least, live, group);
+    const TileScales ts = tile_scales(t.s, shift, live - j * kQTile, lane);
+    if (j * kQTile + kQTile > least) tile_step<true>(c, t, ts, j * kQTile, group);
+    else tile_step<false>(c, t, ts, j * kQTile, group);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -369,37 +426,154 @@ __global__ __launch_bounds__(256) void q_attend_cols_kernel(AttnArgs a) {
 
 // ---- few columns: the keys are split over workgroups and over their waves ----
 
-constexpr int kMinTiles = 4;  // a workgroup's share of the keys is at least this many tiles
-
-// Tiles per split and splits used for `tiles` tiles.
+// Tiles per split for `tiles` tiles over at most `splits` workgroups: all of them
+// where they are few (a split costs 3 to 4 us, the partials' way through memory;
+// eight waves take 8 tiles in 0.7 us more than one), else at least two or one per wave.
+template <int HDP>
 __device__ __forceinline__ int split_tiles(int tiles, int splits) {
-  return max((tiles + splits - 1) / splits, kMinTiles);
+  constexpr int least = HDP == 64 ? 16 : 8;
+  return tiles <= least ? max(tiles, 1) : max((tiles + splits - 1) / splits, least);
 }
 
-// A column's partial: m, l, o[hdp].
-template <int HDP>
+// A column's partial: m, l, o[hdp]. Blocks of W columns.
+template <int HDP, int W>
 __device__ __forceinline__ float* part_of(const AttnArgs& a, int sh, int cb, int z, int col) {
-  return a.part + ((((size_t)sh * a.cblocks + cb) * a.splits + z) * 16 + col) * (HDP + 2);
+  return a.part + ((((size_t)sh * a.cblocks + cb) * a.splits + z) * W + col) * (HDP + 2);
+}
+
+// The waves' results of a workgroup: statistics per column and rows of o.
+template <int HDP, int W, int NW>
+struct Merge {
+  float m[NW][W], l[NW][W];
+  __attribute__((aligned(16))) float o[NW][W][HDP + 4];
+  int last;
+};
+
+// Two neighbouring floats of a partial, past the L2 caches (workgroups of other
+// XCDs read them).
+__device__ __forceinline__ void store2(float* p, float x, float y) {
+  const unsigned long long v = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load2(const float* p) {
+  const unsigned long long v = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32)));
+}
+
+// Joins the waves' results in s (written, not yet synchronised) for the W
+// columns of block cb: to the results where the keys were not split, else to the
+// partials; the last of a block's workgroups to come here joins those.
+template <int HDP, int W, int NW, class T>
+__device__ __forceinline__ void finish(const AttnArgs& a, Merge<HDP, W, NW>& s, const Seq& r, int seq, int sh, int head,
+                                       int cb, int z, int tiles, int per) {
+  constexpr int C4 = HDP / 4, NT = 64 * NW, CPP = NT / C4;
+  const int tid = threadIdx.x, c4 = (tid % C4) * 4;
+  const bool whole = per >= tiles;
+  auto put = [&](int col, float l, const float4& x) {
+    const int ci = cb * W + col, i = ci / a.group, h = head * a.group + ci - i * a.group;
+    const bool any = i < r.count && visible(r, i) > 0;
+    const float inv = 1.f / l;
+    put4<T>(a, seq, i, h, c4,
+            any ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
+  };
+  const int cols = min(W, a.n_q * a.group - cb * W);
+  __syncthreads();
+  for (int col = tid / C4; col < cols; col += CPP) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, s.m[w][col]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(s.m[w][col] - base);
+      const float4 y = *reinterpret_cast<const float4*>(&s.o[w][col][c4]);
+      l = fmaf(f, s.l[w][col], l);
+      x = make_float4(fmaf(f, y.x, x.x), fmaf(f, y.y, x.y), fmaf(f, y.z, x.z), fmaf(f, y.w, x.w));
+    }
+    if (whole) {
+      put(col, l, x);
+    } else {
+      float* p = part_of<HDP, W>(a, sh, cb, z, col);
+      if (c4 == 0) store2(p, m, l);
+      store2(p + 2 + c4, x.x, x.y);
+      store2(p + 4 + c4, x.z, x.w);
+    }
+  }
+  if (whole) return;
+  const int n = (tiles + per - 1) / per;
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the stores have completed
+  __syncthreads();
+  if (tid == 0) {
+    unsigned* count = a.joined + ((size_t)sh * a.cblocks + cb) * kQTicketStride;
+    s.last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)n - 1;
+    if (s.last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!s.last) return;
+  // A split's row over C4 threads; as many such groups to a column as there are
+  // (a power of two), each taking every gpc-th split.
+  constexpr int GPW = 64 / C4;  // groups per wave
+  int gpc = 1;
+  while (gpc * 2 * cols <= CPP) gpc *= 2;
+  const int g = tid / C4, wave = tid >> 6, zg = g & (gpc - 1);
+  for (int col0 = 0; col0 < cols; col0 += CPP / gpc) {
+    const int col = min(col0 + g / gpc, cols - 1);
+    float m = -INFINITY;
+    for (int z2 = tid % C4; z2 < n; z2 += C4) m = fmaxf(m, load2(part_of<HDP, W>(a, sh, cb, z2, col)).x);
+    m = row_max(m);
+    if constexpr (C4 == 32) m = xor16_max_k(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int z2 = zg; z2 < n; z2 += gpc) {
+      const float* p = part_of<HDP, W>(a, sh, cb, z2, col);
+      const float2 ml = load2(p), y0 = load2(p + 2 + c4), y1 = load2(p + 4 + c4);
+      const float f = __builtin_amdgcn_exp2f(ml.x - base);
+      l = fmaf(f, ml.y, l);
+      x = make_float4(fmaf(f, y0.x, x.x), fmaf(f, y0.y, x.y), fmaf(f, y1.x, x.z), fmaf(f, y1.y, x.w));
+    }
+    for (int w = 1; w < gpc && w < GPW; w *= 2) {
+      l += __shfl_xor(l, w * C4);
+      x = make_float4(x.x + __shfl_xor(x.x, w * C4), x.y + __shfl_xor(x.y, w * C4), x.z + __shfl_xor(x.z, w * C4),
+                      x.w + __shfl_xor(x.w, w * C4));
+    }
+    bool first = zg == 0;
+    if (gpc > GPW) {  // (uniform) a column's waves meet in LDS
+      if ((tid & 63) < C4) *reinterpret_cast<float4*>(&s.o[wave][0][c4]) = x;
+      if ((tid & 63) == 0) s.l[wave][0] = l;
+      __syncthreads();
+      if (first)
+        for (int w = 1; w < gpc / GPW; ++w) {
+          const float4 y = *reinterpret_cast<const float4*>(&s.o[wave + w][0][c4]);
+          l += s.l[wave + w][0];
+          x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        }
+      __syncthreads();
+    }
+    if (first && col0 + g / gpc < cols) put(col, l, x);
+  }
 }
 
 template <int HDP, int ND, class T>
 __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
-  constexpr int NW = 4, DT = HDP / 16;
-  __shared__ float sm[NW][16], sl[NW][16];
-  __shared__ __attribute__((aligned(16))) float so[NW][16][HDP + 4];
+  constexpr int NW = 4;
+  __shared__ Merge<HDP, 16, NW> s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
   const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head, cb = blockIdx.y, z = blockIdx.z;
   const Seq r = seq_of(a, seq);
   const int ci = cb * 16 + col, i = ci / a.group, qh = head * a.group + ci - i * a.group;
-  const bool mine = i < a.n_q, used = i < r.count;
+  const bool used = i < r.count;
   const int firstq = cb * 16 / a.group;
   const int last = min((cb * 16 + 15) / a.group, r.count - 1);
   const int live = firstq < r.count ? visible(r, last) : 0;
   const int least = firstq < r.count ? visible(r, firstq) : 0;
-  const int tiles = (live + kQTile - 1) / kQTile, per = split_tiles(tiles, a.splits);
+  const int tiles = (live + kQTile - 1) / kQTile, per = split_tiles<HDP>(tiles, a.splits);
   const int t0 = z * per, t1 = min(t0 + per, tiles);
   if (z > 0 && t0 >= tiles) return;  // (the whole workgroup; split 0 also writes rows without keys)
-  const bool whole = per >= tiles;
   Cols<HDP, ND> c;
   const T* qrow = static_cast<const T*>(a.q.p) + (long)seq * a.q.seq + (long)i * a.q.tok + (long)qh * a.q.head;
   c.init(used ? qrow : nullptr, a.c.hd, a.qvec, group, a.scale, used ? visible(r, i) : 0);
@@ -419,133 +593,259 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
     n.load_s(sp, nj, shift, lane);
     n.load_k(kp, nj, lane);
     n.load_v(vp, nj, lane);
-    tile_step(c, t, shift, j * kQTile, j * kQTile + kQTile > least, live, group);
+    const TileScales ts = tile_scales(t.s, shift, live - j * kQTile, lane);
+    if (j * kQTile + kQTile > least) tile_step<true>(c, t, ts, j * kQTile, group);
+    else tile_step<false>(c, t, ts, j * kQTile, group);
     t = n;
   }
   const float l = xsum(c.l);
   if (group == 0) {
-    sm[wave][col] = c.m;
-    sl[wave][col] = l;
+    s.m[wave][col] = c.m;
+    s.l[wave][col] = l;
   }
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
-    *reinterpret_cast<float4*>(&so[wave][col][d * 16 + group * 4]) = make_float4(c.o[d][0], c.o[d][1], c.o[d][2], c.o[d][3]);
-  __syncthreads();
-  // four threads' worth of columns at a time: thread = (column, 4 results)
-  constexpr int C4 = HDP / 4, CPP = 256 / C4;
-  const int c4 = (threadIdx.x % C4) * 4;
-  for (int cc = threadIdx.x / C4; cc < 16; cc += CPP) {
-    const int cj = cb * 16 + cc, qi = cj / a.group, h = head * a.group + cj - qi * a.group;
-    if (qi >= a.n_q) break;
-    float m = -INFINITY;
+  for (int d = 0; d < HDP / 16; ++d)
+    *reinterpret_cast<float4*>(&s.o[wave][col][d * 16 + group * 4]) = make_float4(c.o[d][0], c.o[d][1], c.o[d][2], c.o[d][3]);
+  finish<HDP, 16, NW, T>(a, s, r, seq, sh, head, cb, z, tiles, per);
+}
+
+// ---- up to four columns: one new token of a head, or of four that share their keys ----
+//
+// The matrix instructions' other way round: the digits of the queries are the
+// rows, the keys of a tile the columns, so the digits' sums of a score lie in one
+// lane's registers 4 g .. 4 g + 2. One column (NC = 1): the 16 keys t of a tile
+// meet a copy of the query that sits in rows 4 t .. 4 t + 2, all into one
+// accumulator, so each of the 64 lanes has the score of one of the 64 keys. Four
+// columns (NC = 4): each has four rows, a lane has four keys of one of them. The
+// probabilities' digits pass through LDS into the same rows for P V, which leaves
+// a lane with one result of 64 (or with every 16th of its column's). A tile then
+// takes 70 (NC = 4: 130) vector instructions where a wave of 16 columns takes 400.
+template <int HDP, int NC>
+struct FewCols {
+  static constexpr int KS = HDP / 64, DT = HDP / 16, NO = NC == 1 ? HDP / 64 : DT;
+  i32x4 q[NC == 1 ? 4 : 1][KS];
+  float sq, m, l;
+  float o[NO];
+  int lim;
+
+  // qrow: this lane's row's column's query (lane & 15: rows); lane >> 4 selects 16 of its elements
+  template <class T>
+  __device__ __forceinline__ void init(const T* qrow, int hd, bool vec, int lane, float scale) {
+    m = -INFINITY;
+    l = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, sm[w][cc]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float ls = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < NO; ++i) o[i] = 0.f;
+    i32x4 d[KS][3];
+    const float sr = fixed_query<KS, 3>(qrow, hd, vec, lane >> 4, scale, d);
+    const int row = lane & 15;
+    i32x4 mine[KS];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sm[w][cc] - base);
-      const float4 y = *reinterpret_cast<const float4*>(&so[w][cc][c4]);
-      ls = fmaf(f, sl[w][cc], ls);
-      x.x = fmaf(f, y.x, x.x);
-      x.y = fmaf(f, y.y, x.y);
-      x.z = fmaf(f, y.z, x.z);
-      x.w = fmaf(f, y.w, x.w);
-    }
-    if (whole) {
-      const bool any = qi < r.count && visible(r, qi) > 0;
-      const float inv = 1.f / ls;
-      put4<T>(a, seq, qi, h, c4,
-              any ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
-    } else {
-      float* p = part_of<HDP>(a, sh, cb, z, cc);
-      if (c4 == 0) {
-        p[0] = m;
-        p[1] = ls;
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int x = (row & 3) == 0 ? d[k][0][e] : (row & 3) == 1 ? d[k][1][e] : d[k][2][e];
+        mine[k][e] = (row & 3) == 3 ? 0 : x;
       }
-      p[2 + c4] = x.x;
-      p[3 + c4] = x.y;
-      p[4 + c4] = x.z;
-      p[5 + c4] = x.w;
+    if constexpr (NC == 1) {
+      sq = sr;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[t][k][e] = row >> 2 == t ? mine[k][e] : 0;
+    } else {
+      // this lane's column is lane >> 4: rows 4 * column + digit
+      sq = __shfl(sr, (lane >> 4) * 4);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) q[0][k] = mine[k];
     }
   }
+};
+
+__device__ __forceinline__ int fixed_sum(const i32x4& d) { return (d[2] << 8) + d[1] + ((d[0] + 128) >> 8); }
+
+// image: this wave's digit planes, [NC][4][4][16] bytes, those of digit 3 zero
+template <int HDP, int NC>
+__device__ __forceinline__ void few_step(FewCols<HDP, NC>& c, const Tile<HDP>& t, int j0, bool edge, int live, int lane,
+                                         unsigned char* image) {
+  constexpr int KS = HDP / 64, DT = HDP / 16, NT = NC == 1 ? 1 : 4;  // keys per lane
+  const int row = lane & 15, group = lane >> 4;
+  const i32x4 zero = {0, 0, 0, 0};
+  float s[NT], sv[NT];
+  // key i of the lane: NC = 1: the lane's own; NC = 4: i * 16 + row
+  auto key = [&](int i) { return NC == 1 ? lane : i * 16 + row; };
+  float top = -INFINITY;
+  if constexpr (NC == 1) {
+    i32x4 d = zero;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.q[i][k], t.k[i][k], d, 0, 0, 0);
+    s[0] = (float)fixed_sum(d) * (c.sq * t.s.x);
+    sv[0] = t.s.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      i32x4 d = zero;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.q[0][k], t.k[i][k], d, 0, 0, 0);
+      s[i] = (float)fixed_sum(d) * (c.sq * lane_of(t.s.x, i * 16));
+      sv[i] = lane_of(t.s.y, i * 16);
+    }
+  }
+  bool poison = false;  // a key that the column sees reads back as NaN
+  if (edge) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const bool see = j0 + key(i) < c.lim;
+      if (!see) {
+        s[i] = -INFINITY;
+        sv[i] = 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    poison |= sv[i] != sv[i];
+    top = fmaxf(top, s[i]);
+  }
+  top = row_max(top);
+  if constexpr (NC == 1) top = xmax(top);
+  const float mn = fmaxf(c.m, top), base = mn == -INFINITY ? 0.f : mn;
+  const float corr = __builtin_amdgcn_exp2f(c.m - base);
+  float sum = 0.f, ptop = 0.f;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const float p = __builtin_amdgcn_exp2f(s[i] - base);
+    sum += p;
+    s[i] = p * sv[i];
+    ptop = fmaxf(ptop, s[i]);
+  }
+  if (poison) sum = NAN;
+  c.l = fmaf(c.l, corr, sum);
+  c.m = mn;
+  ptop = row_max(ptop);
+  if constexpr (NC == 1) ptop = xmax(ptop);
+  const float pinv = ptop >= 1.2e-38f ? __builtin_amdgcn_rcpf(ptop) : 0.f;
+  const float w = ptop * (256.f / fixed_max<3>());
+  const int column = NC == 1 ? 0 : group;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    // 2^23 + 0x8080 + the fixed-point value: its bytes are the digits, plus 128 but for the top one
+    const unsigned u = __float_as_uint(fmaf(s[i] * pinv, fixed_max<3>(), 8421504.f)) ^ 0x8080u;
+    unsigned char* p = image + column * 256 + ((key(i) >> 2) & 3) * 16 + (key(i) >> 4) * 4 + (key(i) & 3);
+    p[0] = (unsigned char)u;
+    p[64] = (unsigned char)(u >> 8);
+    p[128] = (unsigned char)(u >> 16);
+  }
+  // (one wave's LDS accesses are in order; the fences are for the compiler)
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const i32x4 pd = *reinterpret_cast<const i32x4*>(image + (NC == 1 ? 0 : (row >> 2) * 256) + (row & 3) * 64 + group * 16);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  i32x4 r[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) r[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd, t.v[d], zero, 0, 0, 0);
+  if constexpr (NC == 1) {
+    // every group of rows holds the same sums: the lanes of group g take columns 16 g .. 16 g + 15 (of each 64)
+#pragma unroll
+    for (int h = 0; h < HDP / 64; ++h) {
+      i32x4 x;
+#pragma unroll
+      for (int e = 0; e < 3; ++e) {
+        const int lo = (group & 1) ? r[h * 4 + 1][e] : r[h * 4][e], hi = (group & 1) ? r[h * 4 + 3][e] : r[h * 4 + 2][e];
+        x[e] = (group & 2) ? hi : lo;
+      }
+      c.o[h] = fmaf((float)fixed_sum(x), w, c.o[h] * corr);
+    }
+  } else {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) c.o[d] = fmaf((float)fixed_sum(r[d]), w, c.o[d] * corr);
+  }
 }
 
-// Joins the splits of the columns that have more than one: a workgroup per
-// column, its threads 4 results of a split each.
-template <int HDP, class T>
-__global__ __launch_bounds__(256) void q_attend_join_kernel(AttnArgs a) {
-  constexpr int C4 = HDP / 4, ZS = 256 / C4;
-  __shared__ float sm[4];
-  __shared__ __attribute__((aligned(16))) float4 so[4][C4];
-  __shared__ float sl[4];
-  const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int ci = blockIdx.y, cb = ci >> 4, qi = ci / a.group, h = head * a.group + ci - qi * a.group;
+constexpr int kFewWaves = 8;
+
+template <int HDP, int NC, class T>
+__global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a) {
+  constexpr int NW = kFewWaves;
+  __shared__ Merge<HDP, NC, NW> s;
+  __shared__ __attribute__((aligned(16))) unsigned char image[NW][NC * 256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, group = lane >> 4;
+  const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head, z = blockIdx.z;
   const Seq r = seq_of(a, seq);
-  const int last = min((cb * 16 + 15) / a.group, r.count - 1);
-  const int live = cb * 16 / a.group < r.count ? visible(r, last) : 0;
-  const int tiles = (live + kQTile - 1) / kQTile, per = split_tiles(tiles, a.splits);
-  if (per >= tiles) return;
-  const int n = (tiles + per - 1) / per;
-  float m = -INFINITY;
-  for (int z = tid; z < n; z += 256) m = fmaxf(m, part_of<HDP>(a, sh, cb, z, ci & 15)[0]);
-  for (int w = 1; w < 64; w <<= 1) m = fmaxf(m, __shfl_xor(m, w));
-  if (lane == 0) sm[wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  const float base = m == -INFINITY ? 0.f : m;
-  const int c4 = (tid % C4) * 4;
-  float ls = 0.f;
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int z = tid / C4; z < n; z += ZS) {
-    const float* p = part_of<HDP>(a, sh, cb, z, ci & 15);
-    const float f = __builtin_amdgcn_exp2f(p[0] - base);
-    ls = fmaf(f, p[1], ls);
-    x.x = fmaf(f, p[2 + c4], x.x);
-    x.y = fmaf(f, p[3 + c4], x.y);
-    x.z = fmaf(f, p[4 + c4], x.z);
-    x.w = fmaf(f, p[5 + c4], x.w);
+  const int live = r.count > 0 ? visible(r, r.count - 1) : 0, least = r.count > 0 ? visible(r, 0) : 0;
+  const int tiles = (live + kQTile - 1) / kQTile, per = split_tiles<HDP>(tiles, a.splits);
+  const int t0 = z * per, t1 = min(t0 + per, tiles);
+  if (z > 0 && t0 >= tiles) return;  // (the whole workgroup)
+  const int8_t *kp = a.c.k + a.c.codes(sh), *vp = a.c.v + a.c.codes(sh);
+  const float* sp = a.c.s + a.c.scales(sh);
+  const int shift = a.c.block_shift;
+  Tile<HDP> t;
+  int j = t0 + wave;
+  if (j < t1) {
+    t.load_k(kp, j, lane);
+    t.load_v(vp, j, lane);
+    t.load_s64(sp, j, shift, lane);
   }
-  for (int w = C4; w < 64; w <<= 1) {
-    ls += __shfl_xor(ls, w);
-    x.x += __shfl_xor(x.x, w);
-    x.y += __shfl_xor(x.y, w);
-    x.z += __shfl_xor(x.z, w);
-    x.w += __shfl_xor(x.w, w);
+  for (int i = lane; i < NC * 64; i += 64) reinterpret_cast<unsigned*>(image[wave])[i] = 0;
+  FewCols<HDP, NC> c;
+  {
+    const int ci = NC == 1 ? 0 : row >> 2, i = ci / a.group, qh = head * a.group + ci - i * a.group;
+    const T* qrow = static_cast<const T*>(a.q.p) + (long)seq * a.q.seq + (long)i * a.q.tok + (long)qh * a.q.head;
+    c.init(i < r.count ? qrow : nullptr, a.c.hd, a.qvec, lane, a.scale);
   }
-  if (lane < C4) so[wave][lane] = x;
-  if (lane == 0) sl[wave] = ls;
-  __syncthreads();
-  if (tid >= C4) return;
-  ls = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-  const float4 y0 = so[0][tid], y1 = so[1][tid], y2 = so[2][tid], y3 = so[3][tid];
-  const bool any = qi < r.count && visible(r, qi) > 0;
-  const float inv = 1.f / ls;
-  put4<T>(a, seq, qi, h, c4,
-          any ? make_float4(((y0.x + y1.x) + (y2.x + y3.x)) * inv, ((y0.y + y1.y) + (y2.y + y3.y)) * inv,
-                            ((y0.z + y1.z) + (y2.z + y3.z)) * inv, ((y0.w + y1.w) + (y2.w + y3.w)) * inv)
-              : make_float4(0.f, 0.f, 0.f, 0.f));
+  {
+    const int i = (NC == 1 ? 0 : group) / a.group;
+    c.lim = i < r.count ? visible(r, i) : 0;
+  }
+  for (; j < t1; j += NW) {
+    Tile<HDP> n;
+    const int nj = min(j + NW, tiles - 1);
+    n.load_k(kp, nj, lane);
+    n.load_v(vp, nj, lane);
+    n.load_s64(sp, nj, shift, lane);
+    few_step<HDP, NC>(c, t, j * kQTile, j * kQTile + kQTile > least, live, lane, image[wave]);
+    t = n;
+  }
+  float l = row16_sum_k(c.l);
+  if constexpr (NC == 1) l = xsum(l);
+  if (row == 0 && (NC > 1 || group == 0)) {
+    s.m[wave][NC == 1 ? 0 : group] = c.m;
+    s.l[wave][NC == 1 ? 0 : group] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < FewCols<HDP, NC>::NO; ++i) {
+    if constexpr (NC == 1) s.o[wave][0][i * 64 + group * 16 + row] = c.o[i];
+    else s.o[wave][group][i * 16 + row] = c.o[i];
+  }
+  finish<HDP, NC, NW, T>(a, s, r, seq, sh, head, 0, z, tiles, per);
 }
 
-constexpr int kParts = 768;  // (sequence, head, column block, split)s with partials
+// Workgroups of split keys: as many as the device holds at once, which the
+// registers decide (few columns: 106 and 174 of them, 16 columns: 144 and 218).
+template <int HDP>
+constexpr int parts(bool few) {
+  return few ? HDP == 64 ? 512 : 256 : HDP == 64 ? 768 : 512;
+}
+constexpr int kParts = 1024;
 
 template <int HDP, int ND, class T>
 void attend(hipStream_t s, AttnArgs& a) {
   const long heads = (long)a.c.n_seq * a.c.n_head;
-  if (heads * a.cblocks >= 2048) {
+  const int columns = a.n_q * a.group;
+  if (columns <= 4) a.cblocks = 1;
+  if (heads * a.cblocks >= 2048 && columns > 4) {
     const dim3 grid((unsigned)heads, (unsigned)((a.cblocks + 3) / 4));
     q_attend_cols_kernel<HDP, ND, T><<<grid, 256, 0, s>>>(a);
     return;
   }
-  const int most = (a.c.tiles + kMinTiles - 1) / kMinTiles;
-  a.splits = (int)std::max<long>(1, std::min<long>(most, kParts / (heads * a.cblocks)));
+  const int most = (a.c.tiles + 7) / 8;
+  a.splits = (int)std::max<long>(1, std::min<long>(most, parts<HDP>(columns <= 4) / (heads * a.cblocks)));
   const dim3 grid((unsigned)heads, (unsigned)a.cblocks, (unsigned)a.splits);
-  q_attend_split_kernel<HDP, ND, T><<<grid, 256, 0, s>>>(a);
-  if (a.splits > 1)
-    q_attend_join_kernel<HDP, T><<<dim3((unsigned)heads, (unsigned)(a.n_q * a.group)), 256, 0, s>>>(a);
+  if (columns == 1) q_attend_few_kernel<HDP, 1, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  else if (columns <= 4) q_attend_few_kernel<HDP, 4, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  else q_attend_split_kernel<HDP, ND, T><<<grid, 256, 0, s>>>(a);
 }
 
 template <int ND, class T>
@@ -563,7 +863,12 @@ void attend_t(hipStream_t s, AttnArgs& a) {
 
 }  // namespace
 
-size_t qattn_work_bytes(int hdp) { return (size_t)kParts * 16 * (hdp + 2) * 4; }
+// the partials, then the counters
+static size_t part_bytes(int hdp) { return (size_t)kParts * 16 * (hdp + 2) * 4; }
+size_t qattn_work_bytes(int hdp) { return part_bytes(hdp) + (size_t)kParts * kQTicketStride * 4; }
+void qattn_work_clear(hipStream_t s, void* work, int hdp) {
+  (void)hipMemsetAsync(static_cast<char*>(work) + part_bytes(hdp), 0, (size_t)kParts * kQTicketStride * 4, s);
+}
 
 void launch_q_attend(hipStream_t s, const QStore& c, QLen len, int extra, QType type, const QRows& q, int n_q,
                      int n_q_head, const int* counts, float scale, const QOut& out, void* work) {
@@ -581,6 +886,7 @@ void launch_q_attend(hipStream_t s, const QStore& c, QLen len, int extra, QType 
   a.out = out;
   a.cblocks = (int)(((long)n_q * a.group + 15) / 16);
   a.part = static_cast<float*>(work);
+  a.joined = reinterpret_cast<unsigned*>(static_cast<char*>(work) + part_bytes(c.hdp));
   a.splits = 1;
   if (type == Q_F32) attend_t<3, float>(s, a);
   else if (type == Q_BF16) attend_t<2, __bf16>(s, a);

@@ -113,9 +113,10 @@ struct QOut {
 // over the cache: query i sits at position len - count + i and sees the keys up
 // to its own position. extra is added to the lengths. scale: of the dot products.
 // Rows of queries that see no key, and of i >= count, are set to 0.
-// work: qattn_work_bytes() bytes.
+// work: qattn_work_bytes() bytes, cleared once (qattn_work_clear).
 void launch_q_attend(hipStream_t s, const QStore& c, QLen len, int extra, QType type, const QRows& q, int n_q,
                      int n_q_head, const int* counts, float scale, const QOut& out, void* work);
 size_t qattn_work_bytes(int hdp);
+void qattn_work_clear(hipStream_t s, void* work, int hdp);
 
 }  // namespace rtg

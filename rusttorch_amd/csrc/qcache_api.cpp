@@ -130,6 +130,7 @@ rtg_result rtg_qcache_new(size_t n_seq, size_t n_head, size_t head_dim, size_t c
     q->work = static_cast<char*>(q->mem) + head + store;
     e = hipMemset(q->mem, 0, head);
     if (e == hipSuccess) e = hipMemset(q->err, 0xFF, 4);
+    qattn_work_clear(nullptr, q->work, q->c.hdp);
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) return hip_err(e, "rtg_qcache_new");
     *out = q.release();

@@ -450,6 +450,7 @@ static rtg_cache* cache_create(const rtg_model* m, size_t batch, size_t block = 
       HIPX(device_malloc(&c->q_work, qattn_work_bytes(c->q.hdp)));
       HIPX(device_malloc(&c->q_int, 256));
       HIPX(hipMemsetAsync(c->q_int, 0, 256, c->stream));
+      qattn_work_clear(c->stream, c->q_work, c->q.hdp);
     } else {
       HIPX(device_malloc(&c->k, std::max<size_t>(L * c->layer_stride, 1) * 4));
       HIPX(device_malloc(&c->v, std::max<size_t>(L * c->layer_stride, 1) * 4));
