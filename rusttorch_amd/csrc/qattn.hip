@@ -142,6 +142,11 @@ struct Cols {
   }
 };
 
+// The scales (keys', values') of block lane % nb of those that begin at a tile.
+__device__ __forceinline__ float2 block_scale(const float* sp, int tile, int nb, int shift, int lane) {
+  return reinterpret_cast<const float2*>(sp)[(tile << (6 - shift)) + (lane & (nb - 1))];
+}
+
 // A tile of keys and values in registers.
 template <int HDP>
 struct Tile {
@@ -150,7 +155,7 @@ struct Tile {
   float2 s;  // lane i: the scales (keys', values') of the tile's block i, over and over
   // sp: the (sequence, head)'s scales
   __device__ __forceinline__ void load_s(const float* sp, int tile, int shift, int lane) {
-    s = reinterpret_cast<const float2*>(sp)[(tile << (6 - shift)) + (lane & ((1 << (6 - shift)) - 1))];
+    s = block_scale(sp, tile, kQTile >> shift, shift, lane);
   }
   // the same for lane i: the scales of the tile's key i
   __device__ __forceinline__ void load_s64(const float* sp, int tile, int shift, int lane) {
@@ -193,30 +198,34 @@ __device__ __forceinline__ constexpr float p_one() {
 }
 constexpr float kLargeScore = 2097152.f;  // 2^21
 
-// A tile's scales for a wave: of each 16 keys f (scores) and r = max(v scale /
-// vmax, 2^-60) as lr = log2 r and 1 / r. (A block of zeros may take any r.)
+// The scales of NG * 16 keys (one tile, or two) for a wave: of each 16 f (scores)
+// and r = max(v scale / vmax, 2^-60) as lr = log2 r and 1 / r. (A block of zeros
+// may take any r.)
+template <int NG>
 struct TileScales {
-  float f[4], lr[4], rinv[4], vmax;
+  float f[NG], lr[NG], rinv[NG], vmax;
   unsigned bad;  // bit i: the values of the i-th 16 keys read back as NaN
   __device__ __forceinline__ bool nan(int i) const { return bad >> i & 1; }
 };
-// sl: a lane's (keys', values') scales, those of the tile's blocks on lanes 0 ..
-// and over and over; live: keys of the tile that are in the cache (or more).
-__device__ __forceinline__ TileScales tile_scales(float2 sl, int shift, int live, int lane) {
-  TileScales t;
-  const int nb = 64 >> shift;
+// sl: a lane's (keys', values') scales, those of the keys' blocks on lanes 0 ..
+// and over and over; live: keys of these that are in the cache (or more).
+template <int NG>
+__device__ __forceinline__ TileScales<NG> tile_scales(float2 sl, int shift, int live, int lane) {
+  TileScales<NG> t;
+  const int nb = (NG * 16) >> shift;
   const bool in = ((lane & (nb - 1)) << shift) < live;  // blocks behind the last key are not read as numbers
   const float k = in ? sl.x : 0.f, v = in ? sl.y : 0.f;
   const unsigned nans = (unsigned)__builtin_amdgcn_ballot_w64(v != v);
   t.bad = 0;
   float m = fmaxf(v, dpp_row<0xB1>(v));  // (fmaxf skips NaN)
   m = fmaxf(m, dpp_row<0x4E>(m));
+  if (NG == 8) m = fmaxf(m, dpp_row<0x124>(m));
   t.vmax = m;
   // (r to the last place: it is the same for a block's every key)
   const float r = m > 0.f ? fmaxf(v * __builtin_amdgcn_rcpf(m), 8.6736174e-19f) : 1.f;
   const float lr = __builtin_amdgcn_logf(r), ri = __builtin_amdgcn_rcpf(r);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NG; ++i) {
     const int b = (i * 16) >> shift;
     t.f[i] = lane_of(k, b);
     t.lr[i] = lane_of(lr, b);
@@ -226,48 +235,63 @@ __device__ __forceinline__ TileScales tile_scales(float2 sl, int shift, int live
   return t;
 }
 
-// One tile (keys j0 .. j0 + 63) for a wave's columns. EDGE: some column does not
-// see all of its keys. The running maximum is of score + lr, that is of the
-// probability times the value's scale, so that a tile's largest such product is
-// 1 and needs no second reduction; each probability itself is 1 / r of it.
-template <bool EDGE, int HDP, int ND>
-__device__ __forceinline__ void tile_step(Cols<HDP, ND>& c, const Tile<HDP>& t, const TileScales& ts, int j0, int group) {
+// A tile's keys (NG = 4), or two tiles' (8), for a wave's columns. EDGE: some
+// column does not see all of them. The running maximum is of score + lr, that is
+// of the probability times the value's scale, so that the largest such product
+// here is 1 and needs no second reduction; each probability itself is 1 / r of it.
+
+// k: 16 keys; s[4]: a lane's fixed-point sums of them, most: the largest.
+template <int HDP, int ND>
+__device__ __forceinline__ void tile_sums(const Cols<HDP, ND>& c, const i32x4 (&k)[HDP / 64], float (&s)[4],
+                                          float& most) {
+  const i32x4 d = fixed_mfma<ND, HDP / 64>(k, c.q);
+  most = (float)max(max(d[0], d[1]), max(d[2], d[3]));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s[e] = (float)d[e];
+}
+
+// s, most: the keys' fixed-point sums. pd: the probabilities' digits, w: what
+// their products with the values' codes are to be multiplied with.
+template <bool EDGE, int HDP, int ND, int NG>
+__device__ __forceinline__ void tile_probs(Cols<HDP, ND>& c, float (&s)[NG][4], const float (&most)[NG],
+                                           const TileScales<NG>& ts, int j0, int group, i32x4 (&pd)[NG / 4][ND],
+                                           float& w) {
   constexpr int DT = HDP / 16;
-  float s[4][4], f[4];
+  float f[NG];
   float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const i32x4 d = fixed_mfma<ND, Cols<HDP, ND>::KS>(t.k[i], c.q);
+  for (int i = 0; i < NG; ++i) {
     f[i] = c.sq * ts.f[i];
+    if (EDGE) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s[i][e] = (float)d[e];
-      if (EDGE) s[i][e] = j0 + i * 16 + group * 4 + e < c.lim ? fmaf(s[i][e], f[i], ts.lr[i]) : -INFINITY;
+      for (int e = 0; e < 4; ++e) {
+        s[i][e] = j0 + i * 16 + group * 4 + e < c.lim ? fmaf(s[i][e], f[i], ts.lr[i]) : -INFINITY;
+        top = fmaxf(top, s[i][e]);
+      }
+    } else {
+      top = fmaxf(top, fmaf(most[i], f[i], ts.lr[i]));  // (f >= 0)
     }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float m = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
-    top = fmaxf(top, EDGE ? m : fmaf(m, f[i], ts.lr[i]));  // (f >= 0)
   }
   top = xmax(top);
   const float base = top == -INFINITY ? 0.f : top;  // (no key here: every p is 2^-inf = 0)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NG; ++i) {
     const float cc = ts.lr[i] - base;
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[i][e] = EDGE ? s[i][e] - base : fmaf(s[i][e], f[i], cc);
   }
   if (!EDGE && __builtin_amdgcn_ballot_w64(fabsf(top) > kLargeScore)) {
-    asm volatile("");  // (a branch: hardly ever taken)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NG; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] = s[i][e] > 0.f ? 0.f : s[i][e];
+      for (int e = 0; e < 4; ++e) {
+        asm volatile("" : "+v"(s[i][e]));  // (stays behind the branch, which is hardly ever taken)
+        s[i][e] = s[i][e] > 0.f ? 0.f : s[i][e];
+      }
   }
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NG; ++i) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[i][e] = __builtin_amdgcn_exp2f(s[i][e]);
     sum = fmaf((s[i][0] + s[i][1]) + (s[i][2] + s[i][3]), ts.rinv[i], sum);
@@ -276,7 +300,7 @@ __device__ __forceinline__ void tile_step(Cols<HDP, ND>& c, const Tile<HDP>& t, 
     asm volatile("");
     // every column that sees a key of such a block is NaN
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NG; ++i)
       if (ts.nan(i) && j0 + i * 16 + group * 4 < c.lim) sum = NAN;
   }
   const float mn = fmaxf(c.m, top), mb = mn == -INFINITY ? 0.f : mn;
@@ -289,26 +313,26 @@ __device__ __forceinline__ void tile_step(Cols<HDP, ND>& c, const Tile<HDP>& t, 
       for (int i = 0; i < 4; ++i) c.o[d][i] *= corr;
   }
   c.m = mn;
-  const float w = g * ts.vmax * ((ND == 3 ? 256.f : 1.f) / p_one<ND>());
+  w = g * ts.vmax * ((ND == 3 ? 256.f : 1.f) / p_one<ND>());
   // rounded to an integer and biased, in the low bits of the sum with 2^23
   constexpr float magic = ND == 3 ? 8421504.f : 8388608.f + 32896.f;  // 2^23 + 0x8080
-  i32x4 pd[1][ND];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NG; ++i) {
     unsigned u[4], d[ND];
 #pragma unroll
     for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(fmaf(s[i][e], p_one<ND>(), magic));
     planes<ND>(u[0], u[1], u[2], u[3], d);
 #pragma unroll
-    for (int n = 0; n < ND; ++n) pd[0][n][i] = (int)d[n];
+    for (int n = 0; n < ND; ++n) pd[i / 4][n][i & 3] = (int)d[n];
   }
+}
+
+// v: 16 columns of the tiles' values; o[4]: the results of them.
+template <int ND, int NT>
+__device__ __forceinline__ void tile_product(const i32x4 (&v)[NT], const i32x4 (&pd)[NT][ND], float w, float (&o)[4]) {
+  const i32x4 r = fixed_mfma<ND, NT>(v, pd);
 #pragma unroll
-  for (int d = 0; d < DT; ++d) {
-    const i32x4 va[1] = {t.v[d]};
-    const i32x4 r = fixed_mfma<ND, 1>(va, pd);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c.o[d][i] = fmaf((float)r[i], w, c.o[d][i]);
-  }
+  for (int i = 0; i < 4; ++i) o[i] = fmaf((float)r[i], w, o[i]);
 }
 
 struct AttnArgs {
@@ -340,87 +364,179 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs& a, int seq) {
 // Keys that query i sees.
 __device__ __forceinline__ int visible(const Seq& r, int i) { return max(r.len - r.count + i + 1, 0); }
 
-// Four neighbouring results of (sequence, query i, head): columns c4 .. c4 + 3.
-template <class T>
-__device__ __forceinline__ void put4(const AttnArgs& a, int seq, int i, int head, int c4, const float4& x) {
-  const int hd = a.c.hd;
-  if (a.out.kind == QO_ROWS) {
-    T* p = static_cast<T*>(a.out.rows.p) + (long)seq * a.out.rows.seq + (long)i * a.out.rows.tok + (long)head * a.out.rows.head;
-    store4(p, c4, hd, x, a.ovec);
-  } else if (c4 < hd) {
-    const int col = head * hd + c4, d = a.n_q_head * hd;
-    const float xe[4] = {x.x, x.y, x.z, x.w};
-    if (a.out.kind == QO_PAIR) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (c4 + e >= hd) continue;
-        // (the scale brings the bound of the unrounded values to 2^15 at most;
-        // rounded to 8 bits they are below twice that, which f16 just misses)
-        float y = xe[e] * a.out.scale[col + e];
-        if (fabsf(y) > 65504.f && fabsf(y) <= 65536.f) y = copysignf(65504.f, y);
-        unsigned h, l;
-        f16_split(y, &h, &l);
-        uint16_t* p = a.out.pair + pair_index((size_t)seq * a.n_q + i, col + e, d);
-        p[0] = (uint16_t)h;
-        p[32] = (uint16_t)l;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c4 + e < hd) a.out.xt[xt_index(seq, col + e, a.c.n_seq, a.out.tk)] = xe[e];
+// Where the results of (sequence, query i, head) go.
+template <class T, int KIND>
+struct RowOut {
+  T* p;
+  uint16_t* pair;
+  const float* scale;
+  int col0, seq;
+  __device__ __forceinline__ RowOut(const AttnArgs& a, int seq_, int i, int head) {
+    seq = seq_;
+    col0 = head * a.c.hd;
+    if constexpr (KIND == QO_ROWS) {
+      p = static_cast<T*>(a.out.rows.p) + (long)seq * a.out.rows.seq + (long)i * a.out.rows.tok + (long)head * a.out.rows.head;
+    } else if constexpr (KIND == QO_PAIR) {
+      pair = a.out.pair + pair_index((size_t)seq * a.n_q + i, 0, a.n_q_head * a.c.hd);
+      scale = a.out.scale + col0;
     }
   }
-}
+  // columns c4 .. c4 + 3
+  __device__ __forceinline__ void put(const AttnArgs& a, int c4, const float4& x) const {
+    if constexpr (KIND == QO_ROWS) {
+      store4(p, c4, a.c.hd, x, a.ovec);
+    } else {
+      const float xe[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (c4 + e >= a.c.hd) continue;
+        if constexpr (KIND == QO_PAIR) {
+          // (the scale brings the bound of the unrounded values to 2^15 at most;
+          // rounded to 8 bits they are below twice that, which f16 just misses)
+          float y = xe[e] * scale[c4 + e];
+          if (fabsf(y) > 65504.f && fabsf(y) <= 65536.f) y = copysignf(65504.f, y);
+          unsigned h, l;
+          f16_split(y, &h, &l);
+          uint16_t* q = pair + pair_index(0, col0 + c4 + e, 0);
+          q[0] = (uint16_t)h;
+          q[32] = (uint16_t)l;
+        } else {
+          a.out.xt[xt_index(seq, col0 + c4 + e, a.c.n_seq, a.out.tk)] = xe[e];
+        }
+      }
+    }
+  }
+};
 
 // ---- many columns: every wave has 16 of its own and takes all of their keys ----
-template <int HDP, int ND, class T>
+//
+// Two tiles at a time: 128 keys share the maximum, the scales and the conversion
+// of their products with the values (a third of the vector work, which bounds
+// this kernel: about 265 instructions per 64 keys and 16 columns). A workgroup's
+// four waves read them from LDS. The next two tiles' keys are stored there once
+// every wave has this pair's sums, the values once every wave has its products;
+// both come from registers that were loaded half a pair to a pair earlier.
+constexpr int kPair = 2 * kQTile;
+
+template <int HDP>
+struct SharedPair {
+  static constexpr int CH = HDP / 16, U = kPair * CH / 256;  // 16-byte chunks per row; units per thread
+  // Rows of keys lie in chunks xor'ed with the row, so that the 16 rows of a
+  // matrix operand fall on all 64 banks; values lie as in memory.
+  static __device__ __forceinline__ int k_at(int row, int chunk) {
+    return row * CH + (chunk ^ (HDP == 64 ? (row >> 2) & 3 : (row >> 1) & 7));
+  }
+  i32x4 k[kPair * CH], v[kPair * CH];
+};
+
+template <int HDP, int ND, int KIND, class T>
 __global__ __launch_bounds__(256) void q_attend_cols_kernel(AttnArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
+  using Pair = SharedPair<HDP>;
+  constexpr int U = Pair::U, CH = Pair::CH, KS = HDP / 64;
+  __shared__ Pair t;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, group = lane >> 4;
   const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head;
-  const int cb = (a.cblocks - 1 - (int)blockIdx.y * 4) - wave;  // the longest first
-  if (cb < 0) return;
+  const int cb0 = a.cblocks - 1 - (int)blockIdx.y * 4, cb = cb0 - wave;  // the longest first
   const Seq r = seq_of(a, seq);
-  const int ci = cb * 16 + col, i = ci / a.group, qh = head * a.group + ci - i * a.group;
-  const bool mine = i < a.n_q, used = i < r.count;
-  const int last = min((cb * 16 + 15) / a.group, r.count - 1);  // the wave's last query
-  const int firstq = cb * 16 / a.group;
-  if (firstq >= a.n_q) return;
-  Cols<HDP, ND> c;
-  const T* qrow = static_cast<const T*>(a.q.p) + (long)seq * a.q.seq + (long)i * a.q.tok + (long)qh * a.q.head;
-  c.init(used ? qrow : nullptr, a.c.hd, a.qvec, group, a.scale, used ? visible(r, i) : 0);
-  const int live = firstq < r.count ? visible(r, last) : 0;
-  const int least = firstq < r.count ? visible(r, firstq) : 0;
-  const int tiles = (live + kQTile - 1) / kQTile;
-  const int8_t *kp = a.c.k + a.c.codes(sh), *vp = a.c.v + a.c.codes(sh);
+  // keys that the columns of block b see: at least, at most
+  auto least_of = [&](int b) { return b >= 0 && b * 16 / a.group < r.count ? visible(r, b * 16 / a.group) : 0; };
+  auto live_of = [&](int b) {
+    return b >= 0 && b * 16 / a.group < r.count ? visible(r, min((b * 16 + 15) / a.group, r.count - 1)) : 0;
+  };
+  const int live = live_of(cb), least = least_of(cb), mine = (live + kPair - 1) / kPair;
+  int most_live = 0;  // (the later blocks of columns may be padding)
+  for (int w = 0; w < 4; ++w) most_live = max(most_live, live_of(cb0 - w));
+  const int pairs = (most_live + kPair - 1) / kPair;
+  const i32x4* kp = reinterpret_cast<const i32x4*>(a.c.k + a.c.codes(sh));
+  const i32x4* vp = reinterpret_cast<const i32x4*>(a.c.v + a.c.codes(sh));
   const float* sp = a.c.s + a.c.scales(sh);
   const int shift = a.c.block_shift;
-  Tile<HDP> t;
-  if (tiles) {
-    t.load_s(sp, 0, shift, lane);
-    t.load_k(kp, 0, lane);
+  const int end = a.c.tiles * kQTile * CH;  // 16-byte units of the (sequence, head): a pair's second tile may lie behind it
+  i32x4 kr[U], vr[U];
+  auto load = [&](const i32x4* p, int j, i32x4 (&x)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = p[min(j * kPair * CH + u * 256 + tid, end - 1)];
+  };
+  auto store_k = [&]() {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int x = u * 256 + tid;
+      t.k[Pair::k_at(x / CH, x % CH)] = kr[u];
+    }
+  };
+  auto store_v = [&]() {
+#pragma unroll
+    for (int u = 0; u < U; ++u) t.v[u * 256 + tid] = vr[u];
+  };
+  // (blocks of a second tile behind the capacity are those of the last one: no key of theirs is seen)
+  const int nb = kPair >> shift;
+  auto load_s = [&](int j) {
+    const int b = (j * kPair >> shift) + (lane & (nb - 1)), last = (a.c.tiles * kQTile >> shift) - 1;
+    return reinterpret_cast<const float2*>(sp)[min(b, last)];
+  };
+  float2 sl = make_float2(0.f, 0.f);
+  if (pairs) {
+    load(kp, 0, kr);
+    load(vp, 0, vr);
+    sl = load_s(0);
   }
-  for (int j = 0; j < tiles; ++j) {
-    t.load_v(vp, j, lane);
-    Tile<HDP> n;
-    n.load_s(sp, min(j + 1, tiles - 1), shift, lane);
-    n.load_k(kp, min(j + 1, tiles - 1), lane);
-    const TileScales ts = tile_scales(t.s, shift, live - j * kQTile, lane);
-    if (j * kQTile + kQTile > least) tile_step<true>(c, t, ts, j * kQTile, group);
-    else tile_step<false>(c, t, ts, j * kQTile, group);
+  Cols<HDP, ND> c;
+  const int ci = cb * 16 + col, i = ci / a.group, qh = head * a.group + ci - i * a.group;
+  {
+    const T* qrow = static_cast<const T*>(a.q.p) + (long)seq * a.q.seq + (long)i * a.q.tok + (long)qh * a.q.head;
+    const bool used = cb >= 0 && i < r.count;
+    c.init(used ? qrow : nullptr, a.c.hd, a.qvec, group, a.scale, used ? visible(r, i) : 0);
+  }
+  if (pairs) {
+    store_k();
+    store_v();
+    if (pairs > 1) load(kp, 1, kr);
+  }
+  __syncthreads();
+  for (int j = 0; j < pairs; ++j) {
+    const bool more = j + 1 < pairs;
+    const TileScales<8> ts = tile_scales<8>(sl, shift, live - j * kPair, lane);
+    if (more) {
+      load(vp, j + 1, vr);
+      sl = load_s(j + 1);
+    }
+    float s[8][4], most[8], w;
+    if (j < mine) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
+      for (int n = 0; n < 8; ++n) {
+        i32x4 k[KS];
 #pragma unroll
-      for (int y = 0; y < Cols<HDP, ND>::KS; ++y) t.k[x][y] = n.k[x][y];
-    t.s = n.s;
+        for (int e = 0; e < KS; ++e) k[e] = t.k[Pair::k_at(n * 16 + col, e * 4 + group)];
+        tile_sums<HDP, ND>(c, k, s[n], most[n]);
+      }
+    }
+    __syncthreads();  // the keys are read; the values of this pair are there
+    if (more) {
+      store_k();
+      if (j + 2 < pairs) load(kp, j + 2, kr);
+    }
+    if (j < mine) {
+      i32x4 pd[2][ND];
+      if (j * kPair + kPair > least) tile_probs<true>(c, s, most, ts, j * kPair, group, pd, w);
+      else tile_probs<false>(c, s, most, ts, j * kPair, group, pd, w);
+#pragma unroll
+      for (int d = 0; d < HDP / 16; ++d) {
+        const i32x4 v[2] = {t.v[group * HDP + d * 16 + col], t.v[(4 + group) * HDP + d * 16 + col]};
+        tile_product<ND, 2>(v, pd, w, c.o[d]);
+      }
+    }
+    __syncthreads();  // the values are read; the next pair's keys are there
+    if (more) store_v();
   }
   const float l = xsum(c.l);
-  if (!mine) return;
+  if (cb < 0 || i >= a.n_q) return;
   const float inv = c.lim > 0 ? 1.f / l : 0.f;
+  const RowOut<T, KIND> out(a, seq, i, qh);
 #pragma unroll
   for (int d = 0; d < HDP / 16; ++d) {
-    const float4 x = c.lim > 0 ? make_float4(c.o[d][0] * inv, c.o[d][1] * inv, c.o[d][2] * inv, c.o[d][3] * inv)
-                               : make_float4(0.f, 0.f, 0.f, 0.f);
-    put4<T>(a, seq, i, qh, d * 16 + group * 4, x);
+    const float* o = c.o[d];
+    out.put(a, d * 16 + group * 4,
+            c.lim > 0 ? make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
   }
 }
 
@@ -464,7 +580,7 @@ __device__ __forceinline__ float2 load2(const float* p) {
 // Joins the waves' results in s (written, not yet synchronised) for the W
 // columns of block cb: to the results where the keys were not split, else to the
 // partials; the last of a block's workgroups to come here joins those.
-template <int HDP, int W, int NW, class T>
+template <int HDP, int W, int NW, int KIND, class T>
 __device__ __forceinline__ void finish(const AttnArgs& a, Merge<HDP, W, NW>& s, const Seq& r, int seq, int sh, int head,
                                        int cb, int z, int tiles, int per) {
   constexpr int C4 = HDP / 4, NT = 64 * NW, CPP = NT / C4;
@@ -474,8 +590,8 @@ __device__ __forceinline__ void finish(const AttnArgs& a, Merge<HDP, W, NW>& s, 
     const int ci = cb * W + col, i = ci / a.group, h = head * a.group + ci - i * a.group;
     const bool any = i < r.count && visible(r, i) > 0;
     const float inv = 1.f / l;
-    put4<T>(a, seq, i, h, c4,
-            any ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
+    RowOut<T, KIND>(a, seq, i, h).put(
+        a, c4, any ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
   };
   const int cols = min(W, a.n_q * a.group - cb * W);
   __syncthreads();
@@ -558,7 +674,7 @@ __device__ __forceinline__ void finish(const AttnArgs& a, Merge<HDP, W, NW>& s, 
   }
 }
 
-template <int HDP, int ND, class T>
+template <int HDP, int ND, int KIND, class T>
 __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
   constexpr int NW = 4;
   __shared__ Merge<HDP, 16, NW> s;
@@ -593,9 +709,19 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
     n.load_s(sp, nj, shift, lane);
     n.load_k(kp, nj, lane);
     n.load_v(vp, nj, lane);
-    const TileScales ts = tile_scales(t.s, shift, live - j * kQTile, lane);
-    if (j * kQTile + kQTile > least) tile_step<true>(c, t, ts, j * kQTile, group);
-    else tile_step<false>(c, t, ts, j * kQTile, group);
+    const TileScales<4> ts = tile_scales<4>(t.s, shift, live - j * kQTile, lane);
+    float sums[4][4], most[4];
+    i32x4 pd[1][ND];
+    float w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tile_sums<HDP, ND>(c, t.k[i], sums[i], most[i]);
+    if (j * kQTile + kQTile > least) tile_probs<true>(c, sums, most, ts, j * kQTile, group, pd, w);
+    else tile_probs<false>(c, sums, most, ts, j * kQTile, group, pd, w);
+#pragma unroll
+    for (int d = 0; d < HDP / 16; ++d) {
+      const i32x4 v[1] = {t.v[d]};
+      tile_product<ND, 1>(v, pd, w, c.o[d]);
+    }
     t = n;
   }
   const float l = xsum(c.l);
@@ -606,7 +732,7 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
 #pragma unroll
   for (int d = 0; d < HDP / 16; ++d)
     *reinterpret_cast<float4*>(&s.o[wave][col][d * 16 + group * 4]) = make_float4(c.o[d][0], c.o[d][1], c.o[d][2], c.o[d][3]);
-  finish<HDP, 16, NW, T>(a, s, r, seq, sh, head, cb, z, tiles, per);
+  finish<HDP, 16, NW, KIND, T>(a, s, r, seq, sh, head, cb, z, tiles, per);
 }
 
 // ---- up to four columns: one new token of a head, or of four that share their keys ----
@@ -766,7 +892,7 @@ __device__ __forceinline__ void few_step(FewCols<HDP, NC>& c, const Tile<HDP>& t
 
 constexpr int kFewWaves = 8;
 
-template <int HDP, int NC, class T>
+template <int HDP, int NC, int KIND, class T>
 __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a) {
   constexpr int NW = kFewWaves;
   __shared__ Merge<HDP, NC, NW> s;
@@ -819,7 +945,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a
     if constexpr (NC == 1) s.o[wave][0][i * 64 + group * 16 + row] = c.o[i];
     else s.o[wave][group][i * 16 + row] = c.o[i];
   }
-  finish<HDP, NC, NW, T>(a, s, r, seq, sh, head, 0, z, tiles, per);
+  finish<HDP, NC, NW, KIND, T>(a, s, r, seq, sh, head, 0, z, tiles, per);
 }
 
 // Workgroups of split keys: as many as the device holds at once, which the
@@ -830,22 +956,24 @@ constexpr int parts(bool few) {
 }
 constexpr int kParts = 1024;
 
-template <int HDP, int ND, class T>
+template <int HDP, int ND, int KIND, class T>
 void attend(hipStream_t s, AttnArgs& a) {
   const long heads = (long)a.c.n_seq * a.c.n_head;
   const int columns = a.n_q * a.group;
   if (columns <= 4) a.cblocks = 1;
-  if (heads * a.cblocks >= 2048 && columns > 4) {
-    const dim3 grid((unsigned)heads, (unsigned)((a.cblocks + 3) / 4));
-    q_attend_cols_kernel<HDP, ND, T><<<grid, 256, 0, s>>>(a);
-    return;
-  }
   const int most = (a.c.tiles + 7) / 8;
   a.splits = (int)std::max<long>(1, std::min<long>(most, parts<HDP>(columns <= 4) / (heads * a.cblocks)));
   const dim3 grid((unsigned)heads, (unsigned)a.cblocks, (unsigned)a.splits);
-  if (columns == 1) q_attend_few_kernel<HDP, 1, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
-  else if (columns <= 4) q_attend_few_kernel<HDP, 4, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
-  else q_attend_split_kernel<HDP, ND, T><<<grid, 256, 0, s>>>(a);
+  if (columns == 1) {
+    q_attend_few_kernel<HDP, 1, KIND, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  } else if constexpr (KIND != QO_XT) {
+    if (heads * a.cblocks >= 2048 && columns > 4)
+      q_attend_cols_kernel<HDP, ND, KIND, T><<<dim3((unsigned)heads, (unsigned)((a.cblocks + 3) / 4)), 256, 0, s>>>(a);
+    else if (columns <= 4)
+      q_attend_few_kernel<HDP, 4, KIND, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
+    else
+      q_attend_split_kernel<HDP, ND, KIND, T><<<grid, 256, 0, s>>>(a);
+  }
 }
 
 template <int ND, class T>
@@ -857,8 +985,13 @@ void attend_t(hipStream_t s, AttnArgs& a) {
   };
   a.qvec = vec(a.q);
   a.ovec = a.out.kind == QO_ROWS && vec(a.out.rows);
-  if (a.c.hdp == 64) attend<64, ND, T>(s, a);
-  else attend<128, ND, T>(s, a);
+  if constexpr (sizeof(T) == 4) {
+    // (the model's layouts; a step's has one query per sequence and head)
+    if (a.out.kind == QO_PAIR) return attend<64, ND, QO_PAIR, T>(s, a);
+    if (a.out.kind == QO_XT) return attend<64, ND, QO_XT, T>(s, a);
+  }
+  if (a.c.hdp == 64) attend<64, ND, QO_ROWS, T>(s, a);
+  else attend<128, ND, QO_ROWS, T>(s, a);
 }
 
 }  // namespace

@@ -98,7 +98,8 @@ void launch_q_read(hipStream_t s, const QStore& c, QLen len, QType type, const Q
 
 // Attention results: rows (QRows), or the layouts of the model's next GEMM:
 // the pair GEMM's input scaled per column, or the batched decode GEMV's
-// (xt_index with n_seq rows).
+// (xt_index with n_seq rows; one query of as many heads as the cache has). Both
+// for f32 queries and head dims up to 64.
 enum QOutKind { QO_ROWS = 0, QO_PAIR = 1, QO_XT = 2 };
 struct QOut {
   QOutKind kind = QO_ROWS;
