@@ -189,14 +189,11 @@ __device__ __forceinline__ float row_max(float v) {
 __device__ __forceinline__ float xmax(float v) { return xor32_max_k(xor16_max_k(v)); }
 __device__ __forceinline__ float xsum(float v) { return xor32_sum_k(xor16_sum_k(v)); }
 
-// Fixed-point probabilities: at most 2^22 (2^14 for two digits) for the tile's
-// largest, of twice that which the digits hold: its exponent is 0 up to rounding,
-// which stays below 1 for scores up to kLargeScore.
-template <int ND>
-__device__ __forceinline__ constexpr float p_one() {
-  return ND == 3 ? 4150000.f : 16200.f;
-}
-constexpr float kLargeScore = 2097152.f;  // 2^21
+// Scores (in units of log2 e) up to which rounding cannot take the tile's largest
+// probability further above 1 than fixed_max leaves room for; beyond, the
+// exponents are clamped. (A tile's fixed-point probabilities with a bit less
+// doubled the error of f32 results: 8.7e-7 against 4.7e-7 of 64 bits.)
+constexpr float kLargeScore = 256.f;
 
 // The scales of NG * 16 keys (one tile, or two) for a wave: of each 16 f (scores)
 // and r = max(v scale / vmax, 2^-60) as lr = log2 r and 1 / r. (A block of zeros
@@ -313,14 +310,14 @@ __device__ __forceinline__ void tile_probs(Cols<HDP, ND>& c, float (&s)[NG][4], 
       for (int i = 0; i < 4; ++i) c.o[d][i] *= corr;
   }
   c.m = mn;
-  w = g * ts.vmax * ((ND == 3 ? 256.f : 1.f) / p_one<ND>());
+  w = g * ts.vmax * ((ND == 3 ? 256.f : 1.f) / fixed_max<ND>());
   // rounded to an integer and biased, in the low bits of the sum with 2^23
   constexpr float magic = ND == 3 ? 8421504.f : 8388608.f + 32896.f;  // 2^23 + 0x8080
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     unsigned u[4], d[ND];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(fmaf(s[i][e], p_one<ND>(), magic));
+    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(fmaf(s[i][e], fixed_max<ND>(), magic));
     planes<ND>(u[0], u[1], u[2], u[3], d);
 #pragma unroll
     for (int n = 0; n < ND; ++n) pd[i / 4][n][i & 3] = (int)d[n];

@@ -186,6 +186,12 @@ __device__ __forceinline__ bool in_tail(const QStore& c, const Place& p) {
   return p.len > 0 && p.at >> c.block_shift == (p.len - 1) >> c.block_shift;
 }
 
+// Whether the append needs the tail that is there: it goes on in the middle of
+// the block that the tail holds.
+__device__ __forceinline__ bool reads_tail(const QStore& c, const Place& p) {
+  return (p.at & (c.block - 1)) != 0 && in_tail(c, p);
+}
+
 // A value of a full block as it reads back, and its token's own scale: a token
 // that holds code 127 had the block's scale (amax / 127 may round otherwise).
 __device__ __forceinline__ float code_value(int8_t code, float s) { return (float)code * s; }
@@ -193,23 +199,39 @@ __device__ __forceinline__ unsigned read_back_scale(float amax, float s) {
   return amax == 127.f * s ? __float_as_uint(s) : token_scale(amax);
 }
 
-// The tail of an append whose last block starts behind its first tile: written
-// by the first tile's workgroup, which has read the old tail by then.
+// q[i]: byte i of x[0] .. x[3] (and the other way round).
+__device__ __forceinline__ void transpose4(const unsigned (&x)[4], unsigned (&q)[4]) {
+  const unsigned a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400), b = __builtin_amdgcn_perm(x[3], x[2], 0x05010400);
+  const unsigned c = __builtin_amdgcn_perm(x[1], x[0], 0x07030602), d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602);
+  q[0] = __builtin_amdgcn_perm(b, a, 0x05040100);
+  q[1] = __builtin_amdgcn_perm(b, a, 0x07060302);
+  q[2] = __builtin_amdgcn_perm(d, c, 0x05040100);
+  q[3] = __builtin_amdgcn_perm(d, c, 0x07060302);
+}
+
+// The tail of an append that reads the old one and whose last block starts behind
+// its first tile: written by the first tile's workgroup, which has read the old
+// tail by then.
 template <int HDP, class T>
 __device__ void append_tail(const QStore& c, const Place& p, size_t sh, int which, const T* src, long tok_stride,
                             bool vec) {
-  constexpr int LPR = HDP / 4, TPP = 256 / LPR;
+  constexpr int LPR = HDP / 4, TPP = 256 / LPR, ROWS = 64 / TPP;
   const int c4 = (threadIdx.x % LPR) * 4, trow = threadIdx.x / LPR;
   const int last = (p.end - 1) & ~(c.block - 1);
   float* tail = c.tail + c.tails(sh, which);
   float* tail_s = c.tail_s + c.tail_scales(sh, which);
-  for (int t0 = 0; t0 < c.block; t0 += TPP) {  // (whole rows of lanes for row_max_bits)
-    const int t = t0 + trow;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (last + t < p.end) x = load4(src + (long)(last + t - p.at) * tok_stride, c4, c.hd, vec);
-    const float amax = __uint_as_float(row_max_bits<HDP>(max_abs4(x)));
-    if (last + t < p.end) {
-      *reinterpret_cast<float4*>(tail + (size_t)t * HDP + c4) = x;
+  float4 x[ROWS];
+  // (all rows in flight, those behind the end as the last one: one after the
+  // other they took most of a short append's time, 18.9 us against 10)
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i)
+    x[i] = load4(src + (long)(min(last + i * TPP + trow, p.end - 1) - p.at) * tok_stride, c4, c.hd, vec);
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int t = i * TPP + trow;
+    const float amax = __uint_as_float(row_max_bits<HDP>(max_abs4(x[i])));
+    if (last + t < p.end) {  // (t < block)
+      *reinterpret_cast<float4*>(tail + (size_t)t * HDP + c4) = x[i];
       if (c4 == 0) tail_s[t] = __uint_as_float(token_scale(amax));
     }
   }
@@ -219,7 +241,7 @@ __device__ void append_tail(const QStore& c, const Place& p, size_t sh, int whic
 // or values: the y-th tile that the new tokens touch. A thread has 4 columns of
 // 4 neighbouring tokens (a quad), a quad's columns lie on 16 or 32 neighbouring
 // lanes. The first tile's workgroup also quantises the block's earlier tokens
-// anew and writes the tail.
+// anew; the last block's writes the tail.
 template <int HDP, class T>
 __device__ __forceinline__ void append_tile(const QStore& c, const Place& p, size_t sh, int y, int which, const T* src,
                                             long tok_stride, bool vec, unsigned* blkmax, unsigned* image) {
@@ -263,35 +285,52 @@ __device__ __forceinline__ void append_tile(const QStore& c, const Place& p, siz
         ts[i][e] = 0;
       }
     }
-  if (first < p.at) {  // (uniform; y == 0) the block's earlier tokens
+  if (first < p.at) {  // (uniform; y == 0) the block's earlier tokens; rows outside as the nearest of them
+    float4 o[PASSES][4];
+    unsigned os[PASSES][4];
+    auto old = [&](int i, int e) { return min(max(tile0 + (i * QPP + qrow) * 4 + e, first), p.at - 1); };
+    if (tailed) {
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[i][e] = *reinterpret_cast<const float4*>(tail + (size_t)(old(i, e) - blk0) * HDP + c4);
+          os[i][e] = __float_as_uint(tail_s[old(i, e) - blk0]);
+        }
+    } else {
+      const float s = scales[2 * (blk0 >> c.block_shift)];
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        unsigned q[4];
+        if (which) {  // a quad's four tokens lie side by side, by column
+          const int tok = old(i, 0) & ~3;
+          unsigned x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const unsigned*>(codes + value_byte(tok, c4 + j, HDP));
+          transpose4(x, q);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[e] = *reinterpret_cast<const unsigned*>(codes + (size_t)old(i, e) * HDP + c4);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[i][e] = make_float4(code_value((int8_t)q[e], s), code_value((int8_t)(q[e] >> 8), s),
+                                code_value((int8_t)(q[e] >> 16), s), code_value((int8_t)(q[e] >> 24), s));
+      }
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          os[i][e] = read_back_scale(__uint_as_float(row_max_bits<HDP>(max_abs4(o[i][e]))), s);
+    }
 #pragma unroll
     for (int i = 0; i < PASSES; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int tok = tile0 + (i * QPP + qrow) * 4 + e;
-        const bool old = tok >= first && tok < p.at;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        unsigned os = 0;
-        if (old) {
-          if (tailed) {
-            o = *reinterpret_cast<const float4*>(tail + (size_t)(tok - blk0) * HDP + c4);
-            os = __float_as_uint(tail_s[tok - blk0]);
-          } else {
-            const float s = scales[2 * (tok >> c.block_shift)];
-            int8_t q[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              q[j] = codes[which ? value_byte(tok, c4 + j, HDP) : (size_t)tok * HDP + c4 + j];
-            o = make_float4(code_value(q[0], s), code_value(q[1], s), code_value(q[2], s), code_value(q[3], s));
-          }
-        }
-        if (!tailed) {
-          const float amax = __uint_as_float(row_max_bits<HDP>(max_abs4(o)));
-          if (old) os = read_back_scale(amax, scales[2 * (tok >> c.block_shift)]);
-        }
-        if (old) {
-          x[i][e] = o;
-          ts[i][e] = os;
+        if (tok >= first && tok < p.at) {
+          x[i][e] = o[i][e];
+          ts[i][e] = os[i][e];
         }
       }
   }
@@ -315,17 +354,15 @@ __device__ __forceinline__ void append_tile(const QStore& c, const Place& p, siz
         if (tok0 + e >= first && tok0 + e < hi) *reinterpret_cast<unsigned*>(codes + (size_t)(tok0 + e) * HDP + c4) = q[e];
     } else {
       // the quad's bytes by column; they leave in order of the image
-      const unsigned a = __builtin_amdgcn_perm(q[1], q[0], 0x05010400), b = __builtin_amdgcn_perm(q[3], q[2], 0x05010400);
-      const unsigned d = __builtin_amdgcn_perm(q[1], q[0], 0x07030602), f = __builtin_amdgcn_perm(q[3], q[2], 0x07030602);
+      unsigned r[4];
+      transpose4(q, r);
       unsigned* im = image + ((quad & 3) * HDP + c4) * 4 + (quad >> 2);
-      im[0] = __builtin_amdgcn_perm(b, a, 0x05040100);
-      im[4] = __builtin_amdgcn_perm(b, a, 0x07060302);
-      im[8] = __builtin_amdgcn_perm(f, d, 0x05040100);
-      im[12] = __builtin_amdgcn_perm(f, d, 0x07060302);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) im[4 * e] = r[e];
     }
     if (c4 == 0 && (tok0 & (c.block - 1)) == 0 && tok0 >= first && tok0 < hi) scales[2 * (tok0 >> c.block_shift)] = s;
-    // the tail, where the first tile holds the last block (else: append_tail)
-    if (y == 0 && tok0 >> c.block_shift == last) {
+    // the tail, unless the first tile's workgroup may still be reading the old one (then: append_tail)
+    if (tok0 >> c.block_shift == last && (y == 0 || !reads_tail(c, p))) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int tok = tok0 + e;
@@ -373,7 +410,7 @@ __global__ __launch_bounds__(256) void q_append_kernel(QStore c, QLen len, QTick
     const QRows& r = which ? v : k;
     const T* src = static_cast<const T*>(r.p) + seq * r.seq + head * r.head;
     append_tile<HDP, T>(c, p, sh, y, which, src, r.tok, vec, blkmax, image);
-    if (y == 0 && p.end > tile0 + kQTile) append_tail<HDP, T>(c, p, sh, which, src, r.tok, vec);
+    if (y == 0 && p.end > tile0 + kQTile && reads_tail(c, p)) append_tail<HDP, T>(c, p, sh, which, src, r.tok, vec);
   }
   turn.finish(p, c, len, gridDim.y * 2);
 }
@@ -549,12 +586,10 @@ __global__ __launch_bounds__(256) void q_read_kernel(QStore c, const int* __rest
         unsigned x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = t == 0 ? raw[4 * w + e].x : t == 1 ? raw[4 * w + e].y : t == 2 ? raw[4 * w + e].z : raw[4 * w + e].w;
-        const unsigned a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400), b = __builtin_amdgcn_perm(x[3], x[2], 0x05010400);
-        const unsigned d = __builtin_amdgcn_perm(x[1], x[0], 0x07030602), g = __builtin_amdgcn_perm(x[3], x[2], 0x07030602);
-        q[t][0][w] = __builtin_amdgcn_perm(b, a, 0x05040100);
-        q[t][1][w] = __builtin_amdgcn_perm(b, a, 0x07060302);
-        q[t][2][w] = __builtin_amdgcn_perm(g, d, 0x05040100);
-        q[t][3][w] = __builtin_amdgcn_perm(g, d, 0x07060302);
+        unsigned r[4];
+        transpose4(x, r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[t][e][w] = r[e];
       }
   } else {
 #pragma unroll

@@ -130,7 +130,7 @@ class QuantisedCache:
         n, heads = q.shape[1], q.shape[2]
         rows = self._rows("q", q, q.dtype, n, heads)
         if out is None:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q)
         check(self._lib.rtg_qcache_attend(self._h, dtype, rows, n, heads, self._ints("counts", counts),
                                           self.head_dim ** -0.5 if scale is None else scale,
                                           self._rows("out", out, q.dtype, n, heads), stream))
@@ -145,7 +145,7 @@ class QuantisedCache:
             raise Gpt2Error(f"dtype must be f32, bf16 or f16, not {dtype}")
         shape = (self.n_seq, n, self.n_head, self.head_dim)
         k = torch.empty(shape, dtype=dtype, device=self.device) if k is None else k
-        v = k.new_empty(shape) if v is None else v
+        v = torch.empty_like(k) if v is None else v
         check(self._lib.rtg_qcache_read(self._h, _TYPES[dtype], self._rows("k", k, dtype, n, self.n_head),
                                         self._rows("v", v, dtype, n, self.n_head), n, self._ints("first", first),
                                         stream))
