@@ -71,7 +71,7 @@ __device__ __forceinline__ i32x4 fixed_mfma(const i32x4 (&a)[KS], const i32x4 (&
 }
 
 // A query as ND digit planes: this lane's 16 elements (of each 64) group * 16 + e,
-// q[k][digit] bytes e. qrow null: zeros. Returns the score in units of log2 e of a
+// q[k][digit] bytes e. Returns the score in units of log2 e of a
 // unit of the fixed-point sums (of 256 of them for ND = 3), but for the key's
 // scale; NaN for a row with a value that is not finite. The four lanes 16 apart
 // hold a row.
@@ -84,7 +84,7 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
   for (int k = 0; k < KS; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      x[k][e] = qrow ? load4(qrow, k * 64 + group * 16 + e * 4, hd, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[k][e] = load4(qrow, k * 64 + group * 16 + e * 4, hd, vec);
       top = max(max(top, __float_as_uint(x[k][e].x) & 0x7FFFFFFFu), __float_as_uint(x[k][e].y) & 0x7FFFFFFFu);
       top = max(max(top, __float_as_uint(x[k][e].z) & 0x7FFFFFFFu), __float_as_uint(x[k][e].w) & 0x7FFFFFFFu);
     }
@@ -98,7 +98,7 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
   const bool zero = amax < 7.9e-31f;
   // (a negative scale goes into the digits: the factor of the sums is not negative)
   const float inv = fine && !zero ? copysignf(fixed_max<ND>(), scale) / amax : 0.f;
-  constexpr int bias = ND == 3 ? 0x808080 : 0x8080;
+  constexpr float bias = ND == 3 ? 8421504.f : 32896.f;  // 0x808080, 0x8080: every digit plus 128
 #pragma unroll
   for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -106,11 +106,9 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
       const float xe[4] = {x[k][e].x, x[k][e].y, x[k][e].z, x[k][e].w};
       unsigned u[4], d[ND];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u[i] = (unsigned)((int)rintf(fine ? xe[i] * inv : 0.f) + bias);
-        if constexpr (ND == 3) u[i] ^= 0x800000u;  // (the top digit of planes() carries no 128)
-      }
+      for (int i = 0; i < 4; ++i) u[i] = (unsigned)rintf(fmaf(xe[i], inv, bias));  // (NaN and infinity: sq says so)
       planes<ND>(u[0], u[1], u[2], u[3], d);
+      if constexpr (ND == 3) d[2] ^= 0x80808080u;
 #pragma unroll
       for (int i = 0; i < ND; ++i) q[k][i][e] = (int)d[i];
     }
@@ -128,7 +126,7 @@ struct Cols {
   float o[DT][4];
   int lim;  // keys that this lane's column sees
 
-  // qrow: the column's query (null: an unused column)
+  // qrow: the column's query
   template <class T>
   __device__ __forceinline__ void init(const T* qrow, int hd, bool vec, int group, float scale, int lim_) {
     lim = lim_;
@@ -195,39 +193,39 @@ __device__ __forceinline__ float xsum(float v) { return xor32_sum_k(xor16_sum_k(
 // doubled the error of f32 results: 8.7e-7 against 4.7e-7 of 64 bits.)
 constexpr float kLargeScore = 256.f;
 
-// The scales of NG * 16 keys (one tile, or two) for a wave: of each 16 f (scores)
-// and r = max(v scale / vmax, 2^-60) as lr = log2 r and 1 / r. (A block of zeros
-// may take any r.)
-template <int NG>
+// The scales of NG * 16 keys (one tile, or two) in blocks of 2^SH for a wave: of
+// each block f (scores) and r = max(v scale / vmax, 2^-60) as lr = log2 r and 1 /
+// r. (A block of zeros may take any r.)
+template <int NG, int SH>
 struct TileScales {
-  float f[NG], lr[NG], rinv[NG], vmax;
-  unsigned bad;  // bit i: the values of the i-th 16 keys read back as NaN
-  __device__ __forceinline__ bool nan(int i) const { return bad >> i & 1; }
+  static constexpr int NB = NG * 16 >> SH;
+  float f[NB], lr[NB], rinv[NB], vmax;
+  unsigned bad;  // bit b: the values of block b read back as NaN
+  static constexpr int block(int i) { return i * 16 >> SH; }  // of the i-th 16 keys
 };
 // sl: a lane's (keys', values') scales, those of the keys' blocks on lanes 0 ..
 // and over and over; live: keys of these that are in the cache (or more).
-template <int NG>
-__device__ __forceinline__ TileScales<NG> tile_scales(float2 sl, int shift, int live, int lane) {
-  TileScales<NG> t;
-  const int nb = (NG * 16) >> shift;
-  const bool in = ((lane & (nb - 1)) << shift) < live;  // blocks behind the last key are not read as numbers
+template <int NG, int SH>
+__device__ __forceinline__ TileScales<NG, SH> tile_scales(float2 sl, int live, int lane) {
+  TileScales<NG, SH> t;
+  constexpr int NB = TileScales<NG, SH>::NB;
+  const bool in = ((lane & (NB - 1)) << SH) < live;  // blocks behind the last key are not read as numbers
   const float k = in ? sl.x : 0.f, v = in ? sl.y : 0.f;
-  const unsigned nans = (unsigned)__builtin_amdgcn_ballot_w64(v != v);
-  t.bad = 0;
-  float m = fmaxf(v, dpp_row<0xB1>(v));  // (fmaxf skips NaN)
-  m = fmaxf(m, dpp_row<0x4E>(m));
-  if (NG == 8) m = fmaxf(m, dpp_row<0x124>(m));
+  t.bad = (unsigned)__builtin_amdgcn_ballot_w64(v != v) & ((1u << NB) - 1);
+  float m = v;  // (fmaxf skips NaN)
+  if (NB > 1) m = fmaxf(m, dpp_row<0xB1>(m));
+  if (NB > 2) m = fmaxf(m, dpp_row<0x4E>(m));
+  if (NB > 4) m = fmaxf(m, dpp_row<0x124>(m));
+  m = fmaxf(m, 0.f);
   t.vmax = m;
   // (r to the last place: it is the same for a block's every key)
   const float r = m > 0.f ? fmaxf(v * __builtin_amdgcn_rcpf(m), 8.6736174e-19f) : 1.f;
   const float lr = __builtin_amdgcn_logf(r), ri = __builtin_amdgcn_rcpf(r);
 #pragma unroll
-  for (int i = 0; i < NG; ++i) {
-    const int b = (i * 16) >> shift;
-    t.f[i] = lane_of(k, b);
-    t.lr[i] = lane_of(lr, b);
-    t.rinv[i] = lane_of(ri, b);
-    t.bad |= (nans >> b & 1) << i;
+  for (int b = 0; b < NB; ++b) {
+    t.f[b] = lane_of(k, b);
+    t.lr[b] = lane_of(lr, b);
+    t.rinv[b] = lane_of(ri, b);
   }
   return t;
 }
@@ -237,46 +235,45 @@ __device__ __forceinline__ TileScales<NG> tile_scales(float2 sl, int shift, int 
 // of the probability times the value's scale, so that the largest such product
 // here is 1 and needs no second reduction; each probability itself is 1 / r of it.
 
-// k: 16 keys; s[4]: a lane's fixed-point sums of them, most: the largest.
+// k: 16 keys; s[4]: a lane's fixed-point sums of them.
 template <int HDP, int ND>
-__device__ __forceinline__ void tile_sums(const Cols<HDP, ND>& c, const i32x4 (&k)[HDP / 64], float (&s)[4],
-                                          float& most) {
+__device__ __forceinline__ void tile_sums(const Cols<HDP, ND>& c, const i32x4 (&k)[HDP / 64], float (&s)[4]) {
   const i32x4 d = fixed_mfma<ND, HDP / 64>(k, c.q);
-  most = (float)max(max(d[0], d[1]), max(d[2], d[3]));
 #pragma unroll
   for (int e = 0; e < 4; ++e) s[e] = (float)d[e];
 }
 
-// s, most: the keys' fixed-point sums. pd: the probabilities' digits, w: what
+// s: the keys' fixed-point sums. pd: the probabilities' digits, w: what
 // their products with the values' codes are to be multiplied with.
-template <bool EDGE, int HDP, int ND, int NG>
-__device__ __forceinline__ void tile_probs(Cols<HDP, ND>& c, float (&s)[NG][4], const float (&most)[NG],
-                                           const TileScales<NG>& ts, int j0, int group, i32x4 (&pd)[NG / 4][ND],
-                                           float& w) {
-  constexpr int DT = HDP / 16;
-  float f[NG];
+template <bool EDGE, int HDP, int ND, int NG, int SH>
+__device__ __forceinline__ void tile_probs(Cols<HDP, ND>& c, float (&s)[NG][4], const TileScales<NG, SH>& ts, int j0,
+                                           int group, i32x4 (&pd)[NG / 4][ND], float& w) {
+  constexpr int DT = HDP / 16, NB = TileScales<NG, SH>::NB, PER = NG / NB;  // 16s per block
+  float f[NB], cc[NB];
   float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < NG; ++i) {
-    f[i] = c.sq * ts.f[i];
-    if (EDGE) {
+  for (int b = 0; b < NB; ++b) {
+    f[b] = c.sq * ts.f[b];
+    float most = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[i][e] = j0 + i * 16 + group * 4 + e < c.lim ? fmaf(s[i][e], f[i], ts.lr[i]) : -INFINITY;
-        top = fmaxf(top, s[i][e]);
+    for (int i = b * PER; i < (b + 1) * PER; ++i) {
+      if (EDGE) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          s[i][e] = j0 + i * 16 + group * 4 + e < c.lim ? fmaf(s[i][e], f[b], ts.lr[b]) : -INFINITY;
       }
-    } else {
-      top = fmaxf(top, fmaf(most[i], f[i], ts.lr[i]));  // (f >= 0)
+      most = fmaxf(most, fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
     }
+    top = fmaxf(top, EDGE ? most : fmaf(most, f[b], ts.lr[b]));  // (f >= 0)
   }
   top = xmax(top);
   const float base = top == -INFINITY ? 0.f : top;  // (no key here: every p is 2^-inf = 0)
 #pragma unroll
-  for (int i = 0; i < NG; ++i) {
-    const float cc = ts.lr[i] - base;
+  for (int b = 0; b < NB; ++b) cc[b] = ts.lr[b] - base;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[i][e] = EDGE ? s[i][e] - base : fmaf(s[i][e], f[i], cc);
-  }
+  for (int i = 0; i < NG; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[i][e] = EDGE ? s[i][e] - base : fmaf(s[i][e], f[i / PER], cc[i / PER]);
   if (!EDGE && __builtin_amdgcn_ballot_w64(fabsf(top) > kLargeScore)) {
 #pragma unroll
     for (int i = 0; i < NG; ++i)
@@ -288,17 +285,22 @@ __device__ __forceinline__ void tile_probs(Cols<HDP, ND>& c, float (&s)[NG][4], 
   }
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < NG; ++i) {
+  for (int b = 0; b < NB; ++b) {
+    float part = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[i][e] = __builtin_amdgcn_exp2f(s[i][e]);
-    sum = fmaf((s[i][0] + s[i][1]) + (s[i][2] + s[i][3]), ts.rinv[i], sum);
+    for (int i = b * PER; i < (b + 1) * PER; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] = __builtin_amdgcn_exp2f(s[i][e]);
+      part += (s[i][0] + s[i][1]) + (s[i][2] + s[i][3]);
+    }
+    sum = fmaf(part, ts.rinv[b], sum);
   }
   if (ts.bad) {
     asm volatile("");
     // every column that sees a key of such a block is NaN
 #pragma unroll
     for (int i = 0; i < NG; ++i)
-      if (ts.nan(i) && j0 + i * 16 + group * 4 < c.lim) sum = NAN;
+      if ((ts.bad >> i / PER & 1) && j0 + i * 16 + group * 4 < c.lim) sum = NAN;
   }
   const float mn = fmaxf(c.m, top), mb = mn == -INFINITY ? 0.f : mn;
   const float corr = __builtin_amdgcn_exp2f(c.m - mb), g = __builtin_amdgcn_exp2f(top - mb);
@@ -338,6 +340,7 @@ struct AttnArgs {
   int len_stride, extra;
   QRows q;
   int n_q, n_q_head, group;  // group: query heads per key/value head
+  unsigned group_inv;        // ceil(2^32 / group)
   const int* counts;
   float scale;
   QOut out;
@@ -347,6 +350,19 @@ struct AttnArgs {
   unsigned* joined;          // per block of columns: how many of its splits are done (0 between calls)
   int splits;
 };
+
+// Column x of a key/value head's (x < 2^22, group <= 1024): query x / group, and
+// the query head x % group of the head's.
+__device__ __forceinline__ int by_group(const AttnArgs& a, int x) {
+  return a.group == 1 ? x : (int)__umulhi((unsigned)x, a.group_inv);
+}
+struct Column {
+  int i, h;
+};
+__device__ __forceinline__ Column column(const AttnArgs& a, int x) {
+  const int i = by_group(a, x);
+  return Column{i, x - i * a.group};
+}
 
 // The sequence's queries and keys.
 struct Seq {
@@ -360,6 +376,13 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs& a, int seq) {
 }
 // Keys that query i sees.
 __device__ __forceinline__ int visible(const Seq& r, int i) { return max(r.len - r.count + i + 1, 0); }
+
+// The query of a column of key/value head `head`; of one that is none, some row.
+template <class T>
+__device__ __forceinline__ const T* query_row(const AttnArgs& a, int seq, int head, const Column& c) {
+  return static_cast<const T*>(a.q.p) + (long)seq * a.q.seq + (long)min(c.i, a.n_q - 1) * a.q.tok +
+         (long)(head * a.group + c.h) * a.q.head;
+}
 
 // Where the results of (sequence, query i, head) go.
 template <class T, int KIND>
@@ -409,126 +432,121 @@ struct RowOut {
 //
 // Two tiles at a time: 128 keys share the maximum, the scales and the conversion
 // of their products with the values (a third of the vector work, which bounds
-// this kernel: about 265 instructions per 64 keys and 16 columns). A workgroup's
-// four waves read them from LDS. The next two tiles' keys are stored there once
-// every wave has this pair's sums, the values once every wave has its products;
-// both come from registers that were loaded half a pair to a pair earlier.
+// this kernel: about 250 instructions per 64 keys and 16 columns). A workgroup's
+// four waves read them from LDS, where LDS-direct loads put the next pair's keys
+// once every wave has this pair's sums, and its values once every wave has its
+// products. (Codes widened to f16, whose products need no joining of digits, take
+// 340 instead of 513 vector instructions a pair, but twice the LDS reads, which
+// then bound it: 211 against 169 us for 16 x 1023 tokens of 20 heads.)
 constexpr int kPair = 2 * kQTile;
+
+// Lane i's 16 bytes at base + voff go to LDS lds + 16 i (the kernel waits itself).
+__device__ __forceinline__ void load_lds16(unsigned voff, const void* base, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
+}
+// This wave's loads have landed, then the barrier.
+__device__ __forceinline__ void wait_and_sync() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+}
 
 template <int HDP>
 struct SharedPair {
   static constexpr int CH = HDP / 16, U = kPair * CH / 256;  // 16-byte chunks per row; units per thread
   // Rows of keys lie in chunks xor'ed with the row, so that the 16 rows of a
   // matrix operand fall on all 64 banks; values lie as in memory.
-  static __device__ __forceinline__ int k_at(int row, int chunk) {
-    return row * CH + (chunk ^ (HDP == 64 ? (row >> 2) & 3 : (row >> 1) & 7));
-  }
+  static __device__ __forceinline__ int swizzle(int row) { return HDP == 64 ? (row >> 2) & 3 : (row >> 1) & 7; }
+  static __device__ __forceinline__ int k_at(int row, int chunk) { return row * CH + (chunk ^ swizzle(row)); }
   i32x4 k[kPair * CH], v[kPair * CH];
 };
 
-template <int HDP, int ND, int KIND, class T>
-__global__ __launch_bounds__(256) void q_attend_cols_kernel(AttnArgs a) {
+template <int HDP, int ND, int SH, int KIND, class T>
+__global__ __launch_bounds__(256, HDP == 64 || (ND == 2 && SH > 4) ? 3 : 2) void q_attend_cols_kernel(AttnArgs a) {
   using Pair = SharedPair<HDP>;
   constexpr int U = Pair::U, CH = Pair::CH, KS = HDP / 64;
   __shared__ Pair t;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, group = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, group = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head;
   const int cb0 = a.cblocks - 1 - (int)blockIdx.y * 4, cb = cb0 - wave;  // the longest first
   const Seq r = seq_of(a, seq);
   // keys that the columns of block b see: at least, at most
-  auto least_of = [&](int b) { return b >= 0 && b * 16 / a.group < r.count ? visible(r, b * 16 / a.group) : 0; };
   auto live_of = [&](int b) {
-    return b >= 0 && b * 16 / a.group < r.count ? visible(r, min((b * 16 + 15) / a.group, r.count - 1)) : 0;
+    return b >= 0 && by_group(a, b * 16) < r.count ? visible(r, min(by_group(a, b * 16 + 15), r.count - 1)) : 0;
   };
-  const int live = live_of(cb), least = least_of(cb), mine = (live + kPair - 1) / kPair;
-  int most_live = 0;  // (the later blocks of columns may be padding)
-  for (int w = 0; w < 4; ++w) most_live = max(most_live, live_of(cb0 - w));
-  const int pairs = (most_live + kPair - 1) / kPair;
-  const i32x4* kp = reinterpret_cast<const i32x4*>(a.c.k + a.c.codes(sh));
-  const i32x4* vp = reinterpret_cast<const i32x4*>(a.c.v + a.c.codes(sh));
+  const int live = live_of(cb), mine = (live + kPair - 1) / kPair;
+  const int least = live > 0 ? visible(r, by_group(a, cb * 16)) : 0;
+  // (the later blocks of columns may be padding: the last that is not sees most)
+  const int used_cb = r.count > 0 ? (r.count * a.group - 1) / 16 : -1;
+  const int pairs = (live_of(min(cb0, used_cb)) + kPair - 1) / kPair;
+  const int8_t *kp = a.c.k + a.c.codes(sh), *vp = a.c.v + a.c.codes(sh);
   const float* sp = a.c.s + a.c.scales(sh);
-  const int shift = a.c.block_shift;
-  const int end = a.c.tiles * kQTile * CH;  // 16-byte units of the (sequence, head): a pair's second tile may lie behind it
-  i32x4 kr[U], vr[U];
-  auto load = [&](const i32x4* p, int j, i32x4 (&x)[U]) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = p[min(j * kPair * CH + u * 256 + tid, end - 1)];
-  };
-  auto store_k = [&]() {
+  // unit u * 256 + tid of a pair in LDS: a wave's 64 are 1 KB of one tile
+  const unsigned kv = (unsigned)(tid / CH * CH + ((tid % CH) ^ Pair::swizzle(tid / CH))) * 16, vv = (unsigned)tid * 16;
+  const unsigned lk = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)t.k + wave * 1024;
+  const unsigned lv = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)t.v + wave * 1024;
+  auto fetch = [&](const int8_t* p, int j, unsigned voff, unsigned lds) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int x = u * 256 + tid;
-      t.k[Pair::k_at(x / CH, x % CH)] = kr[u];
+      // (a second tile behind the capacity is the first once more: no key of it is seen)
+      const bool second = u >= U / 2;
+      const int tile = second && 2 * j + 1 < a.c.tiles ? 2 * j + 1 : 2 * j;
+      load_lds16(voff, p + (size_t)tile * kQTile * HDP + (u - (second ? U / 2 : 0)) * 4096, lds + u * 4096);
     }
   };
-  auto store_v = [&]() {
-#pragma unroll
-    for (int u = 0; u < U; ++u) t.v[u * 256 + tid] = vr[u];
-  };
-  // (blocks of a second tile behind the capacity are those of the last one: no key of theirs is seen)
-  const int nb = kPair >> shift;
+  // (blocks of a second tile behind the capacity are those of the last one)
   auto load_s = [&](int j) {
-    const int b = (j * kPair >> shift) + (lane & (nb - 1)), last = (a.c.tiles * kQTile >> shift) - 1;
+    const int b = (j * kPair >> SH) + (lane & ((kPair >> SH) - 1)), last = (a.c.tiles * kQTile >> SH) - 1;
     return reinterpret_cast<const float2*>(sp)[min(b, last)];
   };
   float2 sl = make_float2(0.f, 0.f);
   if (pairs) {
-    load(kp, 0, kr);
-    load(vp, 0, vr);
+    fetch(kp, 0, kv, lk);
+    fetch(vp, 0, vv, lv);
     sl = load_s(0);
   }
   Cols<HDP, ND> c;
-  const int ci = cb * 16 + col, i = ci / a.group, qh = head * a.group + ci - i * a.group;
-  {
-    const T* qrow = static_cast<const T*>(a.q.p) + (long)seq * a.q.seq + (long)i * a.q.tok + (long)qh * a.q.head;
-    const bool used = cb >= 0 && i < r.count;
-    c.init(used ? qrow : nullptr, a.c.hd, a.qvec, group, a.scale, used ? visible(r, i) : 0);
-  }
-  if (pairs) {
-    store_k();
-    store_v();
-    if (pairs > 1) load(kp, 1, kr);
-  }
-  __syncthreads();
+  const Column cl = column(a, max(cb, 0) * 16 + col);
+  c.init(query_row<T>(a, seq, head, cl), a.c.hd, a.qvec, group, a.scale, cb >= 0 && cl.i < r.count ? visible(r, cl.i) : 0);
+  wait_and_sync();
   for (int j = 0; j < pairs; ++j) {
     const bool more = j + 1 < pairs;
-    const TileScales<8> ts = tile_scales<8>(sl, shift, live - j * kPair, lane);
-    if (more) {
-      load(vp, j + 1, vr);
-      sl = load_s(j + 1);
-    }
-    float s[8][4], most[8], w;
+    float s[8][4], w;
     if (j < mine) {
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         i32x4 k[KS];
 #pragma unroll
         for (int e = 0; e < KS; ++e) k[e] = t.k[Pair::k_at(n * 16 + col, e * 4 + group)];
-        tile_sums<HDP, ND>(c, k, s[n], most[n]);
+        tile_sums<HDP, ND>(c, k, s[n]);
+        if (n & 1) __builtin_amdgcn_sched_barrier(0);  // (two at a time in flight: registers for four waves)
       }
     }
-    __syncthreads();  // the keys are read; the values of this pair are there
+    wait_and_sync();  // the keys are read; the values of this pair are there
+    const float2 sj = sl;
     if (more) {
-      store_k();
-      if (j + 2 < pairs) load(kp, j + 2, kr);
+      fetch(kp, j + 1, kv, lk);
+      sl = load_s(j + 1);
     }
     if (j < mine) {
+      const TileScales<8, SH> ts = tile_scales<8, SH>(sj, live - j * kPair, lane);
       i32x4 pd[2][ND];
-      if (j * kPair + kPair > least) tile_probs<true>(c, s, most, ts, j * kPair, group, pd, w);
-      else tile_probs<false>(c, s, most, ts, j * kPair, group, pd, w);
+      if (j * kPair + kPair > least) tile_probs<true>(c, s, ts, j * kPair, group, pd, w);
+      else tile_probs<false>(c, s, ts, j * kPair, group, pd, w);
 #pragma unroll
       for (int d = 0; d < HDP / 16; ++d) {
         const i32x4 v[2] = {t.v[group * HDP + d * 16 + col], t.v[(4 + group) * HDP + d * 16 + col]};
         tile_product<ND, 2>(v, pd, w, c.o[d]);
+        if (d & 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
-    __syncthreads();  // the values are read; the next pair's keys are there
-    if (more) store_v();
+    wait_and_sync();  // the values are read; the next pair's keys are there
+    if (more) fetch(vp, j + 1, vv, lv);
   }
   const float l = xsum(c.l);
-  if (cb < 0 || i >= a.n_q) return;
+  if (cb < 0 || cl.i >= a.n_q) return;
   const float inv = c.lim > 0 ? 1.f / l : 0.f;
-  const RowOut<T, KIND> out(a, seq, i, qh);
+  const RowOut<T, KIND> out(a, seq, cl.i, head * a.group + cl.h);
 #pragma unroll
   for (int d = 0; d < HDP / 16; ++d) {
     const float* o = c.o[d];
@@ -584,10 +602,10 @@ __device__ __forceinline__ void finish(const AttnArgs& a, Merge<HDP, W, NW>& s, 
   const int tid = threadIdx.x, c4 = (tid % C4) * 4;
   const bool whole = per >= tiles;
   auto put = [&](int col, float l, const float4& x) {
-    const int ci = cb * W + col, i = ci / a.group, h = head * a.group + ci - i * a.group;
-    const bool any = i < r.count && visible(r, i) > 0;
+    const Column cl = column(a, cb * W + col);
+    const bool any = cl.i < r.count && visible(r, cl.i) > 0;
     const float inv = 1.f / l;
-    RowOut<T, KIND>(a, seq, i, h).put(
+    RowOut<T, KIND>(a, seq, cl.i, head * a.group + cl.h).put(
         a, c4, any ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
   };
   const int cols = min(W, a.n_q * a.group - cb * W);
@@ -671,49 +689,46 @@ __device__ __forceinline__ void finish(const AttnArgs& a, Merge<HDP, W, NW>& s, 
   }
 }
 
-template <int HDP, int ND, int KIND, class T>
+template <int HDP, int ND, int SH, int KIND, class T>
 __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
   constexpr int NW = 4;
   __shared__ Merge<HDP, 16, NW> s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
   const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head, cb = blockIdx.y, z = blockIdx.z;
   const Seq r = seq_of(a, seq);
-  const int ci = cb * 16 + col, i = ci / a.group, qh = head * a.group + ci - i * a.group;
-  const bool used = i < r.count;
-  const int firstq = cb * 16 / a.group;
-  const int last = min((cb * 16 + 15) / a.group, r.count - 1);
+  const Column cl = column(a, cb * 16 + col);
+  const int firstq = by_group(a, cb * 16);
+  const int last = min(by_group(a, cb * 16 + 15), r.count - 1);
   const int live = firstq < r.count ? visible(r, last) : 0;
   const int least = firstq < r.count ? visible(r, firstq) : 0;
   const int tiles = (live + kQTile - 1) / kQTile, per = split_tiles<HDP>(tiles, a.splits);
   const int t0 = z * per, t1 = min(t0 + per, tiles);
   if (z > 0 && t0 >= tiles) return;  // (the whole workgroup; split 0 also writes rows without keys)
   Cols<HDP, ND> c;
-  const T* qrow = static_cast<const T*>(a.q.p) + (long)seq * a.q.seq + (long)i * a.q.tok + (long)qh * a.q.head;
-  c.init(used ? qrow : nullptr, a.c.hd, a.qvec, group, a.scale, used ? visible(r, i) : 0);
+  c.init(query_row<T>(a, seq, head, cl), a.c.hd, a.qvec, group, a.scale, cl.i < r.count ? visible(r, cl.i) : 0);
   const int8_t *kp = a.c.k + a.c.codes(sh), *vp = a.c.v + a.c.codes(sh);
   const float* sp = a.c.s + a.c.scales(sh);
-  const int shift = a.c.block_shift;
   Tile<HDP> t;
   int j = t0 + wave;
   if (j < t1) {
-    t.load_s(sp, j, shift, lane);
+    t.load_s(sp, j, SH, lane);
     t.load_k(kp, j, lane);
     t.load_v(vp, j, lane);
   }
   for (; j < t1; j += NW) {
     Tile<HDP> n;
     const int nj = min(j + NW, tiles - 1);
-    n.load_s(sp, nj, shift, lane);
+    n.load_s(sp, nj, SH, lane);
     n.load_k(kp, nj, lane);
     n.load_v(vp, nj, lane);
-    const TileScales<4> ts = tile_scales<4>(t.s, shift, live - j * kQTile, lane);
-    float sums[4][4], most[4];
+    const TileScales<4, SH> ts = tile_scales<4, SH>(t.s, live - j * kQTile, lane);
+    float sums[4][4];
     i32x4 pd[1][ND];
     float w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tile_sums<HDP, ND>(c, t.k[i], sums[i], most[i]);
-    if (j * kQTile + kQTile > least) tile_probs<true>(c, sums, most, ts, j * kQTile, group, pd, w);
-    else tile_probs<false>(c, sums, most, ts, j * kQTile, group, pd, w);
+    for (int i = 0; i < 4; ++i) tile_sums<HDP, ND>(c, t.k[i], sums[i]);
+    if (j * kQTile + kQTile > least) tile_probs<true>(c, sums, ts, j * kQTile, group, pd, w);
+    else tile_probs<false>(c, sums, ts, j * kQTile, group, pd, w);
 #pragma unroll
     for (int d = 0; d < HDP / 16; ++d) {
       const i32x4 v[1] = {t.v[d]};
@@ -913,15 +928,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a
   }
   for (int i = lane; i < NC * 64; i += 64) reinterpret_cast<unsigned*>(image[wave])[i] = 0;
   FewCols<HDP, NC> c;
-  {
-    const int ci = NC == 1 ? 0 : row >> 2, i = ci / a.group, qh = head * a.group + ci - i * a.group;
-    const T* qrow = static_cast<const T*>(a.q.p) + (long)seq * a.q.seq + (long)i * a.q.tok + (long)qh * a.q.head;
-    c.init(i < r.count ? qrow : nullptr, a.c.hd, a.qvec, lane, a.scale);
-  }
-  {
-    const int i = (NC == 1 ? 0 : group) / a.group;
-    c.lim = i < r.count ? visible(r, i) : 0;
-  }
+  c.init(query_row<T>(a, seq, head, column(a, NC == 1 ? 0 : row >> 2)), a.c.hd, a.qvec, lane, a.scale);
+  const int qi = by_group(a, NC == 1 ? 0 : group);
+  c.lim = qi < r.count ? visible(r, qi) : 0;
   for (; j < t1; j += NW) {
     Tile<HDP> n;
     const int nj = min(j + NW, tiles - 1);
@@ -956,7 +965,7 @@ constexpr int kParts = 1024;
 template <int HDP, int ND, int KIND, class T>
 void attend(hipStream_t s, AttnArgs& a) {
   const long heads = (long)a.c.n_seq * a.c.n_head;
-  const int columns = a.n_q * a.group;
+  const int columns = a.n_q * a.group, sh = a.c.block_shift;
   if (columns <= 4) a.cblocks = 1;
   const int most = (a.c.tiles + 7) / 8;
   a.splits = (int)std::max<long>(1, std::min<long>(most, parts<HDP>(columns <= 4) / (heads * a.cblocks)));
@@ -964,12 +973,18 @@ void attend(hipStream_t s, AttnArgs& a) {
   if (columns == 1) {
     q_attend_few_kernel<HDP, 1, KIND, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
   } else if constexpr (KIND != QO_XT) {
-    if (heads * a.cblocks >= 2048 && columns > 4)
-      q_attend_cols_kernel<HDP, ND, KIND, T><<<dim3((unsigned)heads, (unsigned)((a.cblocks + 3) / 4)), 256, 0, s>>>(a);
-    else if (columns <= 4)
+    if (heads * a.cblocks >= 2048 && columns > 4) {
+      const dim3 wide((unsigned)heads, (unsigned)((a.cblocks + 3) / 4));
+      if (sh == 4) q_attend_cols_kernel<HDP, ND, 4, KIND, T><<<wide, 256, 0, s>>>(a);
+      else if (sh == 5) q_attend_cols_kernel<HDP, ND, 5, KIND, T><<<wide, 256, 0, s>>>(a);
+      else q_attend_cols_kernel<HDP, ND, 6, KIND, T><<<wide, 256, 0, s>>>(a);
+    } else if (columns <= 4) {
       q_attend_few_kernel<HDP, 4, KIND, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
-    else
-      q_attend_split_kernel<HDP, ND, KIND, T><<<grid, 256, 0, s>>>(a);
+    } else {
+      if (sh == 4) q_attend_split_kernel<HDP, ND, 4, KIND, T><<<grid, 256, 0, s>>>(a);
+      else if (sh == 5) q_attend_split_kernel<HDP, ND, 5, KIND, T><<<grid, 256, 0, s>>>(a);
+      else q_attend_split_kernel<HDP, ND, 6, KIND, T><<<grid, 256, 0, s>>>(a);
+    }
   }
 }
 
@@ -1011,6 +1026,7 @@ void launch_q_attend(hipStream_t s, const QStore& c, QLen len, int extra, QType 
   a.n_q = n_q;
   a.n_q_head = n_q_head;
   a.group = n_q_head / c.n_head;
+  a.group_inv = (unsigned)((0x100000000ull + a.group - 1) / a.group);
   a.counts = counts;
   a.scale = scale;
   a.out = out;

@@ -49,6 +49,7 @@ rtg_result err(const char* f, ...) {
 rtg_result hip_err(hipError_t e, const char* what) { return err("HIP error in %s: %s", what, hipGetErrorString(e)); }
 
 constexpr unsigned kNoErr = 0xFFFFFFFFu;
+constexpr size_t kMaxGroup = 1024;
 constexpr size_t kMaxRows = 4000000;  // of one sequence: a grid dimension of 65535 tiles of 64 tokens
 
 // The handle's device as the current one for the length of a call.
@@ -185,8 +186,10 @@ rtg_result rtg_qcache_attend(rtg_qcache* q, rtg_dtype dtype, const rtg_rows* que
   if (!type_of(dtype, &t)) return err("rtg_qcache_attend takes f32, bf16 or f16 rows");
   if (n_q_head == 0 || n_q_head % (size_t)q->c.n_head != 0)
     return err("%zu query heads are not a multiple of the cache's %d heads", n_q_head, q->c.n_head);
+  if (n_q_head / q->c.n_head > kMaxGroup)
+    return err("%zu query heads per key/value head exceed %zu", n_q_head / q->c.n_head, kMaxGroup);
   if (!std::isfinite(scale)) return err("scale must be finite");
-  if (n_q_head / q->c.n_head > kMaxRows || n_q > kMaxRows || n_q * (n_q_head / q->c.n_head) > kMaxRows)
+  if (n_q > kMaxRows || n_q * (n_q_head / q->c.n_head) > kMaxRows)
     return err("%zu queries of %zu heads exceed %zu rows per key/value head", n_q, n_q_head, kMaxRows);
   if (n_q == 0) return ok();
   if (!queries->data || !out->data) return err("null argument");
