@@ -18,6 +18,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_core.h"
 #include "f16_pair.h"
@@ -305,12 +306,11 @@ __device__ __forceinline__ void tile_probs(Cols<HDP, ND>& c, float (&s)[NG][4], 
   const float mn = fmaxf(c.m, top), mb = mn == -INFINITY ? 0.f : mn;
   const float corr = __builtin_amdgcn_exp2f(c.m - mb), g = __builtin_amdgcn_exp2f(top - mb);
   c.l = fmaf(c.l, corr, sum * g);
-  if (__builtin_amdgcn_ballot_w64(mn != c.m)) {
+  // (without a branch for maxima that stay: it cost more copies of registers than it saved)
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c.o[d][i] *= corr;
-  }
+    for (int i = 0; i < 4; ++i) c.o[d][i] *= corr;
   c.m = mn;
   w = g * ts.vmax * ((ND == 3 ? 256.f : 1.f) / fixed_max<ND>());
   // rounded to an integer and biased, in the low bits of the sum with 2^23
@@ -471,14 +471,13 @@ __global__ __launch_bounds__(256, HDP == 64 || (ND == 2 && SH > 4) ? 3 : 2) void
   const int cb0 = a.cblocks - 1 - (int)blockIdx.y * 4, cb = cb0 - wave;  // the longest first
   const Seq r = seq_of(a, seq);
   // keys that the columns of block b see: at least, at most
-  auto live_of = [&](int b) {
-    return b >= 0 && by_group(a, b * 16) < r.count ? visible(r, min(by_group(a, b * 16 + 15), r.count - 1)) : 0;
-  };
-  const int live = live_of(cb), mine = (live + kPair - 1) / kPair;
-  const int least = live > 0 ? visible(r, by_group(a, cb * 16)) : 0;
-  // (the later blocks of columns may be padding: the last that is not sees most)
-  const int used_cb = r.count > 0 ? (r.count * a.group - 1) / 16 : -1;
-  const int pairs = (live_of(min(cb0, used_cb)) + kPair - 1) / kPair;
+  // (the later blocks of columns may be padding: the last that is not sees most;
+  // columns that are none may see anything, their results go nowhere)
+  const int top_cb = r.count > 0 ? min(cb0, (r.count * a.group - 1) / 16) : -1, low_cb = max(cb0 - 3, 0);
+  const int live = top_cb >= 0 ? visible(r, min(by_group(a, top_cb * 16 + 15), r.count - 1)) : 0;
+  const int pairs = (live + kPair - 1) / kPair;
+  // pairs that every column sees whole
+  const int full = top_cb >= low_cb ? min(visible(r, by_group(a, low_cb * 16)) / kPair, pairs) : 0;
   const int8_t *kp = a.c.k + a.c.codes(sh), *vp = a.c.v + a.c.codes(sh);
   const float* sp = a.c.s + a.c.scales(sh);
   // unit u * 256 + tid of a pair in LDS: a wave's 64 are 1 KB of one tile
@@ -509,18 +508,16 @@ __global__ __launch_bounds__(256, HDP == 64 || (ND == 2 && SH > 4) ? 3 : 2) void
   const Column cl = column(a, max(cb, 0) * 16 + col);
   c.init(query_row<T>(a, seq, head, cl), a.c.hd, a.qvec, group, a.scale, cb >= 0 && cl.i < r.count ? visible(r, cl.i) : 0);
   wait_and_sync();
-  for (int j = 0; j < pairs; ++j) {
+  auto step = [&](int j, auto edge) {
     const bool more = j + 1 < pairs;
     float s[8][4], w;
-    if (j < mine) {
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        i32x4 k[KS];
+    for (int n = 0; n < 8; ++n) {
+      i32x4 k[KS];
 #pragma unroll
-        for (int e = 0; e < KS; ++e) k[e] = t.k[Pair::k_at(n * 16 + col, e * 4 + group)];
-        tile_sums<HDP, ND>(c, k, s[n]);
-        if (n & 1) __builtin_amdgcn_sched_barrier(0);  // (two at a time in flight: registers for four waves)
-      }
+      for (int e = 0; e < KS; ++e) k[e] = t.k[Pair::k_at(n * 16 + col, e * 4 + group)];
+      tile_sums<HDP, ND>(c, k, s[n]);
+      if (n & 1) __builtin_amdgcn_sched_barrier(0);  // (two at a time in flight: fewer registers)
     }
     wait_and_sync();  // the keys are read; the values of this pair are there
     const float2 sj = sl;
@@ -528,21 +525,21 @@ __global__ __launch_bounds__(256, HDP == 64 || (ND == 2 && SH > 4) ? 3 : 2) void
       fetch(kp, j + 1, kv, lk);
       sl = load_s(j + 1);
     }
-    if (j < mine) {
-      const TileScales<8, SH> ts = tile_scales<8, SH>(sj, live - j * kPair, lane);
-      i32x4 pd[2][ND];
-      if (j * kPair + kPair > least) tile_probs<true>(c, s, ts, j * kPair, group, pd, w);
-      else tile_probs<false>(c, s, ts, j * kPair, group, pd, w);
+    const TileScales<8, SH> ts = tile_scales<8, SH>(sj, live - j * kPair, lane);
+    i32x4 pd[2][ND];
+    tile_probs<decltype(edge)::value>(c, s, ts, j * kPair, group, pd, w);
 #pragma unroll
-      for (int d = 0; d < HDP / 16; ++d) {
-        const i32x4 v[2] = {t.v[group * HDP + d * 16 + col], t.v[(4 + group) * HDP + d * 16 + col]};
-        tile_product<ND, 2>(v, pd, w, c.o[d]);
-        if (d & 1) __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int d = 0; d < HDP / 16; ++d) {
+      const i32x4 v[2] = {t.v[group * HDP + d * 16 + col], t.v[(4 + group) * HDP + d * 16 + col]};
+      tile_product<ND, 2>(v, pd, w, c.o[d]);
+      if (d & 1) __builtin_amdgcn_sched_barrier(0);
     }
     wait_and_sync();  // the values are read; the next pair's keys are there
     if (more) fetch(vp, j + 1, vv, lv);
-  }
+  };
+  int j = 0;
+  for (; j < full; ++j) step(j, std::false_type());
+  for (; j < pairs; ++j) step(j, std::true_type());
   const float l = xsum(c.l);
   if (cb < 0 || cl.i >= a.n_q) return;
   const float inv = c.lim > 0 ? 1.f / l : 0.f;
