@@ -461,7 +461,7 @@ struct SharedPair {
 };
 
 template <int HDP, int ND, int SH, int KIND, class T>
-__global__ __launch_bounds__(256, HDP == 64 || (ND == 2 && SH > 4) ? 3 : 2) void q_attend_cols_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend_cols_kernel(AttnArgs a) {
   using Pair = SharedPair<HDP>;
   constexpr int U = Pair::U, CH = Pair::CH, KS = HDP / 64;
   __shared__ Pair t;
@@ -959,6 +959,13 @@ constexpr int parts(bool few) {
 }
 constexpr int kParts = 1024;
 
+// Blocks of 16 columns from which every wave takes all keys of its own: 1.4 for
+// each of the device's 1024 SIMDs. Below, splitting the keys fills it better (1264
+// blocks: 184 against 231 us over 15000 keys, 19.2 against 21.0 for prompts of
+// 1023), above it only reads them more often (1548: 13.3 against 10.4, 2000: 46.7
+// against 24.7).
+constexpr long kManyBlocks = 1400;
+
 template <int HDP, int ND, int KIND, class T>
 void attend(hipStream_t s, AttnArgs& a) {
   const long heads = (long)a.c.n_seq * a.c.n_head;
@@ -970,7 +977,7 @@ void attend(hipStream_t s, AttnArgs& a) {
   if (columns == 1) {
     q_attend_few_kernel<HDP, 1, KIND, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
   } else if constexpr (KIND != QO_XT) {
-    if (heads * a.cblocks >= 2048 && columns > 4) {
+    if (columns > 4 && heads * a.cblocks >= kManyBlocks) {
       const dim3 wide((unsigned)heads, (unsigned)((a.cblocks + 3) / 4));
       if (sh == 4) q_attend_cols_kernel<HDP, ND, 4, KIND, T><<<wide, 256, 0, s>>>(a);
       else if (sh == 5) q_attend_cols_kernel<HDP, ND, 5, KIND, T><<<wide, 256, 0, s>>>(a);
