@@ -241,17 +241,19 @@ typedef struct {
   ptrdiff_t stride_seq, stride_token, stride_head;
 } rtg_rows;
 /* Errors: "head_dim <hd> is not supported (1 to 128)", "block <b> is not
- * supported (16, 32 or 64)", capacities over 4000000 tokens. */
+ * supported (16, 32 or 64)", capacities over 4000000 tokens, more than 1000000
+ * pairs of sequence and head. */
 rtg_result rtg_qcache_new(size_t n_seq, size_t n_head, size_t head_dim, size_t capacity, size_t block,
                           rtg_qcache** out);
 void rtg_qcache_destroy(rtg_qcache* cache);
 /* n_new tokens to every sequence, or the first counts[s] (clamped to 0 ..
  * n_new) of its rows; behind its length, or with start from token start[s] on:
  * what lay there and behind is dropped (start of 0: the sequence begins anew;
- * n_new = 0: only dropped). Where a cut falls into a block before
- * the last token's, that block's remaining tokens count as the values they read back as. A
- * sequence whose start is negative or behind its length, or whose tokens would
- * pass the capacity, is left as it was, and rtg_qcache_lengths reports it. */
+ * n_new = 0: only dropped). Where the last token left lies in another block than
+ * the last one did, its block's tokens count as the values they read back as
+ * from then on (their unrounded ones are gone). A sequence whose start is
+ * negative or behind its length, or whose tokens would pass the capacity, is
+ * left as it was, and rtg_qcache_lengths reports it. */
 rtg_result rtg_qcache_append(rtg_qcache* cache, rtg_dtype dtype, const rtg_rows* k, const rtg_rows* v, size_t n_new,
                              const int32_t* counts, const int32_t* start, void* stream);
 /* The values of tokens first[s] (0 for NULL) .. first[s] + n - 1 of every
@@ -262,7 +264,8 @@ rtg_result rtg_qcache_read(const rtg_qcache* cache, rtg_dtype dtype, const rtg_r
  * tokens of every sequence: query i of c sits at position len - c + i and sees
  * the keys up to its own; softmax of scale * q . k, in f32 or better, results
  * rounded to dtype once. Query head h reads key/value head h / (n_q_head /
- * n_head). Rows i >= counts[s], and rows of queries before the sequence's first
+ * n_head), at most 1024 of them one key/value head. A block that reads back as
+ * NaN makes the rows NaN that see a key of it, and no others. Rows i >= counts[s], and rows of queries before the sequence's first
  * token, are set to 0. out must not overlap the queries. */
 rtg_result rtg_qcache_attend(rtg_qcache* cache, rtg_dtype dtype, const rtg_rows* queries, size_t n_q,
                              size_t n_q_head, const int32_t* counts, float scale, const rtg_rows* out, void* stream);

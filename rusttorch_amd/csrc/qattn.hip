@@ -93,12 +93,24 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
   top = max(r[0], r[1]);
   const auto r2 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
   top = max(r2[0], r2[1]);
-  const float amax = __uint_as_float(top);
+  float amax = __uint_as_float(top);
   const bool fine = top < 0x7F800000u;
-  // below 2^-100 a row is as good as 0: no score that exp could tell from 0
-  const bool zero = amax < 7.9e-31f;
+  float unit = fabsf(scale) * 1.4426950408889634f * (ND == 3 ? 256.f : 1.f) / fixed_max<ND>();
+  if (__builtin_amdgcn_ballot_w64(amax < 7.9e-31f)) {
+    asm volatile("");
+    // rows below 2^-100 are taken 2^100 times as large, so that 1 / amax is a number
+    const bool tiny = amax < 7.9e-31f;
+    const float up = tiny ? 1.2676506e30f : 1.f;
+    amax *= up;
+    unit = tiny ? unit * 7.888609e-31f : unit;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[k][e] = make_float4(x[k][e].x * up, x[k][e].y * up, x[k][e].z * up, x[k][e].w * up);
+  }
   // (a negative scale goes into the digits: the factor of the sums is not negative)
-  const float inv = fine && !zero ? copysignf(fixed_max<ND>(), scale) / amax : 0.f;
+  const float inv = fine && amax > 0.f ? copysignf(fixed_max<ND>(), scale) / amax : 0.f;
   constexpr float bias = ND == 3 ? 8421504.f : 32896.f;  // 0x808080, 0x8080: every digit plus 128
 #pragma unroll
   for (int k = 0; k < KS; ++k)
@@ -113,7 +125,7 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
 #pragma unroll
       for (int i = 0; i < ND; ++i) q[k][i][e] = (int)d[i];
     }
-  return !fine ? NAN : zero ? 0.f : amax * (fabsf(scale) * 1.4426950408889634f * (ND == 3 ? 256.f : 1.f) / fixed_max<ND>());
+  return fine ? amax * unit : NAN;
 }
 
 // A wave's 16 columns: lane = group * 16 + column; the group's 16 (of 64) query

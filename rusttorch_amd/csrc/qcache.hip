@@ -59,7 +59,8 @@ namespace {
 // Where an append of a sequence goes: tokens [at, end) over a length of len.
 struct Place {
   int len, at, end;
-  int bad;  // 0, or why it is refused (QTickets)
+  int from;  // a token of the first block to be written: of the last one left where nothing is new
+  int bad;   // 0, or why it is refused (QTickets)
 };
 __device__ __forceinline__ Place place(int seq, const int* len, int len_stride, int n_new, const int* counts,
                                        const int* start, int capacity) {
@@ -69,6 +70,7 @@ __device__ __forceinline__ Place place(int seq, const int* len, int len_stride, 
   const int n = counts ? min(max(counts[seq], 0), n_new) : n_new;
   p.bad = p.at < 0 || p.at > p.len ? 1 : n > capacity - p.at ? 2 : 0;
   p.end = p.bad ? p.at : p.at + n;
+  p.from = p.end > p.at || p.at == 0 ? p.at : p.at - 1;
   return p;
 }
 
@@ -180,16 +182,16 @@ __device__ __forceinline__ size_t value_byte(int tok, int col, int hdp) {
          (tok & 3);
 }
 
-// Whether the block that token `at` lies in is the one that the tail holds: the
-// block of the last token.
+// Whether the first block to be written is the one that the tail holds: the block
+// of the last token.
 __device__ __forceinline__ bool in_tail(const QStore& c, const Place& p) {
-  return p.len > 0 && p.at >> c.block_shift == (p.len - 1) >> c.block_shift;
+  return p.len > 0 && p.from >> c.block_shift == (p.len - 1) >> c.block_shift;
 }
 
 // Whether the append needs the tail that is there: it goes on in the middle of
 // the block that the tail holds.
 __device__ __forceinline__ bool reads_tail(const QStore& c, const Place& p) {
-  return (p.at & (c.block - 1)) != 0 && in_tail(c, p);
+  return (p.from & ~(c.block - 1)) < p.at && in_tail(c, p);
 }
 
 // A value of a full block as it reads back, and its token's own scale: a token
@@ -247,8 +249,8 @@ __device__ __forceinline__ void append_tile(const QStore& c, const Place& p, siz
                                             long tok_stride, bool vec, unsigned* blkmax, unsigned* image) {
   constexpr int LPR = HDP / 4, QPP = 256 / LPR, PASSES = 16 / QPP;  // lanes per quad, quads per pass
   const int tid = threadIdx.x, c4 = (tid % LPR) * 4, qrow = tid / LPR;
-  const int tile0 = (p.at / kQTile + y) * kQTile;  // first token of the tile
-  const int blk0 = p.at & ~(c.block - 1);
+  const int tile0 = (p.from / kQTile + y) * kQTile;  // first token of the tile
+  const int blk0 = p.from & ~(c.block - 1);
   const int first = y == 0 ? blk0 : tile0, hi = min(p.end, tile0 + kQTile);
   const bool tailed = in_tail(c, p);
   float* tail = c.tail + c.tails(sh, which);
@@ -405,7 +407,7 @@ __global__ __launch_bounds__(256) void q_append_kernel(QStore c, QLen len, QTick
   const int sh = blockIdx.x, seq = sh / c.n_head, head = sh - seq * c.n_head, y = blockIdx.y, which = blockIdx.z;
   Turn turn;
   const Place p = turn.begin(&shared, c, sh, len, tickets, n_new, counts, start);
-  const int tile0 = (p.at / kQTile + y) * kQTile;
+  const int tile0 = (p.from / kQTile + y) * kQTile;
   if (!p.bad && (p.end > p.at || p.at < p.len) && (y == 0 || tile0 < p.end)) {
     const QRows& r = which ? v : k;
     const T* src = static_cast<const T*>(r.p) + seq * r.seq + head * r.head;
@@ -448,7 +450,7 @@ __global__ __launch_bounds__(256) void q_append_one_kernel(QStore c, QLen len, Q
   const Place p = turn.begin(&shared, c, sh, len, tickets, n_new, counts, start);
   const bool has = p.end > p.at;  // (false where the append was refused)
   if (!p.bad && (has || p.at < p.len)) {
-    const int blk = p.at >> c.block_shift, in = p.at & (c.block - 1);  // `in` earlier tokens in the block
+    const int blk = p.from >> c.block_shift, in = p.at - (blk << c.block_shift);  // `in` earlier tokens in the block
     const bool tailed = in_tail(c, p);
     float* tail = c.tail + c.tails(sh, which);
     float* tail_s = c.tail_s + c.tail_scales(sh, which);

@@ -32,8 +32,8 @@ class Head:
         self.s = np.zeros(0)            # per block
 
     def cut(self, at):
-        b = at // self.block
-        if at < self.n and b < (self.n - 1) // self.block and at % self.block:
+        b = max(at - 1, 0) // self.block     # the block of the last token left
+        if 0 < at < self.n and b < (self.n - 1) // self.block:
             lo = b * self.block
             s = self.s[b]
             self.x[lo:at] = (self.codes[lo:at].astype(np.float32) * np.float32(s)).astype(np.float64)

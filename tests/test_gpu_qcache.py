@@ -98,6 +98,38 @@ def test_cuts(block):
     b.append(2, start=[300, -1, 4, 1], counts=[2, 2, 2, 2])  # 0, 1: refused
 
 
+@pytest.mark.parametrize("block", [16, 32, 64])
+def test_cuts_to_the_end_of_a_block(block):
+    # what is left ends with a full block, which later calls go back into
+    for by_counts in (False, True):
+        b = Both(3, 2, 64, 300, block, seed=21)
+        b.append(3 * block + 6)
+        ends = [2 * block, 3 * block, block]
+        if by_counts:
+            b.append(4, start=ends, counts=[0, 0, 0])
+        else:
+            b.append(0, start=ends)
+        b.append(1, start=[x - 2 for x in ends])
+        b.append(block + 3, start=[x - 1 for x in ends])
+        b.append(0, start=ends)
+        b.append(0, start=[x - 1 for x in ends])
+        b.append(1)
+        b.append(2)
+        b.append(0, start=[0, 0, 0])
+        b.append(2)
+
+
+def test_many_cuts():
+    rng = np.random.default_rng(22)
+    for block in (16, 64):
+        b = Both(5, 1, 20, 150, block, seed=block)
+        for _ in range(40):
+            n = int(rng.choice([0, 1, 1, 2, 17, 70]))
+            lens = [b.r.length(s) for s in range(5)]
+            start = [int(rng.integers(0, x + 1)) if rng.random() < 0.5 else x for x in lens] if rng.random() < 0.8 else None
+            b.append(n, start=start, counts=rng.integers(0, n + 1, 5) if rng.random() < 0.5 else None, size=float(rng.uniform(0.2, 3)))
+
+
 def test_cut_and_write_again_gives_the_same():
     b = Both(2, 2, 64, 200, 32, seed=11)
     b.append(75)
@@ -277,6 +309,17 @@ def test_large_scores():
         assert np.max(np.abs(got.double().cpu().numpy() - want)) <= 20.0 * (2 * 5 * size * EPS + 200 * EPS)
 
 
+def test_tiny_queries_over_large_keys():
+    b = Both(1, 1, 64, 100, 32, seed=23)
+    (k, kn), (v, vn) = (rows(b.rng, (1, 90, 1, 64)) for _ in range(2))
+    k *= 1e32
+    b.put(k, v, k.double().cpu().numpy(), vn)
+    q, _ = rows(b.rng, (1, 7, 1, 64))
+    for n in (1, 7):
+        x = q[:, :n] * 1e-32
+        near(b.c.attend(x), b.r, x.double().cpu().numpy(), "f32")
+
+
 def test_what_is_not_finite_stays_where_it_is():
     b = Both(1, 1, 64, 200, 16, seed=15)
     (k, kn), (v, vn) = (rows(b.rng, (1, 100, 1, 64)) for _ in range(2))
@@ -397,6 +440,8 @@ def test_refusals():
                        ("counts is on cpu", lambda: c.append(x, x, counts=torch.zeros(2, dtype=torch.int32))),
                        ("start must be", lambda: c.append(x, x, start=torch.zeros(3, dtype=torch.int32, device="cuda"))),
                        ("not a multiple", lambda: c.attend(torch.zeros(2, 3, 3, 64, device="cuda"))),
+                       ("1025 query heads", lambda: c.attend(torch.zeros(2, 1, 2050, 64, device="cuda"))),
+                       ("exceed 4000000 rows", lambda: c.attend(torch.zeros(2, 1, 2, 64, device="cuda").expand(2, 4000001, 2, 64), out=torch.zeros(2, 1, 2, 64, device="cuda").expand(2, 4000001, 2, 64))),
                        ("out must be torch.float32", lambda: c.attend(x, out=x.half())),
                        ("out must be", lambda: c.attend(x, out=torch.zeros(2, 3, 4, 64, device="cuda"))),
                        ("scale must be finite", lambda: c.attend(x, scale=float("nan"))),
