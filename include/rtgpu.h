@@ -234,7 +234,8 @@ rtg_result rtg_generate_cached_quantised(const rtg_model* model, const uint32_t*
  * nothing and may be captured into a graph, each replay acting on the cache as
  * it then is. Lengths live on the device. A cache must not be used by two
  * calls (or replays) at once, the reading ones included: they share a
- * workspace. Calls on different streams need the streams' own ordering. ---- */
+ * workspace. Calls on different streams need the streams' own ordering, and a
+ * cache has to live as long as the graphs that hold its calls. ---- */
 typedef struct rtg_qcache rtg_qcache;
 typedef struct {
   void* data;
@@ -265,8 +266,10 @@ rtg_result rtg_qcache_read(const rtg_qcache* cache, rtg_dtype dtype, const rtg_r
  * the keys up to its own; softmax of scale * q . k, in f32 or better, results
  * rounded to dtype once. Query head h reads key/value head h / (n_q_head /
  * n_head), at most 1024 of them one key/value head. A block that reads back as
- * NaN makes the rows NaN that see a key of it, and no others. Rows i >= counts[s], and rows of queries before the sequence's first
- * token, are set to 0. out must not overlap the queries. */
+ * NaN makes the rows NaN that see a key of it, and no others; a query with a
+ * value that is not finite gives a row of NaN. Rows i >= counts[s], and rows of
+ * queries before the sequence's first token, are set to 0. out must not overlap
+ * the queries. */
 rtg_result rtg_qcache_attend(rtg_qcache* cache, rtg_dtype dtype, const rtg_rows* queries, size_t n_q,
                              size_t n_q_head, const int32_t* counts, float scale, const rtg_rows* out, void* stream);
 /* Waits for the stream and writes the n_seq lengths. Returns an error once

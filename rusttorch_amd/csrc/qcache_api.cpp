@@ -46,7 +46,10 @@ rtg_result err(const char* f, ...) {
   return rtg_result{false, s};
 }
 
-rtg_result hip_err(hipError_t e, const char* what) { return err("HIP error in %s: %s", what, hipGetErrorString(e)); }
+rtg_result hip_err(hipError_t e, const char* what) {
+  (void)hipGetLastError();  // reported here, not by the caller's next check
+  return err("HIP error in %s: %s", what, hipGetErrorString(e));
+}
 
 constexpr unsigned kNoErr = 0xFFFFFFFFu;
 constexpr size_t kMaxGroup = 1024;
@@ -131,8 +134,10 @@ rtg_result rtg_qcache_new(size_t n_seq, size_t n_head, size_t head_dim, size_t c
     q->work = static_cast<char*>(q->mem) + head + store;
     e = hipMemset(q->mem, 0, head);
     if (e == hipSuccess) e = hipMemset(q->err, 0xFF, 4);
-    qattn_work_clear(nullptr, q->work, q->c.hdp);
-    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e == hipSuccess) {
+      qattn_work_clear(nullptr, q->work, q->c.hdp);
+      e = hipDeviceSynchronize();
+    }
     if (e != hipSuccess) return hip_err(e, "rtg_qcache_new");
     *out = q.release();
   } catch (const std::exception& ex) {
@@ -208,6 +213,9 @@ rtg_result rtg_qcache_lengths(rtg_qcache* q, uint32_t* out, void* stream) {
   OnDevice dev(q->device);
   if (dev.status() != hipSuccess) return hip_err(dev.status(), "hipSetDevice");
   hipStream_t s = static_cast<hipStream_t>(stream);
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (s && hipStreamIsCapturing(s, &capture) == hipSuccess && capture != hipStreamCaptureStatusNone)
+    return err("rtg_qcache_lengths: the stream is being captured");  // (a copy would end the capture)
   unsigned bad = kNoErr;
   hipError_t e = hipMemcpyAsync(out, q->len, (size_t)q->c.n_seq * 4, hipMemcpyDeviceToHost, s);
   if (e == hipSuccess) e = hipMemcpyAsync(&bad, q->err, 4, hipMemcpyDeviceToHost, s);

@@ -5,7 +5,8 @@ Programs that run their own layers write keys and values with `append`, run
 attention over them with `attend` and get them back with `read`; the calls go
 to the tensors' current stream and do not wait for it. Tensors are
 [n_seq, tokens, heads, head_dim] on the cache's device, f32, bf16 or f16, in any
-strides whose last is 1. There is no counterpart in the reference.
+strides whose last is 1. Nothing here has a gradient. There is no counterpart in
+the reference.
 """
 from __future__ import annotations
 
@@ -47,6 +48,8 @@ class QuantisedCache:
                         ("block", block)):
             if x < 0:
                 raise Gpt2Error(f"{name} must not be negative")
+            if x >= 1 << 63:
+                raise Gpt2Error(f"{name} is too large")
         self._lib = _lib.load()
         self._index = -1  # of the device
         h = C.c_void_p()
@@ -92,6 +95,8 @@ class QuantisedCache:
             raise Gpt2Error(f"{what} must be {dtype}, not {x.dtype}")
         if x.get_device() != self._index:
             raise Gpt2Error(f"{what} is on {x.device}, the cache on {self.device}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise Gpt2Error(f"{what} requires a gradient, which the cache has none of: detach it or use torch.no_grad()")
         seq, tok, head, col = x.stride()
         if col != 1 and self.head_dim > 1 and x.numel():
             raise Gpt2Error(f"{what}'s last dimension must be contiguous")

@@ -456,3 +456,79 @@ def test_refusals():
     c.close()
     with pytest.raises(Gpt2Error, match="closed"):
         c.lengths()
+
+
+def test_gradients_are_refused():
+    c = QuantisedCache(1, 2, 64, 100)
+    x = torch.zeros(1, 3, 2, 64, device="cuda")
+    leaf = x.clone().requires_grad_()
+    for call in (lambda: c.append(leaf, x), lambda: c.append(x, leaf), lambda: c.attend(leaf)):
+        with pytest.raises(Gpt2Error, match="requires a gradient"):
+            call()
+    with torch.no_grad():
+        c.append(leaf, leaf)
+        c.attend(leaf)
+    assert c.lengths() == [3]
+
+
+def test_a_cache_that_does_not_fit_leaves_no_error_behind():
+    with pytest.raises(Gpt2Error, match="rtg_qcache_new"):
+        QuantisedCache(1000, 1000, 128, 4000000)
+    assert (torch.ones(5, device="cuda") + 1).sum().item() == 10
+
+
+def test_lengths_refuses_a_stream_in_capture():
+    c = QuantisedCache(1, 2, 64, 100)
+    x = torch.ones(1, 3, 2, 64, device="cuda")
+    c.append(x, x)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(Gpt2Error, match="being captured"):
+            c.lengths()
+        c.append(x, x)
+    g.replay()
+    assert c.lengths() == [6]
+
+
+def test_two_graphs_of_one_cache_take_turns():
+    """A step and a check of several tokens (splits of both kinds), each its own graph, share the cache's workspace."""
+    rng = np.random.default_rng(23)
+    c, eager = (QuantisedCache(1, 4, 64, 3000) for _ in range(2))
+    k, v, q, q9 = (rows(rng, (1, n, 4, 64))[0] for n in (1, 1, 1, 9))
+    start = rows(rng, (1, 2500, 4, 64))[0]
+    for x in (c, eager):
+        x.append(start, start)
+    c.attend(q), c.attend(q9)
+    step, nine = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(step):
+        c.append(k, v)
+        out = c.attend(q)
+    with torch.cuda.graph(nine):
+        out9 = c.attend(q9)
+    for i in range(12):
+        for x in (k, v, q, q9):
+            x.copy_(torch.randn(x.shape, device="cuda"))
+        step.replay()
+        nine.replay()
+        eager.append(k, v)
+        assert torch.equal(out, eager.attend(q)) and torch.equal(out9, eager.attend(q9)), i
+
+
+def test_two_caches_on_two_streams_at_once():
+    rng = np.random.default_rng(24)
+    x, q = rows(rng, (2, 5000, 4, 64))[0], rows(rng, (2, 1, 4, 64))[0]
+    caches = [QuantisedCache(2, 4, 64, 5000) for _ in range(2)]
+    for c, y in zip(caches, (x, x.flip(1).contiguous())):
+        c.append(y, y)
+    want = [c.attend(q) for c in caches]
+    streams = [torch.cuda.Stream() for _ in caches]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(caches[i].attend(q))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
