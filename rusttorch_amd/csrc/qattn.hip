@@ -24,6 +24,7 @@
 #include "f16_pair.h"
 #include "qcache.h"
 #include "qrows.h"
+#include "qwrite.h"
 
 namespace rtg {
 namespace {
@@ -361,6 +362,7 @@ struct AttnArgs {
   float* part;               // partial results of split keys
   unsigned* joined;          // per block of columns: how many of its splits are done (0 between calls)
   int splits;
+  QRows new_k, new_v;        // of a decode step: its token's
 };
 
 // Column x of a key/value head's (x < 2^22, group <= 1024): query x / group, and
@@ -913,7 +915,10 @@ __device__ __forceinline__ void few_step(FewCols<HDP, NC>& c, const Tile<HDP>& t
 
 constexpr int kFewWaves = 8;
 
-template <int HDP, int NC, int KIND, class T>
+// STEP: a model's decode step. The key and value of the sequence's new token,
+// whose query this is, are first written into the cache by the workgroup that has
+// the last tile: no other reads a key of the block that this can change.
+template <int HDP, int NC, int KIND, class T, bool STEP>
 __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a) {
   constexpr int NW = kFewWaves;
   __shared__ Merge<HDP, NC, NW> s;
@@ -930,22 +935,32 @@ __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a
   const int shift = a.c.block_shift;
   Tile<HDP> t;
   int j = t0 + wave;
-  if (j < t1) {
-    t.load_k(kp, j, lane);
-    t.load_v(vp, j, lane);
-    t.load_s64(sp, j, shift, lane);
-  }
+  auto load = [&](Tile<HDP>& x, int tile) {
+    x.load_k(kp, tile, lane);
+    x.load_v(vp, tile, lane);
+    x.load_s64(sp, tile, shift, lane);
+  };
+  const bool fresh = STEP && j == tiles - 1;  // (this wave's first tile is the one that is written to)
+  if (j < t1 && !fresh) load(t, j);
   for (int i = lane; i < NC * 64; i += 64) reinterpret_cast<unsigned*>(image[wave])[i] = 0;
   FewCols<HDP, NC> c;
-  c.init(query_row<T>(a, seq, head, column(a, NC == 1 ? 0 : row >> 2)), a.c.hd, a.qvec, lane, a.scale);
+  if constexpr (STEP) {
+    const bool writes = t1 == tiles;
+    const OneToken<HDP, T, NW> token(a.c, seq, head, a.new_k, a.new_v, writes);
+    c.init(query_row<T>(a, seq, head, column(a, 0)), a.c.hd, a.qvec, lane, a.scale);
+    if (writes) {
+      token.write(a.c, Place{r.len - 1, r.len - 1, r.len, r.len - 1, 0}, sh);
+      __syncthreads();  // (a workgroup's stores are seen by its loads behind a barrier)
+      if (fresh) load(t, j);
+    }
+  } else {
+    c.init(query_row<T>(a, seq, head, column(a, NC == 1 ? 0 : row >> 2)), a.c.hd, a.qvec, lane, a.scale);
+  }
   const int qi = by_group(a, NC == 1 ? 0 : group);
   c.lim = qi < r.count ? visible(r, qi) : 0;
   for (; j < t1; j += NW) {
     Tile<HDP> n;
-    const int nj = min(j + NW, tiles - 1);
-    n.load_k(kp, nj, lane);
-    n.load_v(vp, nj, lane);
-    n.load_s64(sp, nj, shift, lane);
+    load(n, min(j + NW, tiles - 1));
     few_step<HDP, NC>(c, t, j * kQTile, j * kQTile + kQTile > least, live, lane, image[wave]);
     t = n;
   }
@@ -978,45 +993,46 @@ constexpr int kParts = 1024;
 // against 24.7).
 constexpr long kManyBlocks = 1400;
 
+// How many workgroups split a (sequence, head)'s block of columns' keys, at most.
+template <int HDP>
+dim3 split_grid(AttnArgs& a, bool few) {
+  const long heads = (long)a.c.n_seq * a.c.n_head;
+  if (few) a.cblocks = 1;
+  const int most = (a.c.tiles + 7) / 8;
+  a.splits = (int)std::max<long>(1, std::min<long>(most, parts<HDP>(few) / (heads * a.cblocks)));
+  return dim3((unsigned)heads, (unsigned)a.cblocks, (unsigned)a.splits);
+}
+
 template <int HDP, int ND, int KIND, class T>
 void attend(hipStream_t s, AttnArgs& a) {
   const long heads = (long)a.c.n_seq * a.c.n_head;
   const int columns = a.n_q * a.group, sh = a.c.block_shift;
-  if (columns <= 4) a.cblocks = 1;
-  const int most = (a.c.tiles + 7) / 8;
-  a.splits = (int)std::max<long>(1, std::min<long>(most, parts<HDP>(columns <= 4) / (heads * a.cblocks)));
-  const dim3 grid((unsigned)heads, (unsigned)a.cblocks, (unsigned)a.splits);
+  const dim3 grid = split_grid<HDP>(a, columns <= 4);
   if (columns == 1) {
-    q_attend_few_kernel<HDP, 1, KIND, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
-  } else if constexpr (KIND != QO_XT) {
-    if (columns > 4 && heads * a.cblocks >= kManyBlocks) {
-      const dim3 wide((unsigned)heads, (unsigned)((a.cblocks + 3) / 4));
-      if (sh == 4) q_attend_cols_kernel<HDP, ND, 4, KIND, T><<<wide, 256, 0, s>>>(a);
-      else if (sh == 5) q_attend_cols_kernel<HDP, ND, 5, KIND, T><<<wide, 256, 0, s>>>(a);
-      else q_attend_cols_kernel<HDP, ND, 6, KIND, T><<<wide, 256, 0, s>>>(a);
-    } else if (columns <= 4) {
-      q_attend_few_kernel<HDP, 4, KIND, T><<<grid, 64 * kFewWaves, 0, s>>>(a);
-    } else {
-      if (sh == 4) q_attend_split_kernel<HDP, ND, 4, KIND, T><<<grid, 256, 0, s>>>(a);
-      else if (sh == 5) q_attend_split_kernel<HDP, ND, 5, KIND, T><<<grid, 256, 0, s>>>(a);
-      else q_attend_split_kernel<HDP, ND, 6, KIND, T><<<grid, 256, 0, s>>>(a);
-    }
+    if constexpr (KIND == QO_ROWS) q_attend_few_kernel<HDP, 1, KIND, T, false><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  } else if (columns <= 4) {
+    q_attend_few_kernel<HDP, 4, KIND, T, false><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  } else if (heads * a.cblocks >= kManyBlocks) {
+    const dim3 wide((unsigned)heads, (unsigned)((a.cblocks + 3) / 4));
+    if (sh == 4) q_attend_cols_kernel<HDP, ND, 4, KIND, T><<<wide, 256, 0, s>>>(a);
+    else if (sh == 5) q_attend_cols_kernel<HDP, ND, 5, KIND, T><<<wide, 256, 0, s>>>(a);
+    else q_attend_cols_kernel<HDP, ND, 6, KIND, T><<<wide, 256, 0, s>>>(a);
+  } else {
+    if (sh == 4) q_attend_split_kernel<HDP, ND, 4, KIND, T><<<grid, 256, 0, s>>>(a);
+    else if (sh == 5) q_attend_split_kernel<HDP, ND, 5, KIND, T><<<grid, 256, 0, s>>>(a);
+    else q_attend_split_kernel<HDP, ND, 6, KIND, T><<<grid, 256, 0, s>>>(a);
   }
+}
+
+bool vec4(const QRows& r, int hd, size_t size) {
+  return hd % 4 == 0 && r.seq % 4 == 0 && r.tok % 4 == 0 && r.head % 4 == 0 &&
+         reinterpret_cast<uintptr_t>(r.p) % (4 * size) == 0;
 }
 
 template <int ND, class T>
 void attend_t(hipStream_t s, AttnArgs& a) {
-  const int hd = a.c.hd;
-  auto vec = [&](const QRows& r) {
-    return hd % 4 == 0 && r.seq % 4 == 0 && r.tok % 4 == 0 && r.head % 4 == 0 &&
-           reinterpret_cast<uintptr_t>(r.p) % (4 * sizeof(T)) == 0;
-  };
-  a.qvec = vec(a.q);
-  a.ovec = a.out.kind == QO_ROWS && vec(a.out.rows);
   if constexpr (sizeof(T) == 4) {
-    // (the model's layouts; a step's has one query per sequence and head)
     if (a.out.kind == QO_PAIR) return attend<64, ND, QO_PAIR, T>(s, a);
-    if (a.out.kind == QO_XT) return attend<64, ND, QO_XT, T>(s, a);
   }
   if (a.c.hdp == 64) attend<64, ND, QO_ROWS, T>(s, a);
   else attend<128, ND, QO_ROWS, T>(s, a);
@@ -1031,8 +1047,9 @@ void qattn_work_clear(hipStream_t s, void* work, int hdp) {
   (void)hipMemsetAsync(static_cast<char*>(work) + part_bytes(hdp), 0, (size_t)kParts * kQTicketStride * 4, s);
 }
 
-void launch_q_attend(hipStream_t s, const QStore& c, QLen len, int extra, QType type, const QRows& q, int n_q,
-                     int n_q_head, const int* counts, float scale, const QOut& out, void* work) {
+namespace {
+AttnArgs attn_args(const QStore& c, QLen len, int extra, QType type, const QRows& q, int n_q, int n_q_head,
+                   const int* counts, float scale, const QOut& out, void* work) {
   AttnArgs a{};
   a.c = c;
   a.len = len.p;
@@ -1046,13 +1063,33 @@ void launch_q_attend(hipStream_t s, const QStore& c, QLen len, int extra, QType 
   a.counts = counts;
   a.scale = scale;
   a.out = out;
+  const size_t size = type == Q_F32 ? 4 : 2;
+  a.qvec = vec4(q, c.hd, size);
+  a.ovec = out.kind == QO_ROWS && vec4(out.rows, c.hd, size);
   a.cblocks = (int)(((long)n_q * a.group + 15) / 16);
   a.part = static_cast<float*>(work);
   a.joined = reinterpret_cast<unsigned*>(static_cast<char*>(work) + part_bytes(c.hdp));
-  a.splits = 1;
+  return a;
+}
+}  // namespace
+
+void launch_q_attend(hipStream_t s, const QStore& c, QLen len, int extra, QType type, const QRows& q, int n_q,
+                     int n_q_head, const int* counts, float scale, const QOut& out, void* work) {
+  AttnArgs a = attn_args(c, len, extra, type, q, n_q, n_q_head, counts, scale, out, work);
   if (type == Q_F32) attend_t<3, float>(s, a);
   else if (type == Q_BF16) attend_t<2, __bf16>(s, a);
   else attend_t<2, _Float16>(s, a);
+}
+
+void launch_q_step(hipStream_t s, const QStore& c, QLen len, const QRows& k, const QRows& v, const QRows& q,
+                   float scale, const QOut& out, void* work) {
+  AttnArgs a = attn_args(c, len, 1, Q_F32, q, 1, c.n_head, nullptr, scale, out, work);
+  a.new_k = k;
+  a.new_v = v;
+  const dim3 grid = split_grid<64>(a, true);
+  if (out.kind == QO_XT) q_attend_few_kernel<64, 1, QO_XT, float, true><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  else if (out.kind == QO_PAIR) q_attend_few_kernel<64, 1, QO_PAIR, float, true><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  else q_attend_few_kernel<64, 1, QO_ROWS, float, true><<<grid, 64 * kFewWaves, 0, s>>>(a);
 }
 
 }  // namespace rtg

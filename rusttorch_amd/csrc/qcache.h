@@ -96,10 +96,10 @@ void launch_q_append(hipStream_t s, const QStore& c, QLen len, QTickets tickets,
 void launch_q_read(hipStream_t s, const QStore& c, QLen len, QType type, const QRows& k, const QRows& v, int n,
                    const int* first);
 
-// Attention results: rows (QRows), or the layouts of the model's next GEMM:
-// the pair GEMM's input scaled per column, or the batched decode GEMV's
-// (xt_index with n_seq rows; one query of as many heads as the cache has). Both
-// for f32 queries and head dims up to 64.
+// Attention results: rows (QRows), or the layouts of the model's next GEMM, for
+// f32 queries and head dims up to 64: the pair GEMM's input scaled per column
+// (as many query heads as the cache has), or the batched decode GEMV's
+// (launch_q_step; xt_index with n_seq rows).
 enum QOutKind { QO_ROWS = 0, QO_PAIR = 1, QO_XT = 2 };
 struct QOut {
   QOutKind kind = QO_ROWS;
@@ -117,6 +117,11 @@ struct QOut {
 // work: qattn_work_bytes() bytes, cleared once (qattn_work_clear).
 void launch_q_attend(hipStream_t s, const QStore& c, QLen len, int extra, QType type, const QRows& q, int n_q,
                      int n_q_head, const int* counts, float scale, const QOut& out, void* work);
+// A model's decode step: one f32 token k, v behind the length of every sequence
+// (which is below the capacity, and stays as it is), and its query's attention
+// over them all. Head dims up to 64, as many query heads as the cache has.
+void launch_q_step(hipStream_t s, const QStore& c, QLen len, const QRows& k, const QRows& v, const QRows& q,
+                   float scale, const QOut& out, void* work);
 size_t qattn_work_bytes(int hdp);
 void qattn_work_clear(hipStream_t s, void* work, int hdp);
 

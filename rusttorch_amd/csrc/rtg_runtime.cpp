@@ -539,9 +539,10 @@ static void q_attention(rtg_cache* c, size_t l, size_t T, const float* q, int ld
     out.rows.head = hd;
   }
   const QLen at{len, 0};
+  const float scale = 1.0f / sqrtf((float)hd);
+  if (T == 1) return launch_q_step(c->stream, st, at, k, v, qr, scale, out, c->q_work);
   launch_q_append(c->stream, st, at, QTickets{}, Q_F32, k, v, (int)T, nullptr, nullptr);
-  launch_q_attend(c->stream, st, at, (int)T, Q_F32, qr, (int)T, (int)m->cfg.n_head, nullptr,
-                  1.0f / sqrtf((float)hd), out, c->q_work);
+  launch_q_attend(c->stream, st, at, (int)T, Q_F32, qr, (int)T, (int)m->cfg.n_head, nullptr, scale, out, c->q_work);
 }
 static QOut q_rows(float* p) {
   QOut o;
