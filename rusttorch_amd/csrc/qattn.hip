@@ -43,12 +43,14 @@ __device__ __forceinline__ unsigned perm(unsigned a, unsigned b, unsigned sel) {
 }
 
 // Digit planes of four fixed-point values whose digits are the bytes of u0 .. u3
-// plus 128 (the top one of ND = 3 as it is): d[i] holds digit i of the four.
-template <int ND>
+// plus 128 (the top one of ND = 3, or of values that are not negative, as it is):
+// d[i] holds digit i of the four.
+template <int ND, bool POSITIVE = false>
 __device__ __forceinline__ void planes(unsigned u0, unsigned u1, unsigned u2, unsigned u3, unsigned (&d)[ND]) {
   const unsigned a = perm(u1, u0, 0x05010400), b = perm(u3, u2, 0x05010400);  // [x0 y0 x1 y1]
   d[0] = perm(b, a, 0x05040100) ^ 0x80808080u;
-  d[1] = perm(b, a, 0x07060302) ^ 0x80808080u;
+  d[1] = perm(b, a, 0x07060302);
+  if (ND == 3 || !POSITIVE) d[1] ^= 0x80808080u;
   if constexpr (ND == 3) d[2] = perm(perm(u3, u2, 0x0c0c0602), perm(u1, u0, 0x0c0c0602), 0x05040100);
 }
 
@@ -326,14 +328,14 @@ __device__ __forceinline__ void tile_probs(Cols<HDP, ND>& c, float (&s)[NG][4], 
     for (int i = 0; i < 4; ++i) c.o[d][i] *= corr;
   c.m = mn;
   w = g * ts.vmax * ((ND == 3 ? 256.f : 1.f) / fixed_max<ND>());
-  // rounded to an integer and biased, in the low bits of the sum with 2^23
-  constexpr float magic = ND == 3 ? 8421504.f : 8388608.f + 32896.f;  // 2^23 + 0x8080
+  // rounded to an integer, the digits below the top one plus 128, in the low bits of the sum with 2^23
+  constexpr float magic = ND == 3 ? 8421504.f : 8388736.f;  // 2^23 + 0x8080, 2^23 + 0x80
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     unsigned u[4], d[ND];
 #pragma unroll
     for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(fmaf(s[i][e], fixed_max<ND>(), magic));
-    planes<ND>(u[0], u[1], u[2], u[3], d);
+    planes<ND, true>(u[0], u[1], u[2], u[3], d);
 #pragma unroll
     for (int n = 0; n < ND; ++n) pd[i / 4][n][i & 3] = (int)d[n];
   }
@@ -507,10 +509,12 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
       load_lds16(voff, p + (size_t)tile * kQTile * HDP + (u - (second ? U / 2 : 0)) * 4096, lds + u * 4096);
     }
   };
+  // a pair whose second tile no column sees is taken by its first alone
+  auto half = [&](int j) { return live - j * kPair <= kQTile; };
   // (blocks of a second tile behind the capacity are those of the last one)
   auto load_s = [&](int j) {
-    const int b = (j * kPair >> SH) + (lane & ((kPair >> SH) - 1)), last = (a.c.tiles * kQTile >> SH) - 1;
-    return reinterpret_cast<const float2*>(sp)[min(b, last)];
+    const int nb = (half(j) ? kQTile : kPair) >> SH, last = (a.c.tiles * kQTile >> SH) - 1;
+    return reinterpret_cast<const float2*>(sp)[min((j * kPair >> SH) + (lane & (nb - 1)), last)];
   };
   float2 sl = make_float2(0.f, 0.f);
   if (pairs) {
@@ -522,11 +526,12 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
   const Column cl = column(a, max(cb, 0) * 16 + col);
   c.init(query_row<T>(a, seq, head, cl), a.c.hd, a.qvec, group, a.scale, cb >= 0 && cl.i < r.count ? visible(r, cl.i) : 0);
   wait_and_sync();
-  auto step = [&](int j, auto edge) {
-    const bool more = j + 1 < pairs;
-    float s[8][4], w;
+  auto step = [&](int j, auto edge, auto groups) {  // groups: of 16 keys
+    constexpr int NG = decltype(groups)::value;
+    const bool more = NG == 8 && j + 1 < pairs;
+    float s[NG][4], w;
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
+    for (int n = 0; n < NG; ++n) {
       i32x4 k[KS];
 #pragma unroll
       for (int e = 0; e < KS; ++e) k[e] = t.k[Pair::k_at(n * 16 + col, e * 4 + group)];
@@ -539,21 +544,27 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
       fetch(kp, j + 1, kv, lk);
       sl = load_s(j + 1);
     }
-    const TileScales<8, SH> ts = tile_scales<8, SH>(sj, live - j * kPair, lane);
-    i32x4 pd[2][ND];
+    const TileScales<NG, SH> ts = tile_scales<NG, SH>(sj, live - j * kPair, lane);
+    i32x4 pd[NG / 4][ND];
     tile_probs<decltype(edge)::value>(c, s, ts, j * kPair, group, pd, w);
 #pragma unroll
     for (int d = 0; d < HDP / 16; ++d) {
-      const i32x4 v[2] = {t.v[group * HDP + d * 16 + col], t.v[(4 + group) * HDP + d * 16 + col]};
-      tile_product<ND, 2>(v, pd, w, c.o[d]);
+      i32x4 v[NG / 4];
+#pragma unroll
+      for (int i = 0; i < NG / 4; ++i) v[i] = t.v[(i * 4 + group) * HDP + d * 16 + col];
+      tile_product<ND, NG / 4>(v, pd, w, c.o[d]);
       if (d & 1) __builtin_amdgcn_sched_barrier(0);
     }
-    wait_and_sync();  // the values are read; the next pair's keys are there
-    if (more) fetch(vp, j + 1, vv, lv);
+    if (more) {
+      wait_and_sync();  // the values are read; the next pair's keys are there
+      fetch(vp, j + 1, vv, lv);
+    }
   };
+  using Pairs = std::integral_constant<int, 8>;
   int j = 0;
-  for (; j < full; ++j) step(j, std::false_type());
-  for (; j < pairs; ++j) step(j, std::true_type());
+  for (; j < full; ++j) step(j, std::false_type(), Pairs());
+  for (; j < pairs && !half(j); ++j) step(j, std::true_type(), Pairs());
+  if (j < pairs) step(j, std::true_type(), std::integral_constant<int, 4>());
   const float l = xsum(c.l);
   if (cb < 0 || cl.i >= a.n_q) return;
   const float inv = c.lim > 0 ? 1.f / l : 0.f;
