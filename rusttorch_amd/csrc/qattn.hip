@@ -674,37 +674,56 @@ __device__ __forceinline__ void finish(const AttnArgs& a, Merge<HDP, W, NW>& s, 
   const int g = tid / C4, wave = tid >> 6, zg = g & (gpc - 1);
   for (int col0 = 0; col0 < cols; col0 += CPP / gpc) {
     const int col = min(col0 + g / gpc, cols - 1);
-    float m = -INFINITY;
-    for (int z2 = tid % C4; z2 < n; z2 += C4) m = fmaxf(m, load2(part_of<HDP, W>(a, sh, cb, z2, col)).x);
-    m = row_max(m);
-    if constexpr (C4 == 32) m = xor16_max_k(m);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
+    float m = -INFINITY, l = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int z2 = zg; z2 < n; z2 += gpc) {
-      const float* p = part_of<HDP, W>(a, sh, cb, z2, col);
-      const float2 ml = load2(p), y0 = load2(p + 2 + c4), y1 = load2(p + 4 + c4);
-      const float f = __builtin_amdgcn_exp2f(ml.x - base);
-      l = fmaf(f, ml.y, l);
-      x = make_float4(fmaf(f, y0.x, x.x), fmaf(f, y0.y, x.y), fmaf(f, y1.x, x.z), fmaf(f, y1.y, x.w));
+    // (their way through memory takes over a microsecond: U at a time)
+    constexpr int U = W == 16 ? 8 : 4;
+    for (int z0 = zg; z0 < n; z0 += gpc * U) {
+      float2 ml[U], y[U][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float* p = part_of<HDP, W>(a, sh, cb, min(z0 + u * gpc, n - 1), col);
+        ml[u] = load2(p);
+        y[u][0] = load2(p + 2 + c4);
+        y[u][1] = load2(p + 4 + c4);
+      }
+      float most = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) most = fmaxf(most, ml[u].x);
+      const float base = most == -INFINITY ? 0.f : most, corr = __builtin_amdgcn_exp2f(m - base);
+      m = most;
+      l *= corr;
+      x = make_float4(x.x * corr, x.y * corr, x.z * corr, x.w * corr);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (z0 + u * gpc >= n) break;
+        const float f = __builtin_amdgcn_exp2f(ml[u].x - base);
+        l = fmaf(f, ml[u].y, l);
+        x = make_float4(fmaf(f, y[u][0].x, x.x), fmaf(f, y[u][0].y, x.y), fmaf(f, y[u][1].x, x.z), fmaf(f, y[u][1].y, x.w));
+      }
     }
-    for (int w = 1; w < gpc && w < GPW; w *= 2) {
-      l += __shfl_xor(l, w * C4);
-      x = make_float4(x.x + __shfl_xor(x.x, w * C4), x.y + __shfl_xor(x.y, w * C4), x.z + __shfl_xor(x.z, w * C4),
-                      x.w + __shfl_xor(x.w, w * C4));
-    }
-    bool first = zg == 0;
+    // takes another group's results m2, l2, x2 in
+    auto add = [&](float m2, float l2, const float4& x2) {
+      const float most = fmaxf(m, m2), base = most == -INFINITY ? 0.f : most;
+      const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+      m = most;
+      l = fmaf(f, l, f2 * l2);
+      x = make_float4(fmaf(f, x.x, f2 * x2.x), fmaf(f, x.y, f2 * x2.y), fmaf(f, x.z, f2 * x2.z), fmaf(f, x.w, f2 * x2.w));
+    };
+    for (int w = 1; w < gpc && w < GPW; w *= 2)
+      add(__shfl_xor(m, w * C4), __shfl_xor(l, w * C4),
+          make_float4(__shfl_xor(x.x, w * C4), __shfl_xor(x.y, w * C4), __shfl_xor(x.z, w * C4), __shfl_xor(x.w, w * C4)));
+    const bool first = zg == 0;
     if (gpc > GPW) {  // (uniform) a column's waves meet in LDS
       if ((tid & 63) < C4) *reinterpret_cast<float4*>(&s.o[wave][0][c4]) = x;
-      if ((tid & 63) == 0) s.l[wave][0] = l;
+      if ((tid & 63) == 0) {
+        s.m[wave][0] = m;
+        s.l[wave][0] = l;
+      }
       __syncthreads();
       if (first)
-        for (int w = 1; w < gpc / GPW; ++w) {
-          const float4 y = *reinterpret_cast<const float4*>(&s.o[wave + w][0][c4]);
-          l += s.l[wave + w][0];
-          x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-        }
+        for (int w = 1; w < gpc / GPW; ++w)
+          add(s.m[wave + w][0], s.l[wave + w][0], *reinterpret_cast<const float4*>(&s.o[wave + w][0][c4]));
       __syncthreads();
     }
     if (first && col0 + g / gpc < cols) put(col, l, x);
@@ -737,12 +756,7 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
     t.load_k(kp, j, lane);
     t.load_v(vp, j, lane);
   }
-  for (; j < t1; j += NW) {
-    Tile<HDP> n;
-    const int nj = min(j + NW, tiles - 1);
-    n.load_s(sp, nj, SH, lane);
-    n.load_k(kp, nj, lane);
-    n.load_v(vp, nj, lane);
+  auto step = [&] {
     const TileScales<4, SH> ts = tile_scales<4, SH>(t.s, live - j * kQTile, lane);
     float sums[4][4];
     i32x4 pd[1][ND];
@@ -756,8 +770,16 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
       const i32x4 v[1] = {t.v[d]};
       tile_product<ND, 1>(v, pd, w, c.o[d]);
     }
+  };
+  for (; j + NW < t1; j += NW) {
+    Tile<HDP> n;
+    n.load_s(sp, j + NW, SH, lane);
+    n.load_k(kp, j + NW, lane);
+    n.load_v(vp, j + NW, lane);
+    step();
     t = n;
   }
+  if (j < t1) step();
   const float l = xsum(c.l);
   if (group == 0) {
     s.m[wave][col] = c.m;
@@ -969,12 +991,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a
   }
   const int qi = by_group(a, NC == 1 ? 0 : group);
   c.lim = qi < r.count ? visible(r, qi) : 0;
-  for (; j < t1; j += NW) {
+  auto step = [&] { few_step<HDP, NC>(c, t, j * kQTile, j * kQTile + kQTile > least, live, lane, image[wave]); };
+  for (; j + NW < t1; j += NW) {
     Tile<HDP> n;
-    load(n, min(j + NW, tiles - 1));
-    few_step<HDP, NC>(c, t, j * kQTile, j * kQTile + kQTile > least, live, lane, image[wave]);
+    load(n, j + NW);
+    step();
     t = n;
   }
+  if (j < t1) step();  // (a load behind the last tile, though nobody needs it, would be waited for)
   float l = row16_sum_k(c.l);
   if constexpr (NC == 1) l = xsum(l);
   if (row == 0 && (NC > 1 || group == 0)) {
