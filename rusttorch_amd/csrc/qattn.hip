@@ -579,13 +579,20 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
 
 // ---- few columns: the keys are split over workgroups and over their waves ----
 
-// Tiles per split for `tiles` tiles over at most `splits` workgroups: all of them
-// where they are few (a split costs 3 to 4 us, the partials' way through memory;
-// eight waves take 8 tiles in 0.7 us more than one), else at least two or one per wave.
-template <int HDP>
+// Tiles per split for `tiles` tiles over at most `splits` workgroups. All of them
+// up to as many as a workgroup takes in the time of a split (2.5 to 3.5 us: the
+// partials' way through memory and back): 8 heads of 128, 1000 tokens: 9.1 us
+// whole, 10.1 split, 1250: 11.2 and 10.5; 16 of 64, 2000: 6.9 and 8.1, 3000: 8.1
+// both; 7 columns a head of 64, 1500: 8.1 and 8.9; 8 a head of 128, 750: 8.4 and
+// 9.6, 1000: 9.7 both. Then at least two or one per wave; for 16 columns, whose
+// join is longer, also so many that the splits to join cost no more than their
+// tiles (16 columns a head of 128, 32000: 15 tiles each 20.3 us, 8 each 26.6).
+template <int HDP, int W>
 __device__ __forceinline__ int split_tiles(int tiles, int splits) {
-  constexpr int least = HDP == 64 ? 16 : 8;
-  return tiles <= least ? max(tiles, 1) : max((tiles + splits - 1) / splits, least);
+  constexpr int whole = W == 16 ? HDP == 64 ? 28 : 12 : HDP == 64 ? 40 : 16, least = HDP == 64 ? 16 : 8;
+  if (tiles <= whole) return max(tiles, 1);
+  const int per = W == 16 ? (int)__builtin_amdgcn_sqrtf((HDP == 64 ? 0.5f : 0.75f) * tiles) / 4 * 4 : 0;
+  return max(max((tiles + splits - 1) / splits, least), per);
 }
 
 // A column's partial: m, l, o[hdp]. Blocks of W columns.
@@ -742,7 +749,7 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
   const int last = min(by_group(a, cb * 16 + 15), r.count - 1);
   const int live = firstq < r.count ? visible(r, last) : 0;
   const int least = firstq < r.count ? visible(r, firstq) : 0;
-  const int tiles = (live + kQTile - 1) / kQTile, per = split_tiles<HDP>(tiles, a.splits);
+  const int tiles = (live + kQTile - 1) / kQTile, per = split_tiles<HDP, 16>(tiles, a.splits);
   const int t0 = z * per, t1 = min(t0 + per, tiles);
   if (z > 0 && t0 >= tiles) return;  // (the whole workgroup; split 0 also writes rows without keys)
   Cols<HDP, ND> c;
@@ -960,7 +967,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a
   const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head, z = blockIdx.z;
   const Seq r = seq_of(a, seq);
   const int live = r.count > 0 ? visible(r, r.count - 1) : 0, least = r.count > 0 ? visible(r, 0) : 0;
-  const int tiles = (live + kQTile - 1) / kQTile, per = split_tiles<HDP>(tiles, a.splits);
+  const int tiles = (live + kQTile - 1) / kQTile, per = split_tiles<HDP, NC>(tiles, a.splits);
   const int t0 = z * per, t1 = min(t0 + per, tiles);
   if (z > 0 && t0 >= tiles) return;  // (the whole workgroup)
   const int8_t *kp = a.c.k + a.c.codes(sh), *vp = a.c.v + a.c.codes(sh);
