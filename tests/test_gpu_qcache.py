@@ -532,3 +532,36 @@ def test_two_caches_on_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+@pytest.mark.parametrize("dim,group,block,length", [
+    (64, 1, 32, 2560), (64, 1, 32, 2561), (64, 3, 16, 2600), (128, 1, 64, 1025), (128, 2, 16, 1100),
+    (64, 7, 32, 1792), (64, 7, 32, 1793), (128, 8, 64, 768), (128, 16, 32, 769), (128, 16, 64, 14000),
+    (64, 16, 64, 52000), (128, 40, 16, 2000)])
+def test_splits(dim, group, block, length):
+    """Lengths from which the keys are split, and splits of more tiles than the fewest."""
+    b = Both(1, 1, dim, length + 20, block, "f16", seed=length)
+    k, kn = rows(b.rng, (1, length, 1, dim), "f16")
+    b.c.append(k, k)
+    b.r.append(kn, kn)
+    q, qn = rows(b.rng, (1, 1, group, dim), "f16", 2.0)
+    near(b.c.attend(q), b.r, qn, "f16")
+
+
+@pytest.mark.parametrize("dim,group,block,dtype", [(64, 20, 16, "f32"), (128, 20, 64, "bf16"), (40, 22, 32, "f16")])
+def test_many_columns_of_several_pairs_of_tiles(dim, group, block, dtype):
+    b = Both(2, 4, dim, 330, block, dtype, seed=dim)
+    b.append(321, counts=[190, 321])
+    q, qn = rows(b.rng, (2, 150, 4 * group, dim), dtype, 2.0)
+    near(b.c.attend(q, counts=ints([150, 141])), b.r, qn, dtype, [150, 141])
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "f32"), (128, "f16"), (20, "bf16")])
+def test_long_reads_of_sequences_of_different_lengths(dim, dtype):
+    b = Both(5, 2, dim, 1700, 32, dtype, seed=dim)
+    k, kn = rows(b.rng, (5, 1700, 2, dim), dtype)
+    lens = [0, 1, 700, 1664, 1700]
+    b.c.append(k, k, counts=ints(lens))
+    b.r.append(kn, kn, lens)
+    b.same(1700)
+    b.same(1600, [0, 5, 690, -70, 200])
