@@ -448,7 +448,10 @@ struct RowOut {
 //
 // Two tiles at a time: 128 keys share the maximum, the scales and the conversion
 // of their products with the values (a third of the vector work, which bounds
-// this kernel: about 250 instructions per 64 keys and 16 columns). A workgroup's
+// this kernel: about 235 instructions per 64 keys and 16 columns in f32 and 220 at
+// 128 columns in 16 bits, 81 to 85 % of the cycles; matrix instructions take 24 to
+// 37 %. 16 x 1023 tokens of 20 heads in f32: 124 us; 2047 tokens of 32 heads of 128
+// behind 12001 in bf16: 510 us, 857 TFLOP/s). A workgroup's
 // four waves read them from LDS, where LDS-direct loads put the next pair's keys
 // once every wave has this pair's sums, and its values once every wave has its
 // products. (Codes widened to f16, whose products need no joining of digits, take
@@ -578,6 +581,9 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
 }
 
 // ---- few columns: the keys are split over workgroups and over their waves ----
+//
+// (five tokens of 16 heads of six sequences behind 700: 7 us, all of it latency:
+// the launch, the queries, a tile or two, the waves' results through LDS)
 
 // Tiles per split for `tiles` tiles over at most `splits` workgroups. All of them
 // up to as many as a workgroup takes in the time of a split (2.5 to 3.5 us: the
@@ -808,7 +814,10 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
 // columns (NC = 4): each has four rows, a lane has four keys of one of them. The
 // probabilities' digits pass through LDS into the same rows for P V, which leaves
 // a lane with one result of 64 (or with every 16th of its column's). A tile then
-// takes 70 (NC = 4: 130) vector instructions where a wave of 16 columns takes 400.
+// takes 70 (NC = 4: 130) vector instructions where a wave of 16 columns takes 400,
+// and memory bounds long caches: 50001 tokens of 16 heads 21 us (4.8 TB/s, where a
+// large copy has 5.4), 8 x 32000 of 8 heads of 128 with four columns each 81 us
+// (4.9 TB/s); 16 x 960 tokens of 25 heads take 10 us, 3 of them latency.
 template <int HDP, int NC>
 struct FewCols {
   static constexpr int KS = HDP / 64, DT = HDP / 16, NO = NC == 1 ? HDP / 64 : DT;
@@ -1021,7 +1030,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a
 }
 
 // Workgroups of split keys: as many as the device holds at once, which the
-// registers decide (few columns: 106 and 174 of them, 16 columns: 144 and 218).
+// registers decide (few columns: 120 and 181 of them, 16 columns: 148 and 238).
 template <int HDP>
 constexpr int parts(bool few) {
   return few ? HDP == 64 ? 512 : 256 : HDP == 64 ? 768 : 512;

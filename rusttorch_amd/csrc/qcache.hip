@@ -324,7 +324,9 @@ __device__ __forceinline__ void append_tile(const QStore& c, const Place& p, siz
   }
 }
 
-// A workgroup per (sequence, head, tile) and side (keys, values).
+// A workgroup per (sequence, head, tile) and side (keys, values). Memory bounds it
+// (8 x 1000 tokens of 12 heads of 64 in f32: 18 us, 3.4 TB/s); short appends are
+// latency: length, rows, the block's earlier tokens (4 x 517 of 8 heads of 128: 12.7 us).
 template <int HDP, class T>
 __global__ __launch_bounds__(256) void q_append_kernel(QStore c, QLen len, QTickets tickets, QRows k, QRows v, int n_new,
                                                        const int* __restrict__ counts, const int* __restrict__ start,
@@ -346,6 +348,7 @@ __global__ __launch_bounds__(256) void q_append_kernel(QStore c, QLen len, QTick
 }
 
 // One new token (or only a cut) for each sequence: a workgroup per (sequence, head).
+// Latency bounds it: 4.1 us for 16 sequences of 25 heads, 400 workgroups.
 template <int HDP, class T>
 __global__ __launch_bounds__(256) void q_append_one_kernel(QStore c, QLen len, QTickets tickets, QRows k, QRows v,
                                                            int n_new, const int* __restrict__ counts,
@@ -391,7 +394,7 @@ __device__ __forceinline__ void put_cols(T* row, int c, int n, const float (&x)[
 // transposed in registers, 4 x 4 bytes at a time. Codes and scales of short reads
 // are loaded before the sequence's length is known (they lie within the capacity):
 // 0.2 to 0.35 us less for 333 and 1000 tokens, but 4 x 20000 and 16 x 2000 of different
-// lengths took 103.6 and 36.5 us where 100.7 and 34.6 do without what lies behind.
+// lengths took 103.6 and 36.5 us where 101.2 (4.5 TB/s) and 34.6 do without what lies behind.
 constexpr int kLongRead = 1500;
 template <int HDP, class T, int CPL>
 __global__ __launch_bounds__(256) void q_read_kernel(QStore c, const int* __restrict__ len, int len_stride, QRows k,

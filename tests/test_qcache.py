@@ -49,3 +49,12 @@ def test_definition():
     assert c.append(x, x, start=[41]) == [0] and c.append(x, x, start=[1], counts=[0]) == []
     assert c.length(0) == 1
     assert np.allclose(c.attend(np.ones((1, 1, 1, 8)))[0, 0, 0], c.read(1)[1][0, 0, 0])
+
+
+@pytest.mark.parametrize("args,what", [((-1, 1, 64, 10), "n_seq must not be negative"),
+                                       ((1, 1, 64, 2 ** 64 + 10), "capacity is too large")])
+def test_sizes_that_the_library_could_not_tell_apart(args, what):
+    from rusttorch_amd.qcache import QuantisedCache
+
+    with pytest.raises(Gpt2Error, match=what):
+        QuantisedCache(*args)
