@@ -135,10 +135,13 @@ class QuantisedCache:
         n, heads = q.shape[1], q.shape[2]
         rows = self._rows("q", q, q.dtype, n, heads)
         if out is None:
-            out = torch.empty_like(q)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            tok = heads * self.head_dim
+            to = _pack_rows(out.data_ptr(), n * tok, tok, self.head_dim)
+        else:
+            to = self._rows("out", out, q.dtype, n, heads)
         check(self._lib.rtg_qcache_attend(self._h, dtype, rows, n, heads, self._ints("counts", counts),
-                                          self.head_dim ** -0.5 if scale is None else scale,
-                                          self._rows("out", out, q.dtype, n, heads), stream))
+                                          self.head_dim ** -0.5 if scale is None else scale, to, stream))
         return out
 
     def read(self, n: int, first=None, dtype: torch.dtype = torch.float32, k=None, v=None):
@@ -148,12 +151,17 @@ class QuantisedCache:
             raise Gpt2Error("n must not be negative")
         if dtype not in _TYPES:
             raise Gpt2Error(f"dtype must be f32, bf16 or f16, not {dtype}")
-        shape = (self.n_seq, n, self.n_head, self.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=self.device) if k is None else k
-        v = torch.empty_like(k) if v is None else v
-        check(self._lib.rtg_qcache_read(self._h, _TYPES[dtype], self._rows("k", k, dtype, n, self.n_head),
-                                        self._rows("v", v, dtype, n, self.n_head), n, self._ints("first", first),
-                                        stream))
+        first = self._ints("first", first)
+        if k is None and v is None:
+            head, tok = self.head_dim, self.n_head * self.head_dim
+            k = torch.empty((self.n_seq, n, self.n_head, head), dtype=dtype, device=self.device)
+            v = torch.empty_like(k)
+            to_k, to_v = (_pack_rows(x.data_ptr(), n * tok, tok, head) for x in (k, v))
+        else:
+            k = torch.empty_like(v) if k is None else k  # (checked below, as the other's are)
+            v = torch.empty_like(k) if v is None else v
+            to_k, to_v = self._rows("k", k, dtype, n, self.n_head), self._rows("v", v, dtype, n, self.n_head)
+        check(self._lib.rtg_qcache_read(self._h, _TYPES[dtype], to_k, to_v, n, first, stream))
         return k, v
 
     def lengths(self) -> list:

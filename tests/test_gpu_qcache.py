@@ -565,3 +565,20 @@ def test_long_reads_of_sequences_of_different_lengths(dim, dtype):
     b.r.append(kn, kn, lens)
     b.same(1700)
     b.same(1600, [0, 5, 690, -70, 200])
+
+
+def test_results_of_other_orders_and_given_ones():
+    rng = np.random.default_rng(25)
+    c = QuantisedCache(2, 3, 64, 200)
+    k, q = rows(rng, (2, 150, 3, 64))[0], rows(rng, (2, 20, 6, 64))[0]
+    c.append(k, k)
+    want = c.attend(q)
+    swapped = q.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(c.attend(swapped), want) and c.attend(swapped).is_contiguous()
+    assert torch.equal(c.attend(q[:, :1].expand(2, 20, 6, 64))[:, :1], c.attend(q[:, :1].repeat(1, 20, 1, 1))[:, :1])
+    out = torch.empty(2, 6, 20, 64, device="cuda").transpose(1, 2)
+    assert c.attend(q, out=out) is out and torch.equal(out, want)
+    both = c.read(170)
+    mine = torch.full((2, 3, 170, 64), 7.0, device="cuda").transpose(1, 2)
+    for got in (c.read(170, k=mine), c.read(170, v=mine)):
+        assert all(torch.equal(a, b) for a, b in zip(got, both))
