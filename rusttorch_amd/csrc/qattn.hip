@@ -1037,12 +1037,15 @@ constexpr int parts(bool few) {
 }
 constexpr int kParts = 1024;
 
-// Blocks of 16 columns from which every wave takes all keys of its own: 1.4 for
-// each of the device's 1024 SIMDs. Below, splitting the keys fills it better (1264
-// blocks: 184 against 231 us over 15000 keys, 19.2 against 21.0 for prompts of
-// 1023), above it only reads them more often (1548: 13.3 against 10.4, 2000: 46.7
-// against 24.7).
-constexpr long kManyBlocks = 1400;
+// Blocks of 16 columns from which every wave takes all keys of its own. hdp 64:
+// 1.4 for each of the device's 1024 SIMDs; below, splitting the keys fills it
+// better (1264 blocks: 184 against 231 us over 15000 keys, 19.2 against 21.0 for
+// prompts of 1023), above it only reads them more often (1548: 13.3 against 10.4,
+// 2000: 46.7 against 24.7). hdp 128: what it reads counts earlier (640: 170
+// against 185 us over 12000 keys, 12.4 against 10.2 for a prompt of 320; 1000: 227
+// against 188, 16.4 against 12.9 for one of 500).
+template <int HDP>
+constexpr long kManyBlocks = HDP == 64 ? 1400 : 800;
 
 // How many workgroups split a (sequence, head)'s block of columns' keys, at most.
 template <int HDP>
@@ -1063,7 +1066,7 @@ void attend(hipStream_t s, AttnArgs& a) {
     if constexpr (KIND == QO_ROWS) q_attend_few_kernel<HDP, 1, KIND, T, false><<<grid, 64 * kFewWaves, 0, s>>>(a);
   } else if (columns <= 4) {
     q_attend_few_kernel<HDP, 4, KIND, T, false><<<grid, 64 * kFewWaves, 0, s>>>(a);
-  } else if (heads * a.cblocks >= kManyBlocks) {
+  } else if (heads * a.cblocks >= kManyBlocks<HDP>) {
     const dim3 wide((unsigned)heads, (unsigned)((a.cblocks + 3) / 4));
     if (sh == 4) q_attend_cols_kernel<HDP, ND, 4, KIND, T><<<wide, 256, 0, s>>>(a);
     else if (sh == 5) q_attend_cols_kernel<HDP, ND, 5, KIND, T><<<wide, 256, 0, s>>>(a);
