@@ -98,7 +98,7 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
   top = max(r2[0], r2[1]);
   float amax = __uint_as_float(top);
   const bool fine = top < 0x7F800000u;
-  float unit = fabsf(scale) * 1.4426950408889634f * (ND == 3 ? 256.f : 1.f) / fixed_max<ND>();
+  float unit = fabsf(scale) * 1.4426950408889634f * (ND == 3 ? 256.f : 1.f);
   if (__builtin_amdgcn_ballot_w64(amax < 7.9e-31f)) {
     asm volatile("");
     // rows below 2^-100 are taken 2^100 times as large, so that 1 / amax is a number
@@ -112,7 +112,8 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
       for (int e = 0; e < 4; ++e)
         x[k][e] = make_float4(x[k][e].x * up, x[k][e].y * up, x[k][e].z * up, x[k][e].w * up);
   }
-  // (a negative scale goes into the digits: the factor of the sums is not negative)
+  // (a negative scale goes into the digits: the factor of the sums is not negative;
+  // it comes from inv as it was rounded, or all scores would be off by its rounding)
   const float inv = fine && amax > 0.f ? copysignf(fixed_max<ND>(), scale) / amax : 0.f;
   constexpr float bias = ND == 3 ? 8421504.f : 32896.f;  // 0x808080, 0x8080: every digit plus 128
 #pragma unroll
@@ -128,7 +129,7 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
 #pragma unroll
       for (int i = 0; i < ND; ++i) q[k][i][e] = (int)d[i];
     }
-  return fine ? amax * unit : NAN;
+  return !fine ? NAN : amax > 0.f ? unit / fabsf(inv) : 0.f;
 }
 
 // A wave's 16 columns: lane = group * 16 + column; the group's 16 (of 64) query
@@ -814,8 +815,8 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
 // columns (NC = 4): each has four rows, a lane has four keys of one of them. The
 // probabilities' digits pass through LDS into the same rows for P V, which leaves
 // a lane with one result of 64 (or with every 16th of its column's). A tile then
-// takes 70 (NC = 4: 130) vector instructions where a wave of 16 columns takes 400,
-// and memory bounds long caches: 50001 tokens of 16 heads 21 us (4.8 TB/s, where a
+// takes about 140 vector instructions at 64 columns (NC = 4: 300 at 128) where a
+// wave of 16 columns takes 400 (700), and memory bounds long caches: 50001 tokens of 16 heads 21 us (4.8 TB/s, where a
 // large copy has 5.4), 8 x 32000 of 8 heads of 128 with four columns each 81 us
 // (4.9 TB/s); 16 x 960 tokens of 25 heads take 10 us, 3 of them latency.
 template <int HDP, int NC>
@@ -862,8 +863,19 @@ struct FewCols {
 };
 
 __device__ __forceinline__ int fixed_sum(const i32x4& d) { return (d[2] << 8) + d[1] + ((d[0] + 128) >> 8); }
+// the same with the row of ones, in units w of 256, plus what there is
+__device__ __forceinline__ float add_sum(const i32x4& d, float w, float o) {
+  return fmaf((float)((d[3] << 15) + (d[2] << 8) + d[1]), w, fmaf((float)d[0], w * 0.00390625f, o));
+}
 
-// image: this wave's digit planes, [NC][4][4][16] bytes, those of digit 3 zero
+// A tile's largest probability as a fixed-point number from 0 to 2^24: its digits
+// are those of 2^23 less, and the row behind them holds ones, whose sum times 2^23
+// is what is missing: a bit more than the three digits have for numbers that are
+// not negative. (Of the integers below 2^24 - 0x8080 less a margin for roundings
+// the one whose inverse is nearest to a float.)
+constexpr float kFewMax = 16741781.f;
+
+// image: this wave's digit planes, [NC][4][4][16] bytes, those of digit 3 one
 template <int HDP, int NC>
 __device__ __forceinline__ void few_step(FewCols<HDP, NC>& c, const Tile<HDP>& t, int j0, bool edge, int live, int lane,
                                          unsigned char* image) {
@@ -926,12 +938,13 @@ __device__ __forceinline__ void few_step(FewCols<HDP, NC>& c, const Tile<HDP>& t
   ptop = row_max(ptop);
   if constexpr (NC == 1) ptop = xmax(ptop);
   const float pinv = ptop >= 1.2e-38f ? __builtin_amdgcn_rcpf(ptop) : 0.f;
-  const float w = ptop * (256.f / fixed_max<3>());
+  // 1 / pinv, not ptop: the instruction's error would be in all results
+  const float w = fmaf(ptop, fmaf(-ptop, pinv, 1.f), ptop) * (256.f / kFewMax);
   const int column = NC == 1 ? 0 : group;
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    // 2^23 + 0x8080 + the fixed-point value: its bytes are the digits, plus 128 but for the top one
-    const unsigned u = __float_as_uint(fmaf(s[i] * pinv, fixed_max<3>(), 8421504.f)) ^ 0x8080u;
+    // the bytes of the number less 2^23 plus 0x8080 are the digits, plus 128 but for the top one
+    const unsigned u = ((unsigned)rintf(s[i] * pinv * kFewMax) - 0x7F7F80u) ^ 0x8080u;
     unsigned char* p = image + column * 256 + ((key(i) >> 2) & 3) * 16 + (key(i) >> 4) * 4 + (key(i) & 3);
     p[0] = (unsigned char)u;
     p[64] = (unsigned char)(u >> 8);
@@ -950,15 +963,15 @@ __device__ __forceinline__ void few_step(FewCols<HDP, NC>& c, const Tile<HDP>& t
     for (int h = 0; h < HDP / 64; ++h) {
       i32x4 x;
 #pragma unroll
-      for (int e = 0; e < 3; ++e) {
+      for (int e = 0; e < 4; ++e) {
         const int lo = (group & 1) ? r[h * 4 + 1][e] : r[h * 4][e], hi = (group & 1) ? r[h * 4 + 3][e] : r[h * 4 + 2][e];
         x[e] = (group & 2) ? hi : lo;
       }
-      c.o[h] = fmaf((float)fixed_sum(x), w, c.o[h] * corr);
+      c.o[h] = add_sum(x, w, c.o[h] * corr);
     }
   } else {
 #pragma unroll
-    for (int d = 0; d < DT; ++d) c.o[d] = fmaf((float)fixed_sum(r[d]), w, c.o[d] * corr);
+    for (int d = 0; d < DT; ++d) c.o[d] = add_sum(r[d], w, c.o[d] * corr);
   }
 }
 
@@ -991,7 +1004,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a
   };
   const bool fresh = STEP && j == tiles - 1;  // (this wave's first tile is the one that is written to)
   if (j < t1 && !fresh) load(t, j);
-  for (int i = lane; i < NC * 64; i += 64) reinterpret_cast<unsigned*>(image[wave])[i] = 0;
+  for (int i = lane; i < NC * 64; i += 64) reinterpret_cast<unsigned*>(image[wave])[i] = (i & 63) < 48 ? 0 : 0x01010101u;
   FewCols<HDP, NC> c;
   if constexpr (STEP) {
     const bool writes = t1 == tiles;
