@@ -389,14 +389,19 @@ __device__ __forceinline__ void put_cols(T* row, int c, int n, const float (&x)[
 }
 
 // A wave per (sequence, head), side and so many 64-token tiles of the cache that
-// its lanes have 16 tokens each: CPL columns (16 bytes of T, one store) of the
-// tokens t * 16 + group * 4 + e. Values come as 16 bytes of a column and are
-// transposed in registers, 4 x 4 bytes at a time. Codes and scales of short reads
-// are loaded before the sequence's length is known (they lie within the capacity):
-// 0.2 to 0.35 us less for 333 and 1000 tokens, but 4 x 20000 and 16 x 2000 of different
-// lengths took 103.6 and 36.5 us where 101.2 (4.5 TB/s) and 34.6 do without what lies behind.
+// its lanes have 4 * TPL tokens each: CPL columns (16 bytes of T, one store) of the
+// tokens (t0 + t) * 16 + group * 4 + e. Values come as 4 * TPL bytes of a column and
+// are transposed in registers, 4 x 4 bytes at a time. Few workgroups are latency and
+// take TPL = 1 (333 tokens of 12 heads of 64: 3.9 us against 5.7 in f32, 4.6 against
+// 8.0 in bf16; 4 x 580 of 8 of 128 in bf16: 6.9 against 9.1), many are memory and
+// take 4 (16 x 1000 of 16 heads of 128: 61.8 against 68.0, 32.4 against 36.5; equal
+// at 600 workgroups). Codes and scales of short reads are loaded before the
+// sequence's length is known (they lie within the capacity): 0.2 to 0.35 us less for
+// 333 and 1000 tokens, but 4 x 20000 and 16 x 2000 of different lengths took 103.6 and
+// 36.5 us where 101.2 (4.5 TB/s) and 34.6 do without what lies behind.
 constexpr int kLongRead = 1500;
-template <int HDP, class T, int CPL>
+constexpr long kFewReads = 600;  // workgroups of TPL = 4
+template <int HDP, class T, int CPL, int TPL>
 __global__ __launch_bounds__(256) void q_read_kernel(QStore c, const int* __restrict__ len, int len_stride, QRows k,
                                                      QRows v, int n, const int* __restrict__ first, bool vec) {
   constexpr int LPG = HDP / CPL;             // lanes per group of 16 tokens
@@ -408,61 +413,62 @@ __global__ __launch_bounds__(256) void q_read_kernel(QStore c, const int* __rest
   const int f = first ? first[seq] : 0;
   // tiles before 0 (a first below 0) are counted too
   const long tile_f = f >= 0 ? f / kQTile : -((-(long)f + kQTile - 1) / kQTile);
-  const long unit = ((long)blockIdx.y * 4 + wave) * GPW + lane / LPG;  // groups of 16 tokens from tile_f's first on
-  const long tile = tile_f + unit / 4;
-  const int group = (int)(unit & 3);
+  const long unit = ((long)blockIdx.y * 4 + wave) * GPW + lane / LPG;  // groups of 4 * TPL tokens from tile_f's first on
+  const long tile = tile_f + unit / (16 / TPL);
+  const int group = (int)(unit & 3), t0 = TPL == 4 ? 0 : (int)(unit >> 2) & 3;
   if (tile * kQTile >= (long)f + n) return;
   const int l = min(len[(size_t)seq * len_stride], c.capacity);
   const bool there = tile >= 0 && tile * kQTile < (n >= kLongRead ? l : c.tiles * kQTile);
   const int8_t* codes = (which ? c.v : c.k) + c.codes(sh) + (there ? tile : 0) * (long)kQTile * HDP;
   const float* scales = c.s + c.scales(sh) + which + 2 * ((there ? tile : 0) * kQTile >> c.block_shift);
-  unsigned q[4][4][CPL / 4];  // [t][token][columns / 4]
-  float s[4];
-  if (!there) {
+  unsigned q[TPL][4][CPL / 4];  // [t][token][columns / 4]
+  float s[TPL];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      s[t] = 0.f;
+  for (int t = 0; t < TPL; ++t) {
+    s[t] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int w = 0; w < CPL / 4; ++w) q[t][e][w] = 0;
+      for (int w = 0; w < CPL / 4; ++w) q[t][e][w] = 0;
+  }
+  if (there && which) {
+    unsigned raw[CPL][TPL];
+#pragma unroll
+    for (int e = 0; e < CPL; ++e) {
+      typedef unsigned UV __attribute__((ext_vector_type(TPL)));
+      const UV r = *reinterpret_cast<const UV*>(codes + (group * HDP + col + e) * 16 + t0 * 4);
+      for (int t = 0; t < TPL; ++t) raw[e][t] = r[t];
     }
-  } else if (which) {
-    uint4 raw[CPL];
-#pragma unroll
-    for (int e = 0; e < CPL; ++e) raw[e] = *reinterpret_cast<const uint4*>(codes + (group * HDP + col + e) * 16);
 #pragma unroll
     for (int w = 0; w < CPL / 4; ++w)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        unsigned x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = t == 0 ? raw[4 * w + e].x : t == 1 ? raw[4 * w + e].y : t == 2 ? raw[4 * w + e].z : raw[4 * w + e].w;
+      for (int t = 0; t < TPL; ++t) {
+        const unsigned x[4] = {raw[4 * w][t], raw[4 * w + 1][t], raw[4 * w + 2][t], raw[4 * w + 3][t]};
         unsigned r[4];
         transpose4(x, r);
 #pragma unroll
         for (int e = 0; e < 4; ++e) q[t][e][w] = r[e];
       }
-  } else {
+  } else if (there) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < TPL; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int8_t* p = codes + (t * 16 + group * 4 + e) * HDP + col;
+        const int8_t* p = codes + ((t0 + t) * 16 + group * 4 + e) * HDP + col;
 #pragma unroll
         for (int w = 0; w < CPL / 4; ++w) q[t][e][w] = reinterpret_cast<const unsigned*>(p)[w];
       }
   }
   if (there) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) s[t] = scales[2 * (t * 16 >> c.block_shift)];
+    for (int t = 0; t < TPL; ++t) s[t] = scales[2 * ((t0 + t) * 16 >> c.block_shift)];
   }
   T* out = static_cast<T*>(o.p) + seq * o.seq + head * o.head;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < TPL; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const long tok = tile * kQTile + t * 16 + group * 4 + e, r = tok - f;
+      const long tok = tile * kQTile + (t0 + t) * 16 + group * 4 + e, r = tok - f;
       if (r < 0 || r >= n) continue;
       const bool in = there && tok < l;
       float x[CPL];
@@ -499,17 +505,27 @@ void append_t(hipStream_t s, const QStore& c, QLen len, QTickets tickets, const 
     q_append_kernel<128, T><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start, vec);
 }
 
+template <int HDP, class T, int CPL>
+void read_rows(hipStream_t s, const QStore& c, QLen len, const QRows& k, const QRows& v, int n, const int* first,
+               bool vec) {
+  const unsigned heads = (unsigned)(c.n_seq * c.n_head);
+  const int tiles = (n + kQTile - 2) / kQTile + 1;  // (whatever the first token's offset in its tile)
+  constexpr int per = 4 * (64 / (HDP / CPL));       // units of 4 * TPL tokens that a workgroup takes
+  const dim3 grid(heads, (unsigned)((tiles * 4 + per - 1) / per), 2);
+  if ((long)grid.x * grid.y * 2 <= kFewReads) {
+    const dim3 fine(heads, (unsigned)((tiles * 16 + per - 1) / per), 2);
+    q_read_kernel<HDP, T, CPL, 1><<<fine, 256, 0, s>>>(c, len.p, len.stride, k, v, n, first, vec);
+  } else {
+    q_read_kernel<HDP, T, CPL, 4><<<grid, 256, 0, s>>>(c, len.p, len.stride, k, v, n, first, vec);
+  }
+}
+
 template <class T>
 void read_t(hipStream_t s, const QStore& c, QLen len, const QRows& k, const QRows& v, int n, const int* first) {
   constexpr int CPL = 16 / sizeof(T);
   const bool vec = vec_ok<T, CPL>(k, c.hd) && vec_ok<T, CPL>(v, c.hd);
-  const int tiles = (n + kQTile - 2) / kQTile + 1;  // (whatever the first token's offset in its tile)
-  const int per = 4 * (64 / (c.hdp / CPL));         // groups of 16 tokens that a workgroup takes
-  const dim3 grid((unsigned)(c.n_seq * c.n_head), (unsigned)((tiles * 4 + per - 1) / per), 2);
-  if (c.hdp == 64)
-    q_read_kernel<64, T, CPL><<<grid, 256, 0, s>>>(c, len.p, len.stride, k, v, n, first, vec);
-  else
-    q_read_kernel<128, T, CPL><<<grid, 256, 0, s>>>(c, len.p, len.stride, k, v, n, first, vec);
+  if (c.hdp == 64) read_rows<64, T, CPL>(s, c, len, k, v, n, first, vec);
+  else read_rows<128, T, CPL>(s, c, len, k, v, n, first, vec);
 }
 
 }  // namespace
