@@ -325,7 +325,7 @@ __device__ __forceinline__ void append_tile(const QStore& c, const Place& p, siz
 }
 
 // A workgroup per (sequence, head, tile) and side (keys, values). Memory bounds it
-// (8 x 1000 tokens of 12 heads of 64 in f32: 18 us, 3.4 TB/s); short appends are
+// (8 x 1000 tokens of 12 heads of 64 in f32: 17.5 us, 3.5 TB/s); short appends are
 // latency: length, rows, the block's earlier tokens (4 x 517 of 8 heads of 128: 12.7 us).
 template <int HDP, class T>
 __global__ __launch_bounds__(256) void q_append_kernel(QStore c, QLen len, QTickets tickets, QRows k, QRows v, int n_new,
