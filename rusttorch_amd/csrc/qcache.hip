@@ -186,6 +186,30 @@ __device__ __forceinline__ void append_tile(const QStore& c, const Place& p, siz
   int8_t* codes = (which ? c.v : c.k) + c.codes(sh);
   float* scales = c.s + c.scales(sh) + which;
 
+  // the block's earlier tokens (uniform; y == 0), rows outside as the nearest of
+  // them: asked for before the new rows, so that both are in flight together
+  const bool earlier = first < p.at;
+  auto old = [&](int i, int e) { return min(max(tile0 + (i * QPP + qrow) * 4 + e, first), p.at - 1); };
+  float4 o[PASSES][4];        // tailed: values
+  unsigned os[PASSES][4];     // and their tokens' scales; else words of codes: a token's, or a quad's by column
+  float old_s;
+  if (earlier && tailed) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[i][e] = *reinterpret_cast<const float4*>(tail + (size_t)(old(i, e) - blk0) * HDP + c4);
+        os[i][e] = __float_as_uint(tail_s[old(i, e) - blk0]);
+      }
+  } else if (earlier) {
+    old_s = scales[2 * (blk0 >> c.block_shift)];
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        os[i][e] = *reinterpret_cast<const unsigned*>(codes + (which ? value_byte(old(i, 0) & ~3, c4 + e, HDP)
+                                                                     : (size_t)old(i, e) * HDP + c4));
+  }
   float4 x[PASSES][4];
   unsigned ts[PASSES][4];
 #pragma unroll
@@ -215,43 +239,22 @@ __device__ __forceinline__ void append_tile(const QStore& c, const Place& p, siz
         ts[i][e] = 0;
       }
     }
-  if (first < p.at) {  // (uniform; y == 0) the block's earlier tokens; rows outside as the nearest of them
-    float4 o[PASSES][4];
-    unsigned os[PASSES][4];
-    auto old = [&](int i, int e) { return min(max(tile0 + (i * QPP + qrow) * 4 + e, first), p.at - 1); };
-    if (tailed) {
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[i][e] = *reinterpret_cast<const float4*>(tail + (size_t)(old(i, e) - blk0) * HDP + c4);
-          os[i][e] = __float_as_uint(tail_s[old(i, e) - blk0]);
-        }
-    } else {
-      const float s = scales[2 * (blk0 >> c.block_shift)];
+  if (earlier) {
+    if (!tailed) {
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) {
-        unsigned q[4];
-        if (which) {  // a quad's four tokens lie side by side, by column
-          const int tok = old(i, 0) & ~3;
-          unsigned x[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const unsigned*>(codes + value_byte(tok, c4 + j, HDP));
-          transpose4(x, q);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) q[e] = *reinterpret_cast<const unsigned*>(codes + (size_t)old(i, e) * HDP + c4);
-        }
+        unsigned q[4] = {os[i][0], os[i][1], os[i][2], os[i][3]};
+        if (which) transpose4(os[i], q);  // (a quad's four tokens lie side by side, by column)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          o[i][e] = make_float4(code_value((int8_t)q[e], s), code_value((int8_t)(q[e] >> 8), s),
-                                code_value((int8_t)(q[e] >> 16), s), code_value((int8_t)(q[e] >> 24), s));
+          o[i][e] = make_float4(code_value((int8_t)q[e], old_s), code_value((int8_t)(q[e] >> 8), old_s),
+                                code_value((int8_t)(q[e] >> 16), old_s), code_value((int8_t)(q[e] >> 24), old_s));
       }
 #pragma unroll
       for (int i = 0; i < PASSES; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          os[i][e] = read_back_scale(__uint_as_float(row_max_bits<HDP>(max_abs4(o[i][e]))), s);
+          os[i][e] = read_back_scale(__uint_as_float(row_max_bits<HDP>(max_abs4(o[i][e]))), old_s);
     }
 #pragma unroll
     for (int i = 0; i < PASSES; ++i)
