@@ -267,9 +267,10 @@ rtg_result rtg_qcache_read(const rtg_qcache* cache, rtg_dtype dtype, const rtg_r
  * rounded to dtype once. Query head h reads key/value head h / (n_q_head /
  * n_head), at most 1024 of them one key/value head. A block that reads back as
  * NaN makes the rows NaN that see a key of it, and no others; a query with a
- * value that is not finite gives a row of NaN. Rows i >= counts[s], and rows of
- * queries before the sequence's first token, are set to 0. out must not overlap
- * the queries. */
+ * value that is not finite gives a row of NaN. Sums are f32 and divided last:
+ * the largest |v| times the number of keys has to be below 3.4e38, and |v| below
+ * 1e-31 lose digits. Rows i >= counts[s], and rows of queries before the
+ * sequence's first token, are set to 0. out must not overlap the queries. */
 rtg_result rtg_qcache_attend(rtg_qcache* cache, rtg_dtype dtype, const rtg_rows* queries, size_t n_q,
                              size_t n_q_head, const int32_t* counts, float scale, const rtg_rows* out, void* stream);
 /* Waits for the stream and writes the n_seq lengths. Returns an error once
