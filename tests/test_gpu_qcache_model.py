@@ -148,3 +148,11 @@ def test_refusals():
     with pytest.raises(Gpt2Error, match="does not take a quantised cache"):
         _lib.check(_lib.load().rtg_forward_cached_noalloc(m._h, c._h, ids.ctypes.data_as(C.c_void_p), 2, None))
     assert c.len() == 0
+
+
+@pytest.mark.parametrize("sh,block,chunks", [
+    (synth.ModelShape(61, 4200, 24, 2, 3), 32, (4094, 1, 1, 1, 1)),      # head_dim 8, the per-launch step
+    (synth.ModelShape(61, 2800, 768, 1, 12), 64, (2623, 1, 1))])         # the batched step
+def test_steps_over_a_context_whose_keys_are_split(sh, block, chunks):
+    """The workgroup that writes the new token is not the one that reads the first keys, and joins what both have."""
+    test_logits_and_cache(sh, "f32", 1, block, chunks)
