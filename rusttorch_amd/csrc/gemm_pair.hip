@@ -154,9 +154,10 @@ __global__ __launch_bounds__(256) void pair_weights_kernel(const void* __restric
 
 // One LDS-direct load instruction: lane i's 16 bytes at base + voff go to LDS
 // lds + 16 i. Written out so that the compiler's wait-count pass does not tie
-// the LDS reads of other stages to it; the kernel waits itself.
+// the LDS reads of other stages to it; the kernel waits itself. (A load to LDS
+// needs a wait state behind the write of M0; nobody adds it within an asm block.)
 __device__ __forceinline__ void dma16(unsigned voff, const void* base, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
 }
 // At most N of this wave's loads outstanding and its LDS reads complete, then
 // the barrier. (The reads' results may be used behind it: nothing but this wait

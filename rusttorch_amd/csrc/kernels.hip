@@ -790,11 +790,12 @@ __device__ __forceinline__ int gl_swz(int row) { return (row >> 2) & 3; }
 // global_load_lds_dwordx4 written out, so that the compiler's wait-count pass
 // does not tie later LDS reads to these loads (it waited for all of them
 // before every fourth tile's reads); the kernel orders them itself with
-// gl_wait_barrier. M0 carries the wave-uniform LDS address.
+// gl_wait_barrier. M0 carries the wave-uniform LDS address. (A load to LDS needs
+// a wait state behind the write of M0; nobody adds it within an asm block.)
 __device__ __forceinline__ void gl_dma16(const float* src, const float* lds_dst) {
   const unsigned m0v =
       __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) float*)lds_dst);
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0v) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0v) : "memory", "m0");
 }
 // Wait until at most N of this wave's vector memory operations are
 // outstanding and its LDS reads are complete (another wave's load may overwrite

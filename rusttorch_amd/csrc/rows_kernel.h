@@ -285,7 +285,8 @@ __device__ __forceinline__ void signal(const RParams& p, u64 val) {
 // 16 bytes per lane from global memory straight into LDS (64 lanes = 1 KiB
 // at dst, lane i at dst + 16 i), streaming (nt). The loads count in vmcnt but
 // occupy no registers; the compiler does not see them, so the wave waits for
-// them itself (lds_dma_wait) before reading dst.
+// them itself (lds_dma_wait) before reading dst. (A load to LDS needs a wait
+// state behind the write of M0; nobody adds it within an asm block.)
 // POL: 0 streaming (nt: weights, read once), 1 cached (data in a region of
 // its own), 2 device scope (data in a shared region).
 template <int POL = 0>
@@ -293,11 +294,11 @@ __device__ __forceinline__ void lds_dma16(const float* src, float* dst) {
   const unsigned m0v =
       __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) float*)dst);
   if constexpr (POL == 0)
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "s"(m0v) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "s"(m0v) : "memory", "m0");
   else if constexpr (POL == 1)
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0v) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0v) : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off sc1" ::"v"(src), "s"(m0v) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off sc1" ::"v"(src), "s"(m0v) : "memory", "m0");
 }
 __device__ __forceinline__ void lds_dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
