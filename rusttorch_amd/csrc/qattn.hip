@@ -7,8 +7,13 @@
 //           the largest |q| of the row: 24 bits, as f32 has;
 //   output  O[column][query] = V^T P^T: p of a tile of 64 keys, times its
 //           block's scale, over the tile's largest such product: 24 bits again.
-// Results of 16-bit types take two digits (16 bits: 1.5e-5 of the row's or the
-// tile's largest value, against 2e-3 and 2.4e-4 half steps of bf16 and f16).
+// The probabilities of bf16 results take two digits (16 bits) in the kernels of
+// 16 columns: each is off by 1.5e-5 of the tile's largest at most, where a half
+// step of bf16 is 2e-3 to 4e-3 of a result; of f16, 2.4e-4 to 4.9e-4, those would
+// show. (2047 tokens of 32 heads of 128 behind 12001 in bf16: 588 us, three digits
+// 677.) Queries take three whatever their type: a channel much larger than the
+// rest would take the others' bits (two digits: 520 us, but f16 results off by 8e-4
+// at a channel 100 times the rest).
 // A wave holds 16 columns, a column being a (query, head) pair that reads one
 // key/value head. Scores are computed transposed, so the lanes of a column hold
 // 16 of a tile's keys each: the softmax statistics are lane-local up to two
@@ -42,15 +47,14 @@ __device__ __forceinline__ unsigned perm(unsigned a, unsigned b, unsigned sel) {
   return __builtin_amdgcn_perm(a, b, sel);  // bytes 0-3 of sel: of b, 4-7: of a
 }
 
-// Digit planes of four fixed-point values whose digits are the bytes of u0 .. u3
-// plus 128 (the top one of ND = 3, or of values that are not negative, as it is):
-// d[i] holds digit i of the four.
-template <int ND, bool POSITIVE = false>
+// Digit planes of four fixed-point values whose digits are the bytes of u0 .. u3,
+// but for the top one plus 128: d[i] holds digit i of the four.
+template <int ND>
 __device__ __forceinline__ void planes(unsigned u0, unsigned u1, unsigned u2, unsigned u3, unsigned (&d)[ND]) {
   const unsigned a = perm(u1, u0, 0x05010400), b = perm(u3, u2, 0x05010400);  // [x0 y0 x1 y1]
   d[0] = perm(b, a, 0x05040100) ^ 0x80808080u;
   d[1] = perm(b, a, 0x07060302);
-  if (ND == 3 || !POSITIVE) d[1] ^= 0x80808080u;
+  if (ND == 3) d[1] ^= 0x80808080u;
   if constexpr (ND == 3) d[2] = perm(perm(u3, u2, 0x0c0c0602), perm(u1, u0, 0x0c0c0602), 0x05040100);
 }
 
@@ -74,14 +78,13 @@ __device__ __forceinline__ i32x4 fixed_mfma(const i32x4 (&a)[KS], const i32x4 (&
   return (hi << 8) + mid;
 }
 
-// A query as ND digit planes: this lane's 16 elements (of each 64) group * 16 + e,
-// q[k][digit] bytes e. Returns the score in units of log2 e of a
-// unit of the fixed-point sums (of 256 of them for ND = 3), but for the key's
-// scale; NaN for a row with a value that is not finite. The four lanes 16 apart
-// hold a row.
-template <int KS, int ND, class T>
+// A query as three digit planes: this lane's 16 elements (of each 64) group * 16 + e,
+// q[k][digit] bytes e. Returns the score in units of log2 e of 256
+// units of the fixed-point sums, but for the key's scale; NaN for a row with a
+// value that is not finite. The four lanes 16 apart hold a row.
+template <int KS, class T>
 __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, int group, float scale,
-                                             i32x4 (&q)[KS][ND]) {
+                                             i32x4 (&q)[KS][3]) {
   float4 x[KS][4];
   unsigned top = 0;  // (bits order like the values, NaN above infinity)
 #pragma unroll
@@ -98,7 +101,7 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
   top = max(r2[0], r2[1]);
   float amax = __uint_as_float(top);
   const bool fine = top < 0x7F800000u;
-  float unit = fabsf(scale) * 1.4426950408889634f * (ND == 3 ? 256.f : 1.f);
+  float unit = fabsf(scale) * 1.4426950408889634f * 256.f;
   if (__builtin_amdgcn_ballot_w64(amax < 7.9e-31f)) {
     asm volatile("");
     // rows below 2^-100 are taken 2^100 times as large, so that 1 / amax is a number
@@ -114,30 +117,30 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
   }
   // (a negative scale goes into the digits: the factor of the sums is not negative;
   // it comes from inv as it was rounded, or all scores would be off by its rounding)
-  const float inv = fine && amax > 0.f ? copysignf(fixed_max<ND>(), scale) / amax : 0.f;
-  constexpr float bias = ND == 3 ? 8421504.f : 32896.f;  // 0x808080, 0x8080: every digit plus 128
+  const float inv = fine && amax > 0.f ? copysignf(fixed_max<3>(), scale) / amax : 0.f;
+  constexpr float bias = 8421504.f;  // 0x808080: every digit plus 128
 #pragma unroll
   for (int k = 0; k < KS; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float xe[4] = {x[k][e].x, x[k][e].y, x[k][e].z, x[k][e].w};
-      unsigned u[4], d[ND];
+      unsigned u[4], d[3];
 #pragma unroll
       for (int i = 0; i < 4; ++i) u[i] = (unsigned)rintf(fmaf(xe[i], inv, bias));  // (NaN and infinity: sq says so)
-      planes<ND>(u[0], u[1], u[2], u[3], d);
-      if constexpr (ND == 3) d[2] ^= 0x80808080u;
+      planes<3>(u[0], u[1], u[2], u[3], d);
+      d[2] ^= 0x80808080u;
 #pragma unroll
-      for (int i = 0; i < ND; ++i) q[k][i][e] = (int)d[i];
+      for (int i = 0; i < 3; ++i) q[k][i][e] = (int)d[i];
     }
   return !fine ? NAN : amax > 0.f ? unit / fabsf(inv) : 0.f;
 }
 
 // A wave's 16 columns: lane = group * 16 + column; the group's 16 (of 64) query
 // elements, and 16 of a tile's keys: t * 16 + group * 4 + i.
-template <int HDP, int ND>
+template <int HDP>
 struct Cols {
   static constexpr int KS = HDP / 64, DT = HDP / 16;
-  i32x4 q[KS][ND];
+  i32x4 q[KS][3];
   float sq;  // score units of log2 e per unit of the fixed-point sums, without the key scale
   float m, l;
   float o[DT][4];
@@ -153,7 +156,7 @@ struct Cols {
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[d][i] = 0.f;
-    sq = fixed_query<KS, ND>(qrow, hd, vec, group, scale, q);
+    sq = fixed_query<KS>(qrow, hd, vec, group, scale, q);
   }
 };
 
@@ -253,9 +256,9 @@ __device__ __forceinline__ TileScales<NG, SH> tile_scales(float2 sl, int live, i
 // here is 1 and needs no second reduction; each probability itself is 1 / r of it.
 
 // k: 16 keys; s[4]: a lane's fixed-point sums of them.
-template <int HDP, int ND>
-__device__ __forceinline__ void tile_sums(const Cols<HDP, ND>& c, const i32x4 (&k)[HDP / 64], float (&s)[4]) {
-  const i32x4 d = fixed_mfma<ND, HDP / 64>(k, c.q);
+template <int HDP>
+__device__ __forceinline__ void tile_sums(const Cols<HDP>& c, const i32x4 (&k)[HDP / 64], float (&s)[4]) {
+  const i32x4 d = fixed_mfma<3, HDP / 64>(k, c.q);
 #pragma unroll
   for (int e = 0; e < 4; ++e) s[e] = (float)d[e];
 }
@@ -263,7 +266,7 @@ __device__ __forceinline__ void tile_sums(const Cols<HDP, ND>& c, const i32x4 (&
 // s: the keys' fixed-point sums. pd: the probabilities' digits, w: what
 // their products with the values' codes are to be multiplied with.
 template <bool EDGE, int HDP, int ND, int NG, int SH>
-__device__ __forceinline__ void tile_probs(Cols<HDP, ND>& c, float (&s)[NG][4], const TileScales<NG, SH>& ts, int j0,
+__device__ __forceinline__ void tile_probs(Cols<HDP>& c, float (&s)[NG][4], const TileScales<NG, SH>& ts, int j0,
                                            int group, i32x4 (&pd)[NG / 4][ND], float& w) {
   constexpr int DT = HDP / 16, NB = TileScales<NG, SH>::NB, PER = NG / NB;  // 16s per block
   float f[NB], cc[NB];
@@ -336,7 +339,7 @@ __device__ __forceinline__ void tile_probs(Cols<HDP, ND>& c, float (&s)[NG][4], 
     unsigned u[4], d[ND];
 #pragma unroll
     for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(fmaf(s[i][e], fixed_max<ND>(), magic));
-    planes<ND, true>(u[0], u[1], u[2], u[3], d);
+    planes<ND>(u[0], u[1], u[2], u[3], d);
 #pragma unroll
     for (int n = 0; n < ND; ++n) pd[i / 4][n][i & 3] = (int)d[n];
   }
@@ -528,7 +531,7 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
     fetch(vp, 0, vv, lv);
     sl = load_s(0);
   }
-  Cols<HDP, ND> c;
+  Cols<HDP> c;
   const Column cl = column(a, max(cb, 0) * 16 + col);
   c.init(query_row<T>(a, seq, head, cl), a.c.hd, a.qvec, group, a.scale, cb >= 0 && cl.i < r.count ? visible(r, cl.i) : 0);
   wait_and_sync();
@@ -541,7 +544,7 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
       i32x4 k[KS];
 #pragma unroll
       for (int e = 0; e < KS; ++e) k[e] = t.k[Pair::k_at(n * 16 + col, e * 4 + group)];
-      tile_sums<HDP, ND>(c, k, s[n]);
+      tile_sums<HDP>(c, k, s[n]);
       if (n & 1) __builtin_amdgcn_sched_barrier(0);  // (two at a time in flight: fewer registers)
     }
     wait_and_sync();  // the keys are read; the values of this pair are there
@@ -761,7 +764,7 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
   const int tiles = (live + kQTile - 1) / kQTile, per = split_tiles<HDP, 16>(tiles, a.splits);
   const int t0 = z * per, t1 = min(t0 + per, tiles);
   if (z > 0 && t0 >= tiles) return;  // (the whole workgroup; split 0 also writes rows without keys)
-  Cols<HDP, ND> c;
+  Cols<HDP> c;
   c.init(query_row<T>(a, seq, head, cl), a.c.hd, a.qvec, group, a.scale, cl.i < r.count ? visible(r, cl.i) : 0);
   const int8_t *kp = a.c.k + a.c.codes(sh), *vp = a.c.v + a.c.codes(sh);
   const float* sp = a.c.s + a.c.scales(sh);
@@ -778,7 +781,7 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
     i32x4 pd[1][ND];
     float w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tile_sums<HDP, ND>(c, t.k[i], sums[i]);
+    for (int i = 0; i < 4; ++i) tile_sums<HDP>(c, t.k[i], sums[i]);
     if (j * kQTile + kQTile > least) tile_probs<true>(c, sums, ts, j * kQTile, group, pd, w);
     else tile_probs<false>(c, sums, ts, j * kQTile, group, pd, w);
 #pragma unroll
@@ -837,7 +840,7 @@ struct FewCols {
 #pragma unroll
     for (int i = 0; i < NO; ++i) o[i] = 0.f;
     i32x4 d[KS][3];
-    const float sr = fixed_query<KS, 3>(qrow, hd, vec, lane >> 4, scale, d);
+    const float sr = fixed_query<KS>(qrow, hd, vec, lane >> 4, scale, d);
     const int row = lane & 15;
     i32x4 mine[KS];
 #pragma unroll
@@ -1147,7 +1150,7 @@ void launch_q_attend(hipStream_t s, const QStore& c, QLen len, int extra, QType 
   AttnArgs a = attn_args(c, len, extra, type, q, n_q, n_q_head, counts, scale, out, work);
   if (type == Q_F32) attend_t<3, float>(s, a);
   else if (type == Q_BF16) attend_t<2, __bf16>(s, a);
-  else attend_t<2, _Float16>(s, a);
+  else attend_t<3, _Float16>(s, a);
 }
 
 void launch_q_step(hipStream_t s, const QStore& c, QLen len, const QRows& k, const QRows& v, const QRows& q,

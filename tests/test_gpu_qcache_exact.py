@@ -1,0 +1,79 @@
+"""Attention over the 8-bit cache against 64 bits, element by element: results
+are those of f32 sums or better and are rounded to their type once, whatever the
+type of the rows and however the values' scales lie."""
+import numpy as np
+import pytest
+
+from tests.test_gpu_qcache import EPS, Both, rows
+
+pytestmark = pytest.mark.gpu
+
+
+def spacing(x, dtype):
+    """Distance of neighbouring numbers of dtype around |x| (the larger one where x is next to a power of two)."""
+    bits, least = {"f32": (23, -126), "bf16": (7, -126), "f16": (10, -14)}[dtype]
+    e = np.frexp(np.abs(x) * (1 + 2.0 ** -bits))[1] - 1
+    return 2.0 ** (np.maximum(e, least) - bits)
+
+
+def check(b, got, q, dtype, counts=None, scale=None, every=1, seqs=None):
+    """Each row of got against 64 bits, of the sequences `seqs` (all), every `every`-th query.
+
+    A result is off by half a step of its type, and before that (EPS = 2^-24, p the probabilities, o the result, n the
+    keys, all as 64 bits have them) by
+      - the query as fixed point: half a step, 1.01 EPS of its largest component, for each of a key's components;
+        8 EPS of the score's size for the roundings on its way to an exponent (the scale, log2 e and their product, the
+        unit of the sums, its product with the key's scale, the sums to f32, the difference to the maximum and the
+        maximum's own), 2 EPS for exp2; a change of the scores by e_j moves o by sum p_j |v_j - o| e_j at most;
+      - the probabilities as fixed point: half a step, 1.01 EPS (bf16 and more than four columns: 2^-16) of the largest
+        product p_j * (largest |v| of the block) of the (up to 128) keys taken together, for each of them;
+      - f32 sums: 4 EPS of sum p_j |v_j| for every 64 keys, 16 times that for joins and the factors of a tile."""
+    D, r = q.shape[-1], b.r
+    scale = D ** -0.5 if scale is None else scale
+    got = got.double().cpu().numpy()
+    group = q.shape[2] // r.heads
+    step = 1.01 * (2.0 ** -16 if dtype == "bf16" and q.shape[1] * group > 4 else EPS)
+    worst = 0.0
+    for s in range(q.shape[0]) if seqs is None else seqs:
+        c = q.shape[1] if counts is None else min(max(int(counts[s]), 0), q.shape[1])
+        n = r.length(s)
+        assert not got[s, c:].any() and not got[s, :max(c - n, 0)].any()
+        for h in range(q.shape[2]):
+            k, v = (x[s][h // group].values().astype(np.float64) for x in (r.k, r.v))
+            if not n:
+                continue
+            top = np.repeat(r.v[s][h // group].s * 127, r.v[0][0].block)[:n]
+            for i in sorted({*range(max(c - n, 0), c, every), max(c - 1, 0)} - set(range(max(c - n, 0)))):
+                if i >= c:
+                    continue
+                see = n - c + i + 1
+                sc = k[:see] @ q[s, i, h] * scale
+                p = np.exp(sc - sc.max())
+                p /= p.sum()
+                o = p @ v[:see]
+                e = abs(scale) * 1.01 * EPS * np.abs(q[s, i, h]).max() * np.abs(k[:see]).sum(1) + 8 * EPS * np.abs(sc) + 2 * EPS
+                off = (p * e) @ np.abs(v[:see] - o)
+                prod = np.concatenate([p * top[:see], np.zeros(-see % 128)]).reshape(-1, 128)
+                off = off + step * 128 * prod.max(1).sum() + 4 * EPS * (see / 64 + 16) * (p @ np.abs(v[:see]))
+                over = np.abs(got[s, i, h] - o) - (spacing(o, dtype) / 2 + off)
+                assert np.all(over <= 0), (s, h, i, over.max(), np.abs(off).max(), np.abs(o).max())
+                worst = max(worst, (np.abs(got[s, i, h] - o) / (spacing(o, dtype) / 2 + off)).max())
+    return worst
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("size", [1.0, 300.0])
+@pytest.mark.parametrize("dim,seqs,heads,group,n_q,length", [
+    (64, 2, 2, 3, 4, 250), (128, 2, 1, 8, 1, 250),          # the keys split over waves
+    (64, 10, 4, 4, 152, 280), (128, 10, 4, 4, 100, 260)])   # every wave all keys
+def test_one_large_channel(dim, seqs, heads, group, n_q, length, size, dtype):
+    """Queries with a channel of `size` times the rest keep the others' bits: five and more columns a head."""
+    b = Both(seqs, heads, dim, length, 32, dtype, seed=dim + n_q)
+    (k, kn), (v, vn) = (rows(b.rng, (seqs, length, heads, dim), dtype) for _ in range(2))
+    k[..., 5] /= size
+    b.c.append(k, v)
+    b.r.append(k.double().cpu().numpy(), vn)
+    q = rows(b.rng, (seqs, n_q, heads * group, dim), dtype, 2.0)[0]
+    q[..., 5] *= size
+    got = b.c.attend(q)
+    print(f"    worst {check(b, got, q.double().cpu().numpy(), dtype, every=37, seqs=[0, seqs - 1]):.3f}", flush=True)
