@@ -214,8 +214,12 @@ __device__ __forceinline__ float xsum(float v) { return xor32_sum_k(xor16_sum_k(
 constexpr float kLargeScore = 256.f;
 
 // The scales of NG * 16 keys (one tile, or two) in blocks of 2^SH for a wave: of
-// each block f (scores) and r = max(v scale / vmax, 2^-60) as lr = log2 r and 1 /
-// r. (A block of zeros may take any r.)
+// each block f (scores) and r = v scale / vmax as lr = log2 r and 1 / r. vmax counts
+// blocks that a column may not see yet, or whose scores keep them out. So where an r
+// is below kLeastRatio (or 0) the blocks are taken one by one, each as the only one:
+// `only` (-1: all of them) says which: it is set to 0 here where that begins, and
+// the tile is taken again with the next one.
+constexpr float kLeastRatio = 0.000244140625f;  // 2^-12: what rounding lr moves a product by stays below 6 EPS
 template <int NG, int SH>
 struct TileScales {
   static constexpr int NB = NG * 16 >> SH;
@@ -226,21 +230,30 @@ struct TileScales {
 // sl: a lane's (keys', values') scales, those of the keys' blocks on lanes 0 ..
 // and over and over; live: keys of these that are in the cache (or more).
 template <int NG, int SH>
-__device__ __forceinline__ TileScales<NG, SH> tile_scales(float2 sl, int live, int lane) {
+__device__ __forceinline__ TileScales<NG, SH> tile_scales(float2 sl, int live, int lane, int& only) {
   TileScales<NG, SH> t;
   constexpr int NB = TileScales<NG, SH>::NB;
-  const bool in = ((lane & (NB - 1)) << SH) < live;  // blocks behind the last key are not read as numbers
-  const float k = in ? sl.x : 0.f, v = in ? sl.y : 0.f;
-  t.bad = (unsigned)__builtin_amdgcn_ballot_w64(v != v) & ((1u << NB) - 1);
+  const int block = lane & (NB - 1);
+  bool in = (block << SH) < live && (only < 0 || block == only);  // blocks behind the last key are not read as numbers
+  float v = in ? sl.y : 0.f;
   float m = v;  // (fmaxf skips NaN)
   if (NB > 1) m = fmaxf(m, dpp_row<0xB1>(m));
   if (NB > 2) m = fmaxf(m, dpp_row<0x4E>(m));
   if (NB > 4) m = fmaxf(m, dpp_row<0x124>(m));
   m = fmaxf(m, 0.f);
+  if (NB > 1 && only < 0 && __builtin_amdgcn_ballot_w64(in && v < m * kLeastRatio)) {
+    only = 0;
+    in = block == 0;
+    v = in ? v : 0.f;
+    m = fmaxf(lane_of(v, 0), 0.f);
+  }
+  const float k = in ? sl.x : 0.f;
+  t.bad = (unsigned)__builtin_amdgcn_ballot_w64(v != v) & ((1u << NB) - 1);
   t.vmax = m;
-  // (r to the last place: it is the same for a block's every key)
-  const float r = m > 0.f ? fmaxf(v * __builtin_amdgcn_rcpf(m), 8.6736174e-19f) : 1.f;
-  const float lr = __builtin_amdgcn_logf(r), ri = __builtin_amdgcn_rcpf(r);
+  // (r to the last place: it is the same for a block's every key. Keys of the other
+  // blocks score 0 * sum - infinity)
+  const float r = m > 0.f && v > 0.f ? v * __builtin_amdgcn_rcpf(m) : 1.f;
+  const float lr = in ? __builtin_amdgcn_logf(r) : -INFINITY, ri = in ? __builtin_amdgcn_rcpf(r) : 0.f;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     t.f[b] = lane_of(k, b);
@@ -248,6 +261,13 @@ __device__ __forceinline__ TileScales<NG, SH> tile_scales(float2 sl, int live, i
     t.rinv[b] = lane_of(ri, b);
   }
   return t;
+}
+// Whether the blocks of NG * 16 keys have all been taken (only is then -1 again);
+// else only is the next one.
+template <int NG, int SH>
+__device__ __forceinline__ bool all_taken(int live, int& only) {
+  only = only < 0 || (only + 1) << SH >= min(live, NG * 16) ? -1 : only + 1;
+  return only < 0;
 }
 
 // A tile's keys (NG = 4), or two tiles' (8), for a wave's columns. EDGE: some
@@ -535,9 +555,9 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
   const Column cl = column(a, max(cb, 0) * 16 + col);
   c.init(query_row<T>(a, seq, head, cl), a.c.hd, a.qvec, group, a.scale, cb >= 0 && cl.i < r.count ? visible(r, cl.i) : 0);
   wait_and_sync();
+  int only = -1;
   auto step = [&](int j, auto edge, auto groups) {  // groups: of 16 keys
     constexpr int NG = decltype(groups)::value;
-    const bool more = NG == 8 && j + 1 < pairs;
     float s[NG][4], w;
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
@@ -548,12 +568,12 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
       if (n & 1) __builtin_amdgcn_sched_barrier(0);  // (two at a time in flight: fewer registers)
     }
     wait_and_sync();  // the keys are read; the values of this pair are there
-    const float2 sj = sl;
+    const TileScales<NG, SH> ts = tile_scales<NG, SH>(sl, live - j * kPair, lane, only);
+    const bool done = all_taken<NG, SH>(live - j * kPair, only), more = done && NG == 8 && j + 1 < pairs;
     if (more) {
       fetch(kp, j + 1, kv, lk);
       sl = load_s(j + 1);
     }
-    const TileScales<NG, SH> ts = tile_scales<NG, SH>(sj, live - j * kPair, lane);
     i32x4 pd[NG / 4][ND];
     tile_probs<decltype(edge)::value>(c, s, ts, j * kPair, group, pd, w);
 #pragma unroll
@@ -568,12 +588,13 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
       wait_and_sync();  // the values are read; the next pair's keys are there
       fetch(vp, j + 1, vv, lv);
     }
+    return (int)done;
   };
   using Pairs = std::integral_constant<int, 8>;
   int j = 0;
-  for (; j < full; ++j) step(j, std::false_type(), Pairs());
-  for (; j < pairs && !half(j); ++j) step(j, std::true_type(), Pairs());
-  if (j < pairs) step(j, std::true_type(), std::integral_constant<int, 4>());
+  while (j < full) j += step(j, std::false_type(), Pairs());
+  while (j < pairs && !half(j)) j += step(j, std::true_type(), Pairs());
+  while (j < pairs) j += step(j, std::true_type(), std::integral_constant<int, 4>());
   const float l = xsum(c.l);
   if (cb < 0 || cl.i >= a.n_q) return;
   const float inv = c.lim > 0 ? 1.f / l : 0.f;
@@ -770,19 +791,19 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
   const float* sp = a.c.s + a.c.scales(sh);
   Tile<HDP> t;
   int j = t0 + wave;
-  if (j < t1) {
-    t.load_s(sp, j, SH, lane);
-    t.load_k(kp, j, lane);
-    t.load_v(vp, j, lane);
-  }
-  auto step = [&] {
-    const TileScales<4, SH> ts = tile_scales<4, SH>(t.s, live - j * kQTile, lane);
+  auto load = [&](Tile<HDP>& x, int tile) {
+    x.load_s(sp, tile, SH, lane);
+    x.load_k(kp, tile, lane);
+    x.load_v(vp, tile, lane);
+  };
+  if (j < t1) load(t, j);
+  auto take = [&](const TileScales<4, SH>& ts, bool edge) {
     float sums[4][4];
     i32x4 pd[1][ND];
     float w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) tile_sums<HDP>(c, t.k[i], sums[i]);
-    if (j * kQTile + kQTile > least) tile_probs<true>(c, sums, ts, j * kQTile, group, pd, w);
+    if (edge) tile_probs<true>(c, sums, ts, j * kQTile, group, pd, w);
     else tile_probs<false>(c, sums, ts, j * kQTile, group, pd, w);
 #pragma unroll
     for (int d = 0; d < HDP / 16; ++d) {
@@ -790,15 +811,32 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
       tile_product<ND, 1>(v, pd, w, c.o[d]);
     }
   };
+  bool left = false;  // tiles whose scales lie far apart
+  auto step = [&] {
+    int only = -1;
+    const TileScales<4, SH> ts = tile_scales<4, SH>(t.s, live - j * kQTile, lane, only);
+    if (only < 0) take(ts, j * kQTile + kQTile > least);
+    else left = true;
+  };
   for (; j + NW < t1; j += NW) {
     Tile<HDP> n;
-    n.load_s(sp, j + NW, SH, lane);
-    n.load_k(kp, j + NW, lane);
-    n.load_v(vp, j + NW, lane);
+    load(n, j + NW);
     step();
     t = n;
   }
   if (j < t1) step();
+  if (left) {
+    // (a loop of its own: above, it would keep more in registers)
+    for (j = t0 + wave; j < t1; j += NW)
+      for (int only = -1;;) {
+        load(t, j);
+        const bool first = only < 0;
+        const TileScales<4, SH> ts = tile_scales<4, SH>(t.s, live - j * kQTile, lane, only);
+        if (first && only < 0) break;
+        take(ts, true);
+        if (all_taken<4, SH>(live - j * kQTile, only)) break;
+      }
+  }
   const float l = xsum(c.l);
   if (group == 0) {
     s.m[wave][col] = c.m;

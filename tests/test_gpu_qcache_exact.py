@@ -3,6 +3,7 @@ are those of f32 sums or better and are rounded to their type once, whatever the
 type of the rows and however the values' scales lie."""
 import numpy as np
 import pytest
+import torch
 
 from tests.test_gpu_qcache import EPS, Both, rows
 
@@ -77,3 +78,41 @@ def test_one_large_channel(dim, seqs, heads, group, n_q, length, size, dtype):
     q[..., 5] *= size
     got = b.c.attend(q)
     print(f"    worst {check(b, got, q.double().cpu().numpy(), dtype, every=37, seqs=[0, seqs - 1]):.3f}", flush=True)
+
+
+@pytest.mark.parametrize("dtype,big,small", [("f32", 1e20, 1.0), ("bf16", 1e20, 1.0), ("f32", 1e5, 1e-30), ("f32", 1e4, 1.0),
+                                             ("bf16", 1e3, 1.0), ("f16", 1e3, 1e-4)])
+@pytest.mark.parametrize("hidden", [False, True])
+@pytest.mark.parametrize("dim,seqs,heads,group,block", [(64, 1, 1, 1, 16), (128, 1, 1, 2, 32), (64, 1, 2, 5, 32),
+                                                        (64, 10, 4, 4, 16), (64, 10, 4, 4, 32), (128, 10, 4, 4, 16)])
+def test_scales_far_apart(dim, seqs, heads, group, block, hidden, dtype, big, small):
+    """Blocks of large and of small values side by side: rows that do not see the large ones yet and, `hidden`, rows whose
+    scores keep them out, are as exact as if those were not there."""
+    n = 152
+    b = Both(seqs, heads, dim, n, block, dtype, seed=block + dim)
+    (k, _), (v, _), (q, _) = (rows(b.rng, (seqs, n, h, dim), dtype) for h in (heads, heads, heads * group))
+    large = (torch.arange(n, device="cuda") // block % 3 == 1)[:, None, None]
+    v *= torch.where(large, big, small).to(v.dtype)
+    if hidden:
+        q[..., 0] = 8.0
+        k[..., 0] = torch.where(large, -25.0 * dim ** 0.5, 0.0)[..., 0].to(k.dtype)
+    b.c.append(k, v)
+    b.r.append(k.double().cpu().numpy(), v.double().cpu().numpy())
+    got = b.c.attend(q)
+    every = 1 if seqs == 1 else 13
+    print(f"    worst {check(b, got, q.double().cpu().numpy(), dtype, every=every, seqs=[seqs - 1]):.3f}", flush=True)
+
+
+@pytest.mark.parametrize("dim,seqs,heads,group", [(64, 1, 1, 1), (128, 1, 1, 2), (64, 10, 4, 4), (128, 10, 4, 4)])
+def test_blocks_of_zeros_that_take_the_probability(dim, seqs, heads, group):
+    """Values of 0 at scores 60 above the rest: what the rest leaves in a result is as exact as ever."""
+    n = 152
+    b = Both(seqs, heads, dim, n, 16, seed=dim)
+    (k, _), (v, _), (q, _) = (rows(b.rng, (seqs, n, h, dim)) for h in (heads, heads, heads * group))
+    zero = (torch.arange(n, device="cuda") // 16 % 3 == 1)[:, None, None]
+    v *= torch.where(zero, 0.0, 1.0)
+    q[..., 0] = 8.0
+    k[..., 0] = torch.where(zero, 7.5 * dim ** 0.5, 0.0)[..., 0]
+    b.c.append(k, v)
+    b.r.append(k.double().cpu().numpy(), v.double().cpu().numpy())
+    check(b, b.c.attend(q), q.double().cpu().numpy(), "f32", every=1 if seqs == 1 else 13, seqs=[seqs - 1])
