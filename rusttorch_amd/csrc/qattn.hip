@@ -219,7 +219,8 @@ constexpr float kLargeScore = 256.f;
 // is below kLeastRatio (or 0) the blocks are taken one by one, each as the only one:
 // `only` (-1: all of them) says which: it is set to 0 here where that begins, and
 // the tile is taken again with the next one.
-constexpr float kLeastRatio = 0.000244140625f;  // 2^-12: what rounding lr moves a product by stays below 6 EPS
+// (The test and the loops' own advance cost many columns of 128 2 to 3 %.)
+constexpr float kLeastRatio = 0.000244140625f;  // 2^-12: lr's last place is 2^-20 or less, of a product's 1
 template <int NG, int SH>
 struct TileScales {
   static constexpr int NB = NG * 16 >> SH;
@@ -519,10 +520,18 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
   // (the later blocks of columns may be padding: the last that is not sees most;
   // columns that are none may see anything, their results go nowhere)
   const int top_cb = r.count > 0 ? min(cb0, (r.count * a.group - 1) / 16) : -1, low_cb = max(cb0 - 3, 0);
-  const int live = top_cb >= 0 ? visible(r, min(by_group(a, top_cb * 16 + 15), r.count - 1)) : 0;
+  const int live = top_cb >= low_cb ? visible(r, min(by_group(a, top_cb * 16 + 15), r.count - 1)) : 0;
+  if (live == 0) {  // (all four blocks are padding, or before the first token)
+    const Column cl = column(a, max(cb, 0) * 16 + col);
+    if (cb < 0 || cl.i >= a.n_q) return;
+    const RowOut<T, KIND> out(a, seq, cl.i, head * a.group + cl.h);
+#pragma unroll
+    for (int d = 0; d < HDP / 16; ++d) out.put(a, d * 16 + group * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+    return;
+  }
   const int pairs = (live + kPair - 1) / kPair;
   // pairs that every column sees whole
-  const int full = top_cb >= low_cb ? min(visible(r, by_group(a, low_cb * 16)) / kPair, pairs) : 0;
+  const int full = min(visible(r, by_group(a, low_cb * 16)) / kPair, pairs);
   const int8_t *kp = a.c.k + a.c.codes(sh), *vp = a.c.v + a.c.codes(sh);
   const float* sp = a.c.s + a.c.scales(sh);
   // unit u * 256 + tid of a pair in LDS: a wave's 64 are 1 KB of one tile
@@ -545,12 +554,9 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
     const int nb = (half(j) ? kQTile : kPair) >> SH, last = (a.c.tiles * kQTile >> SH) - 1;
     return reinterpret_cast<const float2*>(sp)[min((j * kPair >> SH) + (lane & (nb - 1)), last)];
   };
-  float2 sl = make_float2(0.f, 0.f);
-  if (pairs) {
-    fetch(kp, 0, kv, lk);
-    fetch(vp, 0, vv, lv);
-    sl = load_s(0);
-  }
+  fetch(kp, 0, kv, lk);
+  fetch(vp, 0, vv, lv);
+  float2 sl = load_s(0);
   Cols<HDP> c;
   const Column cl = column(a, max(cb, 0) * 16 + col);
   c.init(query_row<T>(a, seq, head, cl), a.c.hd, a.qvec, group, a.scale, cb >= 0 && cl.i < r.count ? visible(r, cl.i) : 0);

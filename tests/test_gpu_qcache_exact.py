@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_qcache import EPS, Both, rows
+from tests.test_gpu_qcache import EPS, Both, ints, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +116,41 @@ def test_blocks_of_zeros_that_take_the_probability(dim, seqs, heads, group):
     b.c.append(k, v)
     b.r.append(k.double().cpu().numpy(), v.double().cpu().numpy())
     check(b, b.c.attend(q), q.double().cpu().numpy(), "f32", every=1 if seqs == 1 else 13, seqs=[seqs - 1])
+
+
+def test_padding_behind_a_prompt_takes_no_time():
+    """Queries that are padding take none of the keys: one token each of long sequences, padded, against whole prompts."""
+    n = 2000
+    b = Both(16, 16, 64, n, 32, seed=7)
+    k, q = (rows(b.rng, (16, n, 16, 64))[0] for _ in range(2))
+    b.c.append(k, k)
+    one = ints([1] * 16)
+    out = torch.empty_like(q)
+
+    def ms(counts):
+        best = 1e9
+        for _ in range(5):
+            t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            t[0].record()
+            b.c.attend(q, counts=counts, out=out)
+            t[1].record()
+            torch.cuda.synchronize()
+            best = min(best, t[0].elapsed_time(t[1]))
+        return best
+
+    whole, padded = ms(None), ms(one)
+    print(f"    whole {1e3 * whole:.0f} us, one token each {1e3 * padded:.0f} us", flush=True)
+    assert padded < whole / 3
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "f32"), (128, "bf16")])
+def test_padded_prompts(dim, dtype):
+    seqs, heads, group, n = 10, 4, 4, 200
+    b = Both(seqs, heads, dim, n, 32, dtype, seed=dim)
+    lens = [0, 1, 66, 200, 63, 64, 65, 128, 129, 199]
+    (k, kn), (v, vn) = (rows(b.rng, (seqs, n, heads, dim), dtype) for _ in range(2))
+    b.c.append(k, v, counts=ints(lens))
+    b.r.append(kn, vn, lens)
+    q, qn = rows(b.rng, (seqs, n, heads * group, dim), dtype)
+    for counts in (lens, [0, 1, 66, 66, 0, 1, 0, 64, 200, 3]):
+        check(b, b.c.attend(q, counts=ints(counts)), qn, dtype, counts, every=23)
