@@ -136,7 +136,9 @@ rtg_result rtg_cache_new(const rtg_model* model, size_t batch, rtg_cache** out);
  * step reads of it), for logits that differ by what the rounding of keys and
  * values to 8 bits moves. Goes wherever a cache of this batch goes except
  * rtg_forward_cached_noalloc; one new token runs the batched step's kernel graph
- * at any batch, more run the prefill kernels. */
+ * at any batch, more run the prefill kernels. Behind a pass that failed the cache
+ * goes on where it was, as an f32 one does; its last block's tokens may then count
+ * as the values that they read back as. */
 rtg_result rtg_cache_new_quantised(const rtg_model* model, size_t batch, size_t block, rtg_cache** out);
 /* KVCache::len / is_empty / clear, gpt2.rs:137-161. */
 size_t rtg_cache_len(const rtg_cache* cache);

@@ -356,6 +356,7 @@ struct rtg_cache {
   void* q_work = nullptr;  // partial results of its attention
   int* q_int = nullptr;    // [0]: tokens before a prefill; [kQZero]: 0
   float* q_new = nullptr;
+  size_t q_reached = 0;    // tokens that a failed pass may have left in it (0: no pass failed)
   bool quantised() const { return q_mem != nullptr; }
 };
 constexpr int kQZero = 32;
@@ -543,6 +544,20 @@ static void q_attention(rtg_cache* c, size_t l, size_t T, const float* q, int ld
   if (T == 1) return launch_q_step(c->stream, st, at, k, v, qr, scale, out, c->q_work);
   launch_q_append(c->stream, st, at, QTickets{}, Q_F32, k, v, (int)T, nullptr, nullptr);
   launch_q_attend(c->stream, st, at, (int)T, Q_F32, qr, (int)T, (int)m->cfg.n_head, nullptr, scale, out, c->q_work);
+}
+// After a failed pass, which a quantised cache may hold in some layers and not in
+// others: where the unrounded values of the last token's block may have gone, that
+// block's tokens count as what they read back as from here on, as behind a cut.
+static void q_after_failure(rtg_cache* c) {
+  const size_t block = (size_t)c->q.block;
+  if (c->q_reached && c->len % block != 0 && (c->q_reached - 1) / block != (c->len - 1) / block) {
+    launch_set_step(c->stream, nullptr, c->q_int, (int)c->len, c->q_int + 1, (int)c->q_reached);
+    for (int i = 0; i < c->q.n_seq; ++i)
+      launch_q_append(c->stream, c->q.from(i, 1), QLen{c->q_int + 1, 0}, QTickets{}, Q_F32, QRows{}, QRows{}, 0, nullptr,
+                      c->q_int);
+    HIPX(hipGetLastError());
+  }
+  c->q_reached = 0;
 }
 static QOut q_rows(float* p) {
   QOut o;
@@ -1013,6 +1028,10 @@ static void forward_cached_impl(rtg_cache* c, const uint32_t* ids, size_t n, flo
   const size_t B = c->batch, V = m->cfg.vocab_size;
   ensure_rows(c, B * n);
   ensure_logits(c, logits_out ? B * n : B);
+  if (c->quantised()) {
+    q_after_failure(c);
+    c->q_reached = c->len + n;
+  }
   if (n == 1 && B == 1 && !c->quantised() && persistent_supported(m->pplan, 1)) {
     // one new token at batch 1: the persistent decode step, the kernel
     // generate_cached runs per token; its token is read from token_dev at
@@ -1063,7 +1082,11 @@ static void forward_cached_impl(rtg_cache* c, const uint32_t* ids, size_t n, flo
     HIPX(hipMemcpyAsync(c->ids_in, ids, B * n * 4, hipMemcpyHostToDevice, c->stream));
     enqueue_prefill(c, cache_work(c), c->ids_in, B, n, c->len, logits_out ? LOGITS_ALL : LOGITS_NONE);
   }
+  // test hook RTG_TEST_FORWARD_FAIL=1: as if the pass failed after its kernels
+  const char* fail = getenv("RTG_TEST_FORWARD_FAIL");
+  if (fail && fail[0] == '1') throw HipError{"forward pass failed (RTG_TEST_FORWARD_FAIL)"};
   copy_out(c->stream, m->device, logits_out, c->logits, logits_out ? B * n * V * 4 : 0, nullptr);
+  c->q_reached = 0;
   c->len += n;
 }
 
@@ -1645,7 +1668,7 @@ rtg_result rtg_cache_new_quantised(const rtg_model* model, size_t batch, size_t 
 size_t rtg_cache_len(const rtg_cache* cache) { return cache ? cache->len : 0; }
 bool rtg_cache_is_empty(const rtg_cache* cache) { return rtg_cache_len(cache) == 0; }
 void rtg_cache_clear(rtg_cache* cache) {
-  if (cache) cache->len = 0;
+  if (cache) cache->len = cache->q_reached = 0;
 }
 
 void rtg_cache_destroy(rtg_cache* c) {
