@@ -101,14 +101,14 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
   top = max(r2[0], r2[1]);
   float amax = __uint_as_float(top);
   const bool fine = top < 0x7F800000u;
-  float unit = fabsf(scale) * 1.4426950408889634f * 256.f;
+  float down = 1.f;
   if (__builtin_amdgcn_ballot_w64(amax < 7.9e-31f)) {
     asm volatile("");
     // rows below 2^-100 are taken 2^100 times as large, so that 1 / amax is a number
     const bool tiny = amax < 7.9e-31f;
     const float up = tiny ? 1.2676506e30f : 1.f;
     amax *= up;
-    unit = tiny ? unit * 7.888609e-31f : unit;
+    down = tiny ? 7.888609e-31f : 1.f;
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -132,7 +132,8 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
 #pragma unroll
       for (int i = 0; i < 3; ++i) q[k][i][e] = (int)d[i];
     }
-  return !fine ? NAN : amax > 0.f ? unit / fabsf(inv) : 0.f;
+  // (in this order neither a large scale of small queries nor a small one of large ones leaves f32's range)
+  return !fine ? NAN : amax > 0.f ? 1.4426950408889634f * 256.f / fabsf(inv) * fabsf(scale) * down : 0.f;
 }
 
 // A wave's 16 columns: lane = group * 16 + column; the group's 16 (of 64) query

@@ -154,3 +154,15 @@ def test_padded_prompts(dim, dtype):
     q, qn = rows(b.rng, (seqs, n, heads * group, dim), dtype)
     for counts in (lens, [0, 1, 66, 66, 0, 1, 0, 64, 200, 3]):
         check(b, b.c.attend(q, counts=ints(counts)), qn, dtype, counts, every=23)
+
+
+@pytest.mark.parametrize("dim,n_q,group", [(64, 1, 1), (128, 1, 4), (64, 7, 2)])
+@pytest.mark.parametrize("scale,q_size,k_size", [(3e36, 1e-36, 0.1), (2e38, 1e-20, 1e-19), (-1e37, 1e-33, 1e-4), (1e-37, 1e30, 1e7)])
+def test_scales_of_the_scores_near_the_ends_of_f32(dim, n_q, group, scale, q_size, k_size):
+    b = Both(2, 2, dim, 100, 32, seed=n_q)
+    (k, _), (v, vn), (q, _) = (rows(b.rng, (2, n, h, dim)) for n, h in ((90, 2), (90, 2), (n_q, 2 * group)))
+    k, q = k * k_size, q * q_size
+    b.c.append(k, v)
+    b.r.append(k.double().cpu().numpy(), vn)
+    got = b.c.attend(q, scale=scale)
+    check(b, got, q.double().cpu().numpy(), "f32", scale=float(np.float32(scale)))
