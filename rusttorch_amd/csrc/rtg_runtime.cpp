@@ -4,6 +4,7 @@
 // (sampling of non-greedy generation aside, which the reference also does on
 // the host, gpt2.rs:871-1017).
 #include <hip/hip_runtime.h>
+#include <limits.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -435,8 +436,15 @@ static void ensure_sample_work(rtg_cache* c) {
   if (!c->sample_work) HIPX(device_malloc(&c->sample_work, sample_work_bytes((int)c->m->cfg.vocab_size)));
 }
 
+// (Sequence, head) pairs of a layer that a quantised cache's launches take, and
+// sequences of all layers that its store counts.
+constexpr size_t kMaxQPairs = 1000000;
+
 // block: of a quantised cache, 0 for an f32 one.
 static rtg_cache* cache_create(const rtg_model* m, size_t batch, size_t block = 0) {
+  if (block && (batch > kMaxQPairs / m->cfg.n_head || batch > (size_t)INT_MAX / std::max<size_t>(m->cfg.n_layer, 1)))
+    throw HipError{fmt("batch %zu is too large for a quantised cache (%zu heads, %zu layers)", batch,
+                       (size_t)m->cfg.n_head, (size_t)m->cfg.n_layer)};
   std::unique_ptr<rtg_cache> c(new rtg_cache());
   c->m = m;
   c->batch = batch;
