@@ -237,7 +237,8 @@ rtg_result rtg_generate_cached_quantised(const rtg_model* model, const uint32_t*
  * it then is. Lengths live on the device. A cache must not be used by two
  * calls (or replays) at once, the reading ones included: they share a
  * workspace. Calls on different streams need the streams' own ordering, and a
- * cache has to live as long as the graphs that hold its calls. ---- */
+ * cache has to live as long as the graphs that hold its calls. Making one and
+ * destroying one (which waits for the device) leave captures under way alone. ---- */
 typedef struct rtg_qcache rtg_qcache;
 typedef struct {
   void* data;

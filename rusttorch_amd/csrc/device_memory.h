@@ -27,4 +27,20 @@ hipError_t device_malloc(T** p, size_t n) {
   return device_malloc_bytes(reinterpret_cast<void**>(p), n);
 }
 
+// Allocating and freeing end a capture that is under way on any stream of the
+// process, unless the thread says that it means neither: a cache may be made or
+// (by a garbage collector) given back at any time. (Stream waits within are for streams
+// that no one captures.)
+class BesideCaptures {
+ public:
+  BesideCaptures() { set_ = hipThreadExchangeStreamCaptureMode(&mode_) == hipSuccess; }
+  ~BesideCaptures() {
+    if (set_) (void)hipThreadExchangeStreamCaptureMode(&mode_);
+  }
+
+ private:
+  hipStreamCaptureMode mode_ = hipStreamCaptureModeRelaxed;
+  bool set_ = false;
+};
+
 }  // namespace rtg

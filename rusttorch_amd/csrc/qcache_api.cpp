@@ -116,6 +116,7 @@ rtg_result rtg_qcache_new(size_t n_seq, size_t n_head, size_t head_dim, size_t c
   if (hipGetDeviceCount(&n) != hipSuccess || n == 0)
     return err("no HIP device available: rtgpu requires an MI355X (gfx950) GPU");
   try {
+    BesideCaptures beside;
     std::unique_ptr<rtg_qcache> q(new rtg_qcache());
     hipDeviceProp_t prop;
     if (hipGetDevice(&q->device) != hipSuccess || hipGetDeviceProperties(&prop, q->device) != hipSuccess)
@@ -132,12 +133,15 @@ rtg_result rtg_qcache_new(size_t n_seq, size_t n_head, size_t head_dim, size_t c
     q->tickets = reinterpret_cast<unsigned*>(static_cast<char*>(q->mem) + lens);
     qstore_place(&q->c, static_cast<char*>(q->mem) + head);
     q->work = static_cast<char*>(q->mem) + head + store;
-    e = hipMemset(q->mem, 0, head);
-    if (e == hipSuccess) e = hipMemset(q->err, 0xFF, 4);
+    hipStream_t s = nullptr;  // (of its own: the default one may be what a capture waits for)
+    e = hipStreamCreateWithFlags(&s, hipStreamNonBlocking);
+    if (e == hipSuccess) e = hipMemsetAsync(q->mem, 0, head, s);
+    if (e == hipSuccess) e = hipMemsetAsync(q->err, 0xFF, 4, s);
     if (e == hipSuccess) {
-      qattn_work_clear(nullptr, q->work, q->c.hdp);
-      e = hipDeviceSynchronize();
+      qattn_work_clear(s, q->work, q->c.hdp);
+      e = hipStreamSynchronize(s);
     }
+    if (s) (void)hipStreamDestroy(s);
     if (e != hipSuccess) return hip_err(e, "rtg_qcache_new");
     *out = q.release();
   } catch (const std::exception& ex) {
@@ -149,6 +153,7 @@ rtg_result rtg_qcache_new(size_t n_seq, size_t n_head, size_t head_dim, size_t c
 void rtg_qcache_destroy(rtg_qcache* q) {
   if (!q) return;
   OnDevice dev(q->device);
+  BesideCaptures beside;
   delete q;  // (hipFree waits for the device)
 }
 

@@ -1642,7 +1642,10 @@ rtg_result rtg_model_from_safetensors(const char* path, const rtg_config* cfg, r
   }
 }
 
-void rtg_model_destroy(rtg_model* model) { delete model; }
+void rtg_model_destroy(rtg_model* model) {
+  BesideCaptures beside;
+  delete model;
+}
 
 size_t rtg_num_parameters(const rtg_model* model) { return model ? model->nparams : 0; }
 
@@ -1681,6 +1684,7 @@ void rtg_cache_clear(rtg_cache* cache) {
 
 void rtg_cache_destroy(rtg_cache* c) {
   if (!c) return;
+  BesideCaptures beside;
   if (c->stream) hipStreamSynchronize(c->stream);
   destroy_graph(c);
   if (c->pstate) persistent_state_destroy(c->pstate);
