@@ -166,3 +166,26 @@ def test_scales_of_the_scores_near_the_ends_of_f32(dim, n_q, group, scale, q_siz
     b.r.append(k.double().cpu().numpy(), vn)
     got = b.c.attend(q, scale=scale)
     check(b, got, q.double().cpu().numpy(), "f32", scale=float(np.float32(scale)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,block,seqs,heads,group,n_q", [
+    (128, 16, 10, 4, 4, 100), (128, 32, 10, 4, 4, 100), (128, 64, 10, 4, 4, 100), (80, 32, 10, 4, 5, 80), (80, 16, 10, 8, 1, 170),
+    (64, 64, 300, 8, 1, 5), (64, 16, 10, 4, 4, 160), (20, 32, 12, 10, 2, 100)])
+def test_many_columns_of_every_form(dim, block, seqs, heads, group, n_q, dtype):
+    """Enough blocks of 16 columns that every wave takes all keys of its own; lengths that end in a pair of tiles' first
+    and second tile and in a block's middle, sequences and queries of different numbers."""
+    blocks = seqs * heads * -(-n_q * group // 16)
+    assert n_q * group > 4 and blocks >= (1400 if dim <= 64 else 800)
+    n = 300
+    b = Both(seqs, heads, dim, n, block, dtype, seed=dim + block)
+    lens = b.rng.integers(0, n + 1, seqs)
+    lens[:5] = [n, 128 + 64, 128 + 65, 40, 1]
+    counts = np.minimum(b.rng.integers(0, n_q + 1, seqs), lens)
+    counts[:3] = np.minimum(n_q, lens[:3])
+    (k, kn), (v, vn) = (rows(b.rng, (seqs, n, heads, dim), dtype) for _ in range(2))
+    b.c.append(k, v, counts=ints(lens))
+    b.r.append(kn, vn, lens)
+    q, qn = rows(b.rng, (seqs, n_q, heads * group, dim), dtype, 2.0)
+    got = b.c.attend(q, counts=ints(counts))
+    check(b, got, qn, dtype, counts, every=31, seqs=[0, 1, 2, 3, 4, 7, seqs - 1])
