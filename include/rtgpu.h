@@ -221,7 +221,8 @@ rtg_result rtg_generate_cached_quantised(const rtg_model* model, const uint32_t*
  * tokens (16, 32 or 64) share one scale:
  *   s = f32(max |x| over the block's tokens so far / 127)   (0 where a token's
  *       maximum is below 127 * 2^-126; NaN where a value is not finite)
- *   code = the integer nearest to x / s, ties to even; it reads back as code * s.
+ *   code = the integer nearest to x / s, ties to even; it reads back as code * s
+ *       in f32 (the largest f32 of all as infinity).
  * The last token's block is quantised from its tokens' unrounded values, which
  * are kept in f32 until the next block begins: what the cache holds does not
  * depend on how the tokens were split over appends. 2 bytes per token, head and

@@ -10,10 +10,10 @@
 // The probabilities of bf16 results take two digits (16 bits) in the kernels of
 // 16 columns: each is off by 1.5e-5 of the tile's largest at most, where a half
 // step of bf16 is 2e-3 to 4e-3 of a result; of f16, 2.4e-4 to 4.9e-4, those would
-// show. (2047 tokens of 32 heads of 128 behind 12001 in bf16: 588 us, three digits
-// 677.) Queries take three whatever their type: a channel much larger than the
-// rest would take the others' bits (two digits: 520 us, but f16 results off by 8e-4
-// at a channel 100 times the rest).
+// show. (2047 tokens of 32 heads of 128 behind 12001 in bf16: 593 us, three digits
+// 690.) Queries take three whatever their type: a channel much larger than the
+// rest would take the others' bits (two digits were 70 us faster there, but f16
+// results off by 8e-4 at a channel 100 times the rest).
 // A wave holds 16 columns, a column being a (query, head) pair that reads one
 // key/value head. Scores are computed transposed, so the lanes of a column hold
 // 16 of a tile's keys each: the softmax statistics are lane-local up to two
@@ -474,10 +474,10 @@ struct RowOut {
 //
 // Two tiles at a time: 128 keys share the maximum, the scales and the conversion
 // of their products with the values (a third of the vector work, which bounds
-// this kernel: about 235 instructions per 64 keys and 16 columns in f32 and 220 at
-// 128 columns in 16 bits, 81 to 85 % of the cycles; matrix instructions take 24 to
-// 37 %. 16 x 1023 tokens of 20 heads in f32: 124 us; 2047 tokens of 32 heads of 128
-// behind 12001 in bf16: 510 us, 857 TFLOP/s). A workgroup's
+// this kernel: about 237 instructions per 64 keys and 16 columns in f32 and 242 at
+// 128 columns in bf16, 87 and 75 % of the cycles; matrix instructions take 24 and
+// 39 %. 16 x 1023 tokens of 20 heads in f32: 122 us; 2047 tokens of 32 heads of 128
+// behind 12001 in bf16: 593 us, 736 TFLOP/s). A workgroup's
 // four waves read them from LDS, where LDS-direct loads put the next pair's keys
 // once every wave has this pair's sums, and its values once every wave has its
 // products. (Codes widened to f16, whose products need no joining of digits, take
@@ -1093,7 +1093,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a
 }
 
 // Workgroups of split keys: as many as the device holds at once, which the
-// registers decide (few columns: 120 and 181 of them, 16 columns: 148 and 238).
+// registers decide (few columns: 120 and 181 of them, 16 columns: 156 and 253).
 template <int HDP>
 constexpr int parts(bool few) {
   return few ? HDP == 64 ? 512 : 256 : HDP == 64 ? 768 : 512;
@@ -1104,9 +1104,9 @@ constexpr int kParts = 1024;
 // 1.4 for each of the device's 1024 SIMDs; below, splitting the keys fills it
 // better (1264 blocks: 184 against 231 us over 15000 keys, 19.2 against 21.0 for
 // prompts of 1023), above it only reads them more often (1548: 13.3 against 10.4,
-// 2000: 46.7 against 24.7). hdp 128: what it reads counts earlier (640: 170
-// against 185 us over 12000 keys, 12.4 against 10.2 for a prompt of 320; 1000: 227
-// against 188, 16.4 against 12.9 for one of 500).
+// 2000: 46.7 against 24.7). hdp 128: what it reads counts earlier (bf16, 640: 194
+// against 220 us over 12000 keys, 13.9 against 11.0 for a prompt of 320; 800: 237
+// against 218, 16.7 against 13.2 for one of 400).
 template <int HDP>
 constexpr long kManyBlocks = HDP == 64 ? 1400 : 800;
 

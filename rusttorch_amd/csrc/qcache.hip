@@ -327,9 +327,12 @@ __device__ __forceinline__ void append_tile(const QStore& c, const Place& p, siz
   }
 }
 
-// A workgroup per (sequence, head, tile) and side (keys, values). Memory bounds it
-// (8 x 1000 tokens of 12 heads of 64 in f32: 17.5 us, 3.5 TB/s); short appends are
-// latency: length, rows, the block's earlier tokens (4 x 517 of 8 heads of 128: 12.7 us).
+// A workgroup per (sequence, head, tile) and side (keys, values). Any such append
+// takes 5.6 us of latency (two tokens of 8 x 12 heads of 64: launch, length, rows,
+// stores; one that goes on in a block of 128 columns 8.9: its earlier tokens too);
+// behind that memory bounds it (8 x 1000 tokens in f32: 14.8 to 17 us; 4000 take 36.6
+// us more, 5.0 TB/s), unless the workgroups do not fill the device (4 x 517 of 8
+// heads of 128 in bf16: 640 of them, 12.6 us, 3.4 TB/s behind its 8.9).
 template <int HDP, class T>
 __global__ __launch_bounds__(256) void q_append_kernel(QStore c, QLen len, QTickets tickets, QRows k, QRows v, int n_new,
                                                        const int* __restrict__ counts, const int* __restrict__ start,
@@ -351,7 +354,10 @@ __global__ __launch_bounds__(256) void q_append_kernel(QStore c, QLen len, QTick
 }
 
 // One new token (or only a cut) for each sequence: a workgroup per (sequence, head).
-// Latency bounds it: 4.1 us for 16 sequences of 25 heads, 400 workgroups.
+// Latency bounds it: 3.8 us for 16 sequences of 25 heads, 400 workgroups, where no
+// token raises its block's scale. Among so many one nearly always does, and its
+// block is written anew, two waves taking its tokens by turns: 5.8 us a token on
+// average over a block of 32, 7.7 of 64 (128 columns, 8 x 8 heads: 7.9 and 10.9).
 template <int HDP, class T>
 __global__ __launch_bounds__(256) void q_append_one_kernel(QStore c, QLen len, QTickets tickets, QRows k, QRows v,
                                                            int n_new, const int* __restrict__ counts,

@@ -3,10 +3,15 @@
 
 Programs that run their own layers write keys and values with `append`, run
 attention over them with `attend` and get them back with `read`; the calls go
-to the tensors' current stream and do not wait for it. Tensors are
-[n_seq, tokens, heads, head_dim] on the cache's device, f32, bf16 or f16, in any
-strides whose last is 1. Nothing here has a gradient. There is no counterpart in
-the reference.
+to the current stream of the cache's device and do not wait for it. Tensors are
+[n_seq, tokens, heads, head_dim] on that device, f32, bf16 or f16, in any strides
+whose last is 1. Nothing here has a gradient. There is no counterpart in the
+reference.
+
+One cache takes one call at a time, reading ones included: they share a
+workspace. Calls on two streams, replays of two graphs, or a replay beside a call
+need the streams' own ordering (`wait_stream`, events); different caches do not.
+A cache has to live as long as the graphs that hold its calls.
 """
 from __future__ import annotations
 
