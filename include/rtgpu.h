@@ -268,10 +268,7 @@ rtg_result rtg_qcache_read(const rtg_qcache* cache, rtg_dtype dtype, const rtg_r
 /* Causal attention of the last counts[s] (n_q for NULL, clamped to 0 .. n_q)
  * tokens of every sequence: query i of c sits at position len - c + i and sees
  * the keys up to its own; softmax of scale * q . k, in f32 or better, results
- * rounded to dtype once. (One thing is less exact than f32: for bf16 results and
- * more than four queries times heads per key/value head, a probability times its
- * value's scale is held in 16 bits of the largest such product among 64 or 128
- * keys.) Query head h reads key/value head h / (n_q_head /
+ * rounded to dtype once. Query head h reads key/value head h / (n_q_head /
  * n_head), at most 1024 of them one key/value head. A block that reads back as
  * NaN makes the rows NaN that see a key of it, and no others; a query with a
  * value that is not finite gives a row of NaN. Sums are f32 and divided last:

@@ -1,19 +1,17 @@
 // Attention over the 8-bit key/value cache (qcache.h) on i8 matrix instructions.
 //
 // The codes go into v_mfma_i32_16x16x64_i8 as they lie in memory; what they
-// multiply is held as fixed-point numbers of ND signed 8-bit digits, an MFMA
+// multiply is held as fixed-point numbers of three signed 8-bit digits, an MFMA
 // for each digit, so every product and sum is exact:
 //   scores  S[key][query] = K Q^T: q = sq * (d2 2^16 + d1 2^8 + d0) with sq from
 //           the largest |q| of the row: 24 bits, as f32 has;
 //   output  O[column][query] = V^T P^T: p of a tile of 64 keys, times its
 //           block's scale, over the tile's largest such product: 24 bits again.
-// The probabilities of bf16 results take two digits (16 bits) in the kernels of
-// 16 columns: each is off by 1.5e-5 of the tile's largest at most, where a half
-// step of bf16 is 2e-3 to 4e-3 of a result; of f16, 2.4e-4 to 4.9e-4, those would
-// show. (2047 tokens of 32 heads of 128 behind 12001 in bf16: 593 us, three digits
-// 690.) Queries take three whatever their type: a channel much larger than the
-// rest would take the others' bits (two digits were 70 us faster there, but f16
-// results off by 8e-4 at a channel 100 times the rest).
+// This goes for 16-bit types too: a query's channel much larger than the rest would
+// take the others' bits (with two digits f16 results were off by 8e-4 at a channel
+// 100 times the rest), and 128 probabilities of 16 bits move a result by 1e-4 of
+// itself, of bf16's steps by one in 40. (2047 tokens of 32 heads of 128 behind 12001
+// in bf16: 693 us; two digits for the probabilities 593, for both 510.)
 // A wave holds 16 columns, a column being a (query, head) pair that reads one
 // key/value head. Scores are computed transposed, so the lanes of a column hold
 // 16 of a tile's keys each: the softmax statistics are lane-local up to two
@@ -36,12 +34,9 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// Largest fixed-point values of 3 and 2 balanced digits (127 * 65536 + 127 * 256
-// + 127 and 127 * 256 + 127), less a margin for the rounding of their scales.
-template <int ND>
-__device__ __forceinline__ constexpr float fixed_max() {
-  return ND == 3 ? 8355000.f : 32600.f;
-}
+// Largest fixed-point value of three balanced digits (127 * 65536 + 127 * 256 +
+// 127), less a margin for the rounding of its scale.
+constexpr float kFixedMax = 8355000.f;
 
 __device__ __forceinline__ unsigned perm(unsigned a, unsigned b, unsigned sel) {
   return __builtin_amdgcn_perm(a, b, sel);  // bytes 0-3 of sel: of b, 4-7: of a
@@ -49,32 +44,25 @@ __device__ __forceinline__ unsigned perm(unsigned a, unsigned b, unsigned sel) {
 
 // Digit planes of four fixed-point values whose digits are the bytes of u0 .. u3,
 // but for the top one plus 128: d[i] holds digit i of the four.
-template <int ND>
-__device__ __forceinline__ void planes(unsigned u0, unsigned u1, unsigned u2, unsigned u3, unsigned (&d)[ND]) {
+__device__ __forceinline__ void planes(unsigned u0, unsigned u1, unsigned u2, unsigned u3, unsigned (&d)[3]) {
   const unsigned a = perm(u1, u0, 0x05010400), b = perm(u3, u2, 0x05010400);  // [x0 y0 x1 y1]
   d[0] = perm(b, a, 0x05040100) ^ 0x80808080u;
-  d[1] = perm(b, a, 0x07060302);
-  if (ND == 3) d[1] ^= 0x80808080u;
-  if constexpr (ND == 3) d[2] = perm(perm(u3, u2, 0x0c0c0602), perm(u1, u0, 0x0c0c0602), 0x05040100);
+  d[1] = perm(b, a, 0x07060302) ^ 0x80808080u;
+  d[2] = perm(perm(u3, u2, 0x0c0c0602), perm(u1, u0, 0x0c0c0602), 0x05040100);
 }
 
-// acc[0 .. ND): sums over the digits -> their value; in units of 256 for ND = 3
-// (the lowest digit's sum enters as its rounded 256th).
-template <int ND, int KS>
-__device__ __forceinline__ i32x4 fixed_mfma(const i32x4 (&a)[KS], const i32x4 (&b)[KS][ND]) {
-  const i32x4 zero = {0, 0, 0, 0};
-  i32x4 lo = ND == 3 ? i32x4{128, 128, 128, 128} : zero, mid, hi = zero;
+// Sums over the digits -> their value, in units of 256 (the lowest digit's sum
+// enters as its rounded 256th).
+template <int KS>
+__device__ __forceinline__ i32x4 fixed_mfma(const i32x4 (&a)[KS], const i32x4 (&b)[KS][3]) {
+  i32x4 lo = {128, 128, 128, 128}, hi = {0, 0, 0, 0};
 #pragma unroll
   for (int k = 0; k < KS; ++k) lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[k], b[k][0], lo, 0, 0, 0);
-  if constexpr (ND == 3) {
-    mid = lo >> 8;
+  i32x4 mid = lo >> 8;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[k], b[k][1], mid, 0, 0, 0);
-  } else {
-    mid = lo;
-  }
+  for (int k = 0; k < KS; ++k) mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[k], b[k][1], mid, 0, 0, 0);
 #pragma unroll
-  for (int k = 0; k < KS; ++k) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[k], b[k][ND - 1], hi, 0, 0, 0);
+  for (int k = 0; k < KS; ++k) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[k], b[k][2], hi, 0, 0, 0);
   return (hi << 8) + mid;
 }
 
@@ -117,7 +105,7 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
   }
   // (a negative scale goes into the digits: the factor of the sums is not negative;
   // it comes from inv as it was rounded, or all scores would be off by its rounding)
-  const float inv = fine && amax > 0.f ? copysignf(fixed_max<3>(), scale) / amax : 0.f;
+  const float inv = fine && amax > 0.f ? copysignf(kFixedMax, scale) / amax : 0.f;
   constexpr float bias = 8421504.f;  // 0x808080: every digit plus 128
 #pragma unroll
   for (int k = 0; k < KS; ++k)
@@ -127,7 +115,7 @@ __device__ __forceinline__ float fixed_query(const T* qrow, int hd, bool vec, in
       unsigned u[4], d[3];
 #pragma unroll
       for (int i = 0; i < 4; ++i) u[i] = (unsigned)rintf(fmaf(xe[i], inv, bias));  // (NaN and infinity: sq says so)
-      planes<3>(u[0], u[1], u[2], u[3], d);
+      planes(u[0], u[1], u[2], u[3], d);
       d[2] ^= 0x80808080u;
 #pragma unroll
       for (int i = 0; i < 3; ++i) q[k][i][e] = (int)d[i];
@@ -280,16 +268,16 @@ __device__ __forceinline__ bool all_taken(int live, int& only) {
 // k: 16 keys; s[4]: a lane's fixed-point sums of them.
 template <int HDP>
 __device__ __forceinline__ void tile_sums(const Cols<HDP>& c, const i32x4 (&k)[HDP / 64], float (&s)[4]) {
-  const i32x4 d = fixed_mfma<3, HDP / 64>(k, c.q);
+  const i32x4 d = fixed_mfma<HDP / 64>(k, c.q);
 #pragma unroll
   for (int e = 0; e < 4; ++e) s[e] = (float)d[e];
 }
 
 // s: the keys' fixed-point sums. pd: the probabilities' digits, w: what
 // their products with the values' codes are to be multiplied with.
-template <bool EDGE, int HDP, int ND, int NG, int SH>
+template <bool EDGE, int HDP, int NG, int SH>
 __device__ __forceinline__ void tile_probs(Cols<HDP>& c, float (&s)[NG][4], const TileScales<NG, SH>& ts, int j0,
-                                           int group, i32x4 (&pd)[NG / 4][ND], float& w) {
+                                           int group, i32x4 (&pd)[NG / 4][3], float& w) {
   constexpr int DT = HDP / 16, NB = TileScales<NG, SH>::NB, PER = NG / NB;  // 16s per block
   float f[NB], cc[NB];
   float top = -INFINITY;
@@ -353,24 +341,24 @@ __device__ __forceinline__ void tile_probs(Cols<HDP>& c, float (&s)[NG][4], cons
 #pragma unroll
     for (int i = 0; i < 4; ++i) c.o[d][i] *= corr;
   c.m = mn;
-  w = g * ts.vmax * ((ND == 3 ? 256.f : 1.f) / fixed_max<ND>());
+  w = g * ts.vmax * (256.f / kFixedMax);
   // rounded to an integer, the digits below the top one plus 128, in the low bits of the sum with 2^23
-  constexpr float magic = ND == 3 ? 8421504.f : 8388736.f;  // 2^23 + 0x8080, 2^23 + 0x80
+  constexpr float magic = 8421504.f;  // 2^23 + 0x8080
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
-    unsigned u[4], d[ND];
+    unsigned u[4], d[3];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(fmaf(s[i][e], fixed_max<ND>(), magic));
-    planes<ND>(u[0], u[1], u[2], u[3], d);
+    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(fmaf(s[i][e], kFixedMax, magic));
+    planes(u[0], u[1], u[2], u[3], d);
 #pragma unroll
-    for (int n = 0; n < ND; ++n) pd[i / 4][n][i & 3] = (int)d[n];
+    for (int n = 0; n < 3; ++n) pd[i / 4][n][i & 3] = (int)d[n];
   }
 }
 
 // v: 16 columns of the tiles' values; o[4]: the results of them.
-template <int ND, int NT>
-__device__ __forceinline__ void tile_product(const i32x4 (&v)[NT], const i32x4 (&pd)[NT][ND], float w, float (&o)[4]) {
-  const i32x4 r = fixed_mfma<ND, NT>(v, pd);
+template <int NT>
+__device__ __forceinline__ void tile_product(const i32x4 (&v)[NT], const i32x4 (&pd)[NT][3], float w, float (&o)[4]) {
+  const i32x4 r = fixed_mfma<NT>(v, pd);
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = fmaf((float)r[i], w, o[i]);
 }
@@ -474,10 +462,10 @@ struct RowOut {
 //
 // Two tiles at a time: 128 keys share the maximum, the scales and the conversion
 // of their products with the values (a third of the vector work, which bounds
-// this kernel: about 237 instructions per 64 keys and 16 columns in f32 and 242 at
-// 128 columns in bf16, 87 and 75 % of the cycles; matrix instructions take 24 and
-// 39 %. 16 x 1023 tokens of 20 heads in f32: 122 us; 2047 tokens of 32 heads of 128
-// behind 12001 in bf16: 593 us, 736 TFLOP/s). A workgroup's
+// this kernel: about 237 instructions per 64 keys and 16 columns of 64 and 277 of
+// 128, 86 and 69 % of the cycles; matrix instructions take 24 and 38 %. 16 x 1023
+// tokens of 20 heads in f32: 120 us; 2047 tokens of 32 heads of 128 behind 12001 in
+// bf16: 693 us, 630 TFLOP/s, its 194 registers leave two waves a SIMD). A workgroup's
 // four waves read them from LDS, where LDS-direct loads put the next pair's keys
 // once every wave has this pair's sums, and its values once every wave has its
 // products. (Codes widened to f16, whose products need no joining of digits, take
@@ -507,8 +495,8 @@ struct SharedPair {
   i32x4 k[kPair * CH], v[kPair * CH];
 };
 
-template <int HDP, int ND, int SH, int KIND, class T>
-__global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend_cols_kernel(AttnArgs a) {
+template <int HDP, int SH, int KIND, class T>
+__global__ __launch_bounds__(256, HDP == 64 ? 4 : 2) void q_attend_cols_kernel(AttnArgs a) {
   using Pair = SharedPair<HDP>;
   constexpr int U = Pair::U, CH = Pair::CH, KS = HDP / 64;
   __shared__ Pair t;
@@ -581,14 +569,14 @@ __global__ __launch_bounds__(256, HDP == 64 ? 4 : ND == 2 ? 3 : 2) void q_attend
       fetch(kp, j + 1, kv, lk);
       sl = load_s(j + 1);
     }
-    i32x4 pd[NG / 4][ND];
+    i32x4 pd[NG / 4][3];
     tile_probs<decltype(edge)::value>(c, s, ts, j * kPair, group, pd, w);
 #pragma unroll
     for (int d = 0; d < HDP / 16; ++d) {
       i32x4 v[NG / 4];
 #pragma unroll
       for (int i = 0; i < NG / 4; ++i) v[i] = t.v[(i * 4 + group) * HDP + d * 16 + col];
-      tile_product<ND, NG / 4>(v, pd, w, c.o[d]);
+      tile_product<NG / 4>(v, pd, w, c.o[d]);
       if (d & 1) __builtin_amdgcn_sched_barrier(0);
     }
     if (more) {
@@ -777,7 +765,7 @@ __device__ __forceinline__ void finish(const AttnArgs& a, Merge<HDP, W, NW>& s, 
   }
 }
 
-template <int HDP, int ND, int SH, int KIND, class T>
+template <int HDP, int SH, int KIND, class T>
 __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
   constexpr int NW = 4;
   __shared__ Merge<HDP, 16, NW> s;
@@ -806,7 +794,7 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
   if (j < t1) load(t, j);
   auto take = [&](const TileScales<4, SH>& ts, bool edge) {
     float sums[4][4];
-    i32x4 pd[1][ND];
+    i32x4 pd[1][3];
     float w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) tile_sums<HDP>(c, t.k[i], sums[i]);
@@ -815,7 +803,7 @@ __global__ __launch_bounds__(256) void q_attend_split_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < HDP / 16; ++d) {
       const i32x4 v[1] = {t.v[d]};
-      tile_product<ND, 1>(v, pd, w, c.o[d]);
+      tile_product<1>(v, pd, w, c.o[d]);
     }
   };
   bool left = false;  // tiles whose scales lie far apart
@@ -1093,7 +1081,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void q_attend_few_kernel(AttnArgs a
 }
 
 // Workgroups of split keys: as many as the device holds at once, which the
-// registers decide (few columns: 120 and 181 of them, 16 columns: 156 and 253).
+// registers decide (few columns: 120 and 181 of them, 16 columns: 156 and 249).
 template <int HDP>
 constexpr int parts(bool few) {
   return few ? HDP == 64 ? 512 : 256 : HDP == 64 ? 768 : 512;
@@ -1104,9 +1092,9 @@ constexpr int kParts = 1024;
 // 1.4 for each of the device's 1024 SIMDs; below, splitting the keys fills it
 // better (1264 blocks: 184 against 231 us over 15000 keys, 19.2 against 21.0 for
 // prompts of 1023), above it only reads them more often (1548: 13.3 against 10.4,
-// 2000: 46.7 against 24.7). hdp 128: what it reads counts earlier (bf16, 640: 194
-// against 220 us over 12000 keys, 13.9 against 11.0 for a prompt of 320; 800: 237
-// against 218, 16.7 against 13.2 for one of 400).
+// 2000: 46.7 against 24.7). hdp 128: what it reads counts earlier (bf16, 640: 204
+// against 244 us over 12000 keys, 14.5 against 11.7 for a prompt of 320; 800: 248
+// against 244, 17.3 against 14.4 for one of 400).
 template <int HDP>
 constexpr long kManyBlocks = HDP == 64 ? 1400 : 800;
 
@@ -1120,7 +1108,7 @@ dim3 split_grid(AttnArgs& a, bool few) {
   return dim3((unsigned)heads, (unsigned)a.cblocks, (unsigned)a.splits);
 }
 
-template <int HDP, int ND, int KIND, class T>
+template <int HDP, int KIND, class T>
 void attend(hipStream_t s, AttnArgs& a) {
   const long heads = (long)a.c.n_seq * a.c.n_head;
   const int columns = a.n_q * a.group, sh = a.c.block_shift;
@@ -1131,13 +1119,13 @@ void attend(hipStream_t s, AttnArgs& a) {
     q_attend_few_kernel<HDP, 4, KIND, T, false><<<grid, 64 * kFewWaves, 0, s>>>(a);
   } else if (heads * a.cblocks >= kManyBlocks<HDP>) {
     const dim3 wide((unsigned)heads, (unsigned)((a.cblocks + 3) / 4));
-    if (sh == 4) q_attend_cols_kernel<HDP, ND, 4, KIND, T><<<wide, 256, 0, s>>>(a);
-    else if (sh == 5) q_attend_cols_kernel<HDP, ND, 5, KIND, T><<<wide, 256, 0, s>>>(a);
-    else q_attend_cols_kernel<HDP, ND, 6, KIND, T><<<wide, 256, 0, s>>>(a);
+    if (sh == 4) q_attend_cols_kernel<HDP, 4, KIND, T><<<wide, 256, 0, s>>>(a);
+    else if (sh == 5) q_attend_cols_kernel<HDP, 5, KIND, T><<<wide, 256, 0, s>>>(a);
+    else q_attend_cols_kernel<HDP, 6, KIND, T><<<wide, 256, 0, s>>>(a);
   } else {
-    if (sh == 4) q_attend_split_kernel<HDP, ND, 4, KIND, T><<<grid, 256, 0, s>>>(a);
-    else if (sh == 5) q_attend_split_kernel<HDP, ND, 5, KIND, T><<<grid, 256, 0, s>>>(a);
-    else q_attend_split_kernel<HDP, ND, 6, KIND, T><<<grid, 256, 0, s>>>(a);
+    if (sh == 4) q_attend_split_kernel<HDP, 4, KIND, T><<<grid, 256, 0, s>>>(a);
+    else if (sh == 5) q_attend_split_kernel<HDP, 5, KIND, T><<<grid, 256, 0, s>>>(a);
+    else q_attend_split_kernel<HDP, 6, KIND, T><<<grid, 256, 0, s>>>(a);
   }
 }
 
@@ -1146,13 +1134,13 @@ bool vec4(const QRows& r, int hd, size_t size) {
          reinterpret_cast<uintptr_t>(r.p) % (4 * size) == 0;
 }
 
-template <int ND, class T>
+template <class T>
 void attend_t(hipStream_t s, AttnArgs& a) {
   if constexpr (sizeof(T) == 4) {
-    if (a.out.kind == QO_PAIR) return attend<64, ND, QO_PAIR, T>(s, a);
+    if (a.out.kind == QO_PAIR) return attend<64, QO_PAIR, T>(s, a);
   }
-  if (a.c.hdp == 64) attend<64, ND, QO_ROWS, T>(s, a);
-  else attend<128, ND, QO_ROWS, T>(s, a);
+  if (a.c.hdp == 64) attend<64, QO_ROWS, T>(s, a);
+  else attend<128, QO_ROWS, T>(s, a);
 }
 
 }  // namespace
@@ -1193,9 +1181,9 @@ AttnArgs attn_args(const QStore& c, QLen len, int extra, QType type, const QRows
 void launch_q_attend(hipStream_t s, const QStore& c, QLen len, int extra, QType type, const QRows& q, int n_q,
                      int n_q_head, const int* counts, float scale, const QOut& out, void* work) {
   AttnArgs a = attn_args(c, len, extra, type, q, n_q, n_q_head, counts, scale, out, work);
-  if (type == Q_F32) attend_t<3, float>(s, a);
-  else if (type == Q_BF16) attend_t<2, __bf16>(s, a);
-  else attend_t<3, _Float16>(s, a);
+  if (type == Q_F32) attend_t<float>(s, a);
+  else if (type == Q_BF16) attend_t<__bf16>(s, a);
+  else attend_t<_Float16>(s, a);
 }
 
 void launch_q_step(hipStream_t s, const QStore& c, QLen len, const QRows& k, const QRows& v, const QRows& q,

@@ -26,14 +26,13 @@ def check(b, got, q, dtype, counts=None, scale=None, every=1, seqs=None):
         8 EPS of the score's size for the roundings on its way to an exponent (the scale, log2 e and their product, the
         unit of the sums, its product with the key's scale, the sums to f32, the difference to the maximum and the
         maximum's own), 2 EPS for exp2; a change of the scores by e_j moves o by sum p_j |v_j - o| e_j at most;
-      - the probabilities as fixed point: half a step, 1.01 EPS (bf16 and more than four columns: 2^-16) of the largest
-        product p_j * (largest |v| of the block) of the (up to 128) keys taken together, for each of them;
+      - the probabilities as fixed point: half a step, 1.01 EPS of the largest product p_j * (largest |v|
+        of the block) of the (up to 128) keys taken together, for each of them;
       - f32 sums: 4 EPS of sum p_j |v_j| for every 64 keys, 16 times that for joins and the factors of a tile."""
     D, r = q.shape[-1], b.r
     scale = D ** -0.5 if scale is None else scale
     got = got.double().cpu().numpy()
     group = q.shape[2] // r.heads
-    step = 1.01 * (2.0 ** -16 if dtype == "bf16" and q.shape[1] * group > 4 else EPS)
     worst = 0.0
     for s in range(q.shape[0]) if seqs is None else seqs:
         c = q.shape[1] if counts is None else min(max(int(counts[s]), 0), q.shape[1])
@@ -55,7 +54,7 @@ def check(b, got, q, dtype, counts=None, scale=None, every=1, seqs=None):
                 e = abs(scale) * 1.01 * EPS * np.abs(q[s, i, h]).max() * np.abs(k[:see]).sum(1) + 8 * EPS * np.abs(sc) + 2 * EPS
                 off = (p * e) @ np.abs(v[:see] - o)
                 prod = np.concatenate([p * top[:see], np.zeros(-see % 128)]).reshape(-1, 128)
-                off = off + step * 128 * prod.max(1).sum() + 4 * EPS * (see / 64 + 16) * (p @ np.abs(v[:see]))
+                off = off + 1.01 * EPS * 128 * prod.max(1).sum() + 4 * EPS * (see / 64 + 16) * (p @ np.abs(v[:see]))
                 over = np.abs(got[s, i, h] - o) - (spacing(o, dtype) / 2 + off)
                 assert np.all(over <= 0), (s, h, i, over.max(), np.abs(off).max(), np.abs(o).max())
                 worst = max(worst, (np.abs(got[s, i, h] - o) / (spacing(o, dtype) / 2 + off)).max())
