@@ -282,6 +282,86 @@ rtg_result rtg_qcache_attend(rtg_qcache* cache, rtg_dtype dtype, const rtg_rows*
  * left a sequence as it was. Not for a stream that is being captured. */
 rtg_result rtg_qcache_lengths(rtg_qcache* cache, uint32_t* out, void* stream);
 
+/* ---- 4-bit key/value cache over device tensors, and its eviction (no
+ * counterpart in the reference). A quarter to an eighth of the memory of f32 and
+ * bf16 rows and half of the 8-bit cache's, for contexts that are long or many.
+ *
+ * For each (sequence, head) and token, keys and values apart, 32 consecutive
+ * channels are numbers of 4 bits (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times a
+ * power of two:
+ *   p = the largest power of two not above the channels' max |x|, twice that
+ *       where the maximum is over 1.75 p; scale = p / 4, within 2^-100 .. 2^125
+ *   the number nearest to x / scale, ties to the one of even code, 6 at most
+ * It reads back as number * scale, which f32 and bf16 hold exactly; the 32
+ * channels read back as NaN where one of them is not finite. A token's numbers
+ * depend on its own values alone. (head_dim / 2 + head_dim / 32) bytes per token
+ * and head for keys and as many for values (head_dim padded to 64 or 128), and 4
+ * for the token's weight: what attention it has got.
+ *
+ * Rows, streams, captures, devices and the order of calls are as for rtg_qcache
+ * above: one call or replay at a time on one cache. ---- */
+typedef struct rtg_fourbit rtg_fourbit;
+/* Errors: "head_dim <hd> is not supported (1 to 128)", capacities over 4000000
+ * tokens, more than 1000000 pairs of sequence and head. */
+rtg_result rtg_fourbit_new(size_t n_seq, size_t n_head, size_t head_dim, size_t capacity, rtg_fourbit** out);
+void rtg_fourbit_destroy(rtg_fourbit* cache);
+/* As rtg_qcache_append. The new tokens' weights are 0. */
+rtg_result rtg_fourbit_append(rtg_fourbit* cache, rtg_dtype dtype, const rtg_rows* k, const rtg_rows* v, size_t n_new,
+                              const int32_t* counts, const int32_t* start, void* stream);
+/* As rtg_qcache_read. */
+rtg_result rtg_fourbit_read(const rtg_fourbit* cache, rtg_dtype dtype, const rtg_rows* k, const rtg_rows* v, size_t n,
+                            const int32_t* first, void* stream);
+/* As rtg_qcache_attend: causal attention of the last counts[s] tokens of every
+ * sequence, rows of padding and of queries before the first token 0. Queries times
+ * scale, scores, and 256 times the largest |v| times the number of keys have to be
+ * within f32. A key that reads back as NaN makes the rows NaN that see it, a value
+ * their channels of the same 32, and no others; a query that is not finite gives a
+ * row of NaN. stats (may be NULL): n_seq * n_q * n_q_head * 2 f32 for
+ * rtg_fourbit_weigh. */
+rtg_result rtg_fourbit_attend(rtg_fourbit* cache, rtg_dtype dtype, const rtg_rows* queries, size_t n_q,
+                              size_t n_q_head, const int32_t* counts, float scale, const rtg_rows* out, float* stats,
+                              void* stream);
+/* The weights of all tokens become decay (0 .. 1; 0 whatever they were) times what
+ * they are, plus the probabilities that the counted queries of all heads of the
+ * token's head give them. Behind an rtg_fourbit_attend of the same cache, queries,
+ * counts and scale, whose stats it takes, with no append between. */
+rtg_result rtg_fourbit_weigh(rtg_fourbit* cache, rtg_dtype dtype, const rtg_rows* queries, size_t n_q,
+                             size_t n_q_head, const int32_t* counts, float scale, const float* stats, float decay,
+                             void* stream);
+/* The weights of tokens 0 .. n - 1 to out [n_seq][n_head][n], 0 where there is no
+ * token; and x [n_seq][n_head][n] added to those of the tokens that there are. */
+rtg_result rtg_fourbit_weights(const rtg_fourbit* cache, float* out, size_t n, void* stream);
+rtg_result rtg_fourbit_add_weights(rtg_fourbit* cache, const float* x, size_t n, void* stream);
+/* Cuts every sequence longer than `keep` to that many tokens: each head keeps the
+ * last `recent` and, of the others, the keep - recent of the largest weights (of
+ * equal ones the first; NaN is larger than all), in their order and with their
+ * weights. kept [n_seq][n_head][keep]: which tokens these were, ascending, -1
+ * behind those of a shorter sequence. Positions count what is left from then on:
+ * keys that hold rotary positions keep those they were written with. */
+rtg_result rtg_fourbit_evict(rtg_fourbit* cache, size_t keep, size_t recent, int32_t* kept, void* stream);
+/* As rtg_qcache_lengths. */
+rtg_result rtg_fourbit_lengths(rtg_fourbit* cache, uint32_t* out, void* stream);
+
+/* ---- Causal attention over packed prompts (no counterpart in the reference,
+ * whose prompts are one sequence, gpt2.rs:639-770): rows of n_seq sequences one
+ * behind the other, each attending to itself; query row i of a sequence sees its
+ * rows 0 .. i. Rows are [n_rows][heads][head_dim] in device memory of the current
+ * device (stride_seq is not used), offsets n_seq + 1 device int32: sequence s has
+ * rows offsets[s] .. offsets[s + 1] - 1; they must not descend, and are clamped to
+ * the rows there are. Rows of no sequence are set to 0. Query head h reads
+ * key/value head h / (n_q_head / n_head), at most 1024 of them one.
+ *
+ * softmax of scale * q . k; sums are f32, results rounded to dtype once, the
+ * probabilities of bf16 rows to bf16 (sums of f16 and bf16 rows: of the rounded
+ * ones). Queries times scale, scores, and 256 times the largest |v| times the
+ * number of keys have to be within f32. A key with a value that is not finite
+ * makes the rows not finite that see it, a value their channel, and no others.
+ * Enqueues one kernel on `stream`, allocates nothing, may be captured; out must
+ * not overlap the others. ---- */
+rtg_result rtg_attend_packed(rtg_dtype dtype, const rtg_rows* q, const rtg_rows* k, const rtg_rows* v, size_t n_rows,
+                             size_t n_q_head, size_t n_head, size_t head_dim, const int32_t* offsets, size_t n_seq,
+                             float scale, const rtg_rows* out, void* stream);
+
 /* ---- BpeTokenizer, rusttorch-core/src/data/tokenizer.rs (host-side text in
  * and out; used by the reference's example at examples/gpt2.rs:77-95).
  * Text is UTF-8 with an explicit length (a Rust &str). Buffers that a call

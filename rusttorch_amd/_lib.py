@@ -93,7 +93,7 @@ SIGNATURES = {
                                              C.c_void_p, C.POINTER(Timing)]),
     "rtg_generate_cached_quantised": (Result, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t,
                                                C.c_void_p, C.POINTER(Timing)]),
-    # (an rtg_rows is passed as its bytes: qcache.py)
+    # (an rtg_rows is passed as its bytes: qcache.py, q4cache.py, attention.py)
     "rtg_qcache_new": (Result, [C.c_size_t] * 5 + [C.POINTER(C.c_void_p)]),
     "rtg_qcache_destroy": (None, [C.c_void_p]),
     "rtg_qcache_append": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_char_p, C.c_size_t, C.c_void_p,
@@ -103,6 +103,22 @@ SIGNATURES = {
     "rtg_qcache_attend": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_size_t, C.c_size_t, C.c_void_p,
                                    C.c_float, C.c_char_p, C.c_void_p]),
     "rtg_qcache_lengths": (Result, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "rtg_fourbit_new": (Result, [C.c_size_t] * 4 + [C.POINTER(C.c_void_p)]),
+    "rtg_fourbit_destroy": (None, [C.c_void_p]),
+    "rtg_fourbit_append": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_char_p, C.c_size_t, C.c_void_p,
+                                    C.c_void_p, C.c_void_p]),
+    "rtg_fourbit_read": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_char_p, C.c_size_t, C.c_void_p,
+                                  C.c_void_p]),
+    "rtg_fourbit_attend": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_size_t, C.c_size_t, C.c_void_p,
+                                    C.c_float, C.c_char_p, C.c_void_p, C.c_void_p]),
+    "rtg_fourbit_weigh": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_size_t, C.c_size_t, C.c_void_p,
+                                   C.c_float, C.c_void_p, C.c_float, C.c_void_p]),
+    "rtg_fourbit_weights": (Result, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "rtg_fourbit_add_weights": (Result, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "rtg_fourbit_evict": (Result, [C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "rtg_fourbit_lengths": (Result, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "rtg_attend_packed": (Result, [C.c_int] + [C.c_char_p] * 3 + [C.c_size_t] * 4 + [C.c_void_p, C.c_size_t, C.c_float,
+                                                                                 C.c_char_p, C.c_void_p]),
     "rtg_tokenizer_from_files": (Result, [C.c_char_p, C.c_char_p, C.POINTER(C.c_void_p)]),
     "rtg_tokenizer_from_strings": (Result, [C.c_char_p, C.c_size_t, C.c_char_p, C.c_size_t, C.POINTER(C.c_void_p)]),
     "rtg_tokenizer_from_vocab_and_merges": (Result, [C.POINTER(C.c_char_p), C.c_size_t, C.POINTER(C.c_char_p),

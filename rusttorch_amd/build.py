@@ -39,7 +39,8 @@ SOURCES = ["kernels.hip", "gemm_pair.hip", "attn_pair.hip", "decode_persistent.h
            "decode_persistent_inst_small.hip", "decode_persistent_inst_medium.hip",
            "decode_persistent_inst_large.hip", "rtg_runtime.cpp", "device_memory.cpp", "safetensors_reader.cpp",
            "tokenizer.cpp", "sampling.hip", "bgemv.hip", "scratch.hip", "decode_tile.hip", "rows.hip",
-           "qcache.hip", "qattn.hip", "qcache_api.cpp"]
+           "qcache.hip", "qattn.hip", "qcache_api.cpp", "fourbit.hip", "fourbit_attn.hip", "attn_tile.hip",
+           "fourbit_api.cpp"]
 
 
 def _compile(src: str) -> str:

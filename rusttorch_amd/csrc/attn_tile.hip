@@ -1,0 +1,520 @@
+// Attention for many queries: packed prompts over their own keys, and the 4-bit
+// cache's (fourbit.h) chunks and prompts.
+//
+// Four waves share the keys and values of one head, 64 at a time in LDS; a wave
+// has 32 rows, a row being a (query, head) pair that reads this key/value head
+// (the heads of a group side by side, so a tile of 128 rows is 128 / group
+// positions and little of it lies above the diagonal).
+//   scores  S[key][row] = K Q^T on v_mfma_f32_32x32x16, computed transposed: a
+//           row's lanes hold 16 of 32 keys each, maximum and sum of the softmax
+//           need the lane 32 further on only, and the probabilities are the
+//           matrix operand of the second product as they lie;
+//   output  O[channel][row] = V^T P^T. Values lie in LDS as rows, like keys; the
+//           operand is read with ds_read_b64_tr_b16, which gives a lane four keys
+//           of one channel.
+// f16 rows are taken as they are by the f16 instructions, bf16 rows by the bf16
+// ones. f32 numbers are the sum of three bf16 parts (24 bits): of the products
+// of parts the six that reach f32's last bits are computed. Over the 4-bit cache
+// keys and values are bf16 exactly, f16 queries two parts. Probabilities: one part
+// for bf16 results (2^-9 of each, as the results' own rounding; their sum is taken
+// of the rounded ones, so that it cancels where values agree), f16 for packed f16
+// ones (from 2^-24 to 2^14 of 2^6), two bf16 parts for f16 over the cache, three
+// for f32. Sums are f32.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "attn_core.h"
+#include "f16_pair.h"
+#include "fourbit_core.h"
+
+namespace rtg {
+namespace {
+
+constexpr int kKeys = 64;      // of a stage in LDS
+constexpr float kSlack = 8.f;  // powers of two that a score may pass the running maximum by
+
+struct Args {
+  QRows q, k, v, out;  // k, v: packed prompts only
+  FStore c;            // the cache, else
+  const int* len;
+  const int* counts;
+  const int* offsets;
+  int n_rows, n_seq, n_head, n_q, n_q_head, group, hd;
+  float query, sum;  // ScoreScale
+  float* stats;
+  bool qvec, kvec, ovec;
+};
+
+// What a workgroup works on: rows [first, first + 128) of the (query, head) pairs
+// of a sequence and key/value head.
+struct Job {
+  int seq, head, tile;
+  int len, count;  // keys, queries
+  int base;        // packed: the sequence's first row
+};
+__device__ __forceinline__ int seen(const Job& j, int i) { return keys_seen(j.len, j.count, i); }
+
+struct Bf16 {
+  typedef __bf16 V2 __attribute__((ext_vector_type(2)));
+  static constexpr float kUp = 0.f;  // probabilities are taken 2^kUp times as large
+  static __device__ __forceinline__ f32x16 mfma(const u4v& a, const u4v& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned two(float x, float y) {
+    const V2 v = {(__bf16)x, (__bf16)y};
+    return __builtin_bit_cast(unsigned, v);
+  }
+  static __device__ __forceinline__ float add2(unsigned x, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(V2, x), __builtin_bit_cast(V2, 0x3F803F80u), c, false);
+  }
+};
+struct F16 {
+  typedef _Float16 V2 __attribute__((ext_vector_type(2)));
+  static constexpr float kUp = 6.f;
+  static __device__ __forceinline__ f32x16 mfma(const u4v& a, const u4v& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned two(float x, float y) {
+    const V2 v = {(_Float16)x, (_Float16)y};
+    return __builtin_bit_cast(unsigned, v);
+  }
+  static __device__ __forceinline__ float add2(unsigned x, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(V2, x), __builtin_bit_cast(V2, 0x3C003C00u), c, false);
+  }
+};
+
+// Eight f32 as N parts of M's type.
+template <class M, int N>
+__device__ __forceinline__ void parts_of(const float (&x)[8], u4v (&p)[N]) {
+  if constexpr (std::is_same_v<M, F16>) {
+    static_assert(N == 1, "f16 rows are one part");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[0][i] = M::two(x[2 * i], x[2 * i + 1]);
+  } else {
+    bf16_parts<N>(x, p);
+  }
+}
+
+// Keys and values of a stage in LDS: rows of HD, 16-byte chunks xor'ed so that the
+// reads below fall on all banks. A matrix operand of keys takes the same chunk of
+// 32 rows; one of values takes four rows of 64 bytes and four rows 4 further on.
+template <int HD, int KP>
+struct Shared {
+  static constexpr int CH = HD / 8;  // chunks of a row
+  static __device__ __forceinline__ int k_at(int key, int chunk) {
+    return key * CH + (chunk ^ (HD == 128 ? key & 15 : (key >> 1) & 7));
+  }
+  static __device__ __forceinline__ int v_at(int key, int chunk) {
+    return key * CH + (chunk ^ (HD == 128 ? (key & 3) << 2 | ((key >> 2) & 3) : (key & 2) << 1 | ((key >> 2) & 3)));
+  }
+  u4v k[KP][kKeys * CH], v[KP][kKeys * CH];
+  int bad[HD];  // the first key whose value in a channel is not finite (and was taken as 0)
+  int any_bad;
+};
+
+// Rows of device memory as a stage: a thread has every 32nd or 16th row's chunk.
+template <class M, int HD, int KP, class T>
+struct RowStage {
+  static constexpr int CH = HD / 8, N = kKeys * CH / 256;
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  T8 k[N], v[N];
+
+  static __device__ __forceinline__ void load1(const T* row, int c8, int n, bool vec, T8& x) {
+    if (vec) {
+      if (c8 < n) x = *reinterpret_cast<const T8*>(row + c8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c8 + e < n) x[e] = row[c8 + e];
+    }
+  }
+  __device__ __forceinline__ void load(const Args& a, const Job& j, int at, int live) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int unit = u * 256 + (int)threadIdx.x, key = at + unit / CH, c8 = unit % CH * 8;
+      k[u] = T8{};
+      v[u] = T8{};
+      if (key < live) {
+        const long row = j.base + key;
+        load1(static_cast<const T*>(a.k.p) + row * a.k.tok + j.head * a.k.head, c8, a.hd, a.kvec, k[u]);
+        load1(static_cast<const T*>(a.v.p) + row * a.v.tok + j.head * a.v.head, c8, a.hd, a.kvec, v[u]);
+      }
+    }
+  }
+  static __device__ __forceinline__ void parts(const T8& x, u4v (&p)[KP]) {
+    if constexpr (sizeof(T) == 2) {
+      p[0] = __builtin_bit_cast(u4v, x);
+    } else {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = x[e];
+      bf16_parts<KP>(f, p);
+    }
+  }
+  __device__ __forceinline__ void store(Shared<HD, KP>& s, int at, int, bool edge) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int unit = u * 256 + (int)threadIdx.x, key = unit / CH, chunk = unit % CH;
+      if (edge) {
+        // (a value times a probability of 0 must be 0 for the rows that do not see it)
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) odd |= !__builtin_isfinite((float)v[u][e]);
+        if (odd) {
+          s.any_bad = 1;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (!__builtin_isfinite((float)v[u][e])) {
+              atomicMin(&s.bad[chunk * 8 + e], at + key);
+              v[u][e] = (T)0.f;
+            }
+        }
+      }
+      u4v p[KP];
+      parts(k[u], p);
+#pragma unroll
+      for (int i = 0; i < KP; ++i) s.k[i][Shared<HD, KP>::k_at(key, chunk)] = p[i];
+      parts(v[u], p);
+#pragma unroll
+      for (int i = 0; i < KP; ++i) s.v[i][Shared<HD, KP>::v_at(key, chunk)] = p[i];
+    }
+  }
+};
+
+// Two tiles of the 4-bit cache as a stage: a thread has HD / 8 bytes of codes of
+// one key, and of four values.
+template <int HD>
+struct CodeStage {
+  typedef unsigned W __attribute__((ext_vector_type(HD / 32)));
+  W k, v;
+  unsigned ks, vs;
+
+  __device__ __forceinline__ void load(const Args& a, const Job& j, int at, int) {
+    const int unit = (int)threadIdx.x & 127, lane = HD == 128 ? unit & 63 : unit >> 1, b = HD == 128 ? unit >> 6 : unit & 1;
+    // (a second tile behind the capacity is the first once more: no key of it is seen)
+    const int tile = min(at / kFTile + ((int)threadIdx.x >> 7), a.c.tiles - 1), g = lane >> 4, m = lane & 15;
+    const size_t sh = (size_t)j.seq * a.c.n_head + j.head, codes = a.c.codes(sh) + (size_t)tile * 16 * HD + unit * (HD / 8);
+    const size_t scales = a.c.scales(sh) + (size_t)tile * HD;
+    k = *reinterpret_cast<const W*>(a.c.k + codes);
+    v = *reinterpret_cast<const W*>(a.c.v + codes);
+    ks = a.c.sk[scales + b * (HD / 2) + (HD == 128 ? lane : (g >> 1) * 16 + m)];
+    vs = *reinterpret_cast<const unsigned*>(a.c.sv + scales + (g * (HD / 32) + m * (HD / 16) / 32) * 8 + b * 4);
+  }
+  __device__ __forceinline__ void store(Shared<HD, 1>& s, int at, int live, bool edge) {
+    const int unit = (int)threadIdx.x & 127, lane = HD == 128 ? unit & 63 : unit >> 1, b = HD == 128 ? unit >> 6 : unit & 1;
+    const int g = lane >> 4, m = lane & 15, first = ((int)threadIdx.x >> 7) * kFTile + b * 16;
+    const float kscale = scale_of(ks);
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i)
+      s.k[0][Shared<HD, 1>::k_at(first + m, g * (HD / 32) + i)] = eight_bf16(k[i], kscale);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = first + 4 * g + i;
+      unsigned byte = (vs >> (8 * i)) & 255u;
+      if (edge && at + key >= live) byte = 0;  // (what lies there is anything)
+      if (byte == 255u) {
+        s.any_bad = 1;
+        for (int e = 0; e < HD / 16; ++e) atomicMin(&s.bad[m * (HD / 16) + e], at + key);
+        byte = 0;
+      }
+      if constexpr (HD == 128) {
+        s.v[0][Shared<HD, 1>::v_at(key, m)] = eight_bf16(v[i], scale_of(byte));
+      } else {
+        const unsigned w = v[i / 2];
+        uint2* to = reinterpret_cast<uint2*>(&s.v[0][Shared<HD, 1>::v_at(key, m >> 1)]) + (m & 1);
+        *to = i & 1 ? make_uint2(two_bf16<2>(w, scale_of(byte)), two_bf16<3>(w, scale_of(byte)))
+                    : make_uint2(two_bf16<0>(w, scale_of(byte)), two_bf16<1>(w, scale_of(byte)));
+      }
+    }
+  }
+};
+
+typedef short s4v __attribute__((ext_vector_type(4)));
+// Four values of 16 bits of one channel, of the rows whose chunks the 16 lanes point at.
+__device__ __forceinline__ uint2 read_tr(const void* p) {
+  typedef s4v __attribute__((address_space(3))) * Lds;
+  const s4v r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)(__attribute__((address_space(3))) const char*)p);
+  return __builtin_bit_cast(uint2, r);
+}
+
+template <class M, int HD, int QP, int KP, int PP, class T, class Stage>
+__device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD, KP>& s) {
+  constexpr int KS = HD / 16, DT = HD / 32;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int first = job.tile * 128, rows = job.count * a.group;
+  // this lane's row: query i of head h
+  const int row = first + wave * 32 + n, i = row / a.group, head = job.head * a.group + row % a.group;
+  const int lim = seen(job, i);
+  // keys that the workgroup's rows see: at most, and at least but for padding
+  const int live = rows > first ? seen(job, (min(first + 128, rows) - 1) / a.group) : 0, least = seen(job, first / a.group);
+  const long qrow = job.base + min(i, max(job.count - 1, 0));
+  u4v q[KS][QP];
+  {
+    const T* p = static_cast<const T*>(a.q.p) + job.seq * a.q.seq + qrow * a.q.tok + head * a.q.head;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      float x[8];
+      load8(p, k * 16 + half * 8, a.hd, a.qvec, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= a.query;
+      parts_of<M, QP>(x, q[k]);
+    }
+  }
+  f32x16 o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = f32x16{};
+  float m = -INFINITY, l = 0.f, l_whole = 0.f;  // l_whole: of unrounded probabilities, for the stats
+  for (int c = tid; c < HD; c += 256) s.bad[c] = INT32_MAX;
+  if (tid == 0) s.any_bad = 0;
+  Stage st;
+  if (live > 0) st.load(a, job, 0, live);
+  for (int at = 0; at < live; at += kKeys) {
+    const bool edge = at + kKeys > least;  // (uniform)
+    __syncthreads();
+    st.store(s, at, live, edge);
+    __syncthreads();
+    if (at + kKeys < live) st.load(a, job, at + kKeys, live);
+    float p[2][16];  // keys at + sub * 32 + e / 4 * 8 + half * 4 + e % 4
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      f32x16 x = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int kp = KP - 1; kp >= 0; --kp) {
+          const u4v f = s.k[kp][Shared<HD, KP>::k_at(sub * 32 + n, k * 2 + half)];
+#pragma unroll
+          for (int qp = QP - 1; qp >= 0; --qp)
+            if (kp + qp < 3) x = M::mfma(f, q[k][qp], x);
+        }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[sub][e] = x[e];
+    }
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (at + e / 16 * 32 + e % 16 / 4 * 8 + half * 4 + e % 4 >= lim) p[e / 16][e % 16] = -INFINITY;
+    }
+    float top = p[0][0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) top = fmaxf(top, p[e / 16][e % 16]);
+    if (__builtin_amdgcn_ballot_w64(top * a.sum > m + kSlack)) {
+      top = xor32_max_k(top) * a.sum;
+      // (each column by itself: its result does not depend on its neighbours')
+      const float f = top > m + kSlack ? __builtin_amdgcn_exp2f(m - top) : 1.f;
+      m = top > m + kSlack ? top : m;
+      l *= f;
+      l_whole *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+    }
+    const float base = (m == -INFINITY ? 0.f : m) - M::kUp;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) p[e / 16][e % 16] = __builtin_amdgcn_exp2f(fmaf(p[e / 16][e % 16], a.sum, -base));
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (at + e / 16 * 32 + e % 16 / 4 * 8 + half * 4 + e % 4 >= lim) p[e / 16][e % 16] = 0.f;
+    }
+    if (PP == 1 && a.stats) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) l_whole += p[e / 16][e % 16];
+    }
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        // keys sub * 32 + u * 16 + e / 4 * 8 + half * 4 + e % 4, e < 8
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = p[sub][u * 8 + e];
+        u4v pp[PP];
+        parts_of<M, PP>(x, pp);
+        if constexpr (PP == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) l = M::add2(pp[0][e], l);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) l += x[e];
+        }
+        const int key = sub * 32 + u * 16 + half * 4 + ((lane & 15) >> 2), chan = (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int kp = KP - 1; kp >= 0; --kp) {
+            u4v f;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const u4v* c = &s.v[kp][Shared<HD, KP>::v_at(key + 8 * r, d * 4 + chan / 8)];
+              const uint2 w = read_tr(reinterpret_cast<const char*>(c) + (chan & 7) * 2);
+              f[2 * r] = w.x;
+              f[2 * r + 1] = w.y;
+            }
+#pragma unroll
+            for (int k = PP - 1; k >= 0; --k)
+              if (kp + k < 3) o[d] = M::mfma(f, pp[k], o[d]);
+          }
+      }
+  }
+  if (row >= a.n_q * a.group) return;
+  l = xor32_sum_k(l);
+  const bool any = lim > 0;
+  const float inv = 1.f / l;
+  T* out = static_cast<T*>(a.out.p) + job.seq * a.out.seq + (job.base + (long)i) * a.out.tok + head * a.out.head;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int c4 = d * 32 + e / 4 * 8 + half * 4;
+      float x[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = any ? o[d][e + r] * inv : 0.f;
+      if (live > 0 && s.any_bad)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (s.bad[c4 + r] < lim) x[r] = NAN;
+      store4(out, c4, a.hd, make_float4(x[0], x[1], x[2], x[3]), a.ovec);
+    }
+  if (a.stats) {
+    if (PP == 1) l = xor32_sum_k(l_whole);
+    if (half == 0)
+      reinterpret_cast<float2*>(a.stats)[((size_t)job.seq * a.n_q + i) * a.n_q_head + head] = make_float2(m - M::kUp, any ? l : 0.f);
+  }
+}
+
+template <int HD, int QP, int PP, class T>
+__global__ __launch_bounds__(256) void f_attend_many_kernel(Args a) {
+  __shared__ Shared<HD, 1> s;
+  Job j;
+  j.seq = (int)blockIdx.x / a.n_head;
+  j.head = (int)blockIdx.x % a.n_head;
+  j.tile = (int)(gridDim.y - 1 - blockIdx.y);  // the longest first
+  j.len = a.len[j.seq];
+  j.count = a.counts ? min(max(a.counts[j.seq], 0), a.n_q) : a.n_q;
+  j.base = 0;
+  attend<Bf16, HD, QP, 1, PP, T, CodeStage<HD>>(a, j, s);
+}
+
+// The workgroups of a packed batch: tile number x / n_head of all sequences'
+// tiles, for head x % n_head; those behind the last tile clear the rows that no
+// sequence has. There is one at least: the sum of the sequences' tiles, rounded up
+// each, is less than the rows' tiles and the number of sequences.
+template <class M, int HD, int P, class T>
+__global__ __launch_bounds__(256) void packed_attend_kernel(Args a) {
+  __shared__ Shared<HD, P> s;
+  const int lane = threadIdx.x & 63;
+  int at = (int)blockIdx.x / a.n_head, end = 0;
+  const int index = at, head = (int)blockIdx.x % a.n_head;
+  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+    const int seq = s0 + lane;
+    int lo = 0, hi = 0;
+    if (seq < a.n_seq) {
+      lo = min(max(a.offsets[seq], 0), a.n_rows);
+      hi = min(max(a.offsets[seq + 1], lo), a.n_rows);
+    }
+    const int tiles = ((hi - lo) * a.group + 127) / 128;
+    int incl = tiles;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += u;
+    }
+    const unsigned long long mine = __builtin_amdgcn_ballot_w64(at >= incl - tiles && at < incl);
+    if (mine) {
+      const int l = __builtin_ctzll(mine);
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+      Job j;
+      j.seq = 0;  // (packed rows have no stride of sequences)
+      j.head = head;
+      j.base = of(lo);
+      j.len = j.count = of(hi) - j.base;
+      j.tile = of(incl) - 1 - at;  // the longest first
+      a.n_q = j.count;
+      attend<M, HD, P, P, P, T, RowStage<M, HD, P, T>>(a, j, s);
+      return;
+    }
+    at -= __builtin_amdgcn_readlane(incl, 63);
+    end = max(end, __builtin_amdgcn_readlane(hi, min(a.n_seq - 1 - s0, 63)));
+  }
+  // `at` workgroups of this head are before this one among those that are left
+  const int start = min(max(a.offsets[0], 0), a.n_rows), spare = start + a.n_rows - end;
+  const int step = (int)(gridDim.x / a.n_head) - (index - at), per = a.group * a.hd;
+  for (int r = at; r < spare; r += step) {
+    const long row = r < start ? r : end + (r - start);
+    for (int c = threadIdx.x; c < per; c += 256)
+      static_cast<T*>(a.out.p)[row * a.out.tok + (long)(head * a.group + c / a.hd) * a.out.head + c % a.hd] = (T)0.f;
+  }
+}
+
+template <int QP, int PP, class T>
+void many_t(hipStream_t s, const Args& a) {
+  const dim3 grid((unsigned)(a.n_seq * a.n_head), (unsigned)((a.n_q * a.group + 127) / 128));
+  if (a.c.hdp == 64) f_attend_many_kernel<64, QP, PP, T><<<grid, 256, 0, s>>>(a);
+  else f_attend_many_kernel<128, QP, PP, T><<<grid, 256, 0, s>>>(a);
+}
+template <class M, int P, class T>
+void packed_t(hipStream_t s, const Args& a) {
+  const unsigned tiles = (unsigned)((a.n_rows * (long)a.group + 127) / 128 + a.n_seq), grid = tiles * (unsigned)a.n_head;
+  if (a.hd <= 64) packed_attend_kernel<M, 64, P, T><<<grid, 256, 0, s>>>(a);
+  else packed_attend_kernel<M, 128, P, T><<<grid, 256, 0, s>>>(a);
+}
+
+}  // namespace
+
+void launch_f_attend_many(hipStream_t s, const FAttn& f) {
+  Args a = {};
+  a.q = f.q;
+  a.out = f.out;
+  a.c = f.c;
+  a.len = f.len;
+  a.counts = f.counts;
+  a.n_seq = f.c.n_seq;
+  a.n_head = f.c.n_head;
+  a.n_q = f.n_q;
+  a.n_q_head = f.n_q_head;
+  a.group = f.n_q_head / f.c.n_head;
+  a.hd = f.c.hd;
+  const ScoreScale sc = score_scale(f.scale);
+  a.query = sc.query;
+  a.sum = sc.sum;
+  a.stats = f.stats;
+  a.qvec = by_eights(f.q, a.hd, f.type);
+  a.ovec = by_eights(f.out, a.hd, f.type);
+  if (f.type == Q_F32) many_t<3, 3, float>(s, a);
+  else if (f.type == Q_BF16) many_t<1, 1, __bf16>(s, a);
+  else many_t<2, 2, _Float16>(s, a);
+}
+
+void launch_packed_attend(hipStream_t s, const PAttn& p) {
+  Args a = {};
+  a.q = p.q;
+  a.k = p.k;
+  a.v = p.v;
+  a.out = p.out;
+  a.offsets = p.offsets;
+  a.n_rows = p.n_rows;
+  a.n_seq = p.n_seq;
+  a.n_head = p.n_head;
+  a.n_q_head = p.n_q_head;
+  a.group = p.n_q_head / p.n_head;
+  a.hd = p.hd;
+  ScoreScale sc = score_scale(p.scale);
+  if (p.type == Q_F16) {
+    // (f16 does not hold the queries times any power of two)
+    sc.sum = (float)std::min(std::max(fabs((double)p.scale) * 1.4426950408889634074, 1.2e-38), 3.4e38);
+    sc.query = p.scale == 0.f ? 0.f : copysignf(1.f, p.scale);
+  }
+  a.query = sc.query;
+  a.sum = sc.sum;
+  a.qvec = by_eights(p.q, a.hd, p.type);
+  a.kvec = by_eights(p.k, a.hd, p.type) && by_eights(p.v, a.hd, p.type);
+  a.ovec = by_eights(p.out, a.hd, p.type);
+  if (p.type == Q_F32) packed_t<Bf16, 3, float>(s, a);
+  else if (p.type == Q_BF16) packed_t<Bf16, 1, __bf16>(s, a);
+  else packed_t<F16, 1, _Float16>(s, a);
+}
+
+}  // namespace rtg

@@ -1,0 +1,511 @@
+// Attention over the 4-bit cache (fourbit.h) for few queries, and the weights
+// that queries give the cache's tokens.
+//
+// A wave holds 16 columns, a column being a (query, head) pair that reads one
+// key/value head, and takes 32 tokens at a time:
+//   scores  S[token][column] = K Q^T on v_mfma_f32_16x16x32_bf16. A lane's 16
+//           bytes of codes are its matrix operands, four codes of channels to a
+//           conversion with the scale in it. bf16 holds every number of the cache
+//           exactly, and a query is the sum of as many bf16 parts as its type has
+//           bits for (f32 three, f16 two), so that products are exact and sums f32;
+//   output  O[channel][column] = V^T P^T. Scores are computed transposed: the
+//           lanes of a column hold 8 of the 32 tokens each, in the order in which
+//           the values' codes lie, so that a lane's probabilities are its matrix
+//           operand. They are taken as two bf16 parts (16 bits) where results are
+//           bf16 or f16, as three (24) where they are f32.
+// The softmax's running maximum is only raised where a score passes it by 2^8: sums
+// stay far within f32, and most tiles need no exchange between lanes.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_core.h"
+#include "fourbit_core.h"
+
+namespace rtg {
+namespace {
+
+constexpr int kCols = 16, kWaves = 4;
+constexpr int kMostSplit = 1024;  // workgroups at most where the keys are split
+constexpr float kSlack = 8.f;     // powers of two that a score may pass the maximum by
+
+struct Args {
+  FStore c;
+  const int* len;
+  QRows q, out;
+  int n_q, n_q_head, group, cblocks;
+  const int* counts;
+  float query, sum;  // ScoreScale
+  float* stats;
+  bool qvec, ovec;
+  int min_tiles;      // of a split
+  unsigned* tickets;  // [sh][cblock][kQTicketStride]
+  float* parts;       // [sh][cblock][split][column][hdp + 2]
+};
+
+struct Column {
+  int i, h;  // query, head within the group; i >= n_q: none
+};
+__device__ __forceinline__ Column column(const Args& a, int col) {
+  Column r;
+  r.i = a.group == 1 ? col : col / a.group;
+  r.h = col - r.i * a.group;
+  return r;
+}
+template <class T>
+__device__ __forceinline__ T* row_of(const QRows& r, int seq, int i, int head) {
+  return static_cast<T*>(r.p) + seq * r.seq + i * r.tok + head * r.head;
+}
+
+__device__ __forceinline__ float2& stats_of(const Args& a, int seq, int i, int head) {
+  return reinterpret_cast<float2*>(a.stats)[((size_t)seq * a.n_q + i) * a.n_q_head + head];
+}
+
+// A column's query as matrix operands, this lane's quarter: channels CK g + 8 j + e.
+template <int HDP, int QP, class T>
+struct Query {
+  static constexpr int J = HDP / 32;
+  u4v q[J][QP];
+  __device__ __forceinline__ void load(const Args& a, int seq, int head, const Column& cl, int g) {
+    const T* row = row_of<const T>(a.q, seq, min(cl.i, a.n_q - 1), head * a.group + cl.h);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      float x[8];
+      load8(row, HDP / 4 * g + 8 * j, a.c.hd, a.qvec, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= a.query;
+      bf16_parts<QP>(x, q[j]);
+    }
+  }
+};
+
+// A tile's keys as they lie: this lane's quarter of tokens m and 16 + m.
+template <int HDP>
+struct Keys {
+  static constexpr int J = HDP / 32;
+  u4v c[HDP / 64];
+  unsigned s[2];
+  __device__ __forceinline__ void load(const uint8_t* k, const uint8_t* sk, int lane) {
+#pragma unroll
+    for (int i = 0; i < HDP / 64; ++i) c[i] = *reinterpret_cast<const u4v*>(k + i * 1024 + lane * 16);
+    const int at = HDP == 128 ? lane : (lane >> 5) * 16 + (lane & 15);
+    s[0] = sk[at];
+    s[1] = sk[HDP / 2 + at];
+  }
+  // scores of tokens b * 16 + 4 g + i
+  template <int QP>
+  __device__ __forceinline__ f32x4 scores(int b, const u4v (&q)[J][QP]) const {
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+    const float scale = scale_of(s[b]);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const unsigned w = HDP == 128 ? c[HDP == 128 ? b : 0][j] : c[0][b * 2 + (j & 1)];
+      const u4v k = eight_bf16(w, scale);
+#pragma unroll
+      for (int p = 0; p < QP; ++p) r = mfma16(k, q[j][p], r);
+    }
+    return r;
+  }
+};
+
+// A tile's values as they lie: this lane's CV channels of tokens b * 16 + 4 g + i,
+// and their scales (byte b * 4 + i).
+template <int HDP>
+struct Values {
+  static constexpr int CV = HDP / 16;
+  u4v c[HDP / 64];
+  unsigned s[2];
+  __device__ __forceinline__ void load(const uint8_t* v, const uint8_t* sv, int lane) {
+#pragma unroll
+    for (int i = 0; i < HDP / 64; ++i) c[i] = *reinterpret_cast<const u4v*>(v + i * 1024 + lane * 16);
+    const int g = lane >> 4, group = (lane & 15) * CV / 32;
+    const uint2 x = *reinterpret_cast<const uint2*>(sv + (g * (HDP / 32) + group) * 8);
+    s[0] = x.x;
+    s[1] = x.y;
+  }
+  // o[d] += the products of channel CV m + d with the columns' probabilities
+  template <int PP>
+  __device__ __forceinline__ void add(const u4v (&p)[PP], f32x4 (&o)[CV]) const {
+    float scale[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) scale[r] = scale_of((s[r / 4] >> (r % 4 * 8)) & 255u);
+    auto pairs = [&](auto pair) {  // channels CV m + 2 pair, + 1
+      constexpr int PR = decltype(pair)::value;
+      unsigned t[8];
+      if constexpr (HDP == 128) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) t[r] = two_bf16<PR>(c[r / 4][r % 4], scale[r]);
+      } else {  // two tokens to a word
+#pragma unroll
+        for (int r = 0; r < 8; r += 2) {
+          t[r] = two_bf16<PR>(c[0][r / 2], scale[r]);
+          t[r + 1] = two_bf16<PR + 2>(c[0][r / 2], scale[r + 1]);
+        }
+      }
+      u4v lo, hi;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[i] = low_halves(t[2 * i], t[2 * i + 1]);
+        hi[i] = high_halves(t[2 * i], t[2 * i + 1]);
+      }
+#pragma unroll
+      for (int k = 0; k < PP; ++k) {
+        o[2 * PR] = mfma16(lo, p[k], o[2 * PR]);
+        o[2 * PR + 1] = mfma16(hi, p[k], o[2 * PR + 1]);
+      }
+    };
+    pairs(std::integral_constant<int, 0>{});
+    pairs(std::integral_constant<int, 1>{});
+    if constexpr (HDP == 128) {
+      pairs(std::integral_constant<int, 2>{});
+      pairs(std::integral_constant<int, 3>{});
+    }
+  }
+  // Whether a value of this lane's reads back as NaN (or lies behind the sequence).
+  __device__ __forceinline__ bool any_nan() const {
+    const unsigned a = ~s[0], b = ~s[1];  // a byte of 0 in one of them
+    return (((a - 0x01010101u) & ~a) | ((b - 0x01010101u) & ~b)) & 0x80808080u;
+  }
+  // Makes the scales of tokens from `live` on, which hold anything, and of values
+  // that read back as NaN 0; the first of these tokens goes to *bad if it is lower.
+  __device__ __forceinline__ void clean(int first, int live, int g, int* bad) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const unsigned byte = (s[r / 4] >> (r % 4 * 8)) & 255u;
+      const int t = first + r / 4 * 16 + 4 * g + r % 4;
+      if (t < live && byte == 255u) *bad = min(*bad, t);
+      if (t >= live || byte == 255u) s[r / 4] &= ~(255u << (r % 4 * 8));
+    }
+  }
+};
+
+struct Seq {
+  int len, count;
+};
+__device__ __forceinline__ Seq seq_of(const Args& a, int seq) {
+  Seq r;
+  r.len = a.len[seq];
+  r.count = a.counts ? min(max(a.counts[seq], 0), a.n_q) : a.n_q;
+  return r;
+}
+
+// Two neighbouring floats of a partial, past the L2 caches (workgroups of other
+// XCDs read them).
+__device__ __forceinline__ void store2(float* p, float x, float y) {
+  const unsigned long long v = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load2(const float* p) {
+  const unsigned long long v = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32)));
+}
+
+template <int HDP>
+struct Shared {
+  float m[kWaves][kCols], l[kWaves][kCols];
+  __attribute__((aligned(16))) float o[kWaves][kCols][HDP + 4];
+  int last;
+};
+
+// Joins the waves' results in s for the columns of block cb: to the results where
+// the keys were not split, else to the partials; the last of the n workgroups of a
+// block to come here joins those.
+template <int HDP, class T>
+__device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq& r, int seq, int head, int sh, int cb,
+                                       int z, int n) {
+  constexpr int C4 = HDP / 4, STEP = 256 / C4;
+  const int tid = threadIdx.x, c4 = tid % C4 * 4;
+  const int cols = min(kCols, a.n_q * a.group - cb * kCols);
+  auto put = [&](int col, float m, float l, const float4& x) {
+    const Column cl = column(a, cb * kCols + col);
+    const bool any = keys_seen(r.len, r.count, cl.i) > 0;
+    const float inv = 1.f / l;
+    store4(row_of<T>(a.out, seq, cl.i, head * a.group + cl.h), c4, a.c.hd,
+           any ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f), a.ovec);
+    if (a.stats && c4 == 0) stats_of(a, seq, cl.i, head * a.group + cl.h) = make_float2(m, any ? l : 0.f);
+  };
+  __syncthreads();
+  for (int col = tid / C4; col < cols; col += STEP) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s.m[w][col]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(s.m[w][col] - base);
+      const float4 y = *reinterpret_cast<const float4*>(&s.o[w][col][c4]);
+      l = fmaf(f, s.l[w][col], l);
+      x = make_float4(fmaf(f, y.x, x.x), fmaf(f, y.y, x.y), fmaf(f, y.z, x.z), fmaf(f, y.w, x.w));
+    }
+    if (n == 1) {
+      put(col, m, l, x);
+    } else {
+      float* p = a.parts + ((((size_t)sh * a.cblocks + cb) * gridDim.z + z) * kCols + col) * (HDP + 2);
+      if (c4 == 0) store2(p, m, l);
+      store2(p + 2 + c4, x.x, x.y);
+      store2(p + 4 + c4, x.z, x.w);
+    }
+  }
+  if (n == 1) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores have completed
+  __syncthreads();
+  if (tid == 0) {
+    unsigned* count = a.tickets + ((size_t)sh * a.cblocks + cb) * kQTicketStride;
+    s.last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)n - 1;
+    if (s.last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!s.last) return;
+  for (int col = tid / C4; col < cols; col += STEP) {
+    const float* p0 = a.parts + ((((size_t)sh * a.cblocks + cb) * gridDim.z) * kCols + col) * (HDP + 2);
+    float m = -INFINITY, l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int U = 8;  // (their way through memory takes over a microsecond: U at a time)
+    for (int z0 = 0; z0 < n; z0 += U) {
+      float2 ml[U], y[U][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float* p = p0 + (size_t)min(z0 + u, n - 1) * kCols * (HDP + 2);
+        ml[u] = load2(p);
+        y[u][0] = load2(p + 2 + c4);
+        y[u][1] = load2(p + 4 + c4);
+      }
+      float most = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) most = fmaxf(most, ml[u].x);
+      const float base = most == -INFINITY ? 0.f : most, corr = __builtin_amdgcn_exp2f(m - base);
+      m = most;
+      l *= corr;
+      x = make_float4(x.x * corr, x.y * corr, x.z * corr, x.w * corr);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (z0 + u >= n) break;
+        const float f = __builtin_amdgcn_exp2f(ml[u].x - base);
+        l = fmaf(f, ml[u].y, l);
+        x = make_float4(fmaf(f, y[u][0].x, x.x), fmaf(f, y[u][0].y, x.y), fmaf(f, y[u][1].x, x.z), fmaf(f, y[u][1].y, x.w));
+      }
+    }
+    put(col, m, l, x);
+  }
+}
+
+template <int HDP, int QP, int PP, class T>
+__global__ __launch_bounds__(256) void f_attend_kernel(Args a) {
+  constexpr int CV = HDP / 16;
+  __shared__ Shared<HDP> s;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head, cb = blockIdx.y, z = blockIdx.z;
+  const Seq r = seq_of(a, seq);
+  // keys that the block's columns see: at most, at least (columns that are none may see anything)
+  const int last_i = min(column(a, cb * kCols + kCols - 1).i, r.count - 1);
+  const int live = last_i >= 0 ? keys_seen(r.len, r.count, last_i) : 0;
+  const int least = keys_seen(r.len, r.count, column(a, cb * kCols).i);
+  const int tiles = (live + kFTile - 1) / kFTile;
+  const int splits = max(min((tiles + a.min_tiles - 1) / a.min_tiles, (int)gridDim.z), 1);
+  if (z >= splits) return;
+  const int per = (tiles + splits - 1) / splits, t0 = z * per, t1 = min(t0 + per, tiles);
+  const Column cl = column(a, cb * kCols + n);
+  const int lim = keys_seen(r.len, r.count, cl.i);
+  Query<HDP, QP, T> q;
+  q.load(a, seq, head, cl, g);
+  f32x4 o[CV];
+#pragma unroll
+  for (int d = 0; d < CV; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  int bad = INT32_MAX;  // the first token whose values of this lane's group of channels are NaN
+  const uint8_t *kc = a.c.k + a.c.codes(sh), *vc = a.c.v + a.c.codes(sh);
+  const uint8_t *ks = a.c.sk + a.c.scales(sh), *vs = a.c.sv + a.c.scales(sh);
+  Keys<HDP> k;
+  Values<HDP> v;
+  auto fetch = [&](int t) {
+    k.load(kc + (size_t)t * 16 * HDP, ks + (size_t)t * HDP, lane);
+    v.load(vc + (size_t)t * 16 * HDP, vs + (size_t)t * HDP, lane);
+  };
+  int t = t0 + wave;
+  if (t < t1) fetch(t);
+  while (t < t1) {
+    const Keys<HDP> k1 = k;
+    Values<HDP> v1 = v;
+    const int at = t * kFTile;
+    t += kWaves;
+    if (t < t1) fetch(t);
+    float p[8];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const f32x4 x = k1.scores(b, q.q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[b * 4 + i] = x[i];
+    }
+    const bool edge = at + kFTile > least;  // (uniform)
+    if (edge || __builtin_amdgcn_ballot_w64(v1.any_nan())) v1.clean(at, live, g, &bad);
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (at + e / 4 * 16 + 4 * g + e % 4 >= lim) p[e] = -INFINITY;
+    }
+    float top = p[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top = fmaxf(top, p[e]);
+    if (__builtin_amdgcn_ballot_w64(top * a.sum > m + kSlack)) {
+      top = xor32_max_k(xor16_max_k(top)) * a.sum;
+      // (each column by itself: its result does not depend on its neighbours')
+      const float f = top > m + kSlack ? __builtin_amdgcn_exp2f(m - top) : 1.f;
+      m = top > m + kSlack ? top : m;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < CV; ++d) o[d] *= f;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], a.sum, -base));
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = at + e / 4 * 16 + 4 * g + e % 4 < lim ? p[e] : 0.f;
+    }
+    u4v pp[PP];
+    bf16_parts<PP>(p, pp);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) l += p[e];
+    v1.add(pp, o);
+  }
+  l = xor32_sum_k(xor16_sum_k(l));
+  if (__builtin_amdgcn_ballot_w64(bad != INT32_MAX)) {
+    // lane (g, m) has looked at the group of m's channels; its results are of the group of channels CV 4 g
+    for (int x = 1; x < 64; x *= 2)
+      if (x >= 16 || x < 32 / CV) bad = min(bad, __shfl_xor(bad, x, 64));
+    bad = __shfl(bad, CV * 4 * g / 32 * (32 / CV), 64);
+#pragma unroll
+    for (int d = 0; d < CV; ++d)
+      if (bad < lim) o[d] = f32x4{NAN, NAN, NAN, NAN};
+  }
+  if (g == 0) {
+    s.m[wave][n] = m;
+    s.l[wave][n] = l;
+  }
+  // o[d][e]: channel CV (4 g + e) + d of column n
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+#pragma unroll
+    for (int d = 0; d < CV; d += 4)
+      *reinterpret_cast<float4*>(&s.o[wave][n][CV * (4 * g + e) + d]) = make_float4(o[d][e], o[d + 1][e], o[d + 2][e], o[d + 3][e]);
+  finish<HDP, T>(a, s, r, seq, head, sh, cb, z, splits);
+}
+
+// ---- weights ----
+
+// A wave takes a tile of 32 tokens and goes over the blocks of 16 columns: the
+// scores once more, and the sum of their exponentials over the columns' sums. Nothing but the keys is read, and each token's
+// weight has one owner: no atomics, and sums in a fixed order.
+template <int HDP, int QP, class T>
+__global__ __launch_bounds__(256) void f_weigh_kernel(Args a, float decay) {
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int tile = (int)blockIdx.y * kWaves + (int)(threadIdx.x >> 6);
+  const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head;
+  const Seq r = seq_of(a, seq);
+  const int at = tile * kFTile;
+  if (at >= r.len) return;
+  Keys<HDP> k;
+  k.load(a.c.k + a.c.codes(sh) + (size_t)tile * 16 * HDP, a.c.sk + a.c.scales(sh) + (size_t)tile * HDP, lane);
+  float sum[8] = {};
+  const int cblocks = (r.count * a.group + kCols - 1) / kCols;
+  for (int cb = 0; cb < cblocks; ++cb) {
+    const Column cl = column(a, cb * kCols + n);
+    const int lim = keys_seen(r.len, r.count, cl.i);
+    Query<HDP, QP, T> q;
+    q.load(a, seq, head, cl, g);
+    const float2 st = stats_of(a, seq, min(cl.i, a.n_q - 1), head * a.group + cl.h);
+    const float inv = 1.f / st.y;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const f32x4 x = k.scores(b, q.q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(x[i], a.sum, -st.x)) * inv;
+        sum[b * 4 + i] += at + b * 16 + 4 * g + i < lim ? p : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[e] = row16_sum_k(sum[e]);
+  // lane n of the 16 that hold the sums writes one of the eight
+  float mine = sum[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) mine = (n & 7) == e ? sum[e] : mine;
+  const int t = at + (n & 7) / 4 * 16 + 4 * g + (n & 3);
+  if (n < 8 && t < r.len) {
+    float* w = a.c.w + a.c.weights(sh) + t;
+    *w = decay == 0.f ? mine : fmaf(decay, *w, mine);
+  }
+}
+
+Args args_of(const FAttn& f) {
+  Args a;
+  a.c = f.c;
+  a.len = f.len;
+  a.q = f.q;
+  a.out = f.out;
+  a.n_q = f.n_q;
+  a.n_q_head = f.n_q_head;
+  a.group = f.n_q_head / f.c.n_head;
+  a.cblocks = (f.n_q * a.group + kCols - 1) / kCols;
+  a.counts = f.counts;
+  const ScoreScale sc = score_scale(f.scale);
+  a.query = sc.query;
+  a.sum = sc.sum;
+  a.stats = f.stats;
+  a.qvec = by_eights(f.q, f.c.hd, f.type);
+  a.ovec = by_eights(f.out, f.c.hd, f.type);
+  a.min_tiles = 1;
+  a.tickets = static_cast<unsigned*>(f.work);
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(f.work) + (size_t)kMostSplit * kQTicketStride * 4);
+  return a;
+}
+
+template <int QP, int PP, class T>
+void attend_t(hipStream_t s, const FAttn& f) {
+  Args a = args_of(f);
+  // Keys are split over workgroups where there are too few blocks of columns to
+  // fill the device; a split has at least 8 tiles.
+  const long blocks = (long)f.c.n_seq * f.c.n_head * a.cblocks;
+  a.min_tiles = 8;
+  const long z = std::max(1l, std::min(kMostSplit / std::max(blocks, 1l), (long)(f.c.tiles + a.min_tiles - 1) / a.min_tiles));
+  const dim3 grid((unsigned)(f.c.n_seq * f.c.n_head), (unsigned)a.cblocks, (unsigned)z);
+  if (f.c.hdp == 64) f_attend_kernel<64, QP, PP, T><<<grid, 256, 0, s>>>(a);
+  else f_attend_kernel<128, QP, PP, T><<<grid, 256, 0, s>>>(a);
+}
+template <int QP, class T>
+void weigh_t(hipStream_t s, const FAttn& f, float decay) {
+  const Args a = args_of(f);
+  const dim3 grid((unsigned)(f.c.n_seq * f.c.n_head), (unsigned)((f.c.tiles + kWaves - 1) / kWaves));
+  if (f.c.hdp == 64) f_weigh_kernel<64, QP, T><<<grid, 256, 0, s>>>(a, decay);
+  else f_weigh_kernel<128, QP, T><<<grid, 256, 0, s>>>(a, decay);
+}
+
+}  // namespace
+
+size_t fattn_work_bytes(int hdp) {
+  return (size_t)kMostSplit * (kQTicketStride * 4 + (size_t)kCols * (hdp + 2) * 4);
+}
+void fattn_work_clear(hipStream_t s, void* work, int) {
+  (void)hipMemsetAsync(work, 0, (size_t)kMostSplit * kQTicketStride * 4, s);
+}
+
+void launch_f_attend(hipStream_t s, const FAttn& f) {
+  if (f.n_q * (f.n_q_head / f.c.n_head) > 128) return launch_f_attend_many(s, f);
+  if (f.type == Q_F32) attend_t<3, 3, float>(s, f);
+  else if (f.type == Q_BF16) attend_t<1, 2, __bf16>(s, f);
+  else attend_t<2, 2, _Float16>(s, f);
+}
+void launch_f_weigh(hipStream_t s, const FAttn& f, float decay) {
+  if (f.type == Q_F32) weigh_t<3, float>(s, f, decay);
+  else if (f.type == Q_BF16) weigh_t<1, __bf16>(s, f, decay);
+  else weigh_t<2, _Float16>(s, f, decay);
+}
+
+}  // namespace rtg
