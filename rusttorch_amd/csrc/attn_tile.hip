@@ -24,10 +24,12 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_core.h"
 #include "f16_pair.h"
 #include "fourbit_core.h"
+#include "lds_direct.h"
 
 namespace rtg {
 namespace {
@@ -69,6 +71,7 @@ struct Bf16 {
   static __device__ __forceinline__ float add2(unsigned x, float c) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(V2, x), __builtin_bit_cast(V2, 0x3F803F80u), c, false);
   }
+  static constexpr unsigned kExponents = 0x7F807F80u, kLowest = 0x00800080u;
 };
 struct F16 {
   typedef _Float16 V2 __attribute__((ext_vector_type(2)));
@@ -83,6 +86,7 @@ struct F16 {
   static __device__ __forceinline__ float add2(unsigned x, float c) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(V2, x), __builtin_bit_cast(V2, 0x3C003C00u), c, false);
   }
+  static constexpr unsigned kExponents = 0x7C007C00u, kLowest = 0x04000400u;
 };
 
 // Eight f32 as N parts of M's type.
@@ -101,26 +105,133 @@ __device__ __forceinline__ void parts_of(const float (&x)[8], u4v (&p)[N]) {
 // reads below fall on all banks. A matrix operand of keys takes the same chunk of
 // 32 rows; one of values takes four rows of 64 bytes and four rows 4 further on.
 template <int HD, int KP>
-struct Shared {
+struct Buffer {
   static constexpr int CH = HD / 8;  // chunks of a row
-  static __device__ __forceinline__ int k_at(int key, int chunk) {
-    return key * CH + (chunk ^ (HD == 128 ? key & 15 : (key >> 1) & 7));
+  static __device__ __forceinline__ int k_swizzle(int key) { return HD == 128 ? key & 15 : (key >> 1) & 7; }
+  static __device__ __forceinline__ int v_swizzle(int key) {
+    return HD == 128 ? (key & 3) << 2 | ((key >> 2) & 3) : (key & 2) << 1 | ((key >> 2) & 3);
   }
-  static __device__ __forceinline__ int v_at(int key, int chunk) {
-    return key * CH + (chunk ^ (HD == 128 ? (key & 3) << 2 | ((key >> 2) & 3) : (key & 2) << 1 | ((key >> 2) & 3)));
-  }
+  static __device__ __forceinline__ int k_at(int key, int chunk) { return key * CH + (chunk ^ k_swizzle(key)); }
+  static __device__ __forceinline__ int v_at(int key, int chunk) { return key * CH + (chunk ^ v_swizzle(key)); }
   u4v k[KP][kKeys * CH], v[KP][kKeys * CH];
-  int bad[HD];  // the first key whose value in a channel is not finite (and was taken as 0)
-  int any_bad;
+};
+// The first key whose value in a channel is not finite (and was taken as 0).
+template <int HD>
+struct Bad {
+  int key[HD];
+  int any;
+};
+template <int HD, int KP, int NB>
+struct Shared {
+  Buffer<HD, KP> b[NB];
+  Bad<HD> bad;
 };
 
-// Rows of device memory as a stage: a thread has every 32nd or 16th row's chunk.
-template <class M, int HD, int KP, class T>
+// Whether one of the 16-bit numbers of x is not finite: its exponent's carry.
+template <class M>
+__device__ __forceinline__ bool any_odd(const u4v& x) {
+  unsigned r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r |= (x[i] & M::kExponents) + M::kLowest;
+  return r & 0x80008000u;
+}
+// The numbers of a chunk of values (of key `key`) that are not finite become 0,
+// and are remembered: a value times a probability of 0 has to be 0 for the rows
+// that do not see it.
+template <class M, int HD>
+__device__ __forceinline__ void clean(u4v& x, Bad<HD>& bad, int channel, int key) {
+  bad.any = 1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned half = 0xFFFFu << (16 * h);
+      if ((((x[i] & M::kExponents) + M::kLowest) & 0x80008000u & half) == 0) continue;
+      atomicMin(&bad.key[channel + 2 * i + h], key);
+      x[i] &= ~half;
+    }
+}
+
+// Rows of 16 bits, aligned, straight to LDS: a wave's load is 1 KB of LDS, each
+// lane picking the chunk that belongs there.
+template <class M, int HD>
+struct DirectStage {
+  static constexpr int KP = 1, NB = 2, CH = HD / 8, N = kKeys * CH / 256;
+  static constexpr bool kDirect = true;
+  typedef Buffer<HD, 1> Buf;
+  const char *k, *v;
+  unsigned kv[N], vv[N];  // this lane's bytes of unit u, keys and values
+  unsigned kstep, vstep;  // bytes of a stage
+  int key[N], wave;
+  bool in[N];  // whether the chunk belongs to the row (of keys', values')
+  bool vin[N];
+
+  __device__ __forceinline__ void init(const Args& a, const Job& j, Shared<HD, 1, 2>& s) {
+    wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    k = static_cast<const char*>(a.k.p) + ((long)j.base * a.k.tok + j.head * a.k.head) * 2;
+    v = static_cast<const char*>(a.v.p) + ((long)j.base * a.v.tok + j.head * a.v.head) * 2;
+    kstep = (unsigned)a.k.tok * 2 * kKeys;
+    vstep = (unsigned)a.v.tok * 2 * kKeys;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int unit = u * 256 + (int)threadIdx.x, pos = unit % CH;
+      key[u] = unit / CH;
+      const int kc = pos ^ Buf::k_swizzle(key[u]), vc = pos ^ Buf::v_swizzle(key[u]);
+      kv[u] = (unsigned)key[u] * (unsigned)a.k.tok * 2 + kc * 16;
+      vv[u] = (unsigned)key[u] * (unsigned)a.v.tok * 2 + vc * 16;
+      in[u] = kc * 8 < a.hd;
+      vin[u] = vc * 8 < a.hd;
+    }
+    if (a.hd < HD) {  // the channels behind the rows' stay 0
+      u4v* p = &s.b[0].k[0][0];
+      for (int i = threadIdx.x; i < (int)(sizeof(s.b) / 16); i += 256) p[i] = u4v{0, 0, 0, 0};
+      __syncthreads();
+    }
+  }
+  // keys at .. + 63 (as far as they are below live) on their way to b
+  __device__ __forceinline__ void issue(Buf& b, int at, int live, bool whole) {
+    const unsigned lk = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)b.k + wave * 1024;
+    const unsigned lv = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)b.v + wave * 1024;
+    const size_t stage = (size_t)(at / kKeys);
+    const char *kp = k + stage * kstep, *vp = v + stage * vstep;
+    if (whole) {
+#pragma unroll
+      for (int u = 0; u < N; ++u) load_lds16(kv[u], kp, lk + u * 4096);
+#pragma unroll
+      for (int u = 0; u < N; ++u) load_lds16(vv[u], vp, lv + u * 4096);
+    } else {
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        if (in[u] && at + key[u] < live) load_lds16(kv[u], kp, lk + u * 4096);
+        if (vin[u] && at + key[u] < live) load_lds16(vv[u], vp, lv + u * 4096);
+      }
+    }
+  }
+  // for a stage that not every row sees whole, once it is there
+  __device__ __forceinline__ void check(Buf& b, Bad<HD>& bad, int at, int live) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      u4v& x = b.v[0][u * 256 + threadIdx.x];
+      if (at + key[u] >= live) x = u4v{0, 0, 0, 0};
+      u4v y = x;
+      if (any_odd<M>(y)) {
+        clean<M>(y, bad, (int)((threadIdx.x % CH) ^ Buf::v_swizzle(key[u])) * 8, at + key[u]);
+        x = y;
+      }
+    }
+  }
+};
+
+// Any rows, through registers: a thread has every 32nd or 16th row's chunk.
+template <class M, int HD, int P, class T>
 struct RowStage {
-  static constexpr int CH = HD / 8, N = kKeys * CH / 256;
+  static constexpr int KP = P, NB = P == 1 ? 2 : 1, CH = HD / 8, N = kKeys * CH / 256;
+  static constexpr bool kDirect = false;
   typedef T T8 __attribute__((ext_vector_type(8)));
+  typedef Buffer<HD, P> Buf;
   T8 k[N], v[N];
 
+  __device__ __forceinline__ void init(const Args&, const Job&, Shared<HD, P, NB>&) {}
   static __device__ __forceinline__ void load1(const T* row, int c8, int n, bool vec, T8& x) {
     if (vec) {
       if (c8 < n) x = *reinterpret_cast<const T8*>(row + c8);
@@ -143,42 +254,39 @@ struct RowStage {
       }
     }
   }
-  static __device__ __forceinline__ void parts(const T8& x, u4v (&p)[KP]) {
+  static __device__ __forceinline__ void parts(const T8& x, u4v (&p)[P]) {
     if constexpr (sizeof(T) == 2) {
       p[0] = __builtin_bit_cast(u4v, x);
     } else {
       float f[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = x[e];
-      bf16_parts<KP>(f, p);
+      bf16_parts<P>(f, p);
     }
   }
-  __device__ __forceinline__ void store(Shared<HD, KP>& s, int at, int, bool edge) {
+  __device__ __forceinline__ void store(Buf& s, Bad<HD>& bad, int at, int, bool edge) {
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       const int unit = u * 256 + (int)threadIdx.x, key = unit / CH, chunk = unit % CH;
-      if (edge) {
-        // (a value times a probability of 0 must be 0 for the rows that do not see it)
-        bool odd = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) odd |= !__builtin_isfinite((float)v[u][e]);
-        if (odd) {
-          s.any_bad = 1;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (!__builtin_isfinite((float)v[u][e])) {
-              atomicMin(&s.bad[chunk * 8 + e], at + key);
-              v[u][e] = (T)0.f;
-            }
-        }
-      }
-      u4v p[KP];
+      u4v p[P];
       parts(k[u], p);
 #pragma unroll
-      for (int i = 0; i < KP; ++i) s.k[i][Shared<HD, KP>::k_at(key, chunk)] = p[i];
+      for (int i = 0; i < P; ++i) s.k[i][Buf::k_at(key, chunk)] = p[i];
       parts(v[u], p);
+      // (the first part of what is not finite is not finite: it is cut or the number itself)
+      if (edge && any_odd<M>(p[0])) {
+        const u4v first = p[0];
+        clean<M>(p[0], bad, chunk * 8, at + key);
 #pragma unroll
-      for (int i = 0; i < KP; ++i) s.v[i][Shared<HD, KP>::v_at(key, chunk)] = p[i];
+        for (int i = 1; i < P; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned kept = ~(first[e] ^ p[0][e]);  // halves that clean() has left alone, and zeros
+            p[i][e] &= ((kept & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((kept & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < P; ++i) s.v[i][Buf::v_at(key, chunk)] = p[i];
     }
   }
 };
@@ -187,10 +295,14 @@ struct RowStage {
 // one key, and of four values.
 template <int HD>
 struct CodeStage {
+  static constexpr int KP = 1, NB = 2;
+  static constexpr bool kDirect = false;
   typedef unsigned W __attribute__((ext_vector_type(HD / 32)));
+  typedef Buffer<HD, 1> Buf;
   W k, v;
   unsigned ks, vs;
 
+  __device__ __forceinline__ void init(const Args&, const Job&, Shared<HD, 1, 2>&) {}
   __device__ __forceinline__ void load(const Args& a, const Job& j, int at, int) {
     const int unit = (int)threadIdx.x & 127, lane = HD == 128 ? unit & 63 : unit >> 1, b = HD == 128 ? unit >> 6 : unit & 1;
     // (a second tile behind the capacity is the first once more: no key of it is seen)
@@ -202,28 +314,27 @@ struct CodeStage {
     ks = a.c.sk[scales + b * (HD / 2) + (HD == 128 ? lane : (g >> 1) * 16 + m)];
     vs = *reinterpret_cast<const unsigned*>(a.c.sv + scales + (g * (HD / 32) + m * (HD / 16) / 32) * 8 + b * 4);
   }
-  __device__ __forceinline__ void store(Shared<HD, 1>& s, int at, int live, bool edge) {
+  __device__ __forceinline__ void store(Buf& s, Bad<HD>& bad, int at, int live, bool edge) {
     const int unit = (int)threadIdx.x & 127, lane = HD == 128 ? unit & 63 : unit >> 1, b = HD == 128 ? unit >> 6 : unit & 1;
     const int g = lane >> 4, m = lane & 15, first = ((int)threadIdx.x >> 7) * kFTile + b * 16;
     const float kscale = scale_of(ks);
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i)
-      s.k[0][Shared<HD, 1>::k_at(first + m, g * (HD / 32) + i)] = eight_bf16(k[i], kscale);
+    for (int i = 0; i < HD / 32; ++i) s.k[0][Buf::k_at(first + m, g * (HD / 32) + i)] = eight_bf16(k[i], kscale);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int key = first + 4 * g + i;
       unsigned byte = (vs >> (8 * i)) & 255u;
       if (edge && at + key >= live) byte = 0;  // (what lies there is anything)
       if (byte == 255u) {
-        s.any_bad = 1;
-        for (int e = 0; e < HD / 16; ++e) atomicMin(&s.bad[m * (HD / 16) + e], at + key);
+        bad.any = 1;
+        for (int e = 0; e < HD / 16; ++e) atomicMin(&bad.key[m * (HD / 16) + e], at + key);
         byte = 0;
       }
       if constexpr (HD == 128) {
-        s.v[0][Shared<HD, 1>::v_at(key, m)] = eight_bf16(v[i], scale_of(byte));
+        s.v[0][Buf::v_at(key, m)] = eight_bf16(v[i], scale_of(byte));
       } else {
         const unsigned w = v[i / 2];
-        uint2* to = reinterpret_cast<uint2*>(&s.v[0][Shared<HD, 1>::v_at(key, m >> 1)]) + (m & 1);
+        uint2* to = reinterpret_cast<uint2*>(&s.v[0][Buf::v_at(key, m >> 1)]) + (m & 1);
         *to = i & 1 ? make_uint2(two_bf16<2>(w, scale_of(byte)), two_bf16<3>(w, scale_of(byte)))
                     : make_uint2(two_bf16<0>(w, scale_of(byte)), two_bf16<1>(w, scale_of(byte)));
       }
@@ -239,9 +350,10 @@ __device__ __forceinline__ uint2 read_tr(const void* p) {
   return __builtin_bit_cast(uint2, r);
 }
 
-template <class M, int HD, int QP, int KP, int PP, class T, class Stage>
-__device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD, KP>& s) {
-  constexpr int KS = HD / 16, DT = HD / 32;
+template <class M, int HD, int QP, int PP, class T, class Stage>
+__device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD, Stage::KP, Stage::NB>& s) {
+  constexpr int KS = HD / 16, DT = HD / 32, KP = Stage::KP, NB = Stage::NB;
+  typedef Buffer<HD, KP> Buf;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int first = job.tile * 128, rows = job.count * a.group;
@@ -250,10 +362,18 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
   const int lim = seen(job, i);
   // keys that the workgroup's rows see: at most, and at least but for padding
   const int live = rows > first ? seen(job, (min(first + 128, rows) - 1) / a.group) : 0, least = seen(job, first / a.group);
-  const long qrow = job.base + min(i, max(job.count - 1, 0));
+  Stage st;
+  st.init(a, job, s);
+  for (int c = tid; c < HD; c += 256) s.bad.key[c] = INT32_MAX;
+  if (tid == 0) s.bad.any = 0;
+  auto edge_at = [&](int at) { return at + kKeys > least; };  // (uniform)
+  if (live > 0) {
+    if constexpr (Stage::kDirect) st.issue(s.b[0], 0, live, kKeys <= live && a.hd == HD);
+    else st.load(a, job, 0, live);
+  }
   u4v q[KS][QP];
   {
-    const T* p = static_cast<const T*>(a.q.p) + job.seq * a.q.seq + qrow * a.q.tok + head * a.q.head;
+    const T* p = static_cast<const T*>(a.q.p) + job.seq * a.q.seq + (job.base + (long)min(i, max(job.count - 1, 0))) * a.q.tok + head * a.q.head;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       float x[8];
@@ -267,16 +387,37 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = f32x16{};
   float m = -INFINITY, l = 0.f, l_whole = 0.f;  // l_whole: of unrounded probabilities, for the stats
-  for (int c = tid; c < HD; c += 256) s.bad[c] = INT32_MAX;
-  if (tid == 0) s.any_bad = 0;
-  Stage st;
-  if (live > 0) st.load(a, job, 0, live);
+  if constexpr (!Stage::kDirect && NB == 2) {
+    if (live > 0) {
+      __syncthreads();
+      st.store(s.b[0], s.bad, 0, live, edge_at(0));
+      if (kKeys < live) st.load(a, job, kKeys, live);
+    }
+  }
   for (int at = 0; at < live; at += kKeys) {
-    const bool edge = at + kKeys > least;  // (uniform)
-    __syncthreads();
-    st.store(s, at, live, edge);
-    __syncthreads();
-    if (at + kKeys < live) st.load(a, job, at + kKeys, live);
+    const bool edge = edge_at(at);
+    const int next = at + kKeys;
+    Buf& b = s.b[NB == 1 ? 0 : at / kKeys & 1];
+    Buf& other = s.b[NB == 1 ? 0 : next / kKeys & 1];
+    if constexpr (Stage::kDirect) {
+      wait_and_sync();  // the stage is there, and nobody reads the other one any more
+      if (edge) {
+        st.check(b, s.bad, at, live);
+        __syncthreads();
+      }
+      if (next < live) st.issue(other, next, live, next + kKeys <= live && a.hd == HD);
+    } else if constexpr (NB == 2) {
+      __syncthreads();
+      if (next < live) {
+        st.store(other, s.bad, next, live, edge_at(next));
+        if (next + kKeys < live) st.load(a, job, next + kKeys, live);
+      }
+    } else {
+      __syncthreads();
+      st.store(b, s.bad, at, live, edge);
+      __syncthreads();
+      if (next < live) st.load(a, job, next, live);
+    }
     float p[2][16];  // keys at + sub * 32 + e / 4 * 8 + half * 4 + e % 4
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
@@ -285,7 +426,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int kp = KP - 1; kp >= 0; --kp) {
-          const u4v f = s.k[kp][Shared<HD, KP>::k_at(sub * 32 + n, k * 2 + half)];
+          const u4v f = b.k[kp][Buf::k_at(sub * 32 + n, k * 2 + half)];
 #pragma unroll
           for (int qp = QP - 1; qp >= 0; --qp)
             if (kp + qp < 3) x = M::mfma(f, q[k][qp], x);
@@ -303,7 +444,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
     for (int e = 1; e < 32; ++e) top = fmaxf(top, p[e / 16][e % 16]);
     if (__builtin_amdgcn_ballot_w64(top * a.sum > m + kSlack)) {
       top = xor32_max_k(top) * a.sum;
-      // (each column by itself: its result does not depend on its neighbours')
+      // (each row by itself: its result does not depend on its neighbours')
       const float f = top > m + kSlack ? __builtin_amdgcn_exp2f(m - top) : 1.f;
       m = top > m + kSlack ? top : m;
       l *= f;
@@ -348,7 +489,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
             u4v f;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const u4v* c = &s.v[kp][Shared<HD, KP>::v_at(key + 8 * r, d * 4 + chan / 8)];
+              const u4v* c = &b.v[kp][Buf::v_at(key + 8 * r, d * 4 + chan / 8)];
               const uint2 w = read_tr(reinterpret_cast<const char*>(c) + (chan & 7) * 2);
               f[2 * r] = w.x;
               f[2 * r + 1] = w.y;
@@ -372,10 +513,10 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       float x[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = any ? o[d][e + r] * inv : 0.f;
-      if (live > 0 && s.any_bad)
+      if (live > 0 && s.bad.any)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (s.bad[c4 + r] < lim) x[r] = NAN;
+          if (s.bad.key[c4 + r] < lim) x[r] = NAN;
       store4(out, c4, a.hd, make_float4(x[0], x[1], x[2], x[3]), a.ovec);
     }
   if (a.stats) {
@@ -386,8 +527,8 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
 }
 
 template <int HD, int QP, int PP, class T>
-__global__ __launch_bounds__(256) void f_attend_many_kernel(Args a) {
-  __shared__ Shared<HD, 1> s;
+__global__ __launch_bounds__(256, HD == 64 || sizeof(T) == 2 ? 2 : 1) void f_attend_many_kernel(Args a) {
+  __shared__ Shared<HD, 1, 2> s;
   Job j;
   j.seq = (int)blockIdx.x / a.n_head;
   j.head = (int)blockIdx.x % a.n_head;
@@ -395,19 +536,23 @@ __global__ __launch_bounds__(256) void f_attend_many_kernel(Args a) {
   j.len = a.len[j.seq];
   j.count = a.counts ? min(max(a.counts[j.seq], 0), a.n_q) : a.n_q;
   j.base = 0;
-  attend<Bf16, HD, QP, 1, PP, T, CodeStage<HD>>(a, j, s);
+  attend<Bf16, HD, QP, PP, T, CodeStage<HD>>(a, j, s);
 }
 
 // The workgroups of a packed batch: tile number x / n_head of all sequences'
 // tiles, for head x % n_head; those behind the last tile clear the rows that no
 // sequence has. There is one at least: the sum of the sequences' tiles, rounded up
 // each, is less than the rows' tiles and the number of sequences.
-template <class M, int HD, int P, class T>
-__global__ __launch_bounds__(256) void packed_attend_kernel(Args a) {
-  __shared__ Shared<HD, P> s;
+template <class M, int HD, int P, class T, class Stage>
+__global__ __launch_bounds__(256, HD == 64 || P == 1 ? 2 : 1) void packed_attend_kernel(Args a) {
+  __shared__ Shared<HD, Stage::KP, Stage::NB> s;
   const int lane = threadIdx.x & 63;
   int at = (int)blockIdx.x / a.n_head, end = 0;
   const int index = at, head = (int)blockIdx.x % a.n_head;
+  Job j;
+  j.seq = 0;  // (packed rows have no stride of sequences)
+  j.head = head;
+  j.tile = -1;
   for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
     const int seq = s0 + lane;
     int lo = 0, hi = 0;
@@ -426,18 +571,17 @@ __global__ __launch_bounds__(256) void packed_attend_kernel(Args a) {
     if (mine) {
       const int l = __builtin_ctzll(mine);
       auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-      Job j;
-      j.seq = 0;  // (packed rows have no stride of sequences)
-      j.head = head;
       j.base = of(lo);
       j.len = j.count = of(hi) - j.base;
       j.tile = of(incl) - 1 - at;  // the longest first
-      a.n_q = j.count;
-      attend<M, HD, P, P, P, T, RowStage<M, HD, P, T>>(a, j, s);
-      return;
+      break;
     }
     at -= __builtin_amdgcn_readlane(incl, 63);
     end = max(end, __builtin_amdgcn_readlane(hi, min(a.n_seq - 1 - s0, 63)));
+  }
+  if (j.tile >= 0) {
+    a.n_q = j.count;
+    return attend<M, HD, P, P, T, Stage>(a, j, s);
   }
   // `at` workgroups of this head are before this one among those that are left
   const int start = min(max(a.offsets[0], 0), a.n_rows), spare = start + a.n_rows - end;
@@ -458,8 +602,20 @@ void many_t(hipStream_t s, const Args& a) {
 template <class M, int P, class T>
 void packed_t(hipStream_t s, const Args& a) {
   const unsigned tiles = (unsigned)((a.n_rows * (long)a.group + 127) / 128 + a.n_seq), grid = tiles * (unsigned)a.n_head;
-  if (a.hd <= 64) packed_attend_kernel<M, 64, P, T><<<grid, 256, 0, s>>>(a);
-  else packed_attend_kernel<M, 128, P, T><<<grid, 256, 0, s>>>(a);
+  auto run = [&](auto width) {
+    constexpr int HD = decltype(width)::value;
+    if constexpr (P == 1) {
+      // (a lane's offset within a stage of 64 rows is 32 bits, unsigned)
+      auto near = [](const QRows& r) { return r.tok >= 0 && r.tok < 1 << 22; };
+      if (a.kvec && near(a.k) && near(a.v)) {
+        packed_attend_kernel<M, HD, P, T, DirectStage<M, HD>><<<grid, 256, 0, s>>>(a);
+        return;
+      }
+    }
+    packed_attend_kernel<M, HD, P, T, RowStage<M, HD, P, T>><<<grid, 256, 0, s>>>(a);
+  };
+  if (a.hd <= 64) run(std::integral_constant<int, 64>{});
+  else run(std::integral_constant<int, 128>{});
 }
 
 }  // namespace

@@ -25,6 +25,7 @@
 
 #include "attn_core.h"
 #include "f16_pair.h"
+#include "lds_direct.h"
 #include "qcache.h"
 #include "qrows.h"
 #include "qwrite.h"
@@ -472,18 +473,6 @@ struct RowOut {
 // 340 instead of 513 vector instructions a pair, but twice the LDS reads, which
 // then bound it: 211 against 169 us for 16 x 1023 tokens of 20 heads.)
 constexpr int kPair = 2 * kQTile;
-
-// Lane i's 16 bytes at base + voff go to LDS lds + 16 i (the kernel waits itself).
-// A load to LDS needs a wait state behind the write of M0; nobody adds it within
-// an asm block.
-__device__ __forceinline__ void load_lds16(unsigned voff, const void* base, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
-}
-// This wave's loads have landed, then the barrier.
-__device__ __forceinline__ void wait_and_sync() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  __syncthreads();
-}
 
 template <int HDP>
 struct SharedPair {
