@@ -343,11 +343,29 @@ struct CodeStage {
 };
 
 typedef short s4v __attribute__((ext_vector_type(4)));
+typedef const u4v __attribute__((address_space(3))) * LdsChunk;
+typedef s4v __attribute__((address_space(3))) * LdsFour;
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
 // Four values of 16 bits of one channel, of the rows whose chunks the 16 lanes point at.
-__device__ __forceinline__ uint2 read_tr(const void* p) {
-  typedef s4v __attribute__((address_space(3))) * Lds;
-  const s4v r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)(__attribute__((address_space(3))) const char*)p);
-  return __builtin_bit_cast(uint2, r);
+__device__ __forceinline__ uint2 read_tr(unsigned at) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour)(uintptr_t)at));
+}
+
+// Of READS reads of LDS in this stretch, the first AHEAD before the first matrix
+// instruction, then STEP of them behind every MFMAS: left to itself the compiler
+// reads each operand right before its use and waits for it, 100 cycles a time.
+template <int READS, int AHEAD, int STEP, int MFMAS>
+__device__ __forceinline__ void reads_ahead() {
+  constexpr int kRead = 0x100, kMfma = 0x8;
+  __builtin_amdgcn_sched_group_barrier(kRead, AHEAD, 0);
+#pragma unroll
+  for (int i = AHEAD; i < READS; i += STEP) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, MFMAS, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, STEP, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(kMfma, (AHEAD + STEP - 1) / STEP * MFMAS, 0);
 }
 
 template <class M, int HD, int QP, int PP, class T, class Stage>
@@ -383,6 +401,19 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       parts_of<M, QP>(x, q[k]);
     }
   }
+  // Where this lane's operands lie in the first buffer, but for multiples of 16 keys
+  // (which the swizzles do not see, and instructions hold as their offsets).
+  unsigned ka[KS], va[DT][2];
+  {
+    const unsigned at_k = lds_address(&s.b[0].k[0][0]), at_v = lds_address(&s.b[0].v[0][0]);
+    const int key = half * 4 + ((lane & 15) >> 2), chan = (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) ka[k] = at_k + Buf::k_at(n, k * 2 + half) * 16;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) va[d][r] = at_v + Buf::v_at(key + 8 * r, d * 4 + chan / 8) * 16 + (chan & 7) * 2;
+  }
   f32x16 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = f32x16{};
@@ -394,11 +425,14 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       if (kKeys < live) st.load(a, job, kKeys, live);
     }
   }
-  for (int at = 0; at < live; at += kKeys) {
-    const bool edge = edge_at(at);
+  // (two forms of the step: the compiler would else select for every score of every stage)
+  auto step = [&](int at, auto edge_stage, auto in_buffer) {
+    constexpr bool edge = decltype(edge_stage)::value;
     const int next = at + kKeys;
-    Buf& b = s.b[NB == 1 ? 0 : at / kKeys & 1];
-    Buf& other = s.b[NB == 1 ? 0 : next / kKeys & 1];
+    const unsigned which = in_buffer;  // (a constant but at the edge)
+    Buf& b = s.b[which];
+    Buf& other = s.b[NB - 1 - which];
+    const unsigned boff = which * (unsigned)sizeof(Buf);
     if constexpr (Stage::kDirect) {
       wait_and_sync();  // the stage is there, and nobody reads the other one any more
       if (edge) {
@@ -426,7 +460,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int kp = KP - 1; kp >= 0; --kp) {
-          const u4v f = b.k[kp][Buf::k_at(sub * 32 + n, k * 2 + half)];
+          const u4v f = *(LdsChunk)(uintptr_t)(ka[k] + (boff + kp * (unsigned)sizeof(b.k[0]) + sub * 512 * Buf::CH));
 #pragma unroll
           for (int qp = QP - 1; qp >= 0; --qp)
             if (kp + qp < 3) x = M::mfma(f, q[k][qp], x);
@@ -434,7 +468,8 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
 #pragma unroll
       for (int e = 0; e < 16; ++e) p[sub][e] = x[e];
     }
-    if (edge) {
+    reads_ahead<2 * KS * KP, 6, 1, KP == 1 ? QP : 2>();
+    if constexpr (edge) {
 #pragma unroll
       for (int e = 0; e < 32; ++e)
         if (at + e / 16 * 32 + e % 16 / 4 * 8 + half * 4 + e % 4 >= lim) p[e / 16][e % 16] = -INFINITY;
@@ -455,7 +490,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
     const float base = (m == -INFINITY ? 0.f : m) - M::kUp;
 #pragma unroll
     for (int e = 0; e < 32; ++e) p[e / 16][e % 16] = __builtin_amdgcn_exp2f(fmaf(p[e / 16][e % 16], a.sum, -base));
-    if (edge) {
+    if constexpr (edge) {
 #pragma unroll
       for (int e = 0; e < 32; ++e)
         if (at + e / 16 * 32 + e % 16 / 4 * 8 + half * 4 + e % 4 >= lim) p[e / 16][e % 16] = 0.f;
@@ -481,7 +516,6 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
 #pragma unroll
           for (int e = 0; e < 8; ++e) l += x[e];
         }
-        const int key = sub * 32 + u * 16 + half * 4 + ((lane & 15) >> 2), chan = (lane >> 4 & 1) * 16 + (lane & 3) * 4;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -489,8 +523,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
             u4v f;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const u4v* c = &b.v[kp][Buf::v_at(key + 8 * r, d * 4 + chan / 8)];
-              const uint2 w = read_tr(reinterpret_cast<const char*>(c) + (chan & 7) * 2);
+              const uint2 w = read_tr(va[d][r] + (boff + kp * (unsigned)sizeof(b.v[0]) + (sub * 32 + u * 16) * 16 * Buf::CH));
               f[2 * r] = w.x;
               f[2 * r + 1] = w.y;
             }
@@ -499,7 +532,18 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
               if (kp + k < 3) o[d] = M::mfma(f, pp[k], o[d]);
           }
       }
+    reads_ahead<8 * DT * KP, 8, 2, KP == 1 ? PP : 2>();
+  };
+  int at = 0;
+  if constexpr (NB == 1) {
+    for (; at < live && !edge_at(at); at += kKeys) step(at, std::false_type{}, std::integral_constant<unsigned, 0>{});
+  } else {
+    for (; at < live && !edge_at(at + kKeys); at += 2 * kKeys) {
+      step(at, std::false_type{}, std::integral_constant<unsigned, 0>{});
+      step(at + kKeys, std::false_type{}, std::integral_constant<unsigned, 1>{});
+    }
   }
+  for (; at < live; at += kKeys) step(at, std::true_type{}, NB == 1 ? 0u : (unsigned)(at / kKeys) & 1u);
   if (row >= a.n_q * a.group) return;
   l = xor32_sum_k(l);
   const bool any = lim > 0;
