@@ -35,6 +35,7 @@ namespace rtg {
 namespace {
 
 constexpr int kKeys = 64;      // of a stage in LDS
+constexpr long kManySplit = 256;  // workgroups at most where the keys are split
 constexpr float kSlack = 8.f;  // powers of two that a score may pass the running maximum by
 
 struct Args {
@@ -47,14 +48,19 @@ struct Args {
   float query, sum;  // ScoreScale
   float* stats;
   bool qvec, kvec, ovec;
+  int min_stages;     // of a split of the keys
+  unsigned* tickets;  // [tile][kQTicketStride], a word for each wave
+  float* parts;       // [tile][split][wave][value][lane]
 };
 
-// What a workgroup works on: rows [first, first + 128) of the (query, head) pairs
-// of a sequence and key/value head.
+// What a workgroup of NT threads works on: NT / 2 rows of the (query, head) pairs of
+// a sequence and key/value head, `tile` times as many before them.
 struct Job {
   int seq, head, tile;
   int len, count;  // keys, queries
   int base;        // packed: the sequence's first row
+  int z = 0, zs = 1;  // which of how many parts of the keys, where they are split
+  int slot = 0;       // where split parts meet: number of the tile among all
 };
 __device__ __forceinline__ int seen(const Job& j, int i) { return keys_seen(j.len, j.count, i); }
 
@@ -121,9 +127,10 @@ struct Bad {
   int key[HD];
   int any;
 };
-template <int HD, int KP, int NB>
+// KG groups of waves, each with NB buffers of its own.
+template <int HD, int KP, int NB, int KG>
 struct Shared {
-  Buffer<HD, KP> b[NB];
+  Buffer<HD, KP> b[KG][NB];
   Bad<HD> bad;
 };
 
@@ -154,9 +161,9 @@ __device__ __forceinline__ void clean(u4v& x, Bad<HD>& bad, int channel, int key
 
 // Rows of 16 bits, aligned, straight to LDS: a wave's load is 1 KB of LDS, each
 // lane picking the chunk that belongs there.
-template <class M, int HD>
+template <class M, int HD, int NW>
 struct DirectStage {
-  static constexpr int KP = 1, NB = 2, CH = HD / 8, N = kKeys * CH / 256;
+  static constexpr int KP = 1, NB = 2, NT = 64 * NW, CH = HD / 8, N = kKeys * CH / NT;
   static constexpr bool kDirect = true;
   typedef Buffer<HD, 1> Buf;
   const char *k, *v;
@@ -166,15 +173,18 @@ struct DirectStage {
   bool in[N];  // whether the chunk belongs to the row (of keys', values')
   bool vin[N];
 
-  __device__ __forceinline__ void init(const Args& a, const Job& j, Shared<HD, 1, 2>& s) {
-    wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  int tid;
+
+  __device__ __forceinline__ void init(const Args& a, const Job& j, Buf (&b)[NB], int thread) {
+    tid = thread;
+    wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     k = static_cast<const char*>(a.k.p) + ((long)j.base * a.k.tok + j.head * a.k.head) * 2;
     v = static_cast<const char*>(a.v.p) + ((long)j.base * a.v.tok + j.head * a.v.head) * 2;
     kstep = (unsigned)a.k.tok * 2 * kKeys;
     vstep = (unsigned)a.v.tok * 2 * kKeys;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int unit = u * 256 + (int)threadIdx.x, pos = unit % CH;
+      const int unit = u * NT + tid, pos = unit % CH;
       key[u] = unit / CH;
       const int kc = pos ^ Buf::k_swizzle(key[u]), vc = pos ^ Buf::v_swizzle(key[u]);
       kv[u] = (unsigned)key[u] * (unsigned)a.k.tok * 2 + kc * 16;
@@ -183,8 +193,8 @@ struct DirectStage {
       vin[u] = vc * 8 < a.hd;
     }
     if (a.hd < HD) {  // the channels behind the rows' stay 0
-      u4v* p = &s.b[0].k[0][0];
-      for (int i = threadIdx.x; i < (int)(sizeof(s.b) / 16); i += 256) p[i] = u4v{0, 0, 0, 0};
+      u4v* p = &b[0].k[0][0];
+      for (int i = tid; i < (int)(sizeof(b) / 16); i += NT) p[i] = u4v{0, 0, 0, 0};
       __syncthreads();
     }
   }
@@ -196,14 +206,14 @@ struct DirectStage {
     const char *kp = k + stage * kstep, *vp = v + stage * vstep;
     if (whole) {
 #pragma unroll
-      for (int u = 0; u < N; ++u) load_lds16(kv[u], kp, lk + u * 4096);
+      for (int u = 0; u < N; ++u) load_lds16(kv[u], kp, lk + u * NT * 16);
 #pragma unroll
-      for (int u = 0; u < N; ++u) load_lds16(vv[u], vp, lv + u * 4096);
+      for (int u = 0; u < N; ++u) load_lds16(vv[u], vp, lv + u * NT * 16);
     } else {
 #pragma unroll
       for (int u = 0; u < N; ++u) {
-        if (in[u] && at + key[u] < live) load_lds16(kv[u], kp, lk + u * 4096);
-        if (vin[u] && at + key[u] < live) load_lds16(vv[u], vp, lv + u * 4096);
+        if (in[u] && at + key[u] < live) load_lds16(kv[u], kp, lk + u * NT * 16);
+        if (vin[u] && at + key[u] < live) load_lds16(vv[u], vp, lv + u * NT * 16);
       }
     }
   }
@@ -211,30 +221,31 @@ struct DirectStage {
   __device__ __forceinline__ void check(Buf& b, Bad<HD>& bad, int at, int live) {
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      u4v& x = b.v[0][u * 256 + threadIdx.x];
+      u4v& x = b.v[0][u * NT + tid];
       if (at + key[u] >= live) x = u4v{0, 0, 0, 0};
       u4v y = x;
       if (any_odd<M>(y)) {
-        clean<M>(y, bad, (int)((threadIdx.x % CH) ^ Buf::v_swizzle(key[u])) * 8, at + key[u]);
+        clean<M>(y, bad, ((tid % CH) ^ Buf::v_swizzle(key[u])) * 8, at + key[u]);
         x = y;
       }
     }
   }
 };
 
-// Any rows, through registers: a thread has every 32nd or 16th row's chunk.
-template <class M, int HD, int P, class T>
+// Rows through registers, NW waves sharing a stage: aligned ones (VEC), or any.
+template <class M, int HD, int P, class T, bool VEC, int NW, int BUFFERS>
 struct RowStage {
-  static constexpr int KP = P, NB = P == 1 ? 2 : 1, CH = HD / 8, N = kKeys * CH / 256;
+  static constexpr int KP = P, NB = BUFFERS, CH = HD / 8, NT = 64 * NW, N = kKeys * CH / NT;
   static constexpr bool kDirect = false;
   typedef T T8 __attribute__((ext_vector_type(8)));
   typedef Buffer<HD, P> Buf;
   T8 k[N], v[N];
+  int tid;
 
-  __device__ __forceinline__ void init(const Args&, const Job&, Shared<HD, P, NB>&) {}
-  static __device__ __forceinline__ void load1(const T* row, int c8, int n, bool vec, T8& x) {
-    if (vec) {
-      if (c8 < n) x = *reinterpret_cast<const T8*>(row + c8);
+  __device__ __forceinline__ void init(const Args&, const Job&, Buf (&)[NB], int thread) { tid = thread; }
+  static __device__ __forceinline__ void load1(const T* row, int c8, int n, T8& x) {
+    if constexpr (VEC) {
+      x = *reinterpret_cast<const T8*>(row + c8);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -242,16 +253,19 @@ struct RowStage {
     }
   }
   __device__ __forceinline__ void load(const Args& a, const Job& j, int at, int live) {
+    const bool whole = VEC && at + kKeys <= live && a.hd == HD;  // (uniform)
+    const T* kp = static_cast<const T*>(a.k.p) + (j.base + (long)at) * a.k.tok + j.head * a.k.head;
+    const T* vp = static_cast<const T*>(a.v.p) + (j.base + (long)at) * a.v.tok + j.head * a.v.head;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int unit = u * 256 + (int)threadIdx.x, key = at + unit / CH, c8 = unit % CH * 8;
-      k[u] = T8{};
-      v[u] = T8{};
-      if (key < live) {
-        const long row = j.base + key;
-        load1(static_cast<const T*>(a.k.p) + row * a.k.tok + j.head * a.k.head, c8, a.hd, a.kvec, k[u]);
-        load1(static_cast<const T*>(a.v.p) + row * a.v.tok + j.head * a.v.head, c8, a.hd, a.kvec, v[u]);
+      const int unit = u * NT + tid, key = unit / CH, c8 = unit % CH * 8;
+      if (!whole) {
+        k[u] = T8{};
+        v[u] = T8{};
+        if (at + key >= live || c8 >= a.hd) continue;
       }
+      load1(kp + key * a.k.tok, c8, a.hd, k[u]);
+      load1(vp + key * a.v.tok, c8, a.hd, v[u]);
     }
   }
   static __device__ __forceinline__ void parts(const T8& x, u4v (&p)[P]) {
@@ -267,7 +281,7 @@ struct RowStage {
   __device__ __forceinline__ void store(Buf& s, Bad<HD>& bad, int at, int, bool edge) {
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int unit = u * 256 + (int)threadIdx.x, key = unit / CH, chunk = unit % CH;
+      const int unit = u * NT + tid, key = unit / CH, chunk = unit % CH;
       u4v p[P];
       parts(k[u], p);
 #pragma unroll
@@ -295,18 +309,19 @@ struct RowStage {
 // one key, and of four values.
 template <int HD>
 struct CodeStage {
-  static constexpr int KP = 1, NB = 2;
+  static constexpr int KP = 1, NB = 2, NT = 256;
   static constexpr bool kDirect = false;
   typedef unsigned W __attribute__((ext_vector_type(HD / 32)));
   typedef Buffer<HD, 1> Buf;
   W k, v;
   unsigned ks, vs;
+  int tid;
 
-  __device__ __forceinline__ void init(const Args&, const Job&, Shared<HD, 1, 2>&) {}
+  __device__ __forceinline__ void init(const Args&, const Job&, Buf (&)[NB], int thread) { tid = thread; }
   __device__ __forceinline__ void load(const Args& a, const Job& j, int at, int) {
-    const int unit = (int)threadIdx.x & 127, lane = HD == 128 ? unit & 63 : unit >> 1, b = HD == 128 ? unit >> 6 : unit & 1;
+    const int unit = tid & 127, lane = HD == 128 ? unit & 63 : unit >> 1, b = HD == 128 ? unit >> 6 : unit & 1;
     // (a second tile behind the capacity is the first once more: no key of it is seen)
-    const int tile = min(at / kFTile + ((int)threadIdx.x >> 7), a.c.tiles - 1), g = lane >> 4, m = lane & 15;
+    const int tile = min(at / kFTile + (tid >> 7), a.c.tiles - 1), g = lane >> 4, m = lane & 15;
     const size_t sh = (size_t)j.seq * a.c.n_head + j.head, codes = a.c.codes(sh) + (size_t)tile * 16 * HD + unit * (HD / 8);
     const size_t scales = a.c.scales(sh) + (size_t)tile * HD;
     k = *reinterpret_cast<const W*>(a.c.k + codes);
@@ -315,8 +330,8 @@ struct CodeStage {
     vs = *reinterpret_cast<const unsigned*>(a.c.sv + scales + (g * (HD / 32) + m * (HD / 16) / 32) * 8 + b * 4);
   }
   __device__ __forceinline__ void store(Buf& s, Bad<HD>& bad, int at, int live, bool edge) {
-    const int unit = (int)threadIdx.x & 127, lane = HD == 128 ? unit & 63 : unit >> 1, b = HD == 128 ? unit >> 6 : unit & 1;
-    const int g = lane >> 4, m = lane & 15, first = ((int)threadIdx.x >> 7) * kFTile + b * 16;
+    const int unit = tid & 127, lane = HD == 128 ? unit & 63 : unit >> 1, b = HD == 128 ? unit >> 6 : unit & 1;
+    const int g = lane >> 4, m = lane & 15, first = (tid >> 7) * kFTile + b * 16;
     const float kscale = scale_of(ks);
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) s.k[0][Buf::k_at(first + m, g * (HD / 32) + i)] = eight_bf16(k[i], kscale);
@@ -368,27 +383,41 @@ __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(kMfma, (AHEAD + STEP - 1) / STEP * MFMAS, 0);
 }
 
-template <class M, int HD, int QP, int PP, class T, class Stage>
-__device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD, Stage::KP, Stage::NB>& s) {
-  constexpr int KS = HD / 16, DT = HD / 32, KP = Stage::KP, NB = Stage::NB;
+template <class M, int HD, int QP, int PP, class T, class Stage, int KG>
+__device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD, Stage::KP, Stage::NB, KG>& s) {
+  constexpr int KS = HD / 16, DT = HD / 32, KP = Stage::KP, NB = Stage::NB, ROWS = Stage::NT / 2;
   typedef Buffer<HD, KP> Buf;
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
+  constexpr int SPAN = KG * kKeys;  // keys of a step: a stage for each group
+  const int tid = threadIdx.x % Stage::NT, lane = tid & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int first = job.tile * 128, rows = job.count * a.group;
+  const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x / Stage::NT);
+  Buf(&bufs)[NB] = s.b[group];
+  const int first = job.tile * ROWS, rows = job.count * a.group;
   // this lane's row: query i of head h
   const int row = first + wave * 32 + n, i = row / a.group, head = job.head * a.group + row % a.group;
   const int lim = seen(job, i);
   // keys that the workgroup's rows see: at most, and at least but for padding
-  const int live = rows > first ? seen(job, (min(first + 128, rows) - 1) / a.group) : 0, least = seen(job, first / a.group);
+  const int all = rows > first ? seen(job, (min(first + ROWS, rows) - 1) / a.group) : 0, least = seen(job, first / a.group);
+  // this workgroup's part of them
+  const int stages = (all + kKeys - 1) / kKeys, splits = job.zs == 1 ? 1 : max(min((stages + a.min_stages - 1) / a.min_stages, job.zs), 1);
+  if (job.z >= splits) return;
+  const int per = splits == 1 ? stages : (stages + splits - 1) / splits;
+  const int begin = job.z * per * kKeys, live = min(all, begin + per * kKeys);
+  const int end = min(first + wave * 32 + 32, rows);  // of this wave's rows
+  const int mine = end > first + wave * 32 ? min(seen(job, (end - 1) / a.group), live) : 0;
   Stage st;
-  st.init(a, job, s);
-  for (int c = tid; c < HD; c += 256) s.bad.key[c] = INT32_MAX;
-  if (tid == 0) s.bad.any = 0;
-  auto edge_at = [&](int at) { return at + kKeys > least; };  // (uniform)
-  if (live > 0) {
-    if constexpr (Stage::kDirect) st.issue(s.b[0], 0, live, kKeys <= live && a.hd == HD);
-    else st.load(a, job, 0, live);
-  }
+  st.init(a, job, bufs, tid);
+  for (int c = threadIdx.x; c < HD; c += KG * Stage::NT) s.bad.key[c] = INT32_MAX;
+  if (threadIdx.x == 0) s.bad.any = 0;
+  const int whole_to = min(least, live);
+  auto edge_at = [&](int at) { return at + SPAN > whole_to; };  // (uniform)
+  const int own = begin + group * kKeys;  // of the first step's keys, this group's
+  auto fetch = [&](int at, Buf& b) {
+    if (at >= live) return;
+    if constexpr (Stage::kDirect) st.issue(b, at, live, at + kKeys <= live && a.hd == HD);
+    else st.load(a, job, at, live);
+  };
+  fetch(own, bufs[0]);
   u4v q[KS][QP];
   {
     const T* p = static_cast<const T*>(a.q.p) + job.seq * a.q.seq + (job.base + (long)min(i, max(job.count - 1, 0))) * a.q.tok + head * a.q.head;
@@ -405,7 +434,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
   // (which the swizzles do not see, and instructions hold as their offsets).
   unsigned ka[KS], va[DT][2];
   {
-    const unsigned at_k = lds_address(&s.b[0].k[0][0]), at_v = lds_address(&s.b[0].v[0][0]);
+    const unsigned at_k = lds_address(&bufs[0].k[0][0]), at_v = lds_address(&bufs[0].v[0][0]);
     const int key = half * 4 + ((lane & 15) >> 2), chan = (lane >> 4 & 1) * 16 + (lane & 3) * 4;
 #pragma unroll
     for (int k = 0; k < KS; ++k) ka[k] = at_k + Buf::k_at(n, k * 2 + half) * 16;
@@ -419,39 +448,36 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
   for (int d = 0; d < DT; ++d) o[d] = f32x16{};
   float m = -INFINITY, l = 0.f, l_whole = 0.f;  // l_whole: of unrounded probabilities, for the stats
   if constexpr (!Stage::kDirect && NB == 2) {
-    if (live > 0) {
-      __syncthreads();
-      st.store(s.b[0], s.bad, 0, live, edge_at(0));
-      if (kKeys < live) st.load(a, job, kKeys, live);
-    }
+    __syncthreads();
+    if (own < live) st.store(bufs[0], s.bad, own, live, edge_at(begin));
+    fetch(own + SPAN, bufs[0]);
   }
   // (two forms of the step: the compiler would else select for every score of every stage)
-  auto step = [&](int at, auto edge_stage, auto in_buffer) {
+  auto step = [&](int from, auto edge_stage, auto in_buffer) {
     constexpr bool edge = decltype(edge_stage)::value;
-    const int next = at + kKeys;
+    const int at = from + group * kKeys, next = at + SPAN;
     const unsigned which = in_buffer;  // (a constant but at the edge)
-    Buf& b = s.b[which];
-    Buf& other = s.b[NB - 1 - which];
+    Buf& b = bufs[which];
+    Buf& other = bufs[NB - 1 - which];
     const unsigned boff = which * (unsigned)sizeof(Buf);
     if constexpr (Stage::kDirect) {
       wait_and_sync();  // the stage is there, and nobody reads the other one any more
       if (edge) {
-        st.check(b, s.bad, at, live);
+        if (at < live) st.check(b, s.bad, at, live);
         __syncthreads();
       }
-      if (next < live) st.issue(other, next, live, next + kKeys <= live && a.hd == HD);
+      fetch(next, other);
     } else if constexpr (NB == 2) {
       __syncthreads();
-      if (next < live) {
-        st.store(other, s.bad, next, live, edge_at(next));
-        if (next + kKeys < live) st.load(a, job, next + kKeys, live);
-      }
+      if (next < live) st.store(other, s.bad, next, live, edge_at(from + SPAN));
+      fetch(next + SPAN, other);
     } else {
       __syncthreads();
-      st.store(b, s.bad, at, live, edge);
+      if (at < live) st.store(b, s.bad, at, live, edge);
       __syncthreads();
-      if (next < live) st.load(a, job, next, live);
+      fetch(next, b);
     }
+    if (edge && at >= mine) return;  // (no row of this wave sees one of these keys)
     float p[2][16];  // keys at + sub * 32 + e / 4 * 8 + half * 4 + e % 4
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
@@ -534,16 +560,91 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       }
     reads_ahead<8 * DT * KP, 8, 2, KP == 1 ? PP : 2>();
   };
-  int at = 0;
+  int at = begin;
   if constexpr (NB == 1) {
-    for (; at < live && !edge_at(at); at += kKeys) step(at, std::false_type{}, std::integral_constant<unsigned, 0>{});
+    for (; at < live && !edge_at(at); at += SPAN) step(at, std::false_type{}, std::integral_constant<unsigned, 0>{});
   } else {
-    for (; at < live && !edge_at(at + kKeys); at += 2 * kKeys) {
+    for (; at < live && !edge_at(at + SPAN); at += 2 * SPAN) {
       step(at, std::false_type{}, std::integral_constant<unsigned, 0>{});
-      step(at + kKeys, std::false_type{}, std::integral_constant<unsigned, 1>{});
+      step(at + SPAN, std::false_type{}, std::integral_constant<unsigned, 1>{});
     }
   }
-  for (; at < live; at += kKeys) step(at, std::true_type{}, NB == 1 ? 0u : (unsigned)(at / kKeys) & 1u);
+  for (; at < live; at += SPAN) step(at, std::true_type{}, NB == 1 ? 0u : (unsigned)((at - begin) / SPAN) & 1u);
+  if constexpr (KG > 1) {
+    // the groups' results meet in LDS, value by value with the lanes side by side
+    constexpr int N = DT * 16 + 3;
+    static_assert(sizeof(s.b) >= (KG - 1) * (Stage::NT / 64) * N * 64 * 4, "room for the results");
+    __syncthreads();
+    float* to = reinterpret_cast<float*>(&s.b) + ((group - 1) * (Stage::NT / 64) + wave) * N * 64 + lane;
+    if (group > 0) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) to[(d * 16 + e) * 64] = o[d][e];
+      to[(N - 3) * 64] = m;
+      to[(N - 2) * 64] = l;
+      to[(N - 1) * 64] = l_whole;
+    }
+    __syncthreads();
+    if (group > 0) return;
+    for (int g = 1; g < KG; ++g) {
+      const float* x = reinterpret_cast<const float*>(&s.b) + ((g - 1) * (Stage::NT / 64) + wave) * N * 64 + lane;
+      const float m2 = x[(N - 3) * 64], most = fmaxf(m, m2), base = most == -INFINITY ? 0.f : most;
+      const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+      m = most;
+      l = fmaf(f, l, f2 * x[(N - 2) * 64]);
+      l_whole = fmaf(f, l_whole, f2 * x[(N - 1) * 64]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = fmaf(f, o[d][e], f2 * x[(d * 16 + e) * 64]);
+    }
+  }
+  if (all > 0 && s.bad.any) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (s.bad.key[d * 32 + e / 4 * 8 + half * 4 + e % 4] < lim) o[d][e] = NAN;
+  }
+  if (splits > 1) {
+    // Every wave's results, in pairs with the lanes side by side, past the L2 caches;
+    // the last of a tile's waves of one number to come here joins theirs, in order.
+    constexpr int N = DT * 16 + 4;
+    float* p = a.parts + ((size_t)(job.slot * job.zs + job.z) * (Stage::NT / 64) + wave) * N * 64 + lane * 2;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) store2(p + (d * 16 + e) * 64, o[d][e], o[d][e + 1]);
+    store2(p + (N - 4) * 64, m, l);
+    store2(p + (N - 2) * 64, l_whole, 0.f);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores have completed
+    unsigned before = 0, *count = a.tickets + (size_t)job.slot * kQTicketStride + wave;
+    if (lane == 0) before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__builtin_amdgcn_readfirstlane(before) != (unsigned)splits - 1) return;
+    if (lane == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    m = -INFINITY;
+    l = l_whole = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = f32x16{};
+    for (int z = 0; z < splits; ++z) {
+      const float* x = a.parts + ((size_t)(job.slot * job.zs + z) * (Stage::NT / 64) + wave) * N * 64 + lane * 2;
+      const float2 ml = load2(x + (N - 4) * 64), lw = load2(x + (N - 2) * 64);
+      const float most = fmaxf(m, ml.x), base = most == -INFINITY ? 0.f : most;
+      const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(ml.x - base);
+      m = most;
+      l = fmaf(f, l, f2 * ml.y);
+      l_whole = fmaf(f, l_whole, f2 * lw.x);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float2 y = load2(x + (d * 16 + e) * 64);
+          o[d][e] = fmaf(f, o[d][e], f2 * y.x);
+          o[d][e + 1] = fmaf(f, o[d][e + 1], f2 * y.y);
+        }
+    }
+  }
   if (row >= a.n_q * a.group) return;
   l = xor32_sum_k(l);
   const bool any = lim > 0;
@@ -553,15 +654,10 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
-      const int c4 = d * 32 + e / 4 * 8 + half * 4;
       float x[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = any ? o[d][e + r] * inv : 0.f;
-      if (live > 0 && s.bad.any)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (s.bad.key[c4 + r] < lim) x[r] = NAN;
-      store4(out, c4, a.hd, make_float4(x[0], x[1], x[2], x[3]), a.ovec);
+      store4(out, d * 32 + e / 4 * 8 + half * 4, a.hd, make_float4(x[0], x[1], x[2], x[3]), a.ovec);
     }
   if (a.stats) {
     if (PP == 1) l = xor32_sum_k(l_whole);
@@ -570,9 +666,9 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
   }
 }
 
-template <int HD, int QP, int PP, class T>
-__global__ __launch_bounds__(256, HD == 64 || sizeof(T) == 2 ? 2 : 1) void f_attend_many_kernel(Args a) {
-  __shared__ Shared<HD, 1, 2> s;
+template <int HD, int QP, int PP, class T, int KG>
+__global__ __launch_bounds__(256 * KG, KG > 1 || HD == 64 || sizeof(T) == 2 ? 2 : 1) void f_attend_many_kernel(Args a) {
+  __shared__ Shared<HD, 1, 2, KG> s;
   Job j;
   j.seq = (int)blockIdx.x / a.n_head;
   j.head = (int)blockIdx.x % a.n_head;
@@ -580,92 +676,173 @@ __global__ __launch_bounds__(256, HD == 64 || sizeof(T) == 2 ? 2 : 1) void f_att
   j.len = a.len[j.seq];
   j.count = a.counts ? min(max(a.counts[j.seq], 0), a.n_q) : a.n_q;
   j.base = 0;
-  attend<Bf16, HD, QP, PP, T, CodeStage<HD>>(a, j, s);
+  j.z = (int)blockIdx.z;
+  j.zs = (int)gridDim.z;
+  j.slot = (int)(blockIdx.x * gridDim.y + blockIdx.y);
+  attend<Bf16, HD, QP, PP, T, CodeStage<HD>, KG>(a, j, s);
 }
 
-// The workgroups of a packed batch: tile number x / n_head of all sequences'
-// tiles, for head x % n_head; those behind the last tile clear the rows that no
-// sequence has. There is one at least: the sum of the sequences' tiles, rounded up
-// each, is less than the rows' tiles and the number of sequences.
-template <class M, int HD, int P, class T, class Stage>
-__global__ __launch_bounds__(256, HD == 64 || P == 1 ? 2 : 1) void packed_attend_kernel(Args a) {
-  __shared__ Shared<HD, Stage::KP, Stage::NB> s;
+// The sum over a wave, in every lane.
+__device__ __forceinline__ int wave_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);   // quad_perm [1,0,3,2]
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);   // quad_perm [2,3,0,1]
+  v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xF, 0xF, false);  // row_ror:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false);  // row_ror:8
+  const auto x = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  v = (int)(x[0] + x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+  return __builtin_amdgcn_readfirstlane((int)(y[0] + y[1]));
+}
+
+// The workgroups of a packed batch: the tiles of all sequences, each for all heads
+// in turn; those behind the last tile clear the rows that no sequence has. There
+// is one at least: the sum of the sequences' tiles, rounded up each, is less than
+// the rows' tiles and the number of sequences.
+// Up to 64 sequences are taken by their lengths, a sequence's tiles by the keys they
+// see, so that what runs last is short (the longest tiles of all sequences first
+// would be shorter still at the end, but 8 sequences' keys do not fit the caches
+// that one's do: 128 us instead of 1XX); where all workgroups are on the device at once (RESIDENT of
+// them on each of its 256 compute units), every second 256 go the other way, so
+// that a compute unit's have about the same to do between them.
+template <class M, int HD, int P, class T, class Stage, int KG, int RESIDENT>
+__global__ __launch_bounds__(Stage::NT * KG, KG > 1 || HD == 64 || P == 1 ? 2 : 1) void packed_attend_kernel(Args a) {
+  constexpr int ROWS = Stage::NT / 2;
+  __shared__ Shared<HD, Stage::KP, Stage::NB, KG> s;
   const int lane = threadIdx.x & 63;
-  int at = (int)blockIdx.x / a.n_head, end = 0;
-  const int index = at, head = (int)blockIdx.x % a.n_head;
+  int block = (int)blockIdx.x, end = 0;
   Job j;
   j.seq = 0;  // (packed rows have no stride of sequences)
-  j.head = head;
   j.tile = -1;
-  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+  // the 64 sequences from s0 on, one per lane
+  int lo = 0, hi = 0;
+  auto sequences = [&](int s0) {
     const int seq = s0 + lane;
-    int lo = 0, hi = 0;
+    lo = hi = 0;
     if (seq < a.n_seq) {
       lo = min(max(a.offsets[seq], 0), a.n_rows);
       hi = min(max(a.offsets[seq + 1], lo), a.n_rows);
     }
-    const int tiles = ((hi - lo) * a.group + 127) / 128;
-    int incl = tiles;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += u;
-    }
-    const unsigned long long mine = __builtin_amdgcn_ballot_w64(at >= incl - tiles && at < incl);
-    if (mine) {
-      const int l = __builtin_ctzll(mine);
-      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-      j.base = of(lo);
-      j.len = j.count = of(hi) - j.base;
-      j.tile = of(incl) - 1 - at;  // the longest first
-      break;
-    }
-    at -= __builtin_amdgcn_readlane(incl, 63);
     end = max(end, __builtin_amdgcn_readlane(hi, min(a.n_seq - 1 - s0, 63)));
+    return ((hi - lo) * a.group + ROWS - 1) / ROWS;
+  };
+  auto take = [&](int lane_of, int tile) {
+    j.base = __builtin_amdgcn_readlane(lo, lane_of);
+    j.len = j.count = __builtin_amdgcn_readlane(hi, lane_of) - j.base;
+    j.tile = tile;
+  };
+  int at, index;  // of this tile among those not yet looked at, among all
+  if (a.n_seq <= 64) {
+    const int tiles = sequences(0), total = wave_sum(tiles), busy = total * a.n_head;
+    if (busy <= 256 * RESIDENT && block < busy && block & 256) {
+      const int row = block & ~255;
+      block = row + min(256, busy - row) - 1 - (block - row);
+    }
+    index = block / a.n_head;
+    j.head = block - index * a.n_head;
+    at = index - total;
+    if (at < 0) {
+      int before = 0;  // tiles of the sequences before this lane's
+      for (int i = 0; i < a.n_seq; ++i) {
+        const int t = __builtin_amdgcn_readlane(tiles, i);
+        before += t > tiles || (t == tiles && i < lane) ? t : 0;
+      }
+      const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(index >= before && index < before + tiles));
+      take(l, __builtin_amdgcn_readlane(before + tiles, l) - 1 - index);
+    }
+  } else {
+    index = block / a.n_head;
+    j.head = block - index * a.n_head;
+    at = index;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+      const int tiles = sequences(s0);
+      int incl = tiles;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += u;
+      }
+      const unsigned long long mine = __builtin_amdgcn_ballot_w64(at >= incl - tiles && at < incl);
+      if (mine) {
+        const int l = __builtin_ctzll(mine);
+        take(l, __builtin_amdgcn_readlane(incl, l) - 1 - at);
+        break;
+      }
+      at -= __builtin_amdgcn_readlane(incl, 63);
+    }
   }
   if (j.tile >= 0) {
     a.n_q = j.count;
-    return attend<M, HD, P, P, T, Stage>(a, j, s);
+    return attend<M, HD, P, P, T, Stage, KG>(a, j, s);
   }
   // `at` workgroups of this head are before this one among those that are left
   const int start = min(max(a.offsets[0], 0), a.n_rows), spare = start + a.n_rows - end;
   const int step = (int)(gridDim.x / a.n_head) - (index - at), per = a.group * a.hd;
   for (int r = at; r < spare; r += step) {
     const long row = r < start ? r : end + (r - start);
-    for (int c = threadIdx.x; c < per; c += 256)
-      static_cast<T*>(a.out.p)[row * a.out.tok + (long)(head * a.group + c / a.hd) * a.out.head + c % a.hd] = (T)0.f;
+    for (int c = threadIdx.x; c < per; c += Stage::NT * KG)
+      static_cast<T*>(a.out.p)[row * a.out.tok + (long)(j.head * a.group + c / a.hd) * a.out.head + c % a.hd] = (T)0.f;
   }
 }
 
 template <int QP, int PP, class T>
-void many_t(hipStream_t s, const Args& a) {
-  const dim3 grid((unsigned)(a.n_seq * a.n_head), (unsigned)((a.n_q * a.group + 127) / 128));
-  if (a.c.hdp == 64) f_attend_many_kernel<64, QP, PP, T><<<grid, 256, 0, s>>>(a);
-  else f_attend_many_kernel<128, QP, PP, T><<<grid, 256, 0, s>>>(a);
+void many_t(hipStream_t s, Args a) {
+  dim3 grid((unsigned)(a.n_seq * a.n_head), (unsigned)((a.n_q * a.group + 127) / 128));
+  const long tiles = (long)grid.x * grid.y;
+  if (tiles <= kManySplit) {
+    // eight waves a workgroup, one workgroup a compute unit; the keys are split where there are fewer
+    a.min_stages = 8;
+    grid.z = (unsigned)std::max(1l, std::min(kManySplit / tiles, ((long)a.c.tiles / 2 + a.min_stages - 1) / a.min_stages));
+    constexpr int KG = QP == 3 ? 1 : 2;  // (f32 queries of 128 columns leave registers for four)
+    if (a.c.hdp == 64) f_attend_many_kernel<64, QP, PP, T, 2><<<grid, 512, 0, s>>>(a);
+    else f_attend_many_kernel<128, QP, PP, T, KG><<<grid, 256 * KG, 0, s>>>(a);
+  } else {
+    if (a.c.hdp == 64) f_attend_many_kernel<64, QP, PP, T, 1><<<grid, 256, 0, s>>>(a);
+    else f_attend_many_kernel<128, QP, PP, T, 1><<<grid, 256, 0, s>>>(a);
+  }
 }
-template <class M, int P, class T>
+template <class M, int HD, int P, class T, class Stage, int KG, int RESIDENT>
+void packed_run(hipStream_t s, const Args& a) {
+  constexpr int ROWS = Stage::NT / 2;
+  const unsigned tiles = (unsigned)((a.n_rows * (long)a.group + ROWS - 1) / ROWS + a.n_seq);
+  packed_attend_kernel<M, HD, P, T, Stage, KG, RESIDENT><<<tiles * (unsigned)a.n_head, Stage::NT * KG, 0, s>>>(a);
+}
+template <class M, int HD, class T>
 void packed_t(hipStream_t s, const Args& a) {
-  const unsigned tiles = (unsigned)((a.n_rows * (long)a.group + 127) / 128 + a.n_seq), grid = tiles * (unsigned)a.n_head;
-  auto run = [&](auto width) {
-    constexpr int HD = decltype(width)::value;
-    if constexpr (P == 1) {
-      // (a lane's offset within a stage of 64 rows is 32 bits, unsigned)
-      auto near = [](const QRows& r) { return r.tok >= 0 && r.tok < 1 << 22; };
-      if (a.kvec && near(a.k) && near(a.v)) {
-        packed_attend_kernel<M, HD, P, T, DirectStage<M, HD>><<<grid, 256, 0, s>>>(a);
-        return;
-      }
-    }
-    packed_attend_kernel<M, HD, P, T, RowStage<M, HD, P, T>><<<grid, 256, 0, s>>>(a);
-  };
-  if (a.hd <= 64) run(std::integral_constant<int, 64>{});
-  else run(std::integral_constant<int, 128>{});
+  if constexpr (sizeof(T) == 4) {
+    // (f32 of 64 columns: eight waves, two buffers of 48 KB)
+    constexpr int NW = HD == 64 ? 8 : 4, NB = HD == 64 ? 2 : 1;
+    if (a.kvec) packed_run<M, HD, 3, T, RowStage<M, HD, 3, T, true, NW, NB>, 1, 1>(s, a);
+    else packed_run<M, HD, 3, T, RowStage<M, HD, 3, T, false, NW, NB>, 1, 1>(s, a);
+  } else {
+    // (a lane's offset within a stage of 64 rows is 32 bits, unsigned)
+    auto near = [](const QRows& r) { return r.tok >= 0 && r.tok < 1 << 22; };
+    const bool direct = a.kvec && near(a.k) && near(a.v);
+    // Where all tiles are on the device at once, the time is the longest's: two groups
+    // of waves have every second stage of its keys each.
+    const bool two = a.n_rows * (long)a.group / 128 * a.n_head <= 512;
+    if (direct && two) packed_run<M, HD, 1, T, DirectStage<M, HD, 4>, 2, 1>(s, a);
+    else if (direct) packed_run<M, HD, 1, T, DirectStage<M, HD, 4>, 1, 2>(s, a);
+    else if (two) packed_run<M, HD, 1, T, RowStage<M, HD, 1, T, false, 4, 2>, 2, 1>(s, a);
+    else packed_run<M, HD, 1, T, RowStage<M, HD, 1, T, false, 4, 2>, 1, 2>(s, a);
+  }
+}
+template <class M, class T>
+void packed(hipStream_t s, const Args& a) {
+  if (a.hd <= 64) packed_t<M, 64, T>(s, a);
+  else packed_t<M, 128, T>(s, a);
 }
 
 }  // namespace
 
-void launch_f_attend_many(hipStream_t s, const FAttn& f) {
+size_t fmany_tickets_bytes() { return (size_t)kManySplit * kQTicketStride * 4; }
+size_t fmany_work_bytes(int hdp) {
+  return fmany_tickets_bytes() + (size_t)kManySplit * 4 * (hdp / 2 + 4) * 64 * 4;
+}
+
+void launch_f_attend_many(hipStream_t s, const FAttn& f, void* work) {
   Args a = {};
+  a.tickets = static_cast<unsigned*>(work);
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(work) + fmany_tickets_bytes());
   a.q = f.q;
   a.out = f.out;
   a.c = f.c;
@@ -712,9 +889,9 @@ void launch_packed_attend(hipStream_t s, const PAttn& p) {
   a.qvec = by_eights(p.q, a.hd, p.type);
   a.kvec = by_eights(p.k, a.hd, p.type) && by_eights(p.v, a.hd, p.type);
   a.ovec = by_eights(p.out, a.hd, p.type);
-  if (p.type == Q_F32) packed_t<Bf16, 3, float>(s, a);
-  else if (p.type == Q_BF16) packed_t<Bf16, 1, __bf16>(s, a);
-  else packed_t<F16, 1, _Float16>(s, a);
+  if (p.type == Q_F32) packed<Bf16, float>(s, a);
+  else if (p.type == Q_BF16) packed<Bf16, __bf16>(s, a);
+  else packed<F16, _Float16>(s, a);
 }
 
 }  // namespace rtg

@@ -79,7 +79,10 @@ struct FAttn {
   void* work = nullptr;
 };
 void launch_f_attend(hipStream_t s, const FAttn& a);
-void launch_f_attend_many(hipStream_t s, const FAttn& a);  // (launch_f_attend chooses it)
+// for many queries (launch_f_attend chooses), and its part of the workspace
+void launch_f_attend_many(hipStream_t s, const FAttn& a, void* work);
+size_t fmany_work_bytes(int hdp);
+size_t fmany_tickets_bytes();
 // w = decay * w + the probabilities that the queries (as in launch_f_attend, whose
 // stats it takes) give a token, summed over the counted queries and the heads of
 // the token's head; decay 0: w as it was is not read.

@@ -191,18 +191,6 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int seq) {
   return r;
 }
 
-// Two neighbouring floats of a partial, past the L2 caches (workgroups of other
-// XCDs read them).
-__device__ __forceinline__ void store2(float* p, float x, float y) {
-  const unsigned long long v = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
-  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 load2(const float* p) {
-  const unsigned long long v = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED,
-                                                 __HIP_MEMORY_SCOPE_AGENT);
-  return make_float2(__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32)));
-}
-
 template <int HDP>
 struct Shared {
   float m[kWaves][kCols], l[kWaves][kCols];
@@ -489,15 +477,18 @@ void weigh_t(hipStream_t s, const FAttn& f, float decay) {
 
 }  // namespace
 
-size_t fattn_work_bytes(int hdp) {
-  return (size_t)kMostSplit * (kQTicketStride * 4 + (size_t)kCols * (hdp + 2) * 4);
-}
-void fattn_work_clear(hipStream_t s, void* work, int) {
+namespace {
+size_t few_work_bytes(int hdp) { return (size_t)kMostSplit * (kQTicketStride * 4 + (size_t)kCols * (hdp + 2) * 4); }
+}  // namespace
+// (one call at a time: both kernels' partial results lie in the same memory, their tickets apart)
+size_t fattn_work_bytes(int hdp) { return few_work_bytes(hdp) + fmany_work_bytes(hdp); }
+void fattn_work_clear(hipStream_t s, void* work, int hdp) {
   (void)hipMemsetAsync(work, 0, (size_t)kMostSplit * kQTicketStride * 4, s);
+  (void)hipMemsetAsync(static_cast<char*>(work) + few_work_bytes(hdp), 0, fmany_tickets_bytes(), s);
 }
 
 void launch_f_attend(hipStream_t s, const FAttn& f) {
-  if (f.n_q * (f.n_q_head / f.c.n_head) > 128) return launch_f_attend_many(s, f);
+  if (f.n_q * (f.n_q_head / f.c.n_head) > 128) return launch_f_attend_many(s, f, static_cast<char*>(f.work) + few_work_bytes(f.c.hdp));
   if (f.type == Q_F32) attend_t<3, 3, float>(s, f);
   else if (f.type == Q_BF16) attend_t<1, 2, __bf16>(s, f);
   else attend_t<2, 2, _Float16>(s, f);

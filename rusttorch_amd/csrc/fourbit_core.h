@@ -116,6 +116,18 @@ inline ScoreScale score_scale(float scale) {
   return {copysignf(ldexpf(1.f, in), scale), (float)ldexp(m, e - in)};
 }
 
+// Two neighbouring floats of a partial, past the L2 caches (workgroups of other
+// XCDs read them).
+__device__ __forceinline__ void store2(float* p, float x, float y) {
+  const unsigned long long v = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load2(const float* p) {
+  const unsigned long long v = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32)));
+}
+
 // Query i of a sequence of len tokens, the last `count` of which ask: keys it sees.
 __device__ __forceinline__ int keys_seen(int len, int count, int i) { return i < count ? max(len - count + i + 1, 0) : 0; }
 

@@ -180,6 +180,8 @@ def test_long_sequences_are_split(dim, dtype):
     b.append(1)
     b.attend(5, 2)
     b.attend(80, 1)
+    b.attend(150, 2, counts=[150, 3])
+    b.attend(70, 4, counts=[0, 70], weigh=1.0)
 
 
 def test_rows_in_any_strides():
