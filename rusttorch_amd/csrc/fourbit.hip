@@ -120,34 +120,56 @@ __global__ __launch_bounds__(256) void f_append_kernel(FStore c, int* len, QTick
   const unsigned per_head = (unsigned)((n + 64 / U - 1) / (64 / U));  // waves' worth of units of a head
   unsigned at = blockIdx.y * 4 + (tid >> 6);
   int head = 0;
-  while (n > 0) {
-    head += (int)(at / per_head);
+  const int c8 = tid % U * 8;
+  // A wave's next unit: its head (n_head behind the last) and the row of this lane's.
+  auto next = [&](int& h, int& row) {
+    if (per_head == 0) {
+      h = c.n_head;
+      return;
+    }
+    head = min(head + (int)(at / per_head), c.n_head);
     at %= per_head;
-    if (head >= c.n_head) break;
-    const int row = (int)at * (64 / U) + (tid & 63) / U, i = min(row, n - 1), c8 = tid % U * 8;
+    h = head;
+    row = (int)at * (64 / U) + (tid & 63) / U;
     at += gridDim.y * 4;
-    float x[8], y[8];
-    load8(static_cast<const T*>(k.p) + seq * k.seq + i * k.tok + head * k.head, c8, c.hd, vec, x);
-    load8(static_cast<const T*>(v.p) + seq * v.seq + i * v.tok + head * v.head, c8, c.hd, vec, y);
-    unsigned kb, vb;
-    const unsigned kw = encode8(x, &kb), vw = encode8(y, &vb);
-    if (row >= n) continue;
-    const size_t sh = (size_t)seq * c.n_head + head;
-    const int t = p.at + i, tile = t / kFTile, tok = t % kFTile;
-    uint8_t *kt = c.k + c.codes(sh) + (size_t)tile * 16 * HDP, *vt = c.v + c.codes(sh) + (size_t)tile * 16 * HDP;
-    *reinterpret_cast<unsigned*>(kt + At<HDP>::k(tok, c8)) = kw;
-    if constexpr (HDP == 128) {
-      *reinterpret_cast<unsigned*>(vt + At<HDP>::v(tok, c8 / 8)) = vw;
-    } else {
-      *reinterpret_cast<uint16_t*>(vt + At<HDP>::v(tok, c8 / 4)) = (uint16_t)vw;
-      *reinterpret_cast<uint16_t*>(vt + At<HDP>::v(tok, c8 / 4 + 1)) = (uint16_t)(vw >> 16);
+  };
+  constexpr int AHEAD = 4;  // loads of so many units are in flight together
+  for (;;) {
+    float x[AHEAD][8], y[AHEAD][8];
+    int h[AHEAD], row[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      row[u] = 0;
+      next(h[u], row[u]);
+      if (h[u] >= c.n_head) continue;
+      const int i = min(row[u], n - 1);
+      load8(static_cast<const T*>(k.p) + seq * k.seq + i * k.tok + h[u] * k.head, c8, c.hd, vec, x[u]);
+      load8(static_cast<const T*>(v.p) + seq * v.seq + i * v.tok + h[u] * v.head, c8, c.hd, vec, y[u]);
     }
-    if (c8 % 32 == 0) {
-      const size_t st = c.scales(sh) + (size_t)tile * HDP;
-      c.sk[st + At<HDP>::k_scale(tok, c8 / 32)] = (uint8_t)kb;
-      c.sv[st + At<HDP>::v_scale(tok, c8 / 32)] = (uint8_t)vb;
-      if (c8 == 0) c.w[c.weights(sh) + t] = 0.f;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (h[u] >= c.n_head) break;
+      unsigned kb, vb;
+      const unsigned kw = encode8(x[u], &kb), vw = encode8(y[u], &vb);
+      if (row[u] >= n) continue;
+      const size_t sh = (size_t)seq * c.n_head + h[u];
+      const int t = p.at + row[u], tile = t / kFTile, tok = t % kFTile;
+      uint8_t *kt = c.k + c.codes(sh) + (size_t)tile * 16 * HDP, *vt = c.v + c.codes(sh) + (size_t)tile * 16 * HDP;
+      *reinterpret_cast<unsigned*>(kt + At<HDP>::k(tok, c8)) = kw;
+      if constexpr (HDP == 128) {
+        *reinterpret_cast<unsigned*>(vt + At<HDP>::v(tok, c8 / 8)) = vw;
+      } else {
+        *reinterpret_cast<uint16_t*>(vt + At<HDP>::v(tok, c8 / 4)) = (uint16_t)vw;
+        *reinterpret_cast<uint16_t*>(vt + At<HDP>::v(tok, c8 / 4 + 1)) = (uint16_t)(vw >> 16);
+      }
+      if (c8 % 32 == 0) {
+        const size_t st = c.scales(sh) + (size_t)tile * HDP;
+        c.sk[st + At<HDP>::k_scale(tok, c8 / 32)] = (uint8_t)kb;
+        c.sv[st + At<HDP>::v_scale(tok, c8 / 32)] = (uint8_t)vb;
+        if (c8 == 0) c.w[c.weights(sh) + t] = 0.f;
+      }
     }
+    if (h[AHEAD - 1] >= c.n_head) break;
   }
   if (readers.last(gridDim.y)) {
     if (p.bad) atomicMin(tickets.err, (unsigned)seq * 4 + p.bad);
@@ -212,6 +234,7 @@ __global__ __launch_bounds__(256) void f_add_weights_kernel(FStore c, const int*
 // ---- eviction ----
 
 constexpr int kPickWaves = 16;
+constexpr int kPickHeld = 24 * 1024;  // weights that stay in LDS between the passes
 
 // Weights in the order in which they are kept: larger is later. -0 and 0 are the
 // same; NaN is larger than infinity.
@@ -224,11 +247,17 @@ __device__ __forceinline__ unsigned pick_key(float x) {
 // One workgroup per (sequence, head) finds the key of the last token to be kept,
 // eight bits at a time, and how many of those that have just this key; then each
 // wave lists what is kept of its stretch of the sequence, behind what the waves
-// before it keep.
+// before it keep. The first pass takes the weights to LDS, eight loads of a thread
+// at a time; longer sequences' are read from memory in every pass (20000 tokens of
+// 32 heads: 30 us that way, XX from LDS).
 __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const int* len, int keep, int recent,
                                                                 int* kept) {
-  constexpr int NT = 64 * kPickWaves, COPIES = 16;
-  __shared__ unsigned hist[COPIES][257];  // (copies: lanes that count the same bin take turns)
+  constexpr int NT = 64 * kPickWaves, AHEAD = 8;
+  // A copy for each lane (lanes that count the same bin would take turns, and most
+  // weights share a few), two bins to a word: a copy counts 4000000 / 64 at most.
+  __shared__ unsigned hist[64][129];
+  __shared__ unsigned totals[256];
+  __shared__ unsigned held[kPickHeld];
   __shared__ unsigned found[2];
   __shared__ int above[kPickWaves], equal[kPickWaves];
   const size_t sh = blockIdx.x;
@@ -240,21 +269,56 @@ __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const
   }
   const float* w = c.w + c.weights(sh);
   const int old = l - recent, some = keep - recent;  // `some` of the `old` first ones; the others are kept
+  const bool inside = old <= kPickHeld;
+  auto key_of = [&](int t) { return inside ? held[t] : pick_key(w[t]); };
+  auto count = [&](unsigned key, int shift) {
+    const unsigned bin = (key >> shift) & 255;
+    atomicAdd(&hist[lane][bin >> 1], 1u << (16 * (bin & 1)));
+  };
   unsigned top = 0, left = (unsigned)some;  // the key's bits so far; how many of those with these bits are kept
   for (int shift = 24; shift >= 0 && some > 0; shift -= 8) {
-    for (int j = tid; j < COPIES * 257; j += NT) (&hist[0][0])[j] = 0;
+    for (int j = tid; j < 64 * 129; j += NT) (&hist[0][0])[j] = 0;
+    if (tid < 256) totals[tid] = 0;
     __syncthreads();
-    for (int t = tid; t < old; t += NT) {
-      const unsigned key = pick_key(w[t]);
-      if (shift == 24 || key >> (shift + 8) == top >> (shift + 8)) atomicAdd(&hist[lane & (COPIES - 1)][(key >> shift) & 255], 1u);
+    if (shift == 24) {
+      for (int t0 = tid; t0 < old; t0 += AHEAD * NT) {
+        float x[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) x[u] = t0 + u * NT < old ? w[t0 + u * NT] : 0.f;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int t = t0 + u * NT;
+          if (t >= old) break;
+          const unsigned key = pick_key(x[u]);
+          if (inside) held[t] = key;
+          count(key, shift);
+        }
+      }
+    } else {
+      for (int t = tid; t < old; t += NT) {
+        const unsigned key = key_of(t);
+        if (key >> (shift + 8) == top >> (shift + 8)) count(key, shift);
+      }
+    }
+    __syncthreads();
+    {
+      const int word = tid & 127, part = tid >> 7;  // eight copies of two bins
+      unsigned low = 0, high = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const unsigned x = hist[part * 8 + k][word];
+        low += x & 0xFFFFu;
+        high += x >> 16;
+      }
+      if (low) atomicAdd(&totals[2 * word], low);
+      if (high) atomicAdd(&totals[2 * word + 1], high);
     }
     __syncthreads();
     if (wave == 0) {
       unsigned n[4], sum = 0;  // bins 255 - 4 lane - i, from the top
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        n[i] = 0;
-        for (int k = 0; k < COPIES; ++k) n[i] += hist[k][255 - 4 * lane - i];
+        n[i] = totals[255 - 4 * lane - i];
         sum += n[i];
       }
       unsigned incl = sum;
@@ -284,7 +348,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const
   if (some > 0) {
     int a = 0, e = 0;
     for (int t = lo + lane; t < hi; t += 64) {
-      const unsigned key = pick_key(w[t]);
+      const unsigned key = key_of(t);
       a += key > top;
       e += key == top;
     }
@@ -306,7 +370,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const
     at += min(ties, (int)left);
     for (int t0 = lo; t0 < hi; t0 += 64) {
       const int t = t0 + lane;
-      const unsigned key = t < hi ? pick_key(w[t]) : 0;
+      const unsigned key = t < hi ? key_of(t) : 0;
       const bool tie = t < hi && key == top;
       const unsigned long long eq = __ballot(tie), below = (1ull << lane) - 1;
       const bool take = t < hi && (key > top || (tie && ties + __popcll(eq & below) < (int)left));
@@ -319,60 +383,87 @@ __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const
   for (int j = tid; j < recent; j += NT) to[some + j] = old + j;
 }
 
-// Moves what is kept to the front, in place. A workgroup goes over the kept
-// tokens in order, STEP at a time: all of them are read before any is written
-// (all_have_read), and those of later steps lie behind everything that is written
-// by then, since token j of the kept ones was never before j. Two workgroups have
-// half of the keys' bytes each, two of the values'.
-__device__ __forceinline__ void all_have_read() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-}
+// A thread's part of a token that is moved: 16 channels of a key, or one lane's of a value.
 template <int HDP>
-__device__ __forceinline__ void move_keys(const FStore& c, size_t sh, int half, int keep, const int* from) {
-  // a thread has 16 channels of a token
-  constexpr int U = HDP / 32, STEP = 256 / U;
-  uint8_t *codes = c.k + c.codes(sh), *scales = c.sk + c.scales(sh);
-  float* w = c.w + c.weights(sh);
-  const int c16 = (half * U + (int)threadIdx.x % U) * 16;
-  const bool scaled = c16 % 32 == 0;
-  for (int j0 = 0; j0 < keep; j0 += STEP) {
-    const int j = j0 + (int)threadIdx.x / U, t = from[min(j, keep - 1)], tile = t / kFTile, tok = t % kFTile;
-    const uint2 x = *reinterpret_cast<const uint2*>(codes + (size_t)tile * 16 * HDP + At<HDP>::k(tok, c16));
-    const uint8_t s = scaled ? scales[(size_t)tile * HDP + At<HDP>::k_scale(tok, c16 / 32)] : 0;
-    const float weight = c16 == 0 ? w[t] : 0.f;
-    all_have_read();
-    if (j >= keep) break;
-    const int to = j / kFTile, tj = j % kFTile;
-    *reinterpret_cast<uint2*>(codes + (size_t)to * 16 * HDP + At<HDP>::k(tj, c16)) = x;
-    if (scaled) scales[(size_t)to * HDP + At<HDP>::k_scale(tj, c16 / 32)] = s;
-    if (c16 == 0) w[j] = weight;
+struct KeyPiece {
+  static constexpr int U = HDP / 32;  // pieces of a token in a half
+  uint2 x;
+  uint8_t s;
+  float w;
+  static __device__ __forceinline__ int channel(int half, int p) { return (half * U + p) * 16; }
+  __device__ __forceinline__ void read(const FStore& c, size_t sh, int t, int ch) {
+    x = *reinterpret_cast<const uint2*>(c.k + c.codes(sh) + (size_t)(t / kFTile) * 16 * HDP + At<HDP>::k(t % kFTile, ch));
+    if (ch % 32 == 0) s = c.sk[c.scales(sh) + (size_t)(t / kFTile) * HDP + At<HDP>::k_scale(t % kFTile, ch / 32)];
+    if (ch == 0) w = c.w[c.weights(sh) + t];
   }
-}
+  __device__ __forceinline__ void write(const FStore& c, size_t sh, int t, int ch) const {
+    *reinterpret_cast<uint2*>(c.k + c.codes(sh) + (size_t)(t / kFTile) * 16 * HDP + At<HDP>::k(t % kFTile, ch)) = x;
+    if (ch % 32 == 0) c.sk[c.scales(sh) + (size_t)(t / kFTile) * HDP + At<HDP>::k_scale(t % kFTile, ch / 32)] = s;
+    if (ch == 0) c.w[c.weights(sh) + t] = w;
+  }
+};
 template <int HDP>
-__device__ __forceinline__ void move_values(const FStore& c, size_t sh, int half, int keep, const int* from) {
-  // a thread has one lane's part of a token
-  constexpr int STEP = 256 / 8;
-  uint8_t *codes = c.v + c.codes(sh), *scales = c.sv + c.scales(sh);
-  const int m = half * 8 + (int)threadIdx.x % 8, channel = m * (HDP / 16);
-  const bool scaled = channel % 32 == 0;
+struct ValuePiece {
+  static constexpr int U = 8, CV = HDP / 16;
+  unsigned x;
+  uint8_t s;
+  static __device__ __forceinline__ int channel(int half, int p) { return (half * U + p) * CV; }
+  __device__ __forceinline__ void read(const FStore& c, size_t sh, int t, int ch) {
+    const uint8_t* p = c.v + c.codes(sh) + (size_t)(t / kFTile) * 16 * HDP + At<HDP>::v(t % kFTile, ch / CV);
+    x = HDP == 128 ? *reinterpret_cast<const unsigned*>(p) : *reinterpret_cast<const uint16_t*>(p);
+    if (ch % 32 == 0) s = c.sv[c.scales(sh) + (size_t)(t / kFTile) * HDP + At<HDP>::v_scale(t % kFTile, ch / 32)];
+  }
+  __device__ __forceinline__ void write(const FStore& c, size_t sh, int t, int ch) const {
+    uint8_t* p = c.v + c.codes(sh) + (size_t)(t / kFTile) * 16 * HDP + At<HDP>::v(t % kFTile, ch / CV);
+    if (HDP == 128) *reinterpret_cast<unsigned*>(p) = x;
+    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)x;
+    if (ch % 32 == 0) c.sv[c.scales(sh) + (size_t)(t / kFTile) * HDP + At<HDP>::v_scale(t % kFTile, ch / 32)] = s;
+  }
+};
+
+// Moves what is kept to the front, in place, in order, STEP tokens at a time: all
+// of a step's are read before any is written (the wait and the barrier), and those
+// of later steps lie behind everything that is written by then, since token j of
+// the kept ones was never before j; so the next step is read meanwhile, and which
+// tokens the one after it has (32 heads' 2048 of 20000: 53 us without, XX with).
+// Two workgroups have half of the keys' bytes each, two of the values'.
+constexpr int kMoveThreads = 1024;
+
+template <class Piece>
+__device__ __forceinline__ void move(const FStore& c, size_t sh, int half, int keep, const int* from) {
+  constexpr int UN = 4, ROWS = kMoveThreads / Piece::U, STEP = UN * ROWS;
+  const int r = (int)threadIdx.x / Piece::U, ch = Piece::channel(half, (int)threadIdx.x % Piece::U);
+  Piece x[UN];
+  int at[UN];
+  auto which = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u) at[u] = from[min(j0 + u * ROWS + r, keep - 1)];
+  };
+  auto read = [&](Piece (&p)[UN]) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u) p[u].read(c, sh, at[u], ch);
+  };
+  which(0);
+  read(x);
+  which(STEP);
   for (int j0 = 0; j0 < keep; j0 += STEP) {
-    const int j = j0 + (int)threadIdx.x / 8, t = from[min(j, keep - 1)], tile = t / kFTile, tok = t % kFTile;
-    const uint8_t* p = codes + (size_t)tile * 16 * HDP + At<HDP>::v(tok, m);
-    const unsigned x = HDP == 128 ? *reinterpret_cast<const unsigned*>(p) : *reinterpret_cast<const uint16_t*>(p);
-    const uint8_t s = scaled ? scales[(size_t)tile * HDP + At<HDP>::v_scale(tok, channel / 32)] : 0;
-    all_have_read();
-    if (j >= keep) break;
-    const int to = j / kFTile, tj = j % kFTile;
-    uint8_t* o = codes + (size_t)to * 16 * HDP + At<HDP>::v(tj, m);
-    if (HDP == 128) *reinterpret_cast<unsigned*>(o) = x;
-    else *reinterpret_cast<uint16_t*>(o) = (uint16_t)x;
-    if (scaled) scales[(size_t)to * HDP + At<HDP>::v_scale(tj, channel / 32)] = s;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    Piece y[UN];
+    read(y);  // (behind the last step: the last token once more)
+    which(j0 + 2 * STEP);
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int j = j0 + u * ROWS + r;
+      if (j < keep) x[u].write(c, sh, j, ch);
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) x[u] = y[u];
   }
 }
 
 template <int HDP>
-__global__ __launch_bounds__(256) void f_move_kernel(FStore c, int* len, QTickets tickets, int keep, const int* kept) {
+__global__ __launch_bounds__(kMoveThreads) void f_move_kernel(FStore c, int* len, QTickets tickets, int keep, const int* kept) {
   __shared__ int length;
   const size_t sh = blockIdx.x / 4;
   const int seq = (int)(sh / c.n_head), part = blockIdx.x % 4;
@@ -382,18 +473,21 @@ __global__ __launch_bounds__(256) void f_move_kernel(FStore c, int* len, QTicket
   Readers readers;
   readers.read(tickets, seq);
   if (l > keep) {
-    if (part < 2) move_keys<HDP>(c, sh, part, keep, kept + sh * keep);
-    else move_values<HDP>(c, sh, part - 2, keep, kept + sh * keep);
+    if (part < 2) move<KeyPiece<HDP>>(c, sh, part, keep, kept + sh * keep);
+    else move<ValuePiece<HDP>>(c, sh, part - 2, keep, kept + sh * keep);
   }
   if (readers.last((unsigned)c.n_head * 4) && l > keep) len[seq] = keep;
 }
 
+constexpr long kAppendGroups = 1024;  // (2048: 4 x 20000 tokens 79 us instead of 81, 1 x 20000 40 instead of 34)
+
 template <class T>
 void append_t(hipStream_t s, const FStore& c, int* len, QTickets tickets, const QRows& k, const QRows& v, int n_new,
               const int* counts, const int* start, bool vec) {
-  // units of 256 threads; at most 64 workgroups of a sequence count themselves on one word
-  const long units = ((long)n_new * (c.hdp / 8) + 63) / 64 * 64 * c.n_head;
-  const dim3 grid((unsigned)c.n_seq, (unsigned)std::max(1l, std::min(64l, (units + 255) / 256)));
+  // Units of 256 threads; enough workgroups to fill the device, but few of a
+  // sequence's, which count themselves on one word (8.6 ns each).
+  const long units = (((long)n_new * (c.hdp / 8) + 63) / 64 * c.n_head + 3) / 4, most = std::max(64l, kAppendGroups / c.n_seq);
+  const dim3 grid((unsigned)c.n_seq, (unsigned)std::max(1l, std::min(most, units)));
   if (c.hdp == 64) f_append_kernel<64, T><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start, vec);
   else f_append_kernel<128, T><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start, vec);
 }
@@ -436,8 +530,8 @@ void launch_f_add_weights(hipStream_t s, const FStore& c, const int* len, const 
 void launch_f_evict(hipStream_t s, const FStore& c, int* len, QTickets tickets, int keep, int recent, int* kept) {
   f_pick_kernel<<<(unsigned)(c.n_seq * c.n_head), 64 * kPickWaves, 0, s>>>(c, len, keep, recent, kept);
   const unsigned grid = (unsigned)(c.n_seq * c.n_head) * 4;
-  if (c.hdp == 64) f_move_kernel<64><<<grid, 256, 0, s>>>(c, len, tickets, keep, kept);
-  else f_move_kernel<128><<<grid, 256, 0, s>>>(c, len, tickets, keep, kept);
+  if (c.hdp == 64) f_move_kernel<64><<<grid, kMoveThreads, 0, s>>>(c, len, tickets, keep, kept);
+  else f_move_kernel<128><<<grid, kMoveThreads, 0, s>>>(c, len, tickets, keep, kept);
 }
 
 }  // namespace rtg

@@ -94,15 +94,17 @@ struct Keys {
     s[0] = sk[at];
     s[1] = sk[HDP / 2 + at];
   }
+  // operand j of tokens b * 16 + m
+  __device__ __forceinline__ u4v eight(int b, int j) const {
+    return eight_bf16(HDP == 128 ? c[HDP == 128 ? b : 0][j] : c[0][b * 2 + (j & 1)], scale_of(s[b]));
+  }
   // scores of tokens b * 16 + 4 g + i
   template <int QP>
   __device__ __forceinline__ f32x4 scores(int b, const u4v (&q)[J][QP]) const {
     f32x4 r = {0.f, 0.f, 0.f, 0.f};
-    const float scale = scale_of(s[b]);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const unsigned w = HDP == 128 ? c[HDP == 128 ? b : 0][j] : c[0][b * 2 + (j & 1)];
-      const u4v k = eight_bf16(w, scale);
+      const u4v k = eight(b, j);
 #pragma unroll
       for (int p = 0; p < QP; ++p) r = mfma16(k, q[j][p], r);
     }
@@ -387,48 +389,94 @@ __global__ __launch_bounds__(256) void f_attend_kernel(Args a) {
 
 // ---- weights ----
 
-// A wave takes a tile of 32 tokens and goes over the blocks of 16 columns: the
-// scores once more, and the sum of their exponentials over the columns' sums. Nothing but the keys is read, and each token's
-// weight has one owner: no atomics, and sums in a fixed order.
+// A workgroup takes some of a head's tiles, a wave every fourth of them, and goes
+// over the columns: the scores once more, and the sum of their exponentials over
+// the columns' sums. Nothing but the keys is read, and each token's weight has one
+// owner: no atomics, and sums in a fixed order. The queries lie in LDS as matrix
+// operands, as many columns at a time as fit; a wave's next tile is loaded while it
+// works on one (one token of 32 heads of 128 over 8 x 16000 in f16: 36 us with a
+// tile or four to a wave and queries from memory, XX so).
+constexpr int kWeighBytes = 32 * 1024;  // of queries in LDS
+
+template <int HDP, int QP>
+struct Weigh {
+  static constexpr int J = HDP / 32, BLOCKS = kWeighBytes / (J * QP * 64 * 16) < 1 ? 1 : kWeighBytes / (J * QP * 64 * 16);
+  u4v q[BLOCKS][J][QP][64];
+  float2 st[BLOCKS][kCols];  // a column's m, and one over its sum
+  int lim[BLOCKS][kCols];    // the keys that it sees
+};
+
 template <int HDP, int QP, class T>
 __global__ __launch_bounds__(256) void f_weigh_kernel(Args a, float decay) {
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int tile = (int)blockIdx.y * kWaves + (int)(threadIdx.x >> 6);
+  typedef Weigh<HDP, QP> W;
+  __shared__ W s;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head;
   const Seq r = seq_of(a, seq);
-  const int at = tile * kFTile;
-  if (at >= r.len) return;
-  Keys<HDP> k;
-  k.load(a.c.k + a.c.codes(sh) + (size_t)tile * 16 * HDP, a.c.sk + a.c.scales(sh) + (size_t)tile * HDP, lane);
-  float sum[8] = {};
+  const int tiles = (r.len + kFTile - 1) / kFTile, step = (int)gridDim.y * kWaves;
+  if ((int)blockIdx.y * kWaves >= tiles) return;
   const int cblocks = (r.count * a.group + kCols - 1) / kCols;
-  for (int cb = 0; cb < cblocks; ++cb) {
-    const Column cl = column(a, cb * kCols + n);
-    const int lim = keys_seen(r.len, r.count, cl.i);
-    Query<HDP, QP, T> q;
-    q.load(a, seq, head, cl, g);
-    const float2 st = stats_of(a, seq, min(cl.i, a.n_q - 1), head * a.group + cl.h);
-    const float inv = 1.f / st.y;
+  const uint8_t *kc = a.c.k + a.c.codes(sh), *ks = a.c.sk + a.c.scales(sh);
+  float* w = a.c.w + a.c.weights(sh);
+  for (int cb0 = 0; cb0 == 0 || cb0 < cblocks; cb0 += W::BLOCKS) {
+    const int blocks = min(W::BLOCKS, cblocks - cb0);
+    if (cb0 > 0) __syncthreads();
+    for (int b = wave; b < blocks; b += kWaves) {
+      const Column cl = column(a, (cb0 + b) * kCols + n);
+      Query<HDP, QP, T> q;
+      q.load(a, seq, head, cl, g);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const f32x4 x = k.scores(b, q.q);
+      for (int j = 0; j < W::J; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(x[i], a.sum, -st.x)) * inv;
-        sum[b * 4 + i] += at + b * 16 + 4 * g + i < lim ? p : 0.f;
+        for (int p = 0; p < QP; ++p) s.q[b][j][p][lane] = q.q[j][p];
+      if (g == 0) {
+        const float2 st = stats_of(a, seq, min(cl.i, a.n_q - 1), head * a.group + cl.h);
+        s.st[b][n] = make_float2(st.x, 1.f / st.y);
+        s.lim[b][n] = keys_seen(r.len, r.count, cl.i);
       }
     }
-  }
+    __syncthreads();
+    int t = (int)blockIdx.y * kWaves + wave;
+    Keys<HDP> next;
+    if (t < tiles) next.load(kc + (size_t)t * 16 * HDP, ks + (size_t)t * HDP, lane);
+    for (; t < tiles; t += step) {
+      const Keys<HDP> k = next;
+      if (t + step < tiles) next.load(kc + (size_t)(t + step) * 16 * HDP, ks + (size_t)(t + step) * HDP, lane);
+      const int at = t * kFTile;
+      float sum[8] = {};
+      for (int b = 0; b < blocks; ++b) {
+        f32x4 x[2] = {};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sum[e] = row16_sum_k(sum[e]);
-  // lane n of the 16 that hold the sums writes one of the eight
-  float mine = sum[0];
+        for (int j = 0; j < W::J; ++j) {
+          const u4v k0 = k.eight(0, j), k1 = k.eight(1, j);
 #pragma unroll
-  for (int e = 1; e < 8; ++e) mine = (n & 7) == e ? sum[e] : mine;
-  const int t = at + (n & 7) / 4 * 16 + 4 * g + (n & 3);
-  if (n < 8 && t < r.len) {
-    float* w = a.c.w + a.c.weights(sh) + t;
-    *w = decay == 0.f ? mine : fmaf(decay, *w, mine);
+          for (int p = 0; p < QP; ++p) {
+            const u4v q = s.q[b][j][p][lane];
+            x[0] = mfma16(k0, q, x[0]);
+            x[1] = mfma16(k1, q, x[1]);
+          }
+        }
+        const float2 st = s.st[b][n];
+        const int lim = s.lim[b][n] - at;  // (of the tile's tokens, in this column)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(x[e / 4][e % 4], a.sum, -st.x)) * st.y;
+          sum[e] += e / 4 * 16 + 4 * g + e % 4 < lim ? p : 0.f;
+        }
+      }
+      // lane n of the 16 that hold the sums writes one of the eight
+      float mine = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = row16_sum_k(sum[e]);
+        mine = (n & 7) == e ? y : mine;
+      }
+      const int tok = at + (n & 7) / 4 * 16 + 4 * g + (n & 3);
+      if (n < 8 && tok < r.len) {
+        const float before = cb0 > 0 ? 1.f : decay;
+        w[tok] = before == 0.f ? mine : fmaf(before, w[tok], mine);
+      }
+    }
   }
 }
 
@@ -470,7 +518,9 @@ void attend_t(hipStream_t s, const FAttn& f) {
 template <int QP, class T>
 void weigh_t(hipStream_t s, const FAttn& f, float decay) {
   const Args a = args_of(f);
-  const dim3 grid((unsigned)(f.c.n_seq * f.c.n_head), (unsigned)((f.c.tiles + kWaves - 1) / kWaves));
+  // as many workgroups as the device takes at once
+  const long sh = (long)f.c.n_seq * f.c.n_head, most = std::max(1l, 1024 / sh);
+  const dim3 grid((unsigned)sh, (unsigned)std::min(most, (long)(f.c.tiles + kWaves - 1) / kWaves));
   if (f.c.hdp == 64) f_weigh_kernel<64, QP, T><<<grid, 256, 0, s>>>(a, decay);
   else f_weigh_kernel<128, QP, T><<<grid, 256, 0, s>>>(a, decay);
 }
