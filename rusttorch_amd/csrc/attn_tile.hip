@@ -478,9 +478,15 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       fetch(next, b);
     }
     if (edge && at >= mine) return;  // (no row of this wave sees one of these keys)
+    const bool short_of = edge && at + 32 >= mine;  // the second 32 keys are seen by no row of this wave
     float p[2][16];  // keys at + sub * 32 + e / 4 * 8 + half * 4 + e % 4
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
+      if (sub == 1 && short_of) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[1][e] = -INFINITY;
+        break;
+      }
       f32x16 x = {};
 #pragma unroll
       for (int k = 0; k < KS; ++k)
@@ -526,7 +532,8 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       for (int e = 0; e < 32; ++e) l_whole += p[e / 16][e % 16];
     }
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
+    for (int sub = 0; sub < 2; ++sub) {
+      if (sub == 1 && short_of) break;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         // keys sub * 32 + u * 16 + e / 4 * 8 + half * 4 + e % 4, e < 8
@@ -558,6 +565,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
               if (kp + k < 3) o[d] = M::mfma(f, pp[k], o[d]);
           }
       }
+    }
     reads_ahead<8 * DT * KP, 8, 2, KP == 1 ? PP : 2>();
   };
   int at = begin;
@@ -808,18 +816,23 @@ void packed_run(hipStream_t s, const Args& a) {
 }
 template <class M, int HD, class T>
 void packed_t(hipStream_t s, const Args& a) {
+  // Where all tiles are on the device at once, the time is that of the tile with most
+  // keys: two groups of waves have every second stage of its keys each, if it has many
+  // of them (4001 tokens of 12 heads of 64 in f32: 171 us, 198 with one group; of 16
+  // in f16: 52 and 58; 16 x up to 1023 of 20 in f32: 191 and 161).
+  const bool two = a.n_rows * (long)a.group / 128 * a.n_head <= 512 && a.n_rows >= 512L * a.n_seq;
   if constexpr (sizeof(T) == 4) {
-    // (f32 of 64 columns: eight waves, two buffers of 48 KB)
-    constexpr int NW = HD == 64 ? 8 : 4, NB = HD == 64 ? 2 : 1;
-    if (a.kvec) packed_run<M, HD, 3, T, RowStage<M, HD, 3, T, true, NW, NB>, 1, 1>(s, a);
-    else packed_run<M, HD, 3, T, RowStage<M, HD, 3, T, false, NW, NB>, 1, 1>(s, a);
+    // (one buffer: with two, 64 columns take 96 KB, which leaves a compute unit one
+    // workgroup, of four waves or eight; 128 columns do so in any case)
+    constexpr int KG = HD == 64 ? 2 : 1, RES = HD == 64 ? 2 : 1;
+    if (a.kvec && two) packed_run<M, HD, 3, T, RowStage<M, HD, 3, T, true, 4, 1>, KG, 1>(s, a);
+    else if (a.kvec) packed_run<M, HD, 3, T, RowStage<M, HD, 3, T, true, 4, 1>, 1, RES>(s, a);
+    else if (two) packed_run<M, HD, 3, T, RowStage<M, HD, 3, T, false, 4, 1>, KG, 1>(s, a);
+    else packed_run<M, HD, 3, T, RowStage<M, HD, 3, T, false, 4, 1>, 1, RES>(s, a);
   } else {
     // (a lane's offset within a stage of 64 rows is 32 bits, unsigned)
     auto near = [](const QRows& r) { return r.tok >= 0 && r.tok < 1 << 22; };
     const bool direct = a.kvec && near(a.k) && near(a.v);
-    // Where all tiles are on the device at once, the time is the longest's: two groups
-    // of waves have every second stage of its keys each.
-    const bool two = a.n_rows * (long)a.group / 128 * a.n_head <= 512;
     if (direct && two) packed_run<M, HD, 1, T, DirectStage<M, HD, 4>, 2, 1>(s, a);
     else if (direct) packed_run<M, HD, 1, T, DirectStage<M, HD, 4>, 1, 2>(s, a);
     else if (two) packed_run<M, HD, 1, T, RowStage<M, HD, 1, T, false, 4, 2>, 2, 1>(s, a);

@@ -244,6 +244,19 @@ __device__ __forceinline__ unsigned pick_key(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// The sum over this lane and those before it.
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+#define RTG_STEP(ctrl, rows) v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
+  RTG_STEP(0x111, 0xF);  // row_shr:1
+  RTG_STEP(0x112, 0xF);  // row_shr:2
+  RTG_STEP(0x114, 0xF);  // row_shr:4
+  RTG_STEP(0x118, 0xF);  // row_shr:8
+  RTG_STEP(0x142, 0xA);  // row_bcast:15
+  RTG_STEP(0x143, 0xC);  // row_bcast:31
+#undef RTG_STEP
+  return v;
+}
+
 // One workgroup per (sequence, head) finds the key of the last token to be kept,
 // eight bits at a time, and how many of those that have just this key; then each
 // wave lists what is kept of its stretch of the sequence, behind what the waves
@@ -321,12 +334,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const
         n[i] = totals[255 - 4 * lane - i];
         sum += n[i];
       }
-      unsigned incl = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const unsigned u = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += u;
-      }
+      const unsigned incl = wave_scan(sum);
       unsigned before = incl - sum;
       if (before < left && left <= incl) {
 #pragma unroll
@@ -479,14 +487,15 @@ __global__ __launch_bounds__(kMoveThreads) void f_move_kernel(FStore c, int* len
   if (readers.last((unsigned)c.n_head * 4) && l > keep) len[seq] = keep;
 }
 
-constexpr long kAppendGroups = 1024;  // (2048: 4 x 20000 tokens 79 us instead of 81, 1 x 20000 40 instead of 34)
-
 template <class T>
 void append_t(hipStream_t s, const FStore& c, int* len, QTickets tickets, const QRows& k, const QRows& v, int n_new,
               const int* counts, const int* start, bool vec) {
-  // Units of 256 threads; enough workgroups to fill the device, but few of a
-  // sequence's, which count themselves on one word (8.6 ns each).
-  const long units = (((long)n_new * (c.hdp / 8) + 63) / 64 * c.n_head + 3) / 4, most = std::max(64l, kAppendGroups / c.n_seq);
+  // Units of 256 threads; enough workgroups to fill the device twice, as sequences
+  // differ in length, but few of a sequence's, which count themselves on one word,
+  // 8.6 ns each (20000 tokens of 8 heads of 128, one sequence: 2048 workgroups 40 us,
+  // 512 of them 33; four: 1024 in all 81, 2048 79).
+  const long units = (((long)n_new * (c.hdp / 8) + 63) / 64 * c.n_head + 3) / 4;
+  const long most = std::max(64l, std::min(512l, 2048l / c.n_seq));
   const dim3 grid((unsigned)c.n_seq, (unsigned)std::max(1l, std::min(most, units)));
   if (c.hdp == 64) f_append_kernel<64, T><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start, vec);
   else f_append_kernel<128, T><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start, vec);

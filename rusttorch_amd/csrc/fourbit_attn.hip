@@ -27,8 +27,9 @@
 namespace rtg {
 namespace {
 
-constexpr int kCols = 16, kWaves = 4;
-constexpr int kMostSplit = 1024;  // workgroups at most where the keys are split
+constexpr int kCols = 16, kWaves = 8, kWeighWaves = 4;
+constexpr int kMostSplit = 256;  // workgroups at most where the keys are split
+constexpr int kWhole = 32, kSplitTiles = 8;  // tiles that are not split; of a split at least
 constexpr float kSlack = 8.f;     // powers of two that a score may pass the maximum by
 
 struct Args {
@@ -40,7 +41,6 @@ struct Args {
   float query, sum;  // ScoreScale
   float* stats;
   bool qvec, ovec;
-  int min_tiles;      // of a split
   unsigned* tickets;  // [sh][cblock][kQTicketStride]
   float* parts;       // [sh][cblock][split][column][hdp + 2]
 };
@@ -206,7 +206,7 @@ struct Shared {
 template <int HDP, class T>
 __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq& r, int seq, int head, int sh, int cb,
                                        int z, int n) {
-  constexpr int C4 = HDP / 4, STEP = 256 / C4;
+  constexpr int C4 = HDP / 4, STEP = 64 * kWaves / C4;
   const int tid = threadIdx.x, c4 = tid % C4 * 4;
   const int cols = min(kCols, a.n_q * a.group - cb * kCols);
   auto put = [&](int col, float m, float l, const float4& x) {
@@ -251,16 +251,21 @@ __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq&
   }
   __syncthreads();
   if (!s.last) return;
-  for (int col = tid / C4; col < cols; col += STEP) {
+  // a column's splits over as many groups of C4 threads as there are, each taking every GPC-th
+  int gpc = 1;
+  while (gpc * 2 * cols <= STEP) gpc *= 2;
+  const int group = tid / C4, zg = group % gpc;
+  for (int col0 = 0; col0 < cols; col0 += STEP / gpc) {
+    const int col = min(col0 + group / gpc, cols - 1);
     const float* p0 = a.parts + ((((size_t)sh * a.cblocks + cb) * gridDim.z) * kCols + col) * (HDP + 2);
     float m = -INFINITY, l = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int U = 8;  // (their way through memory takes over a microsecond: U at a time)
-    for (int z0 = 0; z0 < n; z0 += U) {
+    for (int z0 = zg; z0 < n; z0 += U * gpc) {
       float2 ml[U], y[U][2];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float* p = p0 + (size_t)min(z0 + u, n - 1) * kCols * (HDP + 2);
+        const float* p = p0 + (size_t)min(z0 + u * gpc, n - 1) * kCols * (HDP + 2);
         ml[u] = load2(p);
         y[u][0] = load2(p + 2 + c4);
         y[u][1] = load2(p + 4 + c4);
@@ -274,18 +279,38 @@ __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq&
       x = make_float4(x.x * corr, x.y * corr, x.z * corr, x.w * corr);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (z0 + u >= n) break;
+        if (z0 + u * gpc >= n) break;
         const float f = __builtin_amdgcn_exp2f(ml[u].x - base);
         l = fmaf(f, ml[u].y, l);
         x = make_float4(fmaf(f, y[u][0].x, x.x), fmaf(f, y[u][0].y, x.y), fmaf(f, y[u][1].x, x.z), fmaf(f, y[u][1].y, x.w));
       }
     }
-    put(col, m, l, x);
+    if (gpc > 1) {  // (uniform) the groups meet in LDS: group g in row g
+      __syncthreads();
+      float* row = &s.o[0][0][0] + (size_t)group * (HDP + 4);
+      *reinterpret_cast<float4*>(row + c4) = x;
+      if (c4 == 0) {
+        row[HDP] = m;
+        row[HDP + 1] = l;
+      }
+      __syncthreads();
+      if (zg != 0) continue;
+      for (int g = 1; g < gpc; ++g) {
+        const float* other = row + (size_t)g * (HDP + 4);
+        const float m2 = other[HDP], most = fmaxf(m, m2), base = most == -INFINITY ? 0.f : most;
+        const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+        const float4 y = *reinterpret_cast<const float4*>(other + c4);
+        m = most;
+        l = fmaf(f, l, f2 * other[HDP + 1]);
+        x = make_float4(fmaf(f, x.x, f2 * y.x), fmaf(f, x.y, f2 * y.y), fmaf(f, x.z, f2 * y.z), fmaf(f, x.w, f2 * y.w));
+      }
+    }
+    if (col0 + group / gpc < cols) put(col, m, l, x);
   }
 }
 
 template <int HDP, int QP, int PP, class T>
-__global__ __launch_bounds__(256) void f_attend_kernel(Args a) {
+__global__ __launch_bounds__(64 * kWaves) void f_attend_kernel(Args a) {
   constexpr int CV = HDP / 16;
   __shared__ Shared<HDP> s;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
@@ -297,7 +322,7 @@ __global__ __launch_bounds__(256) void f_attend_kernel(Args a) {
   const int live = last_i >= 0 ? keys_seen(r.len, r.count, last_i) : 0;
   const int least = keys_seen(r.len, r.count, column(a, cb * kCols).i);
   const int tiles = (live + kFTile - 1) / kFTile;
-  const int splits = max(min((tiles + a.min_tiles - 1) / a.min_tiles, (int)gridDim.z), 1);
+  const int splits = tiles <= kWhole ? 1 : min((tiles + kSplitTiles - 1) / kSplitTiles, (int)gridDim.z);
   if (z >= splits) return;
   const int per = (tiles + splits - 1) / splits, t0 = z * per, t1 = min(t0 + per, tiles);
   const Column cl = column(a, cb * kCols + n);
@@ -317,6 +342,7 @@ __global__ __launch_bounds__(256) void f_attend_kernel(Args a) {
     k.load(kc + (size_t)t * 16 * HDP, ks + (size_t)t * HDP, lane);
     v.load(vc + (size_t)t * 16 * HDP, vs + (size_t)t * HDP, lane);
   };
+  // (one tile of a wave ahead: two or three take registers and no time off)
   int t = t0 + wave;
   if (t < t1) fetch(t);
   while (t < t1) {
@@ -413,15 +439,15 @@ __global__ __launch_bounds__(256) void f_weigh_kernel(Args a, float decay) {
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head;
   const Seq r = seq_of(a, seq);
-  const int tiles = (r.len + kFTile - 1) / kFTile, step = (int)gridDim.y * kWaves;
-  if ((int)blockIdx.y * kWaves >= tiles) return;
+  const int tiles = (r.len + kFTile - 1) / kFTile, step = (int)gridDim.y * kWeighWaves;
+  if ((int)blockIdx.y * kWeighWaves >= tiles) return;
   const int cblocks = (r.count * a.group + kCols - 1) / kCols;
   const uint8_t *kc = a.c.k + a.c.codes(sh), *ks = a.c.sk + a.c.scales(sh);
   float* w = a.c.w + a.c.weights(sh);
   for (int cb0 = 0; cb0 == 0 || cb0 < cblocks; cb0 += W::BLOCKS) {
     const int blocks = min(W::BLOCKS, cblocks - cb0);
     if (cb0 > 0) __syncthreads();
-    for (int b = wave; b < blocks; b += kWaves) {
+    for (int b = wave; b < blocks; b += kWeighWaves) {
       const Column cl = column(a, (cb0 + b) * kCols + n);
       Query<HDP, QP, T> q;
       q.load(a, seq, head, cl, g);
@@ -436,7 +462,7 @@ __global__ __launch_bounds__(256) void f_weigh_kernel(Args a, float decay) {
       }
     }
     __syncthreads();
-    int t = (int)blockIdx.y * kWaves + wave;
+    int t = (int)blockIdx.y * kWeighWaves + wave;
     Keys<HDP> next;
     if (t < tiles) next.load(kc + (size_t)t * 16 * HDP, ks + (size_t)t * HDP, lane);
     for (; t < tiles; t += step) {
@@ -497,7 +523,6 @@ Args args_of(const FAttn& f) {
   a.stats = f.stats;
   a.qvec = by_eights(f.q, f.c.hd, f.type);
   a.ovec = by_eights(f.out, f.c.hd, f.type);
-  a.min_tiles = 1;
   a.tickets = static_cast<unsigned*>(f.work);
   a.parts = reinterpret_cast<float*>(static_cast<char*>(f.work) + (size_t)kMostSplit * kQTicketStride * 4);
   return a;
@@ -507,20 +532,22 @@ template <int QP, int PP, class T>
 void attend_t(hipStream_t s, const FAttn& f) {
   Args a = args_of(f);
   // Keys are split over workgroups where there are too few blocks of columns to
-  // fill the device; a split has at least 8 tiles.
+  // fill the device (one workgroup of eight waves a compute unit: 8 x 32000 tokens of
+  // 8 heads of 128 in 49 us, with two of them or twice as many of four waves 58 and
+  // 62, as the partial results take their time), and more than 32 tiles, for a join
+  // takes as long as four rounds of the eight waves.
   const long blocks = (long)f.c.n_seq * f.c.n_head * a.cblocks;
-  a.min_tiles = 8;
-  const long z = std::max(1l, std::min(kMostSplit / std::max(blocks, 1l), (long)(f.c.tiles + a.min_tiles - 1) / a.min_tiles));
+  const long z = f.c.tiles <= kWhole ? 1 : std::max(1l, std::min(kMostSplit / blocks, (long)(f.c.tiles + kSplitTiles - 1) / kSplitTiles));
   const dim3 grid((unsigned)(f.c.n_seq * f.c.n_head), (unsigned)a.cblocks, (unsigned)z);
-  if (f.c.hdp == 64) f_attend_kernel<64, QP, PP, T><<<grid, 256, 0, s>>>(a);
-  else f_attend_kernel<128, QP, PP, T><<<grid, 256, 0, s>>>(a);
+  if (f.c.hdp == 64) f_attend_kernel<64, QP, PP, T><<<grid, 64 * kWaves, 0, s>>>(a);
+  else f_attend_kernel<128, QP, PP, T><<<grid, 64 * kWaves, 0, s>>>(a);
 }
 template <int QP, class T>
 void weigh_t(hipStream_t s, const FAttn& f, float decay) {
   const Args a = args_of(f);
   // as many workgroups as the device takes at once
   const long sh = (long)f.c.n_seq * f.c.n_head, most = std::max(1l, 1024 / sh);
-  const dim3 grid((unsigned)sh, (unsigned)std::min(most, (long)(f.c.tiles + kWaves - 1) / kWaves));
+  const dim3 grid((unsigned)sh, (unsigned)std::min(most, (long)(f.c.tiles + kWeighWaves - 1) / kWeighWaves));
   if (f.c.hdp == 64) f_weigh_kernel<64, QP, T><<<grid, 256, 0, s>>>(a, decay);
   else f_weigh_kernel<128, QP, T><<<grid, 256, 0, s>>>(a, decay);
 }
@@ -537,8 +564,22 @@ void fattn_work_clear(hipStream_t s, void* work, int hdp) {
   (void)hipMemsetAsync(static_cast<char*>(work) + few_work_bytes(hdp), 0, fmany_tickets_bytes(), s);
 }
 
+namespace {
+// The kernel of many rows takes 128 at a time, and 7 us longer at least: it pays
+// where there is much to do (the blocks of 16 columns times the tiles that the
+// sequences may have; the host does not know the lengths) and few of its rows are
+// empty. 32 heads of 128 over 8 behind 32000 tokens in bf16: 32 queries 42 us (60 by
+// the other kernel), 50 72 (59), 150 262 (95); 16 sequences of 12 heads of 64 behind
+// 4000 in f32: 96 queries 75 (82), 128 94 (88).
+bool for_many(const FAttn& f) {
+  const long columns = (long)f.n_q * (f.n_q_head / f.c.n_head), blocks = (columns + kCols - 1) / kCols;
+  const long least = f.type == Q_F32 ? 96 : f.type == Q_F16 || f.c.hdp == 64 ? 64 : 32;
+  return columns > least && blocks * f.c.n_seq * f.c.n_head * f.c.tiles > 60000;
+}
+}  // namespace
+
 void launch_f_attend(hipStream_t s, const FAttn& f) {
-  if (f.n_q * (f.n_q_head / f.c.n_head) > 128) return launch_f_attend_many(s, f, static_cast<char*>(f.work) + few_work_bytes(f.c.hdp));
+  if (for_many(f)) return launch_f_attend_many(s, f, static_cast<char*>(f.work) + few_work_bytes(f.c.hdp));
   if (f.type == Q_F32) attend_t<3, 3, float>(s, f);
   else if (f.type == Q_BF16) attend_t<1, 2, __bf16>(s, f);
   else attend_t<2, 2, _Float16>(s, f);

@@ -24,7 +24,7 @@ def ints(x):
 
 def prob_step(dtype, many):
     """What a probability is rounded by, relative: three bf16 parts for f32, two cut ones (16 bits) for the others,
-    bf16 to nearest for bf16 rows in the kernel of many rows."""
+    bf16 to nearest for bf16 rows where the kernel of many rows may be chosen."""
     return 2.0 ** -24 if dtype == "f32" else 2.0 ** -9 if dtype == "bf16" and many else 2.0 ** -15
 
 
