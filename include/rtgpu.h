@@ -316,18 +316,15 @@ rtg_result rtg_fourbit_read(const rtg_fourbit* cache, rtg_dtype dtype, const rtg
  * scale, scores, and 256 times the largest |v| times the number of keys have to be
  * within f32. A key that reads back as NaN makes the rows NaN that see it, a value
  * their channels of the same 32, and no others; a query that is not finite gives a
- * row of NaN. stats (may be NULL): n_seq * n_q * n_q_head * 2 f32 for
- * rtg_fourbit_weigh. */
+ * row of NaN.
+ *
+ * With stats (n_seq * n_q * n_q_head * 2 f32 to work in, not NULL) the weights of all
+ * tokens then become decay (0 .. 1; 0 whatever they were) times what they are, plus
+ * the probabilities that the counted queries of all heads of the token's head give
+ * them: sums in f32, in a fixed order. */
 rtg_result rtg_fourbit_attend(rtg_fourbit* cache, rtg_dtype dtype, const rtg_rows* queries, size_t n_q,
                               size_t n_q_head, const int32_t* counts, float scale, const rtg_rows* out, float* stats,
-                              void* stream);
-/* The weights of all tokens become decay (0 .. 1; 0 whatever they were) times what
- * they are, plus the probabilities that the counted queries of all heads of the
- * token's head give them. Behind an rtg_fourbit_attend of the same cache, queries,
- * counts and scale, whose stats it takes, with no append between. */
-rtg_result rtg_fourbit_weigh(rtg_fourbit* cache, rtg_dtype dtype, const rtg_rows* queries, size_t n_q,
-                             size_t n_q_head, const int32_t* counts, float scale, const float* stats, float decay,
-                             void* stream);
+                              float decay, void* stream);
 /* The weights of tokens 0 .. n - 1 to out [n_seq][n_head][n], 0 where there is no
  * token; and x [n_seq][n_head][n] added to those of the tokens that there are. */
 rtg_result rtg_fourbit_weights(const rtg_fourbit* cache, float* out, size_t n, void* stream);

@@ -110,9 +110,7 @@ SIGNATURES = {
     "rtg_fourbit_read": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_char_p, C.c_size_t, C.c_void_p,
                                   C.c_void_p]),
     "rtg_fourbit_attend": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_size_t, C.c_size_t, C.c_void_p,
-                                    C.c_float, C.c_char_p, C.c_void_p, C.c_void_p]),
-    "rtg_fourbit_weigh": (Result, [C.c_void_p, C.c_int, C.c_char_p, C.c_size_t, C.c_size_t, C.c_void_p,
-                                   C.c_float, C.c_void_p, C.c_float, C.c_void_p]),
+                                    C.c_float, C.c_char_p, C.c_void_p, C.c_float, C.c_void_p]),
     "rtg_fourbit_weights": (Result, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "rtg_fourbit_add_weights": (Result, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "rtg_fourbit_evict": (Result, [C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p]),

@@ -421,6 +421,19 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
   u4v q[KS][QP];
   {
     const T* p = static_cast<const T*>(a.q.p) + job.seq * a.q.seq + (job.base + (long)min(i, max(job.count - 1, 0))) * a.q.tok + head * a.q.head;
+    bool raw = false;
+    if constexpr (QP == 1 && sizeof(T) == 2) {
+      if (a.qvec && a.query == 1.f) {  // (uniform) as they are
+        raw = true;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const int c8 = k * 16 + half * 8;
+          q[k][0] = u4v{0, 0, 0, 0};
+          if (c8 < a.hd) q[k][0] = *reinterpret_cast<const u4v*>(p + c8);
+        }
+      }
+    }
+    if (!raw)
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       float x[8];

@@ -110,29 +110,6 @@ rtg_result this_gpu(int* device) {
   return ok();
 }
 
-// The arguments that attention and the weights of its keys have in common.
-rtg_result attn_of(const rtg_fourbit* q, rtg_dtype dtype, const rtg_rows* queries, size_t n_q, size_t n_q_head,
-                   const int32_t* counts, float scale, float* stats, FAttn* f, const char* what) {
-  if (!type_of(dtype, &f->type)) return err("%s takes f32, bf16 or f16 rows", what);
-  if (n_q_head == 0 || n_q_head % (size_t)q->c.n_head != 0)
-    return err("%zu query heads are not a multiple of the cache's %d heads", n_q_head, q->c.n_head);
-  if (n_q_head / q->c.n_head > kMaxGroup)
-    return err("%zu query heads per key/value head exceed %zu", n_q_head / q->c.n_head, kMaxGroup);
-  if (!std::isfinite(scale)) return err("scale must be finite");
-  if (n_q > kMaxRows || n_q * (n_q_head / q->c.n_head) > kMaxRows)
-    return err("%zu queries of %zu heads exceed %zu rows per key/value head", n_q, n_q_head, kMaxRows);
-  f->c = q->c;
-  f->len = q->len;
-  f->q = rows(queries);
-  f->n_q = (int)n_q;
-  f->n_q_head = (int)n_q_head;
-  f->counts = counts;
-  f->scale = scale;
-  f->stats = stats;
-  f->work = q->work;
-  return ok();
-}
-
 }  // namespace
 
 extern "C" {
@@ -216,32 +193,37 @@ rtg_result rtg_fourbit_read(const rtg_fourbit* q, rtg_dtype dtype, const rtg_row
 }
 
 rtg_result rtg_fourbit_attend(rtg_fourbit* q, rtg_dtype dtype, const rtg_rows* queries, size_t n_q, size_t n_q_head,
-                              const int32_t* counts, float scale, const rtg_rows* out, float* stats, void* stream) {
+                              const int32_t* counts, float scale, const rtg_rows* out, float* stats, float decay,
+                              void* stream) {
   if (!q || !queries || !out) return err("null argument");
   FAttn f;
-  const rtg_result r = attn_of(q, dtype, queries, n_q, n_q_head, counts, scale, stats, &f, "rtg_fourbit_attend");
-  if (!r.success || n_q == 0) return r;
-  if (!queries->data || !out->data) return err("null argument");
+  if (!type_of(dtype, &f.type)) return err("rtg_fourbit_attend takes f32, bf16 or f16 rows");
+  if (n_q_head == 0 || n_q_head % (size_t)q->c.n_head != 0)
+    return err("%zu query heads are not a multiple of the cache's %d heads", n_q_head, q->c.n_head);
+  if (n_q_head / q->c.n_head > kMaxGroup)
+    return err("%zu query heads per key/value head exceed %zu", n_q_head / q->c.n_head, kMaxGroup);
+  if (!std::isfinite(scale)) return err("scale must be finite");
+  if (stats && !(decay >= 0.f && decay <= 1.f)) return err("decay must be within 0 .. 1");
+  if (n_q > kMaxRows || n_q * (n_q_head / q->c.n_head) > kMaxRows)
+    return err("%zu queries of %zu heads exceed %zu rows per key/value head", n_q, n_q_head, kMaxRows);
+  if (n_q == 0 && !stats) return ok();
+  if (n_q && (!queries->data || !out->data)) return err("null argument");
+  f.c = q->c;
+  f.len = q->len;
+  f.q = rows(queries);
   f.out = rows(out);
+  f.n_q = (int)n_q;
+  f.n_q_head = (int)n_q_head;
+  f.counts = counts;
+  f.scale = scale;
+  f.stats = stats;
+  f.work = q->work;
   OnDevice dev(q->device);
   if (dev.status() != hipSuccess) return hip_err(dev.status(), "hipSetDevice");
-  launch_f_attend(static_cast<hipStream_t>(stream), f);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (n_q) launch_f_attend(s, f);
+  if (stats) launch_f_weigh(s, f, decay);
   return launched("rtg_fourbit_attend");
-}
-
-rtg_result rtg_fourbit_weigh(rtg_fourbit* q, rtg_dtype dtype, const rtg_rows* queries, size_t n_q, size_t n_q_head,
-                             const int32_t* counts, float scale, const float* stats, float decay, void* stream) {
-  if (!q || !queries || !stats) return err("null argument");
-  if (!(decay >= 0.f && decay <= 1.f)) return err("decay must be within 0 .. 1");
-  FAttn f;
-  const rtg_result r = attn_of(q, dtype, queries, n_q, n_q_head, counts, scale, const_cast<float*>(stats), &f,
-                               "rtg_fourbit_weigh");
-  if (!r.success) return r;
-  if (n_q && !queries->data) return err("null argument");
-  OnDevice dev(q->device);
-  if (dev.status() != hipSuccess) return hip_err(dev.status(), "hipSetDevice");
-  launch_f_weigh(static_cast<hipStream_t>(stream), f, decay);
-  return launched("rtg_fourbit_weigh");
 }
 
 rtg_result rtg_fourbit_weights(const rtg_fourbit* q, float* out, size_t n, void* stream) {

@@ -100,9 +100,10 @@ __device__ __forceinline__ f32x4 mfma16(const u4v& a, const u4v& b, const f32x4&
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
 }
 
-// The scale of the scores, as a power of two with its sign that goes into the
-// queries (exactly: parts of bf16 have f32's range) and a factor in [1, 2) of the
-// sums, log2 e included; a scale of 0 makes the queries 0.
+// The scale of the scores: its sign goes into the queries, and where it is far from
+// 1 a power of two, so that sums stay within f32 where the scores do (exactly: parts
+// of bf16 have f32's range); the rest is a factor of the sums, log2 e included. A
+// scale of 0 makes the queries 0.
 struct ScoreScale {
   float query, sum;
 };
@@ -112,7 +113,7 @@ inline ScoreScale score_scale(float scale) {
   const double m = frexp(fabs(x), &e);  // [0.5, 1)
   if (m == 0.0) return {0.f, 1.f};
   // (a power of two that f32 does not hold goes into the factor)
-  const int in = e - 1 < -126 ? -126 : e - 1 > 127 ? 127 : e - 1;
+  const int in = abs(e) <= 20 ? 0 : e - 1 < -126 ? -126 : e - 1 > 127 ? 127 : e - 1;
   return {copysignf(ldexpf(1.f, in), scale), (float)ldexp(m, e - in)};
 }
 

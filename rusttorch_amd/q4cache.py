@@ -95,15 +95,13 @@ class FourBitCache(QuantisedCache):
             to = _pack_rows(out.data_ptr(), n * tok, tok, self.head_dim)
         else:
             to = self._rows("out", out, q.dtype, n, heads)
-        scale = self.head_dim ** -0.5 if scale is None else scale
-        counts = self._ints("counts", counts)
-        stats = None
-        if weigh is not None:
-            stats = torch.empty(max(self.n_seq * n * heads * 2, 1), dtype=torch.float32, device=self.device)
-        at = None if stats is None else stats.data_ptr()
-        check(self._lib.rtg_fourbit_attend(self._h, dtype, rows, n, heads, counts, scale, to, at, stream))
-        if stats is not None:
-            check(self._lib.rtg_fourbit_weigh(self._h, dtype, rows, n, heads, counts, scale, at, weigh, stream))
+        # (the library works in stats; the allocator keeps it from others until this stream is behind the call)
+        stats = None if weigh is None else torch.empty(max(self.n_seq * n * heads * 2, 1), dtype=torch.float32,
+                                                       device=self.device)
+        check(self._lib.rtg_fourbit_attend(self._h, dtype, rows, n, heads, self._ints("counts", counts),
+                                           self.head_dim ** -0.5 if scale is None else scale, to,
+                                           None if stats is None else stats.data_ptr(),
+                                           0.0 if weigh is None else weigh, stream))
         return out
 
     def read(self, n: int, first=None, dtype: torch.dtype = torch.float32, k=None, v=None):

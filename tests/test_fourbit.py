@@ -30,8 +30,8 @@ def test_new_refuses(args, what):
 def test_null_arguments():
     lib, r, out, f = _lib.load(), bytes(32), C.c_uint32(), C.c_void_p(256)
     for res in (lib.rtg_fourbit_new(1, 1, 64, 10, None), lib.rtg_fourbit_append(None, 0, r, r, 1, None, None, None),
-                lib.rtg_fourbit_read(None, 0, r, r, 1, None, None), lib.rtg_fourbit_attend(None, 0, r, 1, 1, None, 1.0, r, None, None),
-                lib.rtg_fourbit_weigh(None, 0, r, 1, 1, None, 1.0, f, 1.0, None), lib.rtg_fourbit_weights(None, f, 1, None),
+                lib.rtg_fourbit_read(None, 0, r, r, 1, None, None), lib.rtg_fourbit_attend(None, 0, r, 1, 1, None, 1.0, r, None, 0.0, None),
+                lib.rtg_fourbit_weights(None, f, 1, None),
                 lib.rtg_fourbit_add_weights(None, f, 1, None), lib.rtg_fourbit_evict(None, 1, 0, f, None),
                 lib.rtg_fourbit_lengths(None, C.byref(out), None),
                 lib.rtg_attend_packed(0, r, r, r, 1, 1, 1, 64, None, 1, 1.0, r, None),
