@@ -703,18 +703,6 @@ __global__ __launch_bounds__(256 * KG, KG > 1 || HD == 64 || sizeof(T) == 2 ? 2 
   attend<Bf16, HD, QP, PP, T, CodeStage<HD>, KG>(a, j, s);
 }
 
-// The sum over a wave, in every lane.
-__device__ __forceinline__ int wave_sum(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);   // quad_perm [1,0,3,2]
-  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);   // quad_perm [2,3,0,1]
-  v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xF, 0xF, false);  // row_ror:4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false);  // row_ror:8
-  const auto x = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
-  v = (int)(x[0] + x[1]);
-  const auto y = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
-  return __builtin_amdgcn_readfirstlane((int)(y[0] + y[1]));
-}
-
 // The workgroups of a packed batch: the tiles of all sequences, each for all heads
 // in turn; those behind the last tile clear the rows that no sequence has. There
 // is one at least: the sum of the sequences' tiles, rounded up each, is less than

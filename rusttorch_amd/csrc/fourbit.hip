@@ -244,19 +244,6 @@ __device__ __forceinline__ unsigned pick_key(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// The sum over this lane and those before it.
-__device__ __forceinline__ unsigned wave_scan(unsigned v) {
-#define RTG_STEP(ctrl, rows) v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
-  RTG_STEP(0x111, 0xF);  // row_shr:1
-  RTG_STEP(0x112, 0xF);  // row_shr:2
-  RTG_STEP(0x114, 0xF);  // row_shr:4
-  RTG_STEP(0x118, 0xF);  // row_shr:8
-  RTG_STEP(0x142, 0xA);  // row_bcast:15
-  RTG_STEP(0x143, 0xC);  // row_bcast:31
-#undef RTG_STEP
-  return v;
-}
-
 // One workgroup per (sequence, head) finds the key of the last token to be kept,
 // eight bits at a time, and how many of those that have just this key; then each
 // wave lists what is kept of its stretch of the sequence, behind what the waves

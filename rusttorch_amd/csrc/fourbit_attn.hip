@@ -41,8 +41,17 @@ struct Args {
   float query, sum;  // ScoreScale
   float* stats;
   bool qvec, ovec;
-  unsigned* tickets;  // [sh][cblock][kQTicketStride]
-  float* parts;       // [sh][cblock][split][column][hdp + 2]
+  bool split;         // keys are split over workgroups
+  unsigned* tickets;  // [seq][head][cblock][kQTicketStride]
+  float* parts;       // [workgroup][column][hdp + 2]
+};
+
+// What a workgroup works on: part z of n of the tiles that a sequence, head and
+// block of columns have, `per` to a part.
+struct Work {
+  int seq, head, cb, z, n, per;
+  int slot0, stride;  // workgroup of part z: slot0 + z * stride
+  int ticket;
 };
 
 struct Column {
@@ -200,12 +209,12 @@ struct Shared {
   int last;
 };
 
-// Joins the waves' results in s for the columns of block cb: to the results where
-// the keys were not split, else to the partials; the last of the n workgroups of a
-// block to come here joins those.
+// Joins the waves' results in s for the columns of a block: to the results where
+// the keys were not split, else to the partials; the last of its workgroups to come
+// here joins those.
 template <int HDP, class T>
-__device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq& r, int seq, int head, int sh, int cb,
-                                       int z, int n) {
+__device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq& r, const Work& wk) {
+  const int seq = wk.seq, head = wk.head, cb = wk.cb, n = wk.n;
   constexpr int C4 = HDP / 4, STEP = 64 * kWaves / C4;
   const int tid = threadIdx.x, c4 = tid % C4 * 4;
   const int cols = min(kCols, a.n_q * a.group - cb * kCols);
@@ -235,7 +244,7 @@ __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq&
     if (n == 1) {
       put(col, m, l, x);
     } else {
-      float* p = a.parts + ((((size_t)sh * a.cblocks + cb) * gridDim.z + z) * kCols + col) * (HDP + 2);
+      float* p = a.parts + ((size_t)(wk.slot0 + wk.z * wk.stride) * kCols + col) * (HDP + 2);
       if (c4 == 0) store2(p, m, l);
       store2(p + 2 + c4, x.x, x.y);
       store2(p + 4 + c4, x.z, x.w);
@@ -245,7 +254,7 @@ __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq&
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores have completed
   __syncthreads();
   if (tid == 0) {
-    unsigned* count = a.tickets + ((size_t)sh * a.cblocks + cb) * kQTicketStride;
+    unsigned* count = a.tickets + (size_t)wk.ticket * kQTicketStride;
     s.last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)n - 1;
     if (s.last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
@@ -257,7 +266,8 @@ __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq&
   const int group = tid / C4, zg = group % gpc;
   for (int col0 = 0; col0 < cols; col0 += STEP / gpc) {
     const int col = min(col0 + group / gpc, cols - 1);
-    const float* p0 = a.parts + ((((size_t)sh * a.cblocks + cb) * gridDim.z) * kCols + col) * (HDP + 2);
+    const float* p0 = a.parts + ((size_t)wk.slot0 * kCols + col) * (HDP + 2);
+    const size_t part = (size_t)wk.stride * kCols * (HDP + 2);
     float m = -INFINITY, l = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int U = 8;  // (their way through memory takes over a microsecond: U at a time)
@@ -265,7 +275,7 @@ __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq&
       float2 ml[U], y[U][2];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float* p = p0 + (size_t)min(z0 + u * gpc, n - 1) * kCols * (HDP + 2);
+        const float* p = p0 + min(z0 + u * gpc, n - 1) * part;
         ml[u] = load2(p);
         y[u][0] = load2(p + 2 + c4);
         y[u][1] = load2(p + 4 + c4);
@@ -309,22 +319,78 @@ __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq&
   }
 }
 
+// Workgroup (sequence and head, block of columns); or, where the keys are split, one
+// of kMostSplit that get about as many tiles each, so that sequences of different
+// lengths are done at the same time (8 of 16000 to 32000 tokens of 8 heads of 128:
+// 54 us with as many parts for each, XX so).
+__device__ __forceinline__ Work work_of(const Args& a) {
+  Work w;
+  w.z = 0;
+  w.n = 1;
+  w.per = 0;
+  if (!a.split) {
+    w.seq = (int)blockIdx.x / a.c.n_head;
+    w.head = (int)blockIdx.x - w.seq * a.c.n_head;
+    w.cb = (int)blockIdx.y;
+    w.slot0 = w.stride = w.ticket = 0;
+    return w;
+  }
+  const int lane = threadIdx.x & 63, inner = a.c.n_head * a.cblocks;
+  auto tiles_at = [&](int s0) { return s0 + lane < a.c.n_seq ? (a.len[s0 + lane] + kFTile - 1) / kFTile : 0; };
+  auto parts_of = [&](int tiles, int each) { return tiles <= kWhole ? 1 : (tiles + each - 1) / each; };
+  int total = 0;
+  for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) total += wave_sum(tiles_at(s0));
+  // the fewest tiles to a part, or up to a 16th more, with which there are not too many parts
+  const int room = kMostSplit / inner;
+  int each = max((total + room - 1) / room, kSplitTiles);
+  for (;; each += each / 16 + 1) {
+    int parts = 0;
+    for (int s0 = 0; s0 < a.c.n_seq; s0 += 64)
+      parts += wave_sum(s0 + lane < a.c.n_seq ? parts_of(tiles_at(s0), each) : 0);
+    if (parts <= room) break;  // (each sequence has one where `each` is large; there are at most room / 2 sequences)
+  }
+  int at = (int)blockIdx.x;
+  w.seq = -1;
+  for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
+    const int tiles = tiles_at(s0), parts = s0 + lane < a.c.n_seq ? parts_of(tiles, each) : 0;
+    const int incl = wave_scan(parts * inner);
+    const unsigned long long mine = __builtin_amdgcn_ballot_w64(at >= incl - parts * inner && at < incl);
+    if (mine) {
+      const int l = __builtin_ctzll(mine);
+      w.seq = s0 + l;
+      w.n = __builtin_amdgcn_readlane(parts, l);
+      w.per = (__builtin_amdgcn_readlane(tiles, l) + w.n - 1) / w.n;
+      const int rest = at - (__builtin_amdgcn_readlane(incl, l) - w.n * inner);
+      w.z = rest / inner;
+      const int pair = rest - w.z * inner;
+      w.head = pair / a.cblocks;
+      w.cb = pair - w.head * a.cblocks;
+      w.stride = inner;
+      w.slot0 = (int)blockIdx.x - w.z * inner;
+      w.ticket = w.seq * inner + pair;
+      return w;
+    }
+    at -= __builtin_amdgcn_readlane(incl, 63);
+  }
+  return w;
+}
+
 template <int HDP, int QP, int PP, class T>
 __global__ __launch_bounds__(64 * kWaves) void f_attend_kernel(Args a) {
   constexpr int CV = HDP / 16;
   __shared__ Shared<HDP> s;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int sh = blockIdx.x, seq = sh / a.c.n_head, head = sh - seq * a.c.n_head, cb = blockIdx.y, z = blockIdx.z;
+  const Work wk = work_of(a);
+  if (wk.seq < 0) return;
+  const int seq = wk.seq, head = wk.head, sh = seq * a.c.n_head + head, cb = wk.cb;
   const Seq r = seq_of(a, seq);
   // keys that the block's columns see: at most, at least (columns that are none may see anything)
   const int last_i = min(column(a, cb * kCols + kCols - 1).i, r.count - 1);
   const int live = last_i >= 0 ? keys_seen(r.len, r.count, last_i) : 0;
   const int least = keys_seen(r.len, r.count, column(a, cb * kCols).i);
   const int tiles = (live + kFTile - 1) / kFTile;
-  const int splits = tiles <= kWhole ? 1 : min((tiles + kSplitTiles - 1) / kSplitTiles, (int)gridDim.z);
-  if (z >= splits) return;
-  const int per = (tiles + splits - 1) / splits, t0 = z * per, t1 = min(t0 + per, tiles);
+  const int t0 = wk.z * wk.per, t1 = wk.n == 1 ? tiles : min(t0 + wk.per, tiles);
   const Column cl = column(a, cb * kCols + n);
   const int lim = keys_seen(r.len, r.count, cl.i);
   Query<HDP, QP, T> q;
@@ -410,7 +476,7 @@ __global__ __launch_bounds__(64 * kWaves) void f_attend_kernel(Args a) {
 #pragma unroll
     for (int d = 0; d < CV; d += 4)
       *reinterpret_cast<float4*>(&s.o[wave][n][CV * (4 * g + e) + d]) = make_float4(o[d][e], o[d + 1][e], o[d + 2][e], o[d + 3][e]);
-  finish<HDP, T>(a, s, r, seq, head, sh, cb, z, splits);
+  finish<HDP, T>(a, s, r, wk);
 }
 
 // ---- weights ----
@@ -523,6 +589,7 @@ Args args_of(const FAttn& f) {
   a.stats = f.stats;
   a.qvec = by_eights(f.q, f.c.hd, f.type);
   a.ovec = by_eights(f.out, f.c.hd, f.type);
+  a.split = false;
   a.tickets = static_cast<unsigned*>(f.work);
   a.parts = reinterpret_cast<float*>(static_cast<char*>(f.work) + (size_t)kMostSplit * kQTicketStride * 4);
   return a;
@@ -537,8 +604,8 @@ void attend_t(hipStream_t s, const FAttn& f) {
   // 62, as the partial results take their time), and more than 32 tiles, for a join
   // takes as long as four rounds of the eight waves.
   const long blocks = (long)f.c.n_seq * f.c.n_head * a.cblocks;
-  const long z = f.c.tiles <= kWhole ? 1 : std::max(1l, std::min(kMostSplit / blocks, (long)(f.c.tiles + kSplitTiles - 1) / kSplitTiles));
-  const dim3 grid((unsigned)(f.c.n_seq * f.c.n_head), (unsigned)a.cblocks, (unsigned)z);
+  a.split = f.c.tiles > kWhole && blocks * 2 <= kMostSplit;
+  const dim3 grid = a.split ? dim3(kMostSplit) : dim3((unsigned)(f.c.n_seq * f.c.n_head), (unsigned)a.cblocks);
   if (f.c.hdp == 64) f_attend_kernel<64, QP, PP, T><<<grid, 64 * kWaves, 0, s>>>(a);
   else f_attend_kernel<128, QP, PP, T><<<grid, 64 * kWaves, 0, s>>>(a);
 }

@@ -129,6 +129,31 @@ __device__ __forceinline__ float2 load2(const float* p) {
   return make_float2(__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32)));
 }
 
+// The sum over a wave, in every lane.
+__device__ __forceinline__ int wave_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);   // quad_perm [1,0,3,2]
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);   // quad_perm [2,3,0,1]
+  v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xF, 0xF, false);  // row_ror:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false);  // row_ror:8
+  const auto x = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  v = (int)(x[0] + x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+  return __builtin_amdgcn_readfirstlane((int)(y[0] + y[1]));
+}
+
+// The sum over this lane and those before it.
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+#define RTG_STEP(ctrl, rows) v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
+  RTG_STEP(0x111, 0xF);  // row_shr:1
+  RTG_STEP(0x112, 0xF);  // row_shr:2
+  RTG_STEP(0x114, 0xF);  // row_shr:4
+  RTG_STEP(0x118, 0xF);  // row_shr:8
+  RTG_STEP(0x142, 0xA);  // row_bcast:15
+  RTG_STEP(0x143, 0xC);  // row_bcast:31
+#undef RTG_STEP
+  return v;
+}
+
 // Query i of a sequence of len tokens, the last `count` of which ask: keys it sees.
 __device__ __forceinline__ int keys_seen(int len, int count, int i) { return i < count ? max(len - count + i + 1, 0) : 0; }
 
