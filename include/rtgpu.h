@@ -344,8 +344,9 @@ rtg_result rtg_fourbit_lengths(rtg_fourbit* cache, uint32_t* out, void* stream);
  * behind the other, each attending to itself; query row i of a sequence sees its
  * rows 0 .. i. Rows are [n_rows][heads][head_dim] in device memory of the current
  * device (stride_seq is not used), offsets n_seq + 1 device int32: sequence s has
- * rows offsets[s] .. offsets[s + 1] - 1; they must not descend, and are clamped to
- * the rows there are. Rows of no sequence are set to 0. Query head h reads
+ * rows offsets[s] .. offsets[s + 1] - 1. Offsets are clamped to the rows there are,
+ * and one that descends counts as the largest before it (its sequence has no row).
+ * Rows of no sequence are set to 0. Query head h reads
  * key/value head h / (n_q_head / n_head), at most 1024 of them one.
  *
  * softmax of scale * q . k; sums are f32, results rounded to dtype once, the

@@ -722,16 +722,16 @@ __global__ __launch_bounds__(Stage::NT * KG, KG > 1 || HD == 64 || P == 1 ? 2 : 
   Job j;
   j.seq = 0;  // (packed rows have no stride of sequences)
   j.tile = -1;
-  // the 64 sequences from s0 on, one per lane
+  // The 64 sequences from s0 on, one per lane. An offset that descends counts as the
+  // largest before it: whatever they hold, sequences lie behind each other within the rows.
   int lo = 0, hi = 0;
+  end = min(max(a.offsets[0], 0), a.n_rows);
   auto sequences = [&](int s0) {
     const int seq = s0 + lane;
-    lo = hi = 0;
-    if (seq < a.n_seq) {
-      lo = min(max(a.offsets[seq], 0), a.n_rows);
-      hi = min(max(a.offsets[seq + 1], lo), a.n_rows);
-    }
-    end = max(end, __builtin_amdgcn_readlane(hi, min(a.n_seq - 1 - s0, 63)));
+    hi = max(wave_max_scan(seq < a.n_seq ? min(max(a.offsets[seq + 1], 0), a.n_rows) : 0), end);
+    lo = __shfl_up(hi, 1, 64);
+    if (lane == 0) lo = end;
+    end = __builtin_amdgcn_readlane(hi, 63);
     return ((hi - lo) * a.group + ROWS - 1) / ROWS;
   };
   auto take = [&](int lane_of, int tile) {

@@ -3,6 +3,7 @@
 #include "fourbit.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fourbit_core.h"
 #include "qwrite.h"
@@ -87,8 +88,8 @@ __device__ __forceinline__ unsigned encode8(const float (&x)[8], unsigned* byte)
   unsigned top = 0;  // (bits order like the values, NaN above infinity)
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-  top = max(top, (unsigned)__shfl_xor((int)top, 1, 64));
-  top = max(top, (unsigned)__shfl_xor((int)top, 2, 64));
+  top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false));  // quad_perm [1,0,3,2]
+  top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false));  // quad_perm [2,3,0,1]
   // 0x1FFFFF carries into the exponent where the fraction is over 0.75
   const int b = min(max((int)((top + 0x1FFFFFu) >> 23) - 2, 27), 252);
   const float scale = scale_of((unsigned)b);
@@ -101,13 +102,16 @@ __device__ __forceinline__ unsigned encode8(const float (&x)[8], unsigned* byte)
   return w;
 }
 
-// Wave by wave, the waves of a sequence's workgroups take every so many'th 64
-// units of it; a unit is eight channels of a new token's key and value. 64 units
-// are 4 or 8 tokens of one head, a workgroup's are 16 or 32: rows are read whole
-// and a tile's bytes are written by neighbours.
-template <int HDP, class T>
+// A unit is 64 times eight channels of a new token's key and value: 4 or 8 tokens of
+// one head. A workgroup's four are behind each other (`wide`), so that lines of the
+// cache are written by one of them, or where there are few tokens of different
+// heads; the heads of the same tokens are the next workgroups', so that rows are
+// read whole at about the same time. 4 x 10000 to 20000 tokens of 8 heads of 128 in
+// bf16 take 74 us (4.2 TB/s in and out; a kernel with branches for rows that are not
+// aligned, and twice as many units in flight, took 95).
+template <int HDP, class T, bool VEC>
 __global__ __launch_bounds__(256) void f_append_kernel(FStore c, int* len, QTickets tickets, QRows k, QRows v, int n_new,
-                                                       const int* counts, const int* start, bool vec) {
+                                                       const int* counts, const int* start) {
   constexpr int U = HDP / 8;
   __shared__ Place shared;
   const int seq = blockIdx.x, tid = threadIdx.x;
@@ -117,23 +121,19 @@ __global__ __launch_bounds__(256) void f_append_kernel(FStore c, int* len, QTick
   Readers readers;
   readers.read(tickets, seq);
   const int n = p.bad ? 0 : p.end - p.at;
-  const unsigned per_head = (unsigned)((n + 64 / U - 1) / (64 / U));  // waves' worth of units of a head
-  unsigned at = blockIdx.y * 4 + (tid >> 6);
-  int head = 0;
+  const bool wide = n_new > 2 * (64 / U);
+  const unsigned heads = (unsigned)c.n_head, units = (unsigned)((n + 64 / U - 1) / (64 / U));  // of a head
+  const unsigned wave = (unsigned)tid >> 6, step = wide ? gridDim.y : gridDim.y * 4;
+  unsigned at = wide ? blockIdx.y : blockIdx.y * 4 + wave;
   const int c8 = tid % U * 8;
   // A wave's next unit: its head (n_head behind the last) and the row of this lane's.
   auto next = [&](int& h, int& row) {
-    if (per_head == 0) {
-      h = c.n_head;
-      return;
-    }
-    head = min(head + (int)(at / per_head), c.n_head);
-    at %= per_head;
-    h = head;
-    row = (int)at * (64 / U) + (tid & 63) / U;
-    at += gridDim.y * 4;
+    const unsigned group = at / heads, unit = wide ? group * 4 + wave : group;
+    h = (int)(unit < units ? at - group * heads : heads);
+    row = (int)unit * (64 / U) + (tid & 63) / U;
+    at += step;
   };
-  constexpr int AHEAD = 4;  // loads of so many units are in flight together
+  constexpr int AHEAD = 2;  // loads of so many units are in flight together
   for (;;) {
     float x[AHEAD][8], y[AHEAD][8];
     int h[AHEAD], row[AHEAD];
@@ -143,12 +143,12 @@ __global__ __launch_bounds__(256) void f_append_kernel(FStore c, int* len, QTick
       next(h[u], row[u]);
       if (h[u] >= c.n_head) continue;
       const int i = min(row[u], n - 1);
-      load8(static_cast<const T*>(k.p) + seq * k.seq + i * k.tok + h[u] * k.head, c8, c.hd, vec, x[u]);
-      load8(static_cast<const T*>(v.p) + seq * v.seq + i * v.tok + h[u] * v.head, c8, c.hd, vec, y[u]);
+      load8(static_cast<const T*>(k.p) + seq * k.seq + i * k.tok + h[u] * k.head, c8, c.hd, VEC, x[u]);
+      load8(static_cast<const T*>(v.p) + seq * v.seq + i * v.tok + h[u] * v.head, c8, c.hd, VEC, y[u]);
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      if (h[u] >= c.n_head) break;
+      if (h[u] >= c.n_head) continue;
       unsigned kb, vb;
       const unsigned kw = encode8(x[u], &kb), vw = encode8(y[u], &vb);
       if (row[u] >= n) continue;
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(256) void f_append_kernel(FStore c, int* len, QTick
         if (c8 == 0) c.w[c.weights(sh) + t] = 0.f;
       }
     }
-    if (h[AHEAD - 1] >= c.n_head) break;
+    if (at / heads * (wide ? 4u : 1u) >= units) break;
   }
   if (readers.last(gridDim.y)) {
     if (p.bad) atomicMin(tickets.err, (unsigned)seq * 4 + p.bad);
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const
         n[i] = totals[255 - 4 * lane - i];
         sum += n[i];
       }
-      const unsigned incl = wave_scan(sum);
+      const unsigned incl = (unsigned)wave_scan((int)sum);
       unsigned before = incl - sum;
       if (before < left && left <= incl) {
 #pragma unroll
@@ -477,15 +477,22 @@ __global__ __launch_bounds__(kMoveThreads) void f_move_kernel(FStore c, int* len
 template <class T>
 void append_t(hipStream_t s, const FStore& c, int* len, QTickets tickets, const QRows& k, const QRows& v, int n_new,
               const int* counts, const int* start, bool vec) {
-  // Units of 256 threads; enough workgroups to fill the device twice, as sequences
-  // differ in length, but few of a sequence's, which count themselves on one word,
-  // 8.6 ns each (20000 tokens of 8 heads of 128, one sequence: 2048 workgroups 40 us,
-  // 512 of them 33; four: 1024 in all 81, 2048 79).
-  const long units = (((long)n_new * (c.hdp / 8) + 63) / 64 * c.n_head + 3) / 4;
-  const long most = std::max(64l, std::min(512l, 2048l / c.n_seq));
+  // Four units a workgroup; enough of them to fill the device three times, as
+  // sequences differ in length, but few of a sequence's, which count themselves on
+  // one word, 8.6 ns each (20000 tokens of 8 heads of 128, one sequence: 2048
+  // workgroups 40 us, 768 of them 30; four of 10000 to 20000: 512 77, 768 74).
+  const int rows = 512 / c.hdp;  // of a unit
+  const long units = n_new > 2 * rows ? (long)c.n_head * ((n_new + 4 * rows - 1) / (4 * rows))
+                                      : ((long)c.n_head * ((n_new + rows - 1) / rows) + 3) / 4;
+  const long most = std::max(64l, std::min(768l, 3072l / c.n_seq));
   const dim3 grid((unsigned)c.n_seq, (unsigned)std::max(1l, std::min(most, units)));
-  if (c.hdp == 64) f_append_kernel<64, T><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start, vec);
-  else f_append_kernel<128, T><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start, vec);
+  auto run = [&](auto width) {
+    constexpr int HDP = decltype(width)::value;
+    if (vec) f_append_kernel<HDP, T, true><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start);
+    else f_append_kernel<HDP, T, false><<<grid, 256, 0, s>>>(c, len, tickets, k, v, n_new, counts, start);
+  };
+  if (c.hdp == 64) run(std::integral_constant<int, 64>{});
+  else run(std::integral_constant<int, 128>{});
 }
 template <class T>
 void read_t(hipStream_t s, const FStore& c, const int* len, const QRows& k, const QRows& v, int n, const int* first,

@@ -291,11 +291,12 @@ rtg_result rtg_attend_packed(rtg_dtype dtype, const rtg_rows* q, const rtg_rows*
   if (n_q_head / n_head > kMaxGroup)
     return err("%zu query heads per key/value head exceed %zu", n_q_head / n_head, kMaxGroup);
   if (n_seq == 0 || n_seq > 1000000) return err("n_seq must be within 1 .. 1000000");
-  constexpr size_t kMost = 100000000;  // of rows and query heads, and of workgroups
-  if (n_rows > kMost || n_q_head > 1000000 || n_rows * n_q_head > kMost * 16)
-    return err("%zu rows of %zu heads exceed %zu", n_rows, n_q_head, kMost * 16);
-  if ((n_rows * (n_q_head / n_head) / 128 + 1 + n_seq) * n_head > kMost)
-    return err("%zu sequences of %zu heads are too many", n_seq, n_head);
+  // (32-bit numbers of rows and heads; a grid of 2^32 threads)
+  constexpr size_t kMostRows = 100000000, kMostPairs = 1600000000, kMostGroups = 8000000;
+  if (n_rows > kMostRows || n_q_head > 1000000 || n_rows * n_q_head > kMostPairs)
+    return err("%zu rows of %zu heads exceed %zu", n_rows, n_q_head, kMostPairs);
+  if ((n_rows * (n_q_head / n_head) / 128 + 1 + n_seq) * n_head > kMostGroups)
+    return err("%zu rows and %zu sequences of %zu heads are too many", n_rows, n_seq, n_head);
   if (!std::isfinite(scale)) return err("scale must be finite");
   if (n_rows == 0) return ok();
   if (!q->data || !k->data || !v->data || !out->data) return err("null argument");

@@ -141,18 +141,27 @@ __device__ __forceinline__ int wave_sum(int v) {
   return __builtin_amdgcn_readfirstlane((int)(y[0] + y[1]));
 }
 
-// The sum over this lane and those before it.
-__device__ __forceinline__ unsigned wave_scan(unsigned v) {
-#define RTG_STEP(ctrl, rows) v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
-  RTG_STEP(0x111, 0xF);  // row_shr:1
-  RTG_STEP(0x112, 0xF);  // row_shr:2
-  RTG_STEP(0x114, 0xF);  // row_shr:4
-  RTG_STEP(0x118, 0xF);  // row_shr:8
-  RTG_STEP(0x142, 0xA);  // row_bcast:15
-  RTG_STEP(0x143, 0xC);  // row_bcast:31
-#undef RTG_STEP
+// The sum over this lane and those before it; the largest of numbers >= 0.
+#define RTG_SCAN(combine)                                                       \
+  RTG_STEP(combine, 0x111, 0xF); /* row_shr:1 */                                \
+  RTG_STEP(combine, 0x112, 0xF); /* row_shr:2 */                                \
+  RTG_STEP(combine, 0x114, 0xF); /* row_shr:4 */                                \
+  RTG_STEP(combine, 0x118, 0xF); /* row_shr:8 */                                \
+  RTG_STEP(combine, 0x142, 0xA); /* row_bcast:15 */                             \
+  RTG_STEP(combine, 0x143, 0xC)  /* row_bcast:31 */
+#define RTG_STEP(combine, ctrl, rows) v = combine(v, __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xF, false))
+__device__ __forceinline__ int wave_scan(int v) {
+  auto sum = [](int a, int b) { return a + b; };
+  RTG_SCAN(sum);
   return v;
 }
+__device__ __forceinline__ int wave_max_scan(int v) {
+  auto most = [](int a, int b) { return max(a, b); };
+  RTG_SCAN(most);
+  return v;
+}
+#undef RTG_STEP
+#undef RTG_SCAN
 
 // Query i of a sequence of len tokens, the last `count` of which ask: keys it sees.
 __device__ __forceinline__ int keys_seen(int len, int count, int i) { return i < count ? max(len - count + i + 1, 0) : 0; }

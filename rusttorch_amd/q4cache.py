@@ -66,6 +66,8 @@ class FourBitCache(QuantisedCache):
             raise Gpt2Error(f"{what} must be contiguous float32 {list(shape)}, not {x.dtype} {list(x.shape)}")
         if x.get_device() != self._index:
             raise Gpt2Error(f"{what} is on {x.device}, the cache on {self.device}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise Gpt2Error(f"{what} requires a gradient, which the cache has none of: detach it or use torch.no_grad()")
         return x.data_ptr()
 
     # -- calls --

@@ -47,7 +47,7 @@ def test_null_arguments():
     (1, 1, 0, 64, 1, 1.0, 0, "multiple"), (1, 1025, 1, 64, 1, 1.0, 0, "exceed 1024"),
     (1, 1, 1, 64, 0, 1.0, 0, "n_seq must be within"), (1, 1, 1, 64, 10 ** 6 + 1, 1.0, 0, "n_seq must be within"),
     (10 ** 8 + 1, 1, 1, 64, 1, 1.0, 0, "exceed"), (10 ** 8, 32, 32, 64, 1, 1.0, 0, "exceed"),
-    (1, 10 ** 6, 10 ** 6, 64, 10 ** 6, 1.0, 0, "too many"), (1, 1, 1, 64, 1, float("inf"), 0, "scale must be finite"),
+    (1, 10 ** 6, 10 ** 6, 64, 10 ** 6, 1.0, 0, "too many"), (4 * 10 ** 7, 32, 32, 64, 1, 1.0, 0, "too many"), (1, 1, 1, 64, 1, float("inf"), 0, "scale must be finite"),
     (1, 1, 1, 64, 1, float("nan"), 0, "scale must be finite"), (1, 1, 1, 64, 1, 1.0, 3, "takes f32, bf16 or f16"),
 ])
 def test_packed_refuses(n_rows, q_heads, heads, dim, n_seq, scale, dtype, what):

@@ -349,6 +349,34 @@ def test_a_cache_within_a_budget(dim, dtype):
         b.attend(3, 8, weigh=0.9)
 
 
+def test_a_cache_past_32_bits():
+    """600 sequences of 8 heads of 128, 16000 tokens each: 4.9 GB of keys' codes; what the last ones hold."""
+    S, H, D, n = 600, 8, 128, 500
+    big, small = FourBitCache(S, H, D, 16000), FourBitCache(2, H, D, 16000)
+    k, v, q = (torch.randn(1, n, h, D, generator=torch.Generator(device="cuda").manual_seed(i), device="cuda").bfloat16()
+               for i, h in ((1, H), (2, H), (3, 4 * H)))
+    counts = torch.zeros(S, dtype=torch.int32, device="cuda")
+    counts[-2:] = n
+    big.append(k.expand(S, n, H, D), v.expand(S, n, H, D), counts=counts)
+    small.append(k.expand(2, n, H, D), v.expand(2, n, H, D))
+    assert big.lengths() == [0] * (S - 2) + [n, n]
+    assert all(torch.equal(a[-2:], b) for a, b in zip(big.read(20), small.read(20)))
+    for m in (1, 40):
+        a = big.attend(q[:, :m].expand(S, m, 4 * H, D), weigh=0.0)
+        b = small.attend(q[:, :m].expand(2, m, 4 * H, D), weigh=0.0)
+        # (the two may be split differently: f32 sums in another order, bf16's last place)
+        assert torch.allclose(a[-2:].float(), b.float(), rtol=2.0 ** -7, atol=2.0 ** -9) and (a[:-2] == 0).all()
+        assert torch.allclose(big.weights(n)[-2:], small.weights(n), rtol=1e-4, atol=1e-6)
+    kept = big.evict(100, recent=10)
+    assert (kept[:-2] == -1).all() and big.lengths()[-2:] == [100, 100]
+    at = kept[-1].long()
+    want = FourBitCache(1, H, D, 600)
+    want.append(k, v)
+    want = want.read(n)[1][0]
+    got = big.read(100)[1][-1]
+    assert all(torch.equal(got[:, h], want[at[h], h]) for h in range(H))
+
+
 # -- streams, captures, refusals --
 
 

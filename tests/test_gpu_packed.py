@@ -153,6 +153,27 @@ def test_offsets_out_of_range_are_clamped():
     assert torch.equal(packed_attention(q, q, q, ints([-2 ** 31, 100, 3 * 10 ** 6])), want)
 
 
+def test_offsets_that_descend():
+    """One counts as the largest before it: its sequence has no row, and no row belongs to two."""
+    g = torch.Generator().manual_seed(5)
+    q = torch.randn(300, 2, 64, generator=g).cuda()
+    for given, meant in (([0, 100, 50, 200], [0, 100, 100, 200]), ([120, 7, 7, 130], [120, 120, 120, 130]), ([300, 0, 0, 0], [300] * 4),
+                         ([50, 300, 0, 300] * 40, [50] + [300] * 159), ([0, 10, -5, 20] + [3] * 100 + [40], [0, 10, 10, 20] + [20] * 100 + [40])):
+        assert torch.equal(packed_attention(q, q, q, ints(given)), packed_attention(q, q, q, ints(meant))), given
+
+
+def test_rows_past_32_bits():
+    """8200 sequences of 64 rows, 32 heads of 128: the last ones' rows lie more than 2^31 elements in."""
+    n, rng = 8200 * 64, torch.Generator(device="cuda").manual_seed(1)
+    some = torch.randn(640, 32 + 2 * 8, 128, generator=rng, device="cuda").bfloat16()
+    qkv = torch.zeros(n, 48, 128, dtype=torch.bfloat16, device="cuda")
+    qkv[-640:] = some
+    offsets = torch.arange(0, n + 64, 64, dtype=torch.int32, device="cuda")
+    got = packed_attention(qkv[:, :32], qkv[:, 32:40], qkv[:, 40:], offsets)
+    assert n * 48 * 128 > 2 ** 31 and torch.equal(got[-640:], packed_attention(some[:, :32], some[:, 32:40], some[:, 40:], offsets[:11]))
+    assert (got[:-640] == 0).all()
+
+
 def test_captured_and_replayed():
     g = torch.Generator().manual_seed(4)
     q, k, v = (torch.randn(300, 4, 64, generator=g).cuda().bfloat16() for _ in range(3))
