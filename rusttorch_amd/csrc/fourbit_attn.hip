@@ -322,7 +322,7 @@ __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq&
 // Workgroup (sequence and head, block of columns); or, where the keys are split, one
 // of kMostSplit that get about as many tiles each, so that sequences of different
 // lengths are done at the same time (8 of 16000 to 32000 tokens of 8 heads of 128:
-// 54 us with as many parts for each, XX so).
+// 54 us with as many parts for each, 50 so).
 __device__ __forceinline__ Work work_of(const Args& a) {
   Work w;
   w.z = 0;
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(64 * kWaves) void f_attend_kernel(Args a) {
 // owner: no atomics, and sums in a fixed order. The queries lie in LDS as matrix
 // operands, as many columns at a time as fit; a wave's next tile is loaded while it
 // works on one (one token of 32 heads of 128 over 8 x 16000 in f16: 36 us with a
-// tile or four to a wave and queries from memory, XX so).
+// tile or four to a wave and queries from memory, 20 so).
 constexpr int kWeighBytes = 32 * 1024;  // of queries in LDS
 
 template <int HDP, int QP>
