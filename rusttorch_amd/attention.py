@@ -75,7 +75,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         to = _rows("out", out, shape, dtype, index)
     call = _call or _load()
     args = (_TYPES[dtype], to_q, to_k, to_v, rows, heads, kv[1], dim, offsets.data_ptr(), n,
-            dim ** -0.5 if scale is None else scale, to, _raw_stream(index))
+            (dim or 1) ** -0.5 if scale is None else scale, to, _raw_stream(index))
     if index == _device():
         check(call(*args))
     else:

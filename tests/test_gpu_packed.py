@@ -251,3 +251,9 @@ def test_refuses():
         with pytest.raises(Gpt2Error, match=what):
             call()
     assert packed_attention(x[:0], x[:0], x[:0], ints([0, 0])).shape == (0, 2, 64)
+
+
+def test_refuses_heads_of_no_channel():
+    x = torch.zeros(4, 1, 0, device="cuda")
+    with pytest.raises(Gpt2Error, match="head_dim 0"):
+        packed_attention(x, x, x, ints([0, 4]))
