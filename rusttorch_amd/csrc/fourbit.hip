@@ -258,7 +258,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const
   __shared__ unsigned hist[64][129];
   __shared__ unsigned totals[256];
   __shared__ unsigned held[kPickHeld];
-  __shared__ unsigned found[2];
+  __shared__ unsigned found[3];
   __shared__ int above[kPickWaves], equal[kPickWaves];
   const size_t sh = blockIdx.x;
   const int l = len[sh / c.n_head], tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -329,6 +329,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const
           if (before < left && left <= before + n[i]) {
             found[0] = (unsigned)(255 - 4 * lane - i);
             found[1] = left - before;
+            found[2] = n[i] == left - before;
           }
           before += n[i];
         }
@@ -337,6 +338,10 @@ __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const
     __syncthreads();
     top |= found[0] << shift;
     left = found[1];
+    if (found[2]) {  // all with these bits are kept: the others do not matter
+      left = INT32_MAX;
+      break;
+    }
   }
   // a wave's stretch of the old tokens
   const int per = (old + kPickWaves - 1) / kPickWaves, lo = min(wave * per, old), hi = min(lo + per, old);

@@ -73,19 +73,23 @@ __device__ __forceinline__ float2& stats_of(const Args& a, int seq, int i, int h
 }
 
 // A column's query as matrix operands, this lane's quarter: channels CK g + 8 j + e.
+// Loads and conversion are apart, so that loads of keys can be asked for in between.
 template <int HDP, int QP, class T>
 struct Query {
   static constexpr int J = HDP / 32;
+  float x[J][8];
   u4v q[J][QP];
   __device__ __forceinline__ void load(const Args& a, int seq, int head, const Column& cl, int g) {
     const T* row = row_of<const T>(a.q, seq, min(cl.i, a.n_q - 1), head * a.group + cl.h);
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      float x[8];
-      load8(row, HDP / 4 * g + 8 * j, a.c.hd, a.qvec, x);
+    for (int j = 0; j < J; ++j) load8(row, HDP / 4 * g + 8 * j, a.c.hd, a.qvec, x[j]);
+  }
+  __device__ __forceinline__ void convert(const Args& a) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= a.query;
-      bf16_parts<QP>(x, q[j]);
+    for (int j = 0; j < J; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[j][e] *= a.query;
+      bf16_parts<QP>(x[j], q[j]);
     }
   }
 };
@@ -384,6 +388,9 @@ __global__ __launch_bounds__(64 * kWaves) void f_attend_kernel(Args a) {
   const Work wk = work_of(a);
   if (wk.seq < 0) return;
   const int seq = wk.seq, head = wk.head, sh = seq * a.c.n_head + head, cb = wk.cb;
+  const Column cl = column(a, cb * kCols + n);
+  Query<HDP, QP, T> q;
+  q.load(a, seq, head, cl, g);
   const Seq r = seq_of(a, seq);
   // keys that the block's columns see: at most, at least (columns that are none may see anything)
   const int last_i = min(column(a, cb * kCols + kCols - 1).i, r.count - 1);
@@ -391,10 +398,7 @@ __global__ __launch_bounds__(64 * kWaves) void f_attend_kernel(Args a) {
   const int least = keys_seen(r.len, r.count, column(a, cb * kCols).i);
   const int tiles = (live + kFTile - 1) / kFTile;
   const int t0 = wk.z * wk.per, t1 = wk.n == 1 ? tiles : min(t0 + wk.per, tiles);
-  const Column cl = column(a, cb * kCols + n);
   const int lim = keys_seen(r.len, r.count, cl.i);
-  Query<HDP, QP, T> q;
-  q.load(a, seq, head, cl, g);
   f32x4 o[CV];
 #pragma unroll
   for (int d = 0; d < CV; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -411,6 +415,7 @@ __global__ __launch_bounds__(64 * kWaves) void f_attend_kernel(Args a) {
   // (one tile of a wave ahead: two or three take registers and no time off)
   int t = t0 + wave;
   if (t < t1) fetch(t);
+  q.convert(a);
   while (t < t1) {
     const Keys<HDP> k1 = k;
     Values<HDP> v1 = v;
@@ -512,11 +517,15 @@ __global__ __launch_bounds__(256) void f_weigh_kernel(Args a, float decay) {
   float* w = a.c.w + a.c.weights(sh);
   for (int cb0 = 0; cb0 == 0 || cb0 < cblocks; cb0 += W::BLOCKS) {
     const int blocks = min(W::BLOCKS, cblocks - cb0);
+    int t = (int)blockIdx.y * kWeighWaves + wave;
+    Keys<HDP> next;
+    if (t < tiles) next.load(kc + (size_t)t * 16 * HDP, ks + (size_t)t * HDP, lane);
     if (cb0 > 0) __syncthreads();
     for (int b = wave; b < blocks; b += kWeighWaves) {
       const Column cl = column(a, (cb0 + b) * kCols + n);
       Query<HDP, QP, T> q;
       q.load(a, seq, head, cl, g);
+      q.convert(a);
 #pragma unroll
       for (int j = 0; j < W::J; ++j)
 #pragma unroll
@@ -528,9 +537,6 @@ __global__ __launch_bounds__(256) void f_weigh_kernel(Args a, float decay) {
       }
     }
     __syncthreads();
-    int t = (int)blockIdx.y * kWeighWaves + wave;
-    Keys<HDP> next;
-    if (t < tiles) next.load(kc + (size_t)t * 16 * HDP, ks + (size_t)t * HDP, lane);
     for (; t < tiles; t += step) {
       const Keys<HDP> k = next;
       if (t + step < tiles) next.load(kc + (size_t)(t + step) * 16 * HDP, ks + (size_t)(t + step) * HDP, lane);
