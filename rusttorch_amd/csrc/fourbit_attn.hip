@@ -541,19 +541,23 @@ __global__ __launch_bounds__(256) void f_weigh_kernel(Args a, float decay) {
       const Keys<HDP> k = next;
       if (t + step < tiles) next.load(kc + (size_t)(t + step) * 16 * HDP, ks + (size_t)(t + step) * HDP, lane);
       const int at = t * kFTile;
+      u4v keys[2][W::J];
+#pragma unroll
+      for (int j = 0; j < W::J; ++j) {
+        keys[0][j] = k.eight(0, j);
+        keys[1][j] = k.eight(1, j);
+      }
       float sum[8] = {};
       for (int b = 0; b < blocks; ++b) {
         f32x4 x[2] = {};
 #pragma unroll
-        for (int j = 0; j < W::J; ++j) {
-          const u4v k0 = k.eight(0, j), k1 = k.eight(1, j);
+        for (int j = 0; j < W::J; ++j)
 #pragma unroll
           for (int p = 0; p < QP; ++p) {
             const u4v q = s.q[b][j][p][lane];
-            x[0] = mfma16(k0, q, x[0]);
-            x[1] = mfma16(k1, q, x[1]);
+            x[0] = mfma16(keys[0][j], q, x[0]);
+            x[1] = mfma16(keys[1][j], q, x[1]);
           }
-        }
         const float2 st = s.st[b][n];
         const int lim = s.lim[b][n] - at;  // (of the tile's tokens, in this column)
 #pragma unroll
@@ -562,15 +566,19 @@ __global__ __launch_bounds__(256) void f_weigh_kernel(Args a, float decay) {
           sum[e] += e / 4 * 16 + 4 * g + e % 4 < lim ? p : 0.f;
         }
       }
-      // lane n of the 16 that hold the sums writes one of the eight
-      float mine = 0.f;
+      // The sums over a row's 16 lanes: of two lanes each hands half of its sums over and
+      // keeps the others, until lane n has number n / 2 (22 instructions, 40 one by one).
+      float four[4], two[2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = row16_sum_k(sum[e]);
-        mine = (n & 7) == e ? y : mine;
-      }
-      const int tok = at + (n & 7) / 4 * 16 + 4 * g + (n & 3);
-      if (n < 8 && tok < r.len) {
+      for (int e = 0; e < 4; ++e)
+        four[e] = (n & 8 ? sum[e + 4] : sum[e]) + dpp_row<0x128>(n & 8 ? sum[e] : sum[e + 4]);  // row_ror:8
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        two[e] = (n & 4 ? four[e + 2] : four[e]) + dpp_row<0x141>(n & 4 ? four[e] : four[e + 2]);  // row_half_mirror
+      float mine = (n & 2 ? two[1] : two[0]) + dpp_row<0x4E>(n & 2 ? two[0] : two[1]);  // quad_perm [2,3,0,1]
+      mine += dpp_row<0xB1>(mine);                                                      // quad_perm [1,0,3,2]
+      const int tok = at + (n >> 3) * 16 + 4 * g + (n >> 1 & 3);
+      if ((n & 1) == 0 && tok < r.len) {
         const float before = cb0 > 0 ? 1.f : decay;
         w[tok] = before == 0.f ? mine : fmaf(before, w[tok], mine);
       }
