@@ -249,7 +249,7 @@ __device__ __forceinline__ unsigned pick_key(float x) {
 // wave lists what is kept of its stretch of the sequence, behind what the waves
 // before it keep. The first pass takes the weights to LDS, eight loads of a thread
 // at a time; longer sequences' are read from memory in every pass (20000 tokens of
-// 32 heads: 30 us that way, 22 from LDS).
+// 32 heads: 30 us that way, 20 from LDS).
 __global__ __launch_bounds__(64 * kPickWaves) void f_pick_kernel(FStore c, const int* len, int keep, int recent,
                                                                 int* kept) {
   constexpr int NT = 64 * kPickWaves, AHEAD = 8;

@@ -492,7 +492,7 @@ __global__ __launch_bounds__(64 * kWaves) void f_attend_kernel(Args a) {
 // owner: no atomics, and sums in a fixed order. The queries lie in LDS as matrix
 // operands, as many columns at a time as fit; a wave's next tile is loaded while it
 // works on one (one token of 32 heads of 128 over 8 x 16000 in f16: 36 us with a
-// tile or four to a wave and queries from memory, 20 so).
+// tile or four to a wave and queries from memory, 17 so).
 constexpr int kWeighBytes = 32 * 1024;  // of queries in LDS
 
 template <int HDP, int QP>
