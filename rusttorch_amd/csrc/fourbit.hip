@@ -482,14 +482,14 @@ __global__ __launch_bounds__(kMoveThreads) void f_move_kernel(FStore c, int* len
 template <class T>
 void append_t(hipStream_t s, const FStore& c, int* len, QTickets tickets, const QRows& k, const QRows& v, int n_new,
               const int* counts, const int* start, bool vec) {
-  // Four units a workgroup; enough of them to fill the device three times, as
+  // Four units a workgroup; enough of them to fill the device three times (768), as
   // sequences differ in length, but few of a sequence's, which count themselves on
   // one word, 8.6 ns each (20000 tokens of 8 heads of 128, one sequence: 2048
   // workgroups 40 us, 768 of them 30; four of 10000 to 20000: 512 77, 768 74).
   const int rows = 512 / c.hdp;  // of a unit
   const long units = n_new > 2 * rows ? (long)c.n_head * ((n_new + 4 * rows - 1) / (4 * rows))
                                       : ((long)c.n_head * ((n_new + rows - 1) / rows) + 3) / 4;
-  const long most = std::max(64l, std::min(768l, 3072l / c.n_seq));
+  const long most = std::max(64l, std::min(768l, 4 * 768l / c.n_seq));
   const dim3 grid((unsigned)c.n_seq, (unsigned)std::max(1l, std::min(most, units)));
   auto run = [&](auto width) {
     constexpr int HDP = decltype(width)::value;
