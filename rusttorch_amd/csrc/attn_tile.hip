@@ -38,6 +38,7 @@ namespace {
 
 constexpr int kKeys = 64;      // of a stage in LDS
 constexpr long kManySplit = 256;  // workgroups at most where the keys are split
+constexpr int kMinStages = 8;     // of a part at least
 constexpr float kSlack = 8.f;  // powers of two that a score may pass the running maximum by
 
 struct Args {
@@ -816,8 +817,8 @@ void many_t(hipStream_t s, Args a) {
   const long tiles = (long)grid.x * grid.y;
   if (tiles <= kManySplit) {
     // eight waves a workgroup, one workgroup a compute unit; the keys are split where there are fewer
-    a.min_stages = 8;
-    grid.z = (unsigned)std::max(1l, std::min(kManySplit / tiles, ((long)a.c.tiles / 2 + a.min_stages - 1) / a.min_stages));
+    a.min_stages = kMinStages;
+    grid.z = (unsigned)fmany_parts(tiles, a.c.tiles);
     constexpr int KG = QP == 3 ? 1 : 2;  // (f32 queries of 128 columns leave registers for four)
     if (a.c.hdp == 64) f_attend_many_kernel<64, QP, PP, T, 2><<<grid, 512, 0, s>>>(a);
     else f_attend_many_kernel<128, QP, PP, T, KG><<<grid, 256 * KG, 0, s>>>(a);
@@ -865,6 +866,9 @@ void packed(hipStream_t s, const Args& a) {
 
 }  // namespace
 
+long fmany_parts(long row_tiles, int tiles) {
+  return std::max(1l, std::min(kManySplit / row_tiles, ((long)tiles / 2 + kMinStages - 1) / kMinStages));
+}
 size_t fmany_tickets_bytes() { return (size_t)kManySplit * kQTicketStride * 4; }
 size_t fmany_work_bytes(int hdp) {
   return fmany_tickets_bytes() + (size_t)kManySplit * 4 * (hdp / 2 + 4) * 64 * 4;

@@ -82,6 +82,7 @@ void launch_f_attend(hipStream_t s, const FAttn& a);
 // for many queries (launch_f_attend chooses), and its part of the workspace
 void launch_f_attend_many(hipStream_t s, const FAttn& a, void* work);
 size_t fmany_work_bytes(int hdp);
+long fmany_parts(long row_tiles, int tiles);  // that the keys are split into, for up to 256 tiles of 128 rows
 size_t fmany_tickets_bytes();
 // w = decay * w + the probabilities that the queries (as in launch_f_attend, whose
 // stats it takes) give a token, summed over the counted queries and the heads of
