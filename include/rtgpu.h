@@ -312,8 +312,9 @@ rtg_result rtg_fourbit_append(rtg_fourbit* cache, rtg_dtype dtype, const rtg_row
 rtg_result rtg_fourbit_read(const rtg_fourbit* cache, rtg_dtype dtype, const rtg_rows* k, const rtg_rows* v, size_t n,
                             const int32_t* first, void* stream);
 /* As rtg_qcache_attend: causal attention of the last counts[s] tokens of every
- * sequence, rows of padding and of queries before the first token 0. Queries times
- * scale, scores, and 256 times the largest |v| times the number of keys have to be
+ * sequence, rows of padding and of queries before the first token 0. Sums are f32,
+ * probabilities have 24 bits for f32 results and 16 for the others (2^-16 of each),
+ * whatever the capacity; results are rounded to dtype once. Queries times scale, scores, and 256 times the largest |v| times the number of keys have to be
  * within f32. A key that reads back as NaN makes the rows NaN that see it, a value
  * their channels of the same 32, and no others; a query that is not finite gives a
  * row of NaN.

@@ -15,13 +15,14 @@
 // f16 rows are taken as they are by the f16 instructions, bf16 rows by the bf16
 // ones. f32 numbers are the sum of three bf16 parts (24 bits): of the products
 // of parts the six that reach f32's last bits are computed. Over the 4-bit cache
-// keys and values are bf16 exactly, f16 queries two parts. Probabilities: one part
-// for bf16 results (2^-9 of each, as the results' own rounding; their sum is taken
-// of the rounded ones, so that it cancels where values agree. With two the results
-// of 2047 tokens behind 12001 are 1.7e-3 off instead of 2.2e-3, nearly all of it their
-// own rounding, and take 536 us instead of 397; 16000 packed 2515 and 1832), f16 for packed f16
-// ones (from 2^-24 to 2^14 of 2^6), two bf16 parts for f16 over the cache, three
-// for f32. Sums are f32.
+// keys and values are bf16 exactly, f16 queries two parts. Probabilities over the cache: two
+// bf16 parts (16 bits) for 16-bit results, three for f32, as in the kernel of few columns: a
+// result's bits must not hang on the capacity that chooses between the two. (One part for
+// bf16 results takes 393 us instead of 536 for 2047 tokens behind 12001, and is off by 2^-9
+// of each probability, a result whose values cancel by many times its own rounding.) Of
+// packed rows: one bf16 part for bf16 (2^-9 of each, as the results' own rounding; their sum
+// is taken of the rounded ones, so that it cancels where values agree), f16 for f16 (from
+// 2^-24 to 2^14 of 2^6), three bf16 parts for f32. Sums are f32.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -896,7 +897,7 @@ void launch_f_attend_many(hipStream_t s, const FAttn& f, void* work) {
   a.qvec = by_eights(f.q, a.hd, f.type);
   a.ovec = by_eights(f.out, a.hd, f.type);
   if (f.type == Q_F32) many_t<3, 3, float>(s, a);
-  else if (f.type == Q_BF16) many_t<1, 1, __bf16>(s, a);
+  else if (f.type == Q_BF16) many_t<1, 2, __bf16>(s, a);
   else many_t<2, 2, _Float16>(s, a);
 }
 
