@@ -314,10 +314,11 @@ rtg_result rtg_fourbit_read(const rtg_fourbit* cache, rtg_dtype dtype, const rtg
 /* As rtg_qcache_attend: causal attention of the last counts[s] tokens of every
  * sequence, rows of padding and of queries before the first token 0. Sums are f32,
  * probabilities have 24 bits for f32 results and 16 for the others (2^-16 of each),
- * whatever the capacity; results are rounded to dtype once. Queries times scale, scores, and 256 times the largest |v| times the number of keys have to be
- * within f32. A key that reads back as NaN makes the rows NaN that see it, a value
- * their channels of the same 32, and no others; a query that is not finite gives a
- * row of NaN.
+ * whatever the capacity; results are rounded to dtype once. Queries times scale,
+ * scores, and 256 times the largest |v| times the number of keys have to be within
+ * f32. A key that reads back as NaN makes the rows NaN that see it, a value their
+ * channels of the same 32, and no others; a query that is not finite gives a row of
+ * NaN.
  *
  * With stats (n_seq * n_q * n_q_head * 2 f32 to work in, not NULL) the weights of all
  * tokens then become decay (0 .. 1; 0 whatever they were) times what they are, plus
@@ -350,11 +351,12 @@ rtg_result rtg_fourbit_lengths(rtg_fourbit* cache, uint32_t* out, void* stream);
  * Rows of no sequence are set to 0. Query head h reads
  * key/value head h / (n_q_head / n_head), at most 1024 of them one.
  *
- * softmax of scale * q . k; sums are f32, results rounded to dtype once, the
- * probabilities of bf16 rows to bf16 (sums of f16 and bf16 rows: of the rounded
- * ones). Queries times scale, scores, and 256 times the largest |v| times the
- * number of keys have to be within f32. A key with a value that is not finite
- * makes the rows not finite that see it, a value their channel, and no others.
+ * softmax of scale * q . k; sums are f32, results rounded to dtype once.
+ * Probabilities have 24 bits for f32 rows, 16 for bf16 (2^-16 of each) and 22 for
+ * f16, there in steps of 2^-30 of the row's largest. Queries times scale, scores, and
+ * 256 times the largest |v| times the number of keys have to be within f32. A key with
+ * a value that is not finite makes the rows not finite that see it, a value their
+ * channel, and no others.
  * Enqueues one kernel on `stream`, allocates nothing, may be captured; out must
  * not overlap the others. ---- */
 rtg_result rtg_attend_packed(rtg_dtype dtype, const rtg_rows* q, const rtg_rows* k, const rtg_rows* v, size_t n_rows,

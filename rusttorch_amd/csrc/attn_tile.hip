@@ -15,14 +15,14 @@
 // f16 rows are taken as they are by the f16 instructions, bf16 rows by the bf16
 // ones. f32 numbers are the sum of three bf16 parts (24 bits): of the products
 // of parts the six that reach f32's last bits are computed. Over the 4-bit cache
-// keys and values are bf16 exactly, f16 queries two parts. Probabilities over the cache: two
-// bf16 parts (16 bits) for 16-bit results, three for f32, as in the kernel of few columns: a
-// result's bits must not hang on the capacity that chooses between the two. (One part for
-// bf16 results takes 393 us instead of 536 for 2047 tokens behind 12001, and is off by 2^-9
-// of each probability, a result whose values cancel by many times its own rounding.) Of
-// packed rows: one bf16 part for bf16 (2^-9 of each, as the results' own rounding; their sum
-// is taken of the rounded ones, so that it cancels where values agree), f16 for f16 (from
-// 2^-24 to 2^14 of 2^6), three bf16 parts for f32. Sums are f32.
+// keys and values are bf16 exactly, f16 queries two parts. Probabilities have two parts for
+// 16-bit results, three for f32: bf16's to 2^-16 of each over the cache and of packed bf16
+// rows, as in the kernel of few columns (a result's bits must not hang on the capacity that
+// chooses between the two); f16's of packed f16 rows, from 2^14 to 2^-24 of 2^6, to 2^-22.
+// (One part takes 393 us instead of 525 for 2047 bf16 tokens behind 12001, 1751 instead of
+// 2380 for 16000 packed ones of 32 heads over 8 of 128, 154 instead of 216 for 8000 in f16 of
+// 16 heads of 64, and is off by 2^-9 of each probability, 2^-11 in f16: a result whose values
+// cancel by many times its own rounding.) Sums are f32.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -74,13 +74,6 @@ struct Bf16 {
   static __device__ __forceinline__ f32x16 mfma(const u4v& a, const u4v& b, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ unsigned two(float x, float y) {
-    const V2 v = {(__bf16)x, (__bf16)y};
-    return __builtin_bit_cast(unsigned, v);
-  }
-  static __device__ __forceinline__ float add2(unsigned x, float c) {
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(V2, x), __builtin_bit_cast(V2, 0x3F803F80u), c, false);
-  }
   static constexpr unsigned kExponents = 0x7F807F80u, kLowest = 0x00800080u;
 };
 struct F16 {
@@ -93,9 +86,6 @@ struct F16 {
     const V2 v = {(_Float16)x, (_Float16)y};
     return __builtin_bit_cast(unsigned, v);
   }
-  static __device__ __forceinline__ float add2(unsigned x, float c) {
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(V2, x), __builtin_bit_cast(V2, 0x3C003C00u), c, false);
-  }
   static constexpr unsigned kExponents = 0x7C007C00u, kLowest = 0x04000400u;
 };
 
@@ -103,9 +93,13 @@ struct F16 {
 template <class M, int N>
 __device__ __forceinline__ void parts_of(const float (&x)[8], u4v (&p)[N]) {
   if constexpr (std::is_same_v<M, F16>) {
-    static_assert(N == 1, "f16 rows are one part");
+    static_assert(N <= 2, "f16 rows are one part, probabilities two");
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[0][i] = M::two(x[2 * i], x[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) {
+      const typename M::V2 hi = {(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+      p[0][i] = __builtin_bit_cast(unsigned, hi);
+      if constexpr (N == 2) p[1][i] = M::two(x[2 * i] - (float)hi[0], x[2 * i + 1] - (float)hi[1]);
+    }
   } else {
     bf16_parts<N>(x, p);
   }
@@ -463,7 +457,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
   f32x16 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = f32x16{};
-  float m = -INFINITY, l = 0.f, l_whole = 0.f;  // l_whole: of unrounded probabilities, for the stats
+  float m = -INFINITY, l = 0.f;
   if constexpr (!Stage::kDirect && NB == 2) {
     __syncthreads();
     if (own < live) st.store(bufs[0], s.bad, own, live, edge_at(begin));
@@ -544,7 +538,6 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       const float f = top > m + kSlack ? __builtin_amdgcn_exp2f(m - top) : 1.f;
       m = top > m + kSlack ? top : m;
       l *= f;
-      l_whole *= f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= f;
     }
@@ -555,10 +548,6 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
 #pragma unroll
       for (int e = 0; e < 32; ++e)
         if (at + e / 16 * 32 + e % 16 / 4 * 8 + half * 4 + e % 4 >= lim) p[e / 16][e % 16] = 0.f;
-    }
-    if (PP == 1 && a.stats) {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) l_whole += p[e / 16][e % 16];
     }
     in_products(true);
 #pragma unroll
@@ -572,13 +561,8 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
         for (int e = 0; e < 8; ++e) x[e] = p[sub][u * 8 + e];
         u4v pp[PP];
         parts_of<M, PP>(x, pp);
-        if constexpr (PP == 1) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) l = M::add2(pp[0][e], l);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) l += x[e];
-        }
+        for (int e = 0; e < 8; ++e) l += x[e];
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -611,7 +595,7 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
   for (; at < live; at += SPAN) step(at, std::true_type{}, NB == 1 ? 0u : (unsigned)((at - begin) / SPAN) & 1u);
   if constexpr (KG > 1) {
     // the groups' results meet in LDS, value by value with the lanes side by side
-    constexpr int N = DT * 16 + 3;
+    constexpr int N = DT * 16 + 2;
     static_assert(sizeof(s.b) >= (KG - 1) * (Stage::NT / 64) * N * 64 * 4, "room for the results");
     __syncthreads();
     float* to = reinterpret_cast<float*>(&s.b) + ((group - 1) * (Stage::NT / 64) + wave) * N * 64 + lane;
@@ -620,19 +604,17 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) to[(d * 16 + e) * 64] = o[d][e];
-      to[(N - 3) * 64] = m;
-      to[(N - 2) * 64] = l;
-      to[(N - 1) * 64] = l_whole;
+      to[(N - 2) * 64] = m;
+      to[(N - 1) * 64] = l;
     }
     __syncthreads();
     if (group > 0) return;
     for (int g = 1; g < KG; ++g) {
       const float* x = reinterpret_cast<const float*>(&s.b) + ((g - 1) * (Stage::NT / 64) + wave) * N * 64 + lane;
-      const float m2 = x[(N - 3) * 64], most = fmaxf(m, m2), base = most == -INFINITY ? 0.f : most;
+      const float m2 = x[(N - 2) * 64], most = fmaxf(m, m2), base = most == -INFINITY ? 0.f : most;
       const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
       m = most;
-      l = fmaf(f, l, f2 * x[(N - 2) * 64]);
-      l_whole = fmaf(f, l_whole, f2 * x[(N - 1) * 64]);
+      l = fmaf(f, l, f2 * x[(N - 1) * 64]);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -649,31 +631,29 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
   if (splits > 1) {
     // Every wave's results, in pairs with the lanes side by side, past the L2 caches;
     // the last of a tile's waves of one number to come here joins theirs, in order.
-    constexpr int N = DT * 16 + 4;
+    constexpr int N = DT * 16 + 2;
     float* p = a.parts + ((size_t)(job.slot * job.zs + job.z) * (Stage::NT / 64) + wave) * N * 64 + lane * 2;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 16; e += 2) store2(p + (d * 16 + e) * 64, o[d][e], o[d][e + 1]);
-    store2(p + (N - 4) * 64, m, l);
-    store2(p + (N - 2) * 64, l_whole, 0.f);
+    store2(p + (N - 2) * 64, m, l);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores have completed
     unsigned before = 0, *count = a.tickets + (size_t)job.slot * kQTicketStride + wave;
     if (lane == 0) before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (__builtin_amdgcn_readfirstlane(before) != (unsigned)splits - 1) return;
     if (lane == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     m = -INFINITY;
-    l = l_whole = 0.f;
+    l = 0.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = f32x16{};
     for (int z = 0; z < splits; ++z) {
       const float* x = a.parts + ((size_t)(job.slot * job.zs + z) * (Stage::NT / 64) + wave) * N * 64 + lane * 2;
-      const float2 ml = load2(x + (N - 4) * 64), lw = load2(x + (N - 2) * 64);
+      const float2 ml = load2(x + (N - 2) * 64);
       const float most = fmaxf(m, ml.x), base = most == -INFINITY ? 0.f : most;
       const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(ml.x - base);
       m = most;
       l = fmaf(f, l, f2 * ml.y);
-      l_whole = fmaf(f, l_whole, f2 * lw.x);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -698,11 +678,8 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
       for (int r = 0; r < 4; ++r) x[r] = any ? o[d][e + r] * inv : 0.f;
       store4(out, d * 32 + e / 4 * 8 + half * 4, a.hd, make_float4(x[0], x[1], x[2], x[3]), a.ovec);
     }
-  if (a.stats) {
-    if (PP == 1) l = xor32_sum_k(l_whole);
-    if (half == 0)
-      reinterpret_cast<float2*>(a.stats)[((size_t)job.seq * a.n_q + i) * a.n_q_head + head] = make_float2(m - M::kUp, any ? l : 0.f);
-  }
+  if (a.stats && half == 0)
+    reinterpret_cast<float2*>(a.stats)[((size_t)job.seq * a.n_q + i) * a.n_q_head + head] = make_float2(m - M::kUp, any ? l : 0.f);
 }
 
 template <int HD, int QP, int PP, class T, int KG>
@@ -800,7 +777,7 @@ __global__ __launch_bounds__(Stage::NT * KG, KG > 1 || HD == 64 || P == 1 ? 2 : 
   }
   if (j.tile >= 0) {
     a.n_q = j.count;
-    return attend<M, HD, P, P, T, Stage, KG>(a, j, s);
+    return attend<M, HD, P, P == 1 ? 2 : P, T, Stage, KG>(a, j, s);
   }
   // `at` workgroups of this head are before this one among those that are left
   const int start = min(max(a.offsets[0], 0), a.n_rows), spare = start + a.n_rows - end;
@@ -872,7 +849,7 @@ long fmany_parts(long row_tiles, int tiles) {
 }
 size_t fmany_tickets_bytes() { return (size_t)kManySplit * kQTicketStride * 4; }
 size_t fmany_work_bytes(int hdp) {
-  return fmany_tickets_bytes() + (size_t)kManySplit * 4 * (hdp / 2 + 4) * 64 * 4;
+  return fmany_tickets_bytes() + (size_t)kManySplit * 4 * (hdp / 2 + 2) * 64 * 4;
 }
 
 void launch_f_attend_many(hipStream_t s, const FAttn& f, void* work) {

@@ -4,14 +4,16 @@ import numpy as np
 import pytest
 import torch
 
+from rusttorch_amd.attention import packed_attention
 from rusttorch_amd.q4cache import FourBitCache
 from tests.fourbit_ref import attention, held
 from tests.test_gpu_fourbit import TYPES, ints, near
 
 pytestmark = pytest.mark.gpu
 
-# A probability as two parts: 8 bits cut and 8 of the rest to nearest, 2^-7 2^-9; as three for f32.
+# A probability as two parts: 8 bits cut and 8 of the rest to nearest, 2^-7 2^-9; two of f16, 2^-11 2^-11.
 STEP = {"f32": 2.0 ** -24, "bf16": 2.0 ** -16, "f16": 2.0 ** -16}
+PACKED_STEP = {"f32": 2.0 ** -24, "bf16": 2.0 ** -16, "f16": 2.0 ** -22}
 
 
 def pairs(n, heads, kv, dim, dtype, seed):
@@ -23,6 +25,20 @@ def pairs(n, heads, kv, dim, dtype, seed):
     v[1::2] = -v[0::2]
     out = [torch.from_numpy(x).to(TYPES[dtype]) for x in (q, k, v)]
     return [x.cuda() for x in out], [x.double().numpy() for x in out]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("n", [48, 700])
+def test_packed(dim, dtype, n):
+    print(f"[gpu] packed pairs {n} x 4 over 2 of {dim}, {dtype}", flush=True)
+    (q, k, v), (qn, kn, vn) = pairs(n, 4, 2, dim, dtype, n + dim)
+    got = packed_attention(q, k, v, ints([0, n]))
+    want, off = np.zeros(qn.shape), np.zeros(qn.shape)
+    for h in range(4):
+        want[:, h], off[:, h], *_ = attention(qn[:, h], kn[:, h // 2], vn[:, h // 2], np.arange(n) + 1, dim ** -0.5,
+                                              PACKED_STEP[dtype], 2.0 ** -31 if dtype == "f16" else 2.0 ** -125)
+    near(got, want, off, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
