@@ -326,7 +326,8 @@ __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq&
 // Workgroup (sequence and head, block of columns); or, where the keys are split, one
 // of kMostSplit that get about as many tiles each, so that sequences of different
 // lengths are done at the same time (8 of 16000 to 32000 tokens of 8 heads of 128:
-// 54 us with as many parts for each, 50 so).
+// 54 us with as many parts for each, 50 so). Blocks of padding take one each, which
+// only writes zeros, and leave the others to those that read keys.
 __device__ __forceinline__ Work work_of(const Args& a) {
   Work w;
   w.z = 0;
@@ -339,39 +340,51 @@ __device__ __forceinline__ Work work_of(const Args& a) {
     w.slot0 = w.stride = w.ticket = 0;
     return w;
   }
-  const int lane = threadIdx.x & 63, inner = a.c.n_head * a.cblocks;
+  const int lane = threadIdx.x & 63, heads = a.c.n_head, inner = heads * a.cblocks;
+  // the tiles, and the blocks of columns with queries in them, of the sequences s0 + lane
   auto tiles_at = [&](int s0) { return s0 + lane < a.c.n_seq ? (a.len[s0 + lane] + kFTile - 1) / kFTile : 0; };
+  auto busy_at = [&](int s0) { return s0 + lane < a.c.n_seq ? (seq_of(a, s0 + lane).count * a.group + kCols - 1) / kCols : 0; };
   auto parts_of = [&](int tiles, int each) { return tiles <= kWhole ? 1 : (tiles + each - 1) / each; };
-  int total = 0;
-  for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) total += wave_sum(tiles_at(s0));
+  int total = 0, idle = a.c.n_seq * inner;
+  for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
+    const int busy = busy_at(s0) * heads;
+    total += wave_sum(tiles_at(s0) * busy);
+    idle -= wave_sum(busy);
+  }
   // the fewest tiles to a part, or up to a 16th more, with which there are not too many parts
-  const int room = kMostSplit / inner;
+  const int room = kMostSplit - idle;
   int each = max((total + room - 1) / room, kSplitTiles);
   for (;; each += each / 16 + 1) {
     int parts = 0;
-    for (int s0 = 0; s0 < a.c.n_seq; s0 += 64)
-      parts += wave_sum(s0 + lane < a.c.n_seq ? parts_of(tiles_at(s0), each) : 0);
-    if (parts <= room) break;  // (each sequence has one where `each` is large; there are at most room / 2 sequences)
+    for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) parts += wave_sum(busy_at(s0) * heads * parts_of(tiles_at(s0), each));
+    if (parts <= room) break;  // (each block has one where `each` is large; there are at most kMostSplit / 2 blocks)
   }
   int at = (int)blockIdx.x;
   w.seq = -1;
   for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) {
-    const int tiles = tiles_at(s0), parts = s0 + lane < a.c.n_seq ? parts_of(tiles, each) : 0;
-    const int incl = wave_scan(parts * inner);
-    const unsigned long long mine = __builtin_amdgcn_ballot_w64(at >= incl - parts * inner && at < incl);
+    const int tiles = tiles_at(s0), parts = parts_of(tiles, each), busy = busy_at(s0);
+    const int mine_all = s0 + lane < a.c.n_seq ? inner + busy * heads * (parts - 1) : 0;
+    const int incl = wave_scan(mine_all);
+    const unsigned long long mine = __builtin_amdgcn_ballot_w64(at >= incl - mine_all && at < incl);
     if (mine) {
-      const int l = __builtin_ctzll(mine);
+      const int l = __builtin_ctzll(mine), n = __builtin_amdgcn_readlane(parts, l), b = __builtin_amdgcn_readlane(busy, l);
       w.seq = s0 + l;
-      w.n = __builtin_amdgcn_readlane(parts, l);
-      w.per = (__builtin_amdgcn_readlane(tiles, l) + w.n - 1) / w.n;
-      const int rest = at - (__builtin_amdgcn_readlane(incl, l) - w.n * inner);
-      w.z = rest / inner;
-      const int pair = rest - w.z * inner;
-      w.head = pair / a.cblocks;
-      w.cb = pair - w.head * a.cblocks;
-      w.stride = inner;
-      w.slot0 = (int)blockIdx.x - w.z * inner;
-      w.ticket = w.seq * inner + pair;
+      const int rest = at - __builtin_amdgcn_readlane(incl - mine_all, l), split = b * heads * n;
+      w.stride = b * heads;
+      if (rest < split) {
+        w.n = n;
+        w.per = (__builtin_amdgcn_readlane(tiles, l) + n - 1) / n;
+        w.z = rest / w.stride;
+        const int pair = rest - w.z * w.stride;
+        w.head = pair / b;
+        w.cb = pair - w.head * b;
+      } else {
+        const int none = a.cblocks - b;
+        w.head = (rest - split) / none;
+        w.cb = b + rest - split - w.head * none;
+      }
+      w.slot0 = (int)blockIdx.x - w.z * w.stride;
+      w.ticket = w.seq * inner + w.head * a.cblocks + w.cb;
       return w;
     }
     at -= __builtin_amdgcn_readlane(incl, 63);
@@ -393,9 +406,11 @@ __global__ __launch_bounds__(64 * kWaves) void f_attend_kernel(Args a) {
   q.load(a, seq, head, cl, g);
   const Seq r = seq_of(a, seq);
   // keys that the block's columns see: at most, at least (columns that are none may see anything)
-  const int last_i = min(column(a, cb * kCols + kCols - 1).i, r.count - 1);
-  const int live = last_i >= 0 ? keys_seen(r.len, r.count, last_i) : 0;
-  const int least = keys_seen(r.len, r.count, column(a, cb * kCols).i);
+  // (a block of padding none: 60 queries' room for one of each of 64 sequences, 8 heads of 64
+  // behind 8000 tokens in f32, takes 76 us, 303 where they all go over the keys)
+  const int first_i = column(a, cb * kCols).i, last_i = min(column(a, cb * kCols + kCols - 1).i, r.count - 1);
+  const int live = first_i < r.count ? keys_seen(r.len, r.count, last_i) : 0;
+  const int least = keys_seen(r.len, r.count, first_i);
   const int tiles = (live + kFTile - 1) / kFTile;
   const int t0 = wk.z * wk.per, t1 = wk.n == 1 ? tiles : min(t0 + wk.per, tiles);
   const int lim = keys_seen(r.len, r.count, cl.i);
@@ -638,7 +653,7 @@ void weigh_t(hipStream_t s, const FAttn& f, float decay) {
 namespace {
 size_t few_work_bytes(int hdp) { return (size_t)kMostSplit * (kQTicketStride * 4 + (size_t)kCols * (hdp + 2) * 4); }
 }  // namespace
-// (one call at a time: both kernels' partial results lie in the same memory, their tickets apart)
+// (each kernel's tickets and partial results, one behind the other)
 size_t fattn_work_bytes(int hdp) { return few_work_bytes(hdp) + fmany_work_bytes(hdp); }
 void fattn_work_clear(hipStream_t s, void* work, int hdp) {
   (void)hipMemsetAsync(work, 0, (size_t)kMostSplit * kQTicketStride * 4, s);
