@@ -758,7 +758,50 @@ __global__ __launch_bounds__(Stage::NT * KG, KG > 1 || HD == 64 || P == 1 ? 2 : 
     index = block / a.n_head;
     j.head = block - index * a.n_head;
     at = index;
-    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+    int s0 = 0;
+    // Sequences that end before this tile, 256 N at a time: a lane has four in a row of
+    // each 256, the next ones' offsets are on their way (10000 sequences of 20 tokens, 12
+    // heads of 64 in f32: 3.4 ms, 13.3 by 64 at a time).
+    auto skip = [&](auto chunks) {
+      constexpr int N = decltype(chunks)::value, SPAN = 256 * N;
+      typedef int I4 __attribute__((ext_vector_type(4), aligned(4)));
+      I4 next[N];
+      auto load = [&](int s) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) next[u] = *reinterpret_cast<const I4*>(a.offsets + s + 1 + u * 256 + lane * 4);
+      };
+      if (s0 + SPAN <= a.n_seq) load(s0);
+      for (; s0 + SPAN <= a.n_seq; s0 += SPAN) {
+        I4 o[N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) o[u] = next[u];
+        if (s0 + 2 * SPAN <= a.n_seq) load(s0 + SPAN);
+        int last = end, tiles = 0;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          int h[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) h[i] = max(min(max(o[u][i], 0), a.n_rows), i ? h[i ? i - 1 : 0] : 0);
+          const int upto = max(wave_max_scan(h[3]), last);
+          int from = __shfl_up(upto, 1, 64);
+          if (lane == 0) from = last;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int to = max(h[i], from);
+            tiles += ((to - from) * a.group + ROWS - 1) / ROWS;
+            from = to;
+          }
+          last = __builtin_amdgcn_readlane(upto, 63);
+        }
+        const int sum = wave_sum(tiles);
+        if (at < sum) return;
+        at -= sum;
+        end = last;
+      }
+    };
+    skip(std::integral_constant<int, 4>{});
+    skip(std::integral_constant<int, 1>{});
+    for (; s0 < a.n_seq; s0 += 64) {
       const int tiles = sequences(s0);
       int incl = tiles;
 #pragma unroll
