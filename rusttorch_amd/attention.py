@@ -7,7 +7,7 @@ import torch
 
 from . import _lib
 from ._lib import Gpt2Error, check
-from .qcache import _TYPES, _one_runtime, _pack_rows, _raw_stream
+from .qcache import _TYPES, _no_gradient, _one_runtime, _pack_rows, _raw_stream
 
 __all__ = ["packed_attention"]
 
@@ -33,8 +33,7 @@ def _rows(what: str, x: torch.Tensor, shape, dtype, index: int) -> bytes:
         raise Gpt2Error(f"{what} must be {dtype}, not {x.dtype}")
     if x.get_device() != index:
         raise Gpt2Error(f"{what} is on {x.device}, q on GPU {index}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise Gpt2Error(f"{what} requires a gradient, which packed_attention has none of: detach it or use torch.no_grad()")
+    _no_gradient(what, x, "packed_attention")
     row, head, col = x.stride()
     if col != 1 and shape[2] > 1 and x.numel():
         raise Gpt2Error(f"{what}'s last dimension must be contiguous")

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from ._lib import Gpt2Error, check
-from .qcache import _TYPES, QuantisedCache, _one_runtime, _pack_rows
+from .qcache import _TYPES, QuantisedCache, _no_gradient, _one_runtime, _pack_rows
 
 __all__ = ["FourBitCache"]
 
@@ -66,8 +66,7 @@ class FourBitCache(QuantisedCache):
             raise Gpt2Error(f"{what} must be contiguous float32 {list(shape)}, not {x.dtype} {list(x.shape)}")
         if x.get_device() != self._index:
             raise Gpt2Error(f"{what} is on {x.device}, the cache on {self.device}")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise Gpt2Error(f"{what} requires a gradient, which the cache has none of: detach it or use torch.no_grad()")
+        _no_gradient(what, x, "the cache")
         return x.data_ptr()
 
     # -- calls --

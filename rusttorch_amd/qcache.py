@@ -19,6 +19,7 @@ import ctypes as C
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import Gpt2Error, check
@@ -41,6 +42,14 @@ def _one_runtime() -> None:
     if len(paths) > 1:
         raise Gpt2Error("two HIP runtimes are loaded (" + ", ".join(sorted(paths)) +
                         "): import torch before the library is first used")
+
+
+def _no_gradient(what: str, x: torch.Tensor, whose: str) -> None:
+    """Refuses an x whose gradient, backward or forward, would be lost."""
+    if x.requires_grad and torch.is_grad_enabled():
+        raise Gpt2Error(f"{what} requires a gradient, which {whose} has none of: detach it or use torch.no_grad()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise Gpt2Error(f"{what} has a forward-mode tangent, which {whose} does not carry on: take its primal")
 
 
 class QuantisedCache:
@@ -100,8 +109,7 @@ class QuantisedCache:
             raise Gpt2Error(f"{what} must be {dtype}, not {x.dtype}")
         if x.get_device() != self._index:
             raise Gpt2Error(f"{what} is on {x.device}, the cache on {self.device}")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise Gpt2Error(f"{what} requires a gradient, which the cache has none of: detach it or use torch.no_grad()")
+        _no_gradient(what, x, "the cache")
         seq, tok, head, col = x.stride()
         if col != 1 and self.head_dim > 1 and x.numel():
             raise Gpt2Error(f"{what}'s last dimension must be contiguous")
