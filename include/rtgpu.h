@@ -354,9 +354,11 @@ rtg_result rtg_fourbit_lengths(rtg_fourbit* cache, uint32_t* out, void* stream);
  * softmax of scale * q . k; sums are f32, results rounded to dtype once.
  * Probabilities have 24 bits for f32 rows, 16 for bf16 (2^-16 of each) and 22 for
  * f16, there in steps of 2^-30 of the row's largest. Queries times scale, scores, and
- * 256 times the largest |v| times the number of keys have to be within f32. A key with
- * a value that is not finite makes the rows not finite that see it, a value their
- * channel, and no others.
+ * 256 times the largest |v| times the number of keys have to be within f32.
+ * What is not finite: a query makes its row NaN, a value the channel not finite of the
+ * rows that see it, a NaN in a key the rows NaN that see it. An infinity in a key does
+ * the same for f32 rows; of bf16 and f16 ones it counts as the score that it gives, so
+ * a score of -infinity takes no part in its row. No other results depend on them.
  * Enqueues one kernel on `stream`, allocates nothing, may be captured; out must
  * not overlap the others. ---- */
 rtg_result rtg_attend_packed(rtg_dtype dtype, const rtg_rows* q, const rtg_rows* k, const rtg_rows* v, size_t n_rows,
