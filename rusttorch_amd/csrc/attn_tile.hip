@@ -236,6 +236,7 @@ struct RowStage {
   static constexpr int KP = P, NB = BUFFERS, CH = HD / 8, NT = 64 * NW, N = kKeys * CH / NT;
   static constexpr bool kDirect = false;
   typedef T T8 __attribute__((ext_vector_type(8)));
+  typedef T Aligned8 __attribute__((ext_vector_type(8), aligned(16)));  // (eight f32 are not aligned to their size)
   typedef Buffer<HD, P> Buf;
   T8 k[N], v[N];
   int tid;
@@ -243,7 +244,7 @@ struct RowStage {
   __device__ __forceinline__ void init(const Args&, const Job&, Buf (&)[NB], int thread) { tid = thread; }
   static __device__ __forceinline__ void load1(const T* row, int c8, int n, T8& x) {
     if constexpr (VEC) {
-      x = *reinterpret_cast<const T8*>(row + c8);
+      x = *reinterpret_cast<const Aligned8*>(row + c8);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
