@@ -283,8 +283,9 @@ rtg_result rtg_qcache_attend(rtg_qcache* cache, rtg_dtype dtype, const rtg_rows*
 rtg_result rtg_qcache_lengths(rtg_qcache* cache, uint32_t* out, void* stream);
 
 /* ---- 4-bit key/value cache over device tensors, and its eviction (no
- * counterpart in the reference). A quarter to an eighth of the memory of f32 and
- * bf16 rows and half of the 8-bit cache's, for contexts that are long or many.
+ * counterpart in the reference). An eighth and a quarter of the memory of f32 and
+ * bf16 rows and half of the 8-bit cache's, for contexts that are long or many; up to
+ * half as much again, 17 MB at most, for attention's partial results.
  *
  * For each (sequence, head) and token, keys and values apart, 32 consecutive
  * channels are numbers of 4 bits (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times a

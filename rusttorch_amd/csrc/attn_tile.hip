@@ -38,7 +38,6 @@ namespace rtg {
 namespace {
 
 constexpr int kKeys = 64;      // of a stage in LDS
-constexpr long kManySplit = 256;  // workgroups at most where the keys are split
 constexpr int kMinStages = 8;     // of a part at least
 constexpr float kSlack = 8.f;  // powers of two that a score may pass the running maximum by
 
@@ -837,10 +836,10 @@ template <int QP, int PP, class T>
 void many_t(hipStream_t s, Args a) {
   dim3 grid((unsigned)(a.n_seq * a.n_head), (unsigned)((a.n_q * a.group + 127) / 128));
   const long tiles = (long)grid.x * grid.y;
-  if (tiles <= kManySplit) {
+  if (tiles <= kSplits) {
     // eight waves a workgroup, one workgroup a compute unit; the keys are split where there are fewer
     a.min_stages = kMinStages;
-    grid.z = (unsigned)fmany_parts(tiles, a.c.tiles);
+    grid.z = (unsigned)fmany_parts(tiles, a.c);
     constexpr int KG = QP == 3 ? 1 : 2;  // (f32 queries of 128 columns leave registers for four)
     if (a.c.hdp == 64) f_attend_many_kernel<64, QP, PP, T, 2><<<grid, 512, 0, s>>>(a);
     else f_attend_many_kernel<128, QP, PP, T, KG><<<grid, 256 * KG, 0, s>>>(a);
@@ -888,18 +887,14 @@ void packed(hipStream_t s, const Args& a) {
 
 }  // namespace
 
-long fmany_parts(long row_tiles, int tiles) {
-  return std::max(1l, std::min(kManySplit / row_tiles, ((long)tiles / 2 + kMinStages - 1) / kMinStages));
-}
-size_t fmany_tickets_bytes() { return (size_t)kManySplit * kQTicketStride * 4; }
-size_t fmany_work_bytes(int hdp) {
-  return fmany_tickets_bytes() + (size_t)kManySplit * 4 * (hdp / 2 + 2) * 64 * 4;
+long fmany_parts(long row_tiles, const FStore& c) {
+  return std::max(1l, std::min(many_room(c) / row_tiles, ((long)c.tiles / 2 + kMinStages - 1) / kMinStages));
 }
 
-void launch_f_attend_many(hipStream_t s, const FAttn& f, void* work) {
+void launch_f_attend_many(hipStream_t s, const FAttn& f) {
   Args a = {};
-  a.tickets = static_cast<unsigned*>(work);
-  a.parts = reinterpret_cast<float*>(static_cast<char*>(work) + fmany_tickets_bytes());
+  a.tickets = reinterpret_cast<unsigned*>(static_cast<char*>(f.work) + kTicketBytes);
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(f.work) + 2 * kTicketBytes);
   a.q = f.q;
   a.out = f.out;
   a.c = f.c;

@@ -66,7 +66,9 @@ void launch_f_evict(hipStream_t s, const FStore& c, int* len, QTickets tickets, 
 
 // Attention as launch_q_attend, results as rows; stats [seq][n_q][n_q_head][2] (may
 // be null): for each query's scores x (times log2 e) an m and the sum of 2^(x - m),
-// 0 where it sees no key. work: fattn_work_bytes() bytes, cleared once (fattn_work_clear).
+// 0 where it sees no key. work: fattn_work_bytes() bytes, cleared once (fattn_work_clear):
+// tickets of the kernels of few columns and of many rows, kSplits of each, then partial
+// results of either (one call at a time works on a cache).
 struct FAttn {
   FStore c;
   const int* len = nullptr;
@@ -79,17 +81,34 @@ struct FAttn {
   void* work = nullptr;
 };
 void launch_f_attend(hipStream_t s, const FAttn& a);
-// for many queries (launch_f_attend chooses), and its part of the workspace
-void launch_f_attend_many(hipStream_t s, const FAttn& a, void* work);
-size_t fmany_work_bytes(int hdp);
-long fmany_parts(long row_tiles, int tiles);  // that the keys are split into, for up to 256 tiles of 128 rows
-size_t fmany_tickets_bytes();
+// for many queries (launch_f_attend chooses)
+void launch_f_attend_many(hipStream_t s, const FAttn& a);
+long fmany_parts(long row_tiles, const FStore& c);  // that the keys are split into, for up to kSplits tiles of 128 rows
 // w = decay * w + the probabilities that the queries (as in launch_f_attend, whose
 // stats it takes) give a token, summed over the counted queries and the heads of
 // the token's head; decay 0: w as it was is not read.
 void launch_f_weigh(hipStream_t s, const FAttn& a, float decay);
-size_t fattn_work_bytes(int hdp);
-void fattn_work_clear(hipStream_t s, void* work, int hdp);
+size_t fattn_work_bytes(const FStore& c);
+void fattn_work_clear(hipStream_t s, void* work);
+
+// Workgroups at most where the keys are split, and how many of them there is room for.
+// One's results take 4 KB (16 columns) or 34 (128 rows) for heads up to 64 channels,
+// twice that above: room for all of them, 9 or 17 MB, would be more than the keys and
+// values of a cache of up to 10000 tokens of 12 heads, and there is one for each layer;
+// so there is room for half as many bytes as the cache holds.
+constexpr int kSplits = 256;
+constexpr size_t kTicketBytes = (size_t)kSplits * kQTicketStride * 4;
+inline size_t few_part_bytes(const FStore& c) { return 16 * (size_t)(c.hdp + 2) * 4; }
+inline size_t many_part_bytes(const FStore& c) { return 128 * (size_t)(c.hdp + 4) * 4; }
+inline size_t fattn_parts_bytes(const FStore& c) {
+  const size_t half = fstore_bytes(c) / 2 / 256 * 256, all = kSplits * many_part_bytes(c);
+  return half < all ? half : all;
+}
+inline int few_room(const FStore& c) {
+  const size_t n = fattn_parts_bytes(c) / few_part_bytes(c);
+  return n < kSplits ? (int)n : kSplits;
+}
+inline int many_room(const FStore& c) { return (int)(fattn_parts_bytes(c) / many_part_bytes(c)); }
 
 // Causal attention of packed sequences, each over itself: rows [n_rows][head][hd]
 // (the rows' seq strides are not used), sequence s at rows offsets[s] ..

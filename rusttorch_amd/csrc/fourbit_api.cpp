@@ -130,7 +130,7 @@ rtg_result rtg_fourbit_new(size_t n_seq, size_t n_head, size_t head_dim, size_t 
     q->device = device;
     fstore_shape(&q->c, (int)n_seq, (int)n_head, (int)head_dim, (int)capacity);
     const size_t lens = (n_seq * 4 + 4 + 255) / 256 * 256, head = lens + n_seq * kQTicketStride * 4;
-    hipError_t e = device_malloc(&q->mem, (head + 255) / 256 * 256 + fstore_bytes(q->c) + fattn_work_bytes(q->c.hdp));
+    hipError_t e = device_malloc(&q->mem, (head + 255) / 256 * 256 + fstore_bytes(q->c) + fattn_work_bytes(q->c));
     if (e != hipSuccess) return hip_err(e, "rtg_fourbit_new");
     char* mem = static_cast<char*>(q->mem);
     q->len = static_cast<int*>(q->mem);
@@ -144,7 +144,7 @@ rtg_result rtg_fourbit_new(size_t n_seq, size_t n_head, size_t head_dim, size_t 
     if (e == hipSuccess) e = hipMemsetAsync(q->mem, 0, head, s);
     if (e == hipSuccess) e = hipMemsetAsync(q->tickets.err, 0xFF, 4, s);
     if (e == hipSuccess) {
-      fattn_work_clear(s, q->work, q->c.hdp);
+      fattn_work_clear(s, q->work);
       e = hipStreamSynchronize(s);
     }
     if (s) (void)hipStreamDestroy(s);

@@ -28,7 +28,6 @@ namespace rtg {
 namespace {
 
 constexpr int kCols = 16, kWaves = 8, kWeighWaves = 4;
-constexpr int kMostSplit = 256;  // workgroups at most where the keys are split
 constexpr int kWhole = 32, kSplitTiles = 8;  // tiles that are not split; of a split at least
 constexpr float kSlack = 8.f;     // powers of two that a score may pass the maximum by
 
@@ -41,7 +40,7 @@ struct Args {
   float query, sum;  // ScoreScale
   float* stats;
   bool qvec, ovec;
-  bool split;         // keys are split over workgroups
+  int room;           // workgroups that the keys are split over; 0: they are not
   unsigned* tickets;  // [seq][head][cblock][kQTicketStride]
   float* parts;       // [workgroup][column][hdp + 2]
 };
@@ -324,7 +323,7 @@ __device__ __forceinline__ void finish(const Args& a, Shared<HDP>& s, const Seq&
 }
 
 // Workgroup (sequence and head, block of columns); or, where the keys are split, one
-// of kMostSplit that get about as many tiles each, so that sequences of different
+// of `room` that get about as many tiles each, so that sequences of different
 // lengths are done at the same time (8 of 16000 to 32000 tokens of 8 heads of 128:
 // 54 us with as many parts for each, 50 so). Blocks of padding take one each, which
 // only writes zeros, and leave the others to those that read keys.
@@ -333,7 +332,7 @@ __device__ __forceinline__ Work work_of(const Args& a) {
   w.z = 0;
   w.n = 1;
   w.per = 0;
-  if (!a.split) {
+  if (a.room == 0) {
     w.seq = (int)blockIdx.x / a.c.n_head;
     w.head = (int)blockIdx.x - w.seq * a.c.n_head;
     w.cb = (int)blockIdx.y;
@@ -352,12 +351,12 @@ __device__ __forceinline__ Work work_of(const Args& a) {
     idle -= wave_sum(busy);
   }
   // the fewest tiles to a part, or up to a 16th more, with which there are not too many parts
-  const int room = kMostSplit - idle;
+  const int room = a.room - idle;
   int each = max((total + room - 1) / room, kSplitTiles);
   for (;; each += each / 16 + 1) {
     int parts = 0;
     for (int s0 = 0; s0 < a.c.n_seq; s0 += 64) parts += wave_sum(busy_at(s0) * heads * parts_of(tiles_at(s0), each));
-    if (parts <= room) break;  // (each block has one where `each` is large; there are at most kMostSplit / 2 blocks)
+    if (parts <= room) break;  // (each block has one where `each` is large; there are at most half as many blocks as workgroups)
   }
   int at = (int)blockIdx.x;
   w.seq = -1;
@@ -618,9 +617,9 @@ Args args_of(const FAttn& f) {
   a.stats = f.stats;
   a.qvec = by_eights(f.q, f.c.hd, f.type);
   a.ovec = by_eights(f.out, f.c.hd, f.type);
-  a.split = false;
+  a.room = 0;
   a.tickets = static_cast<unsigned*>(f.work);
-  a.parts = reinterpret_cast<float*>(static_cast<char*>(f.work) + (size_t)kMostSplit * kQTicketStride * 4);
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(f.work) + 2 * kTicketBytes);
   return a;
 }
 
@@ -633,8 +632,8 @@ void attend_t(hipStream_t s, const FAttn& f) {
   // 62, as the partial results take their time), and more than 32 tiles, for a join
   // takes as long as four rounds of the eight waves.
   const long blocks = (long)f.c.n_seq * f.c.n_head * a.cblocks;
-  a.split = f.c.tiles > kWhole && blocks * 2 <= kMostSplit;
-  const dim3 grid = a.split ? dim3(kMostSplit) : dim3((unsigned)(f.c.n_seq * f.c.n_head), (unsigned)a.cblocks);
+  if (f.c.tiles > kWhole && blocks * 2 <= few_room(f.c)) a.room = few_room(f.c);
+  const dim3 grid = a.room ? dim3((unsigned)a.room) : dim3((unsigned)(f.c.n_seq * f.c.n_head), (unsigned)a.cblocks);
   if (f.c.hdp == 64) f_attend_kernel<64, QP, PP, T><<<grid, 64 * kWaves, 0, s>>>(a);
   else f_attend_kernel<128, QP, PP, T><<<grid, 64 * kWaves, 0, s>>>(a);
 }
@@ -650,15 +649,8 @@ void weigh_t(hipStream_t s, const FAttn& f, float decay) {
 
 }  // namespace
 
-namespace {
-size_t few_work_bytes(int hdp) { return (size_t)kMostSplit * (kQTicketStride * 4 + (size_t)kCols * (hdp + 2) * 4); }
-}  // namespace
-// (each kernel's tickets and partial results, one behind the other)
-size_t fattn_work_bytes(int hdp) { return few_work_bytes(hdp) + fmany_work_bytes(hdp); }
-void fattn_work_clear(hipStream_t s, void* work, int hdp) {
-  (void)hipMemsetAsync(work, 0, (size_t)kMostSplit * kQTicketStride * 4, s);
-  (void)hipMemsetAsync(static_cast<char*>(work) + few_work_bytes(hdp), 0, fmany_tickets_bytes(), s);
-}
+size_t fattn_work_bytes(const FStore& c) { return 2 * kTicketBytes + fattn_parts_bytes(c); }
+void fattn_work_clear(hipStream_t s, void* work) { (void)hipMemsetAsync(work, 0, 2 * kTicketBytes, s); }
 
 namespace {
 // What the two kernels take, in us, fitted to 702 calls (24 to 3200 columns of 2 to 320
@@ -688,13 +680,13 @@ bool for_many(const FAttn& f) {
   const Costs& c = kCosts[f.type == Q_F32 ? 0 : f.type == Q_BF16 ? 1 : 2][f.c.hdp == 128];
   const float b = heads * blocks / 256.f, few = c.few + b * (c.few_block + c.few_tile * (keys / 32.f));
   if (rows > 256) return few > c.many + rows / 512.f * (c.many_block + c.many_tile * (keys / 32.f));
-  const long parts = fmany_parts(rows, f.c.tiles);
+  const long parts = fmany_parts(rows, f.c);
   return few > c.many + (parts > 1 ? c.many_join : 0.f) + c.many_split * ((keys + parts - 1) / parts / 32.f);
 }
 }  // namespace
 
 void launch_f_attend(hipStream_t s, const FAttn& f) {
-  if (for_many(f)) return launch_f_attend_many(s, f, static_cast<char*>(f.work) + few_work_bytes(f.c.hdp));
+  if (for_many(f)) return launch_f_attend_many(s, f);
   if (f.type == Q_F32) attend_t<3, 3, float>(s, f);
   else if (f.type == Q_BF16) attend_t<1, 2, __bf16>(s, f);
   else attend_t<2, 2, _Float16>(s, f);
