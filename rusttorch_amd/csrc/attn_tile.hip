@@ -38,7 +38,6 @@ namespace rtg {
 namespace {
 
 constexpr int kKeys = 64;      // of a stage in LDS
-constexpr int kMinStages = 8;     // of a part at least
 constexpr float kSlack = 8.f;  // powers of two that a score may pass the running maximum by
 
 struct Args {
@@ -839,7 +838,7 @@ void many_t(hipStream_t s, Args a) {
   if (tiles <= kSplits) {
     // eight waves a workgroup, one workgroup a compute unit; the keys are split where there are fewer
     a.min_stages = kMinStages;
-    grid.z = (unsigned)fmany_parts(tiles, a.c);
+    grid.z = (unsigned)fmany_parts(tiles, a.c.sizes());
     constexpr int KG = QP == 3 ? 1 : 2;  // (f32 queries of 128 columns leave registers for four)
     if (a.c.hdp == 64) f_attend_many_kernel<64, QP, PP, T, 2><<<grid, 512, 0, s>>>(a);
     else f_attend_many_kernel<128, QP, PP, T, KG><<<grid, 256 * KG, 0, s>>>(a);
@@ -886,10 +885,6 @@ void packed(hipStream_t s, const Args& a) {
 }
 
 }  // namespace
-
-long fmany_parts(long row_tiles, const FStore& c) {
-  return std::max(1l, std::min(many_room(c) / row_tiles, ((long)c.tiles / 2 + kMinStages - 1) / kMinStages));
-}
 
 void launch_f_attend_many(hipStream_t s, const FAttn& f) {
   Args a = {};

@@ -16,6 +16,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "fourbit_choice.h"
 #include "qcache.h"
 
 namespace rtg {
@@ -41,12 +42,12 @@ struct FStore {
   uint8_t *sk = nullptr, *sv = nullptr;  // scales [seq][head][tile][hdp]
   float* w = nullptr;  // what attention the tokens have got [seq][head][tiles * 32]
 
+  FSizes sizes() const { return {n_seq, n_head, hdp, tiles}; }
   __host__ __device__ size_t codes(size_t sh) const { return sh * tiles * (size_t)(16 * hdp); }
   __host__ __device__ size_t scales(size_t sh) const { return sh * tiles * (size_t)hdp; }
   __host__ __device__ size_t weights(size_t sh) const { return sh * tiles * (size_t)kFTile; }
 };
 
-size_t fstore_bytes(const FStore& c);
 void fstore_shape(FStore* c, int n_seq, int n_head, int hd, int capacity);
 void fstore_place(FStore* c, void* mem);
 
@@ -83,32 +84,13 @@ struct FAttn {
 void launch_f_attend(hipStream_t s, const FAttn& a);
 // for many queries (launch_f_attend chooses)
 void launch_f_attend_many(hipStream_t s, const FAttn& a);
-long fmany_parts(long row_tiles, const FStore& c);  // that the keys are split into, for up to kSplits tiles of 128 rows
 // w = decay * w + the probabilities that the queries (as in launch_f_attend, whose
 // stats it takes) give a token, summed over the counted queries and the heads of
 // the token's head; decay 0: w as it was is not read.
 void launch_f_weigh(hipStream_t s, const FAttn& a, float decay);
 size_t fattn_work_bytes(const FStore& c);
 void fattn_work_clear(hipStream_t s, void* work);
-
-// Workgroups at most where the keys are split, and how many of them there is room for.
-// One's results take 4 KB (16 columns) or 34 (128 rows) for heads up to 64 channels,
-// twice that above: room for all of them, 9 or 17 MB, would be more than the keys and
-// values of a cache of up to 10000 tokens of 12 heads, and there is one for each layer;
-// so there is room for half as many bytes as the cache holds.
-constexpr int kSplits = 256;
 constexpr size_t kTicketBytes = (size_t)kSplits * kQTicketStride * 4;
-inline size_t few_part_bytes(const FStore& c) { return 16 * (size_t)(c.hdp + 2) * 4; }
-inline size_t many_part_bytes(const FStore& c) { return 128 * (size_t)(c.hdp + 4) * 4; }
-inline size_t fattn_parts_bytes(const FStore& c) {
-  const size_t half = fstore_bytes(c) / 2 / 256 * 256, all = kSplits * many_part_bytes(c);
-  return half < all ? half : all;
-}
-inline int few_room(const FStore& c) {
-  const size_t n = fattn_parts_bytes(c) / few_part_bytes(c);
-  return n < kSplits ? (int)n : kSplits;
-}
-inline int many_room(const FStore& c) { return (int)(fattn_parts_bytes(c) / many_part_bytes(c)); }
 
 // Causal attention of packed sequences, each over itself: rows [n_rows][head][hd]
 // (the rows' seq strides are not used), sequence s at rows offsets[s] ..

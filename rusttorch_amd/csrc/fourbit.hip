@@ -19,23 +19,13 @@ void fstore_shape(FStore* c, int n_seq, int n_head, int hd, int capacity) {
   c->tiles = (capacity + kFTile - 1) / kFTile;
 }
 
-namespace {
-size_t up256(size_t x) { return (x + 255) / 256 * 256; }
-}  // namespace
-
-size_t fstore_bytes(const FStore& c) {
-  const size_t sh = (size_t)c.n_seq * c.n_head;
-  return 2 * up256(c.codes(sh)) + 2 * up256(c.scales(sh)) + up256(c.weights(sh) * 4);
-}
-
 void fstore_place(FStore* c, void* mem) {
-  const size_t sh = (size_t)c->n_seq * c->n_head, codes = up256(c->codes(sh)), scales = up256(c->scales(sh));
-  uint8_t* m = static_cast<uint8_t*>(mem);
-  c->k = m;
-  c->v = c->k + codes;
-  c->sk = c->v + codes;
-  c->sv = c->sk + scales;
-  c->w = reinterpret_cast<float*>(c->sv + scales);
+  const FSizes size = c->sizes();
+  c->k = static_cast<uint8_t*>(mem);
+  c->v = c->k + size.code_bytes();
+  c->sk = c->v + size.code_bytes();
+  c->sv = c->sk + size.scale_bytes();
+  c->w = reinterpret_cast<float*>(c->sv + size.scale_bytes());
 }
 
 namespace {

@@ -130,7 +130,7 @@ rtg_result rtg_fourbit_new(size_t n_seq, size_t n_head, size_t head_dim, size_t 
     q->device = device;
     fstore_shape(&q->c, (int)n_seq, (int)n_head, (int)head_dim, (int)capacity);
     const size_t lens = (n_seq * 4 + 4 + 255) / 256 * 256, head = lens + n_seq * kQTicketStride * 4;
-    hipError_t e = device_malloc(&q->mem, (head + 255) / 256 * 256 + fstore_bytes(q->c) + fattn_work_bytes(q->c));
+    hipError_t e = device_malloc(&q->mem, (head + 255) / 256 * 256 + q->c.sizes().bytes() + fattn_work_bytes(q->c));
     if (e != hipSuccess) return hip_err(e, "rtg_fourbit_new");
     char* mem = static_cast<char*>(q->mem);
     q->len = static_cast<int*>(q->mem);
@@ -138,7 +138,7 @@ rtg_result rtg_fourbit_new(size_t n_seq, size_t n_head, size_t head_dim, size_t 
     q->tickets.count = reinterpret_cast<unsigned*>(mem + lens);
     mem += (head + 255) / 256 * 256;
     fstore_place(&q->c, mem);
-    q->work = mem + fstore_bytes(q->c);
+    q->work = mem + q->c.sizes().bytes();
     hipStream_t s = nullptr;  // (of its own: the default one may be what a capture waits for)
     e = hipStreamCreateWithFlags(&s, hipStreamNonBlocking);
     if (e == hipSuccess) e = hipMemsetAsync(q->mem, 0, head, s);

@@ -27,7 +27,7 @@
 namespace rtg {
 namespace {
 
-constexpr int kCols = 16, kWaves = 8, kWeighWaves = 4;
+constexpr int kWaves = 8, kWeighWaves = 4;
 constexpr int kWhole = 32, kSplitTiles = 8;  // tiles that are not split; of a split at least
 constexpr float kSlack = 8.f;     // powers of two that a score may pass the maximum by
 
@@ -632,7 +632,8 @@ void attend_t(hipStream_t s, const FAttn& f) {
   // 62, as the partial results take their time), and more than 32 tiles, for a join
   // takes as long as four rounds of the eight waves.
   const long blocks = (long)f.c.n_seq * f.c.n_head * a.cblocks;
-  if (f.c.tiles > kWhole && blocks * 2 <= few_room(f.c)) a.room = few_room(f.c);
+  const int room = few_room(f.c.sizes());
+  if (f.c.tiles > kWhole && blocks * 2 <= room) a.room = room;
   const dim3 grid = a.room ? dim3((unsigned)a.room) : dim3((unsigned)(f.c.n_seq * f.c.n_head), (unsigned)a.cblocks);
   if (f.c.hdp == 64) f_attend_kernel<64, QP, PP, T><<<grid, 64 * kWaves, 0, s>>>(a);
   else f_attend_kernel<128, QP, PP, T><<<grid, 64 * kWaves, 0, s>>>(a);
@@ -649,44 +650,12 @@ void weigh_t(hipStream_t s, const FAttn& f, float decay) {
 
 }  // namespace
 
-size_t fattn_work_bytes(const FStore& c) { return 2 * kTicketBytes + fattn_parts_bytes(c); }
+size_t fattn_work_bytes(const FStore& c) { return 2 * kTicketBytes + fattn_parts_bytes(c.sizes()); }
 void fattn_work_clear(hipStream_t s, void* work) { (void)hipMemsetAsync(work, 0, 2 * kTicketBytes, s); }
 
-namespace {
-// What the two kernels take, in us, fitted to 702 calls (24 to 3200 columns of 2 to 320
-// sequences' heads, 40 to 4400 tokens) within 9 and 6 % on average: by blocks of 16
-// columns, tiles of 128 rows, and the keys' tiles that a sequence may have, as the host
-// does not know the lengths (both take less where they are shorter). The kernel that is
-// chosen so takes 2 % longer than the better one on average, at most 59 %; by a least
-// number of columns and of blocks times tiles it was 5 % and 143 %: 24 sequences of 8
-// heads of 80, 202 queries behind 554 tokens in f16, took 64 us, now 36. Far behind the
-// fitted lengths it can miss by as much: 84 queries of 20 heads of 64 behind 2 x 30000
-// in f16 take 112 us, by the other kernel 92.
-struct Costs {
-  float few, few_block, few_tile;        // a call; 256 blocks; 256 blocks of 32 tiles of keys
-  float many, many_join, many_split;     // up to 256 tiles of rows: a call; parts to join; 32 tiles of keys of a part
-  float many_block, many_tile;           // more: 512 of them; 512 of 32 tiles of keys
-};
-constexpr Costs kCosts[3][2] = {
-    {{7.5f, 0.5f, 3.4f, 8.9f, 3.3f, 19.5f, 0.9f, 46.6f}, {6.3f, 2.8f, 6.2f, 10.0f, 3.9f, 40.5f, 15.4f, 88.5f}},  // f32
-    {{7.3f, 0.3f, 2.6f, 7.7f, 3.2f, 11.7f, 0.7f, 23.5f}, {6.4f, 2.1f, 4.6f, 9.6f, 6.2f, 15.6f, 1.5f, 38.3f}},    // bf16
-    {{7.2f, 0.4f, 2.8f, 7.9f, 3.4f, 16.7f, 1.0f, 33.1f}, {6.4f, 2.2f, 5.0f, 10.4f, 6.0f, 23.1f, 1.7f, 56.2f}},   // f16
-};
-bool for_many(const FAttn& f) {
-  const long columns = (long)f.n_q * (f.n_q_head / f.c.n_head), blocks = (columns + kCols - 1) / kCols;
-  if (columns <= 32) return false;   // (a quarter of the rows at most)
-  if (blocks > 65535) return true;   // (what a grid holds)
-  const long heads = (long)f.c.n_seq * f.c.n_head, rows = heads * ((columns + 127) / 128), keys = f.c.tiles;
-  const Costs& c = kCosts[f.type == Q_F32 ? 0 : f.type == Q_BF16 ? 1 : 2][f.c.hdp == 128];
-  const float b = heads * blocks / 256.f, few = c.few + b * (c.few_block + c.few_tile * (keys / 32.f));
-  if (rows > 256) return few > c.many + rows / 512.f * (c.many_block + c.many_tile * (keys / 32.f));
-  const long parts = fmany_parts(rows, f.c);
-  return few > c.many + (parts > 1 ? c.many_join : 0.f) + c.many_split * ((keys + parts - 1) / parts / 32.f);
-}
-}  // namespace
-
 void launch_f_attend(hipStream_t s, const FAttn& f) {
-  if (for_many(f)) return launch_f_attend_many(s, f);
+  const int type = f.type == Q_F32 ? 0 : f.type == Q_BF16 ? 1 : 2;
+  if (for_many(f.c.sizes(), type, (long)f.n_q * (f.n_q_head / f.c.n_head))) return launch_f_attend_many(s, f);
   if (f.type == Q_F32) attend_t<3, 3, float>(s, f);
   else if (f.type == Q_BF16) attend_t<1, 2, __bf16>(s, f);
   else attend_t<2, 2, _Float16>(s, f);
