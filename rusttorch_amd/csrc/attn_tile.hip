@@ -463,8 +463,8 @@ __device__ __forceinline__ void attend(const Args& a, const Job& job, Shared<HD,
     fetch(own + SPAN, bufs[0]);
   }
   // Between their matrix instructions a SIMD's two waves leave each other room, so the
-  // one that is at its products goes first (2047 tokens behind 12001 in bf16: 428 us
-  // without, 398 with; 16000 packed 1903 and 1853). With f32's six products it does
+  // one that is at its products goes first (2047 tokens behind 12001 in bf16: 559 us
+  // without, 532 with; 16000 packed 2547 and 2519). With f32's six products it does
   // not pay (500 behind 4 x 4000: 89 us, 95 with).
   auto in_products = [](bool yes) {
     if constexpr (QP < 3) {
@@ -703,8 +703,9 @@ __global__ __launch_bounds__(256 * KG, KG > 1 || HD == 64 || sizeof(T) == 2 ? 2 
 // the rows' tiles and the number of sequences.
 // Up to 64 sequences are taken by their lengths, a sequence's tiles by the keys they
 // see, so that what runs last is short (8 x up to 1500 tokens of 32 heads of 128 over
-// 8 in bf16: 117 us; the longest tiles of all sequences first would be shorter still
-// at the end, but the keys of 8 sequences do not fit the caches that one's do: 128).
+// 8 in bf16: 142 us; the longest tiles of all sequences first would be shorter still
+// at the end, but the keys of 8 sequences do not fit the caches that one's do: 128 us
+// instead of 117 with one part of probabilities). More are taken in their order.
 // Where all workgroups are on the device at once, RESIDENT of them on each of its 256
 // compute units, every second 256 go the other way, so that those of a compute unit
 // have about the same to do between them.
@@ -858,7 +859,9 @@ void packed_t(hipStream_t s, const Args& a) {
   // Where all tiles are on the device at once, the time is that of the tile with most
   // keys: two groups of waves have every second stage of its keys each, if it has many
   // of them (4001 tokens of 12 heads of 64 in f32: 171 us, 198 with one group; of 16
-  // in f16: 52 and 58; 16 x up to 1023 of 20 in f32: 191 and 161).
+  // in f16: 73 and 79; 16 x up to 1023 of 20 in f32: 191 and 161). (Rows of 16 bits that
+  // are not aligned, in heads above 64: all registers are taken, and two to four that the
+  // results need at the end wait in scratch meanwhile.)
   const bool two = a.n_rows * (long)a.group / 128 * a.n_head <= 512 && a.n_rows >= 512L * a.n_seq;
   if constexpr (sizeof(T) == 4) {
     // (one buffer: with two, 64 columns take 96 KB, which leaves a compute unit one
